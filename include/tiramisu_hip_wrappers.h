@@ -162,6 +162,54 @@ float tiramisu_hip_event_elapsed_ms(void *start, void *stop); /* waits for `stop
 int tiramisu_hip_event_destroy(void *event);
 int tiramisu_hip_device_count(void);
 
+/* ---- operators of a transformer's feed-forward sublayer on this build's own kernels, forward and backward (the reference has
+ *      nothing of the kind).  All pointers are GPU memory; all launches go to the calling thread's stream and nothing waits.
+ *      Matrices are row-major with their columns dense and `ld...` elements from row to row (0: dense rows too); results are dense and must not
+ *      overlap inputs.  Weights are [outputs][inputs].  Operands may begin at any element; rows that the
+ *      matrix kernels cannot load in place (odd strides of 16-bit elements) are moved to scratch first.  Sums are kept in 32 bits and rounded once.
+ *      Types and activations are the numbers below.  Arguments that do not fit together are refused: a message on stderr,
+ *      return value 1, nothing launched.  Scratch is kept per thread and stream like tiramisu_hip_sgemm's; a call that is
+ *      recorded into a graph has to have run before on that thread and stream at that size, so that the scratch is there. ---- */
+enum tiramisu_hip_element_t { TIRAMISU_HIP_FLOAT32 = 0, TIRAMISU_HIP_FLOAT16 = 1, TIRAMISU_HIP_BFLOAT16 = 2, TIRAMISU_HIP_FLOAT8_E4M3 = 3 };
+enum tiramisu_hip_activation_t {
+    TIRAMISU_HIP_NONE = 0, TIRAMISU_HIP_RELU = 1, TIRAMISU_HIP_GELU = 2 /* erf */, TIRAMISU_HIP_GELU_TANH = 3, TIRAMISU_HIP_SILU = 4
+};
+
+/* sum = x + residual (both or neither; else x itself), rstd = 1 / sqrt(mean(sum^2) + eps) of each row, y = sum rstd weight, of the
+ * sum ahead of its rounding.  x, residual, weight, sum: `type` (float32, float16, bfloat16); y: the same, or y_type float8_e4m3:
+ * y / scale with scale = max|y| / 448 of each row (1 for a row of zeros).  rstd may be null. */
+int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum, float *scale, float *rstd,
+                          uint64_t rows, uint64_t columns, uint64_t ldx, uint64_t ldr, float eps, int32_t type, int32_t y_type);
+/* dx = rstd (g - sum rstd^2 mean(g sum)) + dsum with g = dy weight; dweight = sum over the rows of dy sum rstd.  dsum (the
+ * gradient that arrives at the sum itself) may be null.  dx is the gradient of x and of the residual.  Deterministic. */
+int tiramisu_hip_rms_norm_backward(const void *dy, const void *sum, const void *weight, const float *rstd, const void *dsum, void *dx,
+                                   void *dweight, uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t lds, uint64_t ldd, int32_t type);
+/* q = x / scale in float8_e4m3, scale = max|x| / 448 of each row (1 for a row of zeros). */
+int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type);
+
+/* z = x weight^T [x_scale of the row, weight_scale of the column] + bias; pre = z; y = activation(z) + residual.  x is M x K, weight N x K, both of
+ * `type`: float16 or bfloat16 (then y_type is the same), or float8_e4m3 with scales (y_type float16 or bfloat16).  bias,
+ * residual, y and pre are of y_type; bias, residual and pre may be null. */
+int tiramisu_hip_linear(const void *x, const void *weight, const void *bias, const void *residual, const float *x_scale,
+                        const float *weight_scale, void *y, void *pre, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldw,
+                        uint64_t ldr, int32_t activation, int32_t type, int32_t y_type);
+/* dz = dy activation'(pre), dx = dz weight, dweight = dz^T x, dbias = sum over the rows of dz (the residual's gradient is dy).  Of
+ * float16 or bfloat16 throughout; dz is rounded to that type ahead of the products.  dx, dweight, dbias may be null; pre is null where
+ * the activation is none. */
+int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weight, const void *pre, void *dx, void *dweight, void *dbias,
+                                 uint64_t M, uint64_t N, uint64_t K, uint64_t ldy, uint64_t ldx, uint64_t ldw, uint64_t ldp, int32_t activation,
+                                 int32_t type);
+/* gate = x gate_weight^T, up = x up_weight^T (scaled like tiramisu_hip_linear), h = activation(gate) up, in one kernel.  gate and up are stored
+ * where both are given (what the backward pass reads). */
+int tiramisu_hip_gated_linear(const void *x, const void *gate_weight, const void *up_weight, const float *x_scale, const float *gate_scale,
+                              const float *up_scale, void *h, void *gate, void *up, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldg,
+                              uint64_t ldu, int32_t activation, int32_t type, int32_t h_type);
+/* dgate = dh up activation'(gate), dup = dh activation(gate), dx = dgate gate_weight + dup up_weight, dgate_weight = dgate^T x, dup_weight =
+ * dup^T x.  dgate and dup are rounded to `type` ahead of the products.  dx may be null, and so may both weights' gradients. */
+int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate,
+                                       const void *up, void *dx, void *dgate_weight, void *dup_weight, uint64_t M, uint64_t N, uint64_t K, uint64_t ldh,
+                                       uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
+
 /* ---- per-launch timing.  Between profile_start and profile_stop every tiramisu_hip_launch
  *      (and GEMM library call), from any thread, is bracketed by two events on its current
  *      stream; profile_stop waits for them and keeps one (kernel name, milliseconds) record

@@ -12,6 +12,7 @@ Three kinds of artefacts, all in-tree so that they travel to the GPU machine:
 
 Nothing here needs a GPU: hipcc cross-compiles for gfx950.
 """
+import concurrent.futures
 import os
 import subprocess
 import sys
@@ -72,15 +73,25 @@ def build_compiler(force=True):
     return out
 
 
+# The runtime's translation units: (object, source, what it is compiled with).  The matrix products' kernels are one unit for each type of operand.
+WRAPPER_UNITS = [("hip_wrappers", "hip_wrappers.hip", []), ("operators", "operators.hip", [])] + \
+    [("linear_tiles_" + e.lower(), "linear_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16", "F8")]
+
+
 def build_wrappers(force=True):
-    src = os.path.join(CSRC, "hip_wrappers.hip")
     kdir = os.path.join(CSRC, "kernels")
-    deps = [src, os.path.join(INCLUDE, "tiramisu_hip_wrappers.h")] + \
-        [os.path.join(kdir, h) for h in os.listdir(kdir)]
+    deps = sorted({os.path.join(CSRC, source) for _, source, _ in WRAPPER_UNITS}) + \
+        [os.path.join(CSRC, "operators.h"), os.path.join(INCLUDE, "tiramisu_hip_wrappers.h")] + [os.path.join(kdir, h) for h in os.listdir(kdir)]
     out = wrappers_library()
     if not force and _newer(out, deps):
         return out
-    _run([HIPCC] + HIP_FLAGS + ["-fPIC", "-shared", "-o", out, src])
+    odir = os.path.join(PKG, "build")
+    os.makedirs(odir, exist_ok=True)
+    objects = [os.path.join(odir, name + ".o") for name, _, _ in WRAPPER_UNITS]
+    with concurrent.futures.ThreadPoolExecutor(len(WRAPPER_UNITS)) as pool:         # (each thread waits for a compiler of its own)
+        list(pool.map(lambda unit: _run([HIPCC] + HIP_FLAGS + unit[2] + ["-fPIC", "-c", "-o", os.path.join(odir, unit[0] + ".o"), os.path.join(CSRC, unit[1])]),
+                      WRAPPER_UNITS))
+    _run([HIPCC] + HIP_FLAGS + ["-fPIC", "-shared", "-o", out] + objects)
     return out
 
 

@@ -22,6 +22,7 @@
 #include "kernels/gemm_mfma_f64.hip.h"
 #include "kernels/gemm_mfma_split.hip.h"
 #include "kernels/target_gfx950.h"
+#include "operators.h"
 
 namespace {
 
@@ -454,6 +455,23 @@ void launch_dgemm(bool transposeA, bool transposeB, const double *A, const doubl
 }
 
 }  // namespace
+
+// What the operators' translation units use of this one's state (operators.h)
+namespace tiramisu_runtime {
+
+hipStream_t stream() { return current_stream; }
+void check(hipError_t e, const char *function) { ::check(e, function); }
+timed::timed(const char *name) : stop(nullptr) {
+    if (!profiling) return;
+    scoped_record r(name);
+    std::swap(stop, r.stop);
+    r.on = false;                            // the record ends with this object
+}
+timed::~timed() {
+    if (stop) ::check(hipEventRecord(stop, current_stream), "tiramisu_hip_profile");
+}
+
+}  // namespace tiramisu_runtime
 
 extern "C" {
 

@@ -1,0 +1,318 @@
+// Root-mean-square norm of rows, with the addition of a residual ahead of it and rows of 8-bit numbers with a scale behind it:
+//     s = x + r,   rstd = 1 / sqrt(mean(s^2) + eps),   y = s rstd w,   or   q = e4m3(y / scale), scale = max|y| / 448
+// and backward, from the gradient dy of y and ds that arrives along the residual stream:
+//     dx = rstd (g - s rstd^2 mean(g s)) + ds with g = dy w,      dw = sum over rows of dy s rstd.
+// Each input is read once and each output written once: a row stays in the registers of its team (64, 256 or 1024 threads, PER
+// pieces of 16 bytes of the widest input each), which reduces it by lane exchanges and, where it is more than a wavefront, through LDS.  The norm
+// is of the unrounded sum.  Rows too long for that are read a second time.
+// Sums of the backward pass over rows are kept per team in registers, written once, and added by a second launch in a fixed
+// order: results do not depend on the order of workgroups.
+#ifndef TIRAMISU_AMD_RMS_NORM_HIP_H
+#define TIRAMISU_AMD_RMS_NORM_HIP_H
+#include "operator_elements.hip.h"
+
+namespace tops {
+
+struct norm_arguments {
+    const void *x, *residual, *weight;      // residual: may be null; weight: null for quantize_rows
+    void *y, *sum;                          // sum: may be null
+    float *scale, *rstd;                    // may be null
+    long rows, columns, ldx, ldr;
+    float eps;
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// the larger of two, and NaN where one is
+__device__ __forceinline__ float max_or_nan(float a, float b) { return a > b || a != a ? a : b; }
+__device__ __forceinline__ float wave_max_or_nan(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max_or_nan(v, __shfl_xor(v, o));
+    return v;
+}
+
+// Reductions over a team of TEAM threads.  `slot`: TEAM / 64 floats of LDS that no other reduction in flight uses; a team larger than a
+// wavefront is the whole workgroup, and its slots alternate, so that one barrier a reduction is enough.
+template <int TEAM, bool MAX>
+__device__ __forceinline__ float team_reduce(float v, float *slot) {
+    v = MAX ? wave_max_or_nan(v) : wave_sum(v);
+    if constexpr (TEAM > 64) {
+        constexpr int WAVES = TEAM / 64;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        if (lane == 0) slot[wave] = v;
+        __syncthreads();
+        v = slot[lane & (WAVES - 1)];
+#pragma unroll
+        for (int o = WAVES / 2; o > 0; o >>= 1) {
+            const float other = __shfl_xor(v, o);
+            v = MAX ? max_or_nan(v, other) : v + other;
+        }
+    }
+    return v;
+}
+
+// Y: element type of y (E, or F8).  HELD: the row fits TEAM x PER pieces; else it is read again.
+template <int E, int Y, int TEAM, int PER, bool HELD>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void rms_norm_kernel(norm_arguments a) {
+    constexpr int N = E == F32 ? 4 : 8;                      // elements of a piece
+    constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+    __shared__ float slots[2][TEAM > 64 ? TEAM / 64 : 1];
+    const int t = threadIdx.x % TEAM;
+    const long row = (long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
+    if (TEAMS > 1 && row >= a.rows) return;                  // a whole wavefront, and no barrier follows in teams of one
+    typedef stored<E> T;
+    const T *x = (const T *)a.x + row * a.ldx, *r = a.residual ? (const T *)a.residual + row * a.ldr : nullptr, *w = (const T *)a.weight;
+    T *sum = a.sum ? (T *)a.sum + row * a.columns : nullptr;
+    stored<Y> *y = (stored<Y> *)a.y + row * a.columns;
+    const int pieces = HELD ? PER : (int)((a.columns + TEAM * N - 1) / (TEAM * N));
+
+    float held[HELD ? PER : 1][N];
+    float squares = 0.f;
+    auto read = [&](int p, float (&v)[N]) {
+        const long c = ((long)p * TEAM + t) * N;
+        const int n = (int)min((long)N, a.columns - c);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = 0.f;
+        if (n <= 0) return;
+        load_some<E>(x + c, n, v);
+        if (r) {
+            float other[N];
+            load_some<E>(r + c, n, other);
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] += other[i];
+        }
+    };
+    auto finish = [&](int p, float (&v)[N], float factor) {  // v: s; becomes y
+        const long c = ((long)p * TEAM + t) * N;
+        const int n = (int)min((long)N, a.columns - c);
+        if (n <= 0) {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = 0.f;
+            return;
+        }
+        float g[N];
+        if (w) load_some<E>(w + c, n, g);
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = w ? v[i] * factor * g[i] : v[i];
+    };
+    auto write_sum = [&](int p, float (&v)[N]) {
+        const long c = ((long)p * TEAM + t) * N;
+        const int n = (int)min((long)N, a.columns - c);
+        if (n > 0) store_some<E>(sum + c, n, v);
+    };
+
+    if constexpr (HELD) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) read(p, held[p]);
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+#pragma unroll
+            for (int i = 0; i < N; i++) squares += held[p][i] * held[p][i];
+            if (sum) write_sum(p, held[p]);
+        }
+    } else {
+        for (int p = 0; p < pieces; p++) {
+            float v[N];
+            read(p, v);
+#pragma unroll
+            for (int i = 0; i < N; i++) squares += v[i] * v[i];
+        }
+    }
+    float rstd = 1.f;
+    if (w) {
+        squares = team_reduce<TEAM, false>(squares, slots[0]);
+        rstd = 1.f / sqrtf(squares / (float)a.columns + a.eps);
+        if (a.rstd && t == 0) a.rstd[row] = rstd;
+    }
+    float most = 0.f;
+    if constexpr (Y == F8) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int p = 0; p < PER; p++) {
+                finish(p, held[p], rstd);
+#pragma unroll
+                for (int i = 0; i < N; i++) most = max_or_nan(fabsf(held[p][i]), most);
+            }
+        } else {
+            for (int p = 0; p < pieces; p++) {
+                float v[N];
+                read(p, v);
+                finish(p, v, rstd);
+#pragma unroll
+                for (int i = 0; i < N; i++) most = max_or_nan(fabsf(v[i]), most);
+            }
+        }
+        most = team_reduce<TEAM, true>(most, slots[1]);
+        most = most == 0.f ? 1.f : most / E4M3_MOST;         // the scale; a row of zeros has 1
+        if (t == 0) a.scale[row] = most;
+    }
+    auto write = [&](int p, float (&v)[N]) {
+        const long c = ((long)p * TEAM + t) * N;
+        const int n = (int)min((long)N, a.columns - c);
+        if (n <= 0) return;
+        if constexpr (Y == F8) {
+            // (a scale below the normal numbers is rounded coarsely: what then lies beyond the format's largest number is set to it)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                v[i] /= most;
+                v[i] = v[i] > E4M3_MOST ? E4M3_MOST : v[i] < -E4M3_MOST ? -E4M3_MOST : v[i];
+            }
+        }
+        store_some<Y>(y + c, n, v);
+    };
+    if constexpr (HELD) {
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            if constexpr (Y != F8) finish(p, held[p], rstd);
+            write(p, held[p]);
+        }
+    } else {
+        for (int p = 0; p < pieces; p++) {
+            float v[N];
+            read(p, v);
+            if (sum) write_sum(p, v);
+            finish(p, v, rstd);
+            write(p, v);
+        }
+    }
+}
+
+struct norm_backward_arguments {
+    const void *dy, *sum, *weight, *dsum;   // dsum: may be null
+    const float *rstd;
+    void *dx;
+    float *partial;                         // [teams][columns]
+    long rows, columns, ldy, lds, ldd;
+    int teams;
+};
+
+// Teams walk over the rows, team g taking rows g, g + teams, ...
+template <int E, int TEAM, int PER>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void rms_norm_backward_kernel(norm_backward_arguments a) {
+    constexpr int N = E == F32 ? 4 : 8;
+    constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+    __shared__ float slots[2][TEAM > 64 ? TEAM / 64 : 1];
+    typedef stored<E> T;
+    const int t = threadIdx.x % TEAM;
+    const long team = (long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
+    if (TEAMS > 1 && team >= a.teams) return;
+    float dw[PER][N];
+#pragma unroll
+    for (int p = 0; p < PER; p++)
+#pragma unroll
+        for (int i = 0; i < N; i++) dw[p][i] = 0.f;
+    int turn = 0;
+    for (long row = team; row < a.rows; row += a.teams, turn ^= 1) {
+        const T *dy = (const T *)a.dy + row * a.ldy, *s = (const T *)a.sum + row * a.lds, *w = (const T *)a.weight;
+        const float rstd = a.rstd[row];
+        float xhat[PER][N], g[PER][N];
+        float dot = 0.f;
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const long c = ((long)p * TEAM + t) * N;
+            const int n = (int)min((long)N, a.columns - c);
+#pragma unroll
+            for (int i = 0; i < N; i++) xhat[p][i] = g[p][i] = 0.f;
+            if (n > 0) {
+                load_some<E>(s + c, n, xhat[p]);
+                load_some<E>(dy + c, n, g[p]);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const long c = ((long)p * TEAM + t) * N;
+            const int n = (int)min((long)N, a.columns - c);
+            float f[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) f[i] = 0.f;
+            if (n > 0) load_some<E>(w + c, n, f);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                xhat[p][i] *= rstd;
+                dw[p][i] += g[p][i] * xhat[p][i];
+                g[p][i] *= f[i];
+                dot += g[p][i] * xhat[p][i];
+            }
+        }
+        dot = team_reduce<TEAM, false>(dot, slots[turn]) / (float)a.columns;
+        T *dx = (T *)a.dx + row * a.columns;
+        const T *ds = a.dsum ? (const T *)a.dsum + row * a.ldd : nullptr;
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const long c = ((long)p * TEAM + t) * N;
+            const int n = (int)min((long)N, a.columns - c);
+            if (n <= 0) continue;
+            float v[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = rstd * (g[p][i] - xhat[p][i] * dot);
+            if (ds) {
+                float d[N];
+                load_some<E>(ds + c, n, d);
+#pragma unroll
+                for (int i = 0; i < N; i++) v[i] += d[i];
+            }
+            store_some<E>(dx + c, n, v);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PER; p++) {
+        const long c = ((long)p * TEAM + t) * N;
+        const int n = (int)min((long)N, a.columns - c);
+        if (n > 0) store_some<F32>(a.partial + team * a.columns + c, n, dw[p]);
+    }
+}
+
+// Rows that no team holds: dx by a workgroup for each row, reading it twice, and the columns' sums by threads that walk down them.
+template <int E>
+__global__ __launch_bounds__(1024) void rms_norm_backward_long_rows_kernel(norm_backward_arguments a) {
+    __shared__ float slots[16];
+    typedef stored<E> T;
+    const long row = blockIdx.x;
+    const T *dy = (const T *)a.dy + row * a.ldy, *s = (const T *)a.sum + row * a.lds, *w = (const T *)a.weight;
+    const T *ds = a.dsum ? (const T *)a.dsum + row * a.ldd : nullptr;
+    const float rstd = a.rstd[row];
+    float dot = 0.f;
+    for (long c = threadIdx.x; c < a.columns; c += 1024) dot += (float)dy[c] * (float)w[c] * ((float)s[c] * rstd);
+    dot = team_reduce<1024, false>(dot, slots) / (float)a.columns;
+    for (long c = threadIdx.x; c < a.columns; c += 1024) {
+        float v = rstd * ((float)dy[c] * (float)w[c] - (float)s[c] * rstd * dot);
+        if (ds) v += (float)ds[c];
+        ((T *)a.dx)[row * a.columns + c] = (T)v;
+    }
+}
+template <int E>
+__global__ __launch_bounds__(256) void rms_norm_backward_long_columns_kernel(norm_backward_arguments a) {
+    typedef stored<E> T;
+    const long c = (long)blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.columns) return;
+    float sum = 0.f;
+    for (long row = blockIdx.y; row < a.rows; row += a.teams)
+        sum += (float)((const T *)a.dy)[row * a.ldy + c] * ((float)((const T *)a.sum)[row * a.lds + c] * a.rstd[row]);
+    a.partial[(long)blockIdx.y * a.columns + c] = sum;
+}
+
+// out[c] = sum over `parts` rows of partial[][c], in a fixed order: 32 columns to a workgroup, 32 threads down each.
+template <int E>
+__global__ __launch_bounds__(1024) void sum_parts_kernel(const float *partial, int parts, long columns, stored<E> *out) {
+    __shared__ float s[32][33];
+    const int x = threadIdx.x & 31, yy = threadIdx.x >> 5;
+    const long c = (long)blockIdx.x * 32 + x;
+    float v = 0.f;
+    if (c < columns) {
+#pragma unroll 8
+        for (int p = yy; p < parts; p += 32) v += partial[(long)p * columns + c];
+    }
+    s[yy][x] = v;
+    __syncthreads();
+    v = s[x][yy];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    const long out_c = (long)blockIdx.x * 32 + yy;
+    if (x == 0 && out_c < columns) store_one<E>(out + out_c, v);
+}
+
+}  // namespace tops
+#endif

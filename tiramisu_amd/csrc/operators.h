@@ -1,0 +1,36 @@
+// What operators.hip (the entry points), linear_tiles.hip (the matrix products' kernels, compiled once for each operand type) and
+// hip_wrappers.hip (the runtime's state) share.
+#ifndef TIRAMISU_AMD_OPERATORS_H
+#define TIRAMISU_AMD_OPERATORS_H
+#include <hip/hip_runtime.h>
+
+namespace tops {
+
+struct product_arguments;
+
+// How a product's operands lie: k along the rows of both (forward), of A alone (gradient of the input), of neither (gradient of the weights).
+enum product_layout { FORWARD, INPUT_GRADIENT, WEIGHT_GRADIENT };
+
+// Launches on `stream`; splits > 1: partial sums to arguments.partial, without the epilogue.  y: element type of the outputs.
+void launch_tiles_F16(int edge, product_layout, int epilogue, int y, const product_arguments &, int splits, hipStream_t stream);
+void launch_tiles_BF16(int edge, product_layout, int epilogue, int y, const product_arguments &, int splits, hipStream_t stream);
+void launch_tiles_F8(int edge, product_layout, int epilogue, int y, const product_arguments &, int splits, hipStream_t stream);
+
+}  // namespace tops
+
+namespace tiramisu_runtime {
+
+// The calling thread's stream, the failure model of the runtime, and a record of what lies between construction and destruction for
+// tiramisu_hip_profile_start / _stop.
+hipStream_t stream();
+void check(hipError_t e, const char *function);
+class timed {
+public:
+    explicit timed(const char *name);
+    ~timed();
+private:
+    hipEvent_t stop;
+};
+
+}  // namespace tiramisu_runtime
+#endif

@@ -1,0 +1,439 @@
+// Entry points of the transformer operators (include/tiramisu_hip_wrappers.h): what they refuse, which kernel a call goes to, and the launches.
+// Every launch goes to the calling thread's stream; scratch is the runtime's (tiramisu_hip_kept_scratch), kept per thread and stream.
+#include "operators.h"
+
+#include <algorithm>
+#include <atomic>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/tiramisu_hip_wrappers.h"
+#include "kernels/linear_few_tokens.hip.h"
+#include "kernels/linear_tiles.hip.h"
+#include "kernels/operator_backward.hip.h"
+#include "kernels/rms_norm.hip.h"
+#include "kernels/target_gfx950.h"
+
+namespace tops {
+namespace {
+
+using tiramisu_runtime::check;
+using tiramisu_runtime::stream;
+using tiramisu_runtime::timed;
+
+__attribute__((format(printf, 2, 3))) int refuse(const char *fn, const char *format, ...) {
+    fprintf(stderr, "Error at %s: ", fn);
+    va_list args;
+    va_start(args, format);
+    vfprintf(stderr, format, args);
+    va_end(args);
+    fprintf(stderr, "\n");
+    return 1;
+}
+
+constexpr uint64_t MOST = 0x7fffffff;                    // rows and columns are counted in 31 bits
+constexpr int64_t MOST_ROW_BYTES = 1 << 22;              // of an operand with k along its rows: a tile's offsets stay below 2^31
+constexpr int64_t MOST_STEP = 1 << 23;                   // elements from k to k of one with k down its columns: the same
+
+bool known_type(int type, bool with_f32) { return type == F16 || type == BF16 || (with_f32 && type == F32); }
+int bytes_of(int type) { return type == F32 ? 4 : type == F8 ? 1 : 2; }
+
+// ---- scratch.  A block for each use and power of two of bytes: a block, once given, stays where it is until
+// tiramisu_hip_release_cached_memory(), so that launches recorded into a graph keep theirs.
+enum scratch_use { GRADIENT, PARTIAL, MOVED_A, MOVED_B, MOVED_C, MOVED_D, COLUMN_SUMS, SCRATCH_USES };
+void *scratch(scratch_use use, uint64_t bytes) {
+    static char sites[SCRATCH_USES][64];
+    int log2 = 16;
+    while ((1ull << log2) < bytes) log2++;
+    return tiramisu_hip_kept_scratch(&sites[use][log2], 1ull << log2, nullptr);
+}
+
+// ---- operands as the tiles can load them: rows that begin at multiples of 4 bytes, and strides within the limits above.  Others are
+// moved to scratch, rows at multiples of 16 bytes.
+struct operand { const void *p; long ld; };
+bool loadable(const operand &o, int bytes, bool k_along_rows) {
+    return (uintptr_t)o.p % 4 == 0 && (o.ld * bytes) % 4 == 0 && (k_along_rows ? o.ld * bytes <= MOST_ROW_BYTES : o.ld <= MOST_STEP);
+}
+operand moved_where_needed(const operand &o, long rows, long columns, int bytes, bool k_along_rows, scratch_use use) {
+    if (rows <= 0 || columns <= 0 || loadable(o, bytes, k_along_rows)) return o;
+    const long to = (columns * bytes + 15) / 16 * 16;
+    char *out = (char *)scratch(use, (uint64_t)(to * rows));
+    const unsigned blocks = (unsigned)((to / 16 * rows + 255) / 256);
+    if (bytes == 1) hipLaunchKernelGGL(move_rows_kernel<1>, dim3(blocks), dim3(256), 0, stream(), (const char *)o.p, out, rows, columns * bytes, o.ld * bytes, to);
+    else hipLaunchKernelGGL(move_rows_kernel<2>, dim3(blocks), dim3(256), 0, stream(), (const char *)o.p, out, rows, columns * bytes, o.ld * bytes, to);
+    check(hipGetLastError(), "tiramisu_hip_linear");
+    return {out, to / bytes};
+}
+
+// ---- which tile, and how many workgroups share the k of one.  A launch is modelled as `fixed` microseconds, and per slice of 128 bytes of k `first` for
+// the first round of tiles over the compute units and `further` for each round after it; splitting adds a launch and the partial sums' bytes.
+struct tile_model { int edge; double fixed, first, further; };
+constexpr tile_model TILE_MODELS[] = {{256, 9.0, 1.1, 1.7}, {128, 3.9, 0.50, 0.48}, {64, 3.35, 0.264, 0.234}};
+struct tile_plan { int edge, splits, slices; };
+tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
+    const long slices = std::max(1L, (K * bytes + 127) / 128);
+    tile_plan best = {0, 1, 0};
+    double best_cost = 0;
+    for (const tile_model &t : TILE_MODELS) {
+        const long rows = t.edge, columns = gated ? std::max(t.edge / 2, 64) : t.edge, weight = gated && t.edge == 64 ? 2 : 1;
+        const long tiles = ((M + rows - 1) / rows) * ((N + columns - 1) / columns);
+        for (long splits = 1; splits <= 16 && splits <= slices; splits++) {
+            const long each = (slices + splits - 1) / splits, used = (slices + each - 1) / each;
+            if (used != splits) continue;
+            const double rounds = (double)((tiles * splits + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
+            double cost = t.fixed + (double)each * weight * (t.first + (rounds - 1) * t.further);
+            if (splits > 1) cost += 4.0 + (double)(gated ? 2 : 1) * M * N * 4 * 2 * splits / 4e6;
+            if (!best.edge || cost < best_cost) { best = {t.edge, (int)splits, (int)each}; best_cost = cost; }
+        }
+    }
+    return best;
+}
+
+int launch_product(const char *fn, int type, product_layout layout, int epilogue, int y, product_arguments p) {
+    if (p.M == 0 || p.N == 0) return 0;
+    const bool gated = epilogue == GATED;
+    const long work = p.a_more ? 2L * p.K : p.K;
+    tile_plan plan = plan_for(p.M, p.N, work, bytes_of(type), gated);
+    if (p.a_more && plan.splits > 1) plan.slices = (plan.slices + 1) / 2, plan.splits = (int)std::max(1L, ((long)p.K + 64L * plan.slices - 1) / (64L * plan.slices));
+    p.partial = nullptr;
+    p.slices_per_split = plan.slices;
+    if (plan.splits > 1) p.partial = (float *)scratch(PARTIAL, (uint64_t)plan.splits * (gated ? 2 : 1) * p.M * p.N * 4);
+    if (type == BF16) launch_tiles_BF16(plan.edge, layout, epilogue, y, p, plan.splits, stream());
+    else if (type == F16) launch_tiles_F16(plan.edge, layout, epilogue, y, p, plan.splits, stream());
+    else launch_tiles_F8(plan.edge, layout, epilogue, y, p, plan.splits, stream());
+    if (plan.splits > 1) {
+        const unsigned blocks = (unsigned)(((p.N + 7L) / 8 * p.M + 255) / 256);
+        auto kernel = gated ? (y == BF16 ? finish_kernel<BF16, GATED> : finish_kernel<F16, GATED>) : (y == BF16 ? finish_kernel<BF16, LINEAR> : finish_kernel<F16, LINEAR>);
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream(), p, plan.splits);
+        check(hipGetLastError(), fn);
+    }
+    return 0;
+}
+
+// Rows of x for which the weights are streamed through registers (linear_few_tokens.hip.h).
+constexpr long FEW_TOKENS = 64;
+
+template <int E, int Y, int EPILOGUE, int TILES>
+void launch_few(const char *fn, const product_arguments &p) {
+    auto kernel = few_tokens_kernel<E, Y, EPILOGUE, TILES>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.N + FEW_ROWS - 1L) / FEW_ROWS)), dim3(64 * FEW_WAVES), few_lds_bytes(TILES, EPILOGUE == GATED), stream(), p);
+    check(hipGetLastError(), fn);
+}
+template <int E, int Y, int EPILOGUE>
+void launch_few(const char *fn, const product_arguments &p) {
+    if (p.M <= 16) launch_few<E, Y, EPILOGUE, 1>(fn, p);
+    else if (p.M <= 32) launch_few<E, Y, EPILOGUE, 2>(fn, p);
+    else launch_few<E, Y, EPILOGUE, 4>(fn, p);
+}
+template <int EPILOGUE>
+void launch_few(const char *fn, int type, int y, const product_arguments &p) {
+    if (type == BF16) launch_few<BF16, BF16, EPILOGUE>(fn, p);
+    else if (type == F16) launch_few<F16, F16, EPILOGUE>(fn, p);
+    else if (y == BF16) launch_few<F8, BF16, EPILOGUE>(fn, p);
+    else launch_few<F8, F16, EPILOGUE>(fn, p);
+}
+
+// A forward product: few tokens, or tiles
+int forward(const char *fn, int type, int y, int epilogue, product_arguments p) {
+    if (p.M == 0 || p.N == 0) return 0;
+    if (p.M <= FEW_TOKENS && p.K > 0) {
+        epilogue == GATED ? launch_few<GATED>(fn, type, y, p) : launch_few<LINEAR>(fn, type, y, p);
+        return 0;
+    }
+    const int bytes = bytes_of(type);
+    auto take = [&](const void *&q, long &ld, long rows, scratch_use use) {
+        const operand o = moved_where_needed({q, ld}, rows, p.K, bytes, true, use);
+        q = o.p;
+        ld = o.ld;
+    };
+    take(p.a, p.lda, p.M, MOVED_A);
+    take(p.b, p.ldb, p.N, MOVED_B);
+    if (epilogue == GATED) take(p.b2, p.ldb2, p.N, MOVED_C);
+    return launch_product(fn, type, FORWARD, epilogue, y, p);
+}
+
+// ---- rows
+template <int E, int Y>
+void launch_norm(const char *fn, const norm_arguments &a) {
+    constexpr int N = E == F32 ? 4 : 8;
+    const long pieces = (a.columns + N - 1) / N;
+    auto go = [&](auto kernel, int threads, int rows) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(threads), 0, stream(), a);
+    };
+    if (pieces <= 64) go(rms_norm_kernel<E, Y, 64, 1, true>, 256, 4);
+    else if (pieces <= 256) go(rms_norm_kernel<E, Y, 256, 1, true>, 256, 1);
+    else if (pieces <= 512) go(rms_norm_kernel<E, Y, 256, 2, true>, 256, 1);
+    else if (pieces <= 1024) go(rms_norm_kernel<E, Y, 256, 4, true>, 256, 1);
+    else if (pieces <= 4096) go(rms_norm_kernel<E, Y, 1024, 4, true>, 1024, 1);
+    else go(rms_norm_kernel<E, Y, 1024, 1, false>, 1024, 1);
+    check(hipGetLastError(), fn);
+}
+int norm(const char *fn, int type, int y, const norm_arguments &a) {
+    if (a.rows == 0 || a.columns == 0) return 0;
+    if (type == F32) y == F8 ? launch_norm<F32, F8>(fn, a) : launch_norm<F32, F32>(fn, a);
+    else if (type == F16) y == F8 ? launch_norm<F16, F8>(fn, a) : launch_norm<F16, F16>(fn, a);
+    else y == F8 ? launch_norm<BF16, F8>(fn, a) : launch_norm<BF16, BF16>(fn, a);
+    return 0;
+}
+
+template <int E>
+void sum_parts(const char *fn, const float *partial, int parts, long columns, void *out) {
+    hipLaunchKernelGGL(sum_parts_kernel<E>, dim3((unsigned)((columns + 31) / 32)), dim3(1024), 0, stream(), partial, parts, columns, (stored<E> *)out);
+    check(hipGetLastError(), fn);
+}
+
+template <int E>
+void launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweight) {
+    constexpr int N = E == F32 ? 4 : 8;
+    const long pieces = (a.columns + N - 1) / N;
+    // teams: enough for every compute unit, few enough that their sums are little beside the rows
+    auto go = [&](auto kernel, int threads, int teams_each) {
+        a.teams = (int)std::max(1L, std::min(a.rows, 512L * teams_each));
+        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.teams * a.columns * 4);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.teams + teams_each - 1) / teams_each)), dim3(threads), 0, stream(), a);
+    };
+    if (pieces <= 64) go(rms_norm_backward_kernel<E, 64, 1>, 256, 4);
+    else if (pieces <= 256) go(rms_norm_backward_kernel<E, 256, 1>, 256, 1);
+    else if (pieces <= 512) go(rms_norm_backward_kernel<E, 256, 2>, 256, 1);
+    else if (pieces <= 1024) go(rms_norm_backward_kernel<E, 256, 4>, 256, 1);
+    else if (pieces <= 4096) go(rms_norm_backward_kernel<E, 1024, 4>, 1024, 1);
+    else {
+        a.teams = (int)std::max(1L, std::min(a.rows, 64L));
+        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.teams * a.columns * 4);
+        if (a.rows > 0) hipLaunchKernelGGL(rms_norm_backward_long_rows_kernel<E>, dim3((unsigned)a.rows), dim3(1024), 0, stream(), a);
+        hipLaunchKernelGGL(rms_norm_backward_long_columns_kernel<E>, dim3((unsigned)((a.columns + 255) / 256), (unsigned)a.teams), dim3(256), 0, stream(), a);
+    }
+    check(hipGetLastError(), fn);
+    sum_parts<E>(fn, a.partial, a.teams, a.columns, dweight);
+}
+
+// dz and the bias's gradient; what is null is not computed
+template <int E>
+void launch_activation_backward(const char *fn, activation_backward_arguments a, void *dbias) {
+    a.across = 1;
+    while (a.across < 64 && a.across * 8 < a.N) a.across *= 2;
+    const long columns = (a.N + 8L * a.across - 1) / (8L * a.across), down = 256 / a.across;
+    const long chunks = std::max(1L, std::min((a.M + 4 * down - 1) / (4 * down), std::max(1L, 1024 / columns)));
+    a.rows = std::max(1L, (a.M + chunks - 1) / chunks);
+    const int used = (int)std::max(1L, (a.M + a.rows - 1) / a.rows);
+    a.partial = dbias ? (float *)scratch(COLUMN_SUMS, (uint64_t)used * a.N * 4) : nullptr;
+    hipLaunchKernelGGL(activation_backward_kernel<E>, dim3((unsigned)columns, (unsigned)used), dim3(256), 0, stream(), a);
+    check(hipGetLastError(), fn);
+    if (dbias) sum_parts<E>(fn, a.partial, used, a.N, dbias);
+}
+
+product_arguments product_of(long M, long N, long K) {
+    product_arguments p = {};
+    p.M = (int)M;
+    p.N = (int)N;
+    p.K = (int)K;
+    p.rows_above = p.split_row = p.M;
+    return p;
+}
+
+// What both products refuse alike
+int refuse_product(const char *fn, uint64_t M, uint64_t N, uint64_t K, int activation, int type, int y) {
+    if (M > MOST || N > MOST || K > MOST) return refuse(fn, "dimension exceeds 2^31-1");
+    if ((int64_t)K * bytes_of(type) > MOST_ROW_BYTES) return refuse(fn, "K of %llu: rows of at most %lld bytes", (unsigned long long)K, (long long)MOST_ROW_BYTES);
+    if (activation < NONE || activation > SILU) return refuse(fn, "activation %d is not known", activation);
+    if (!known_type(type, false) && type != F8) return refuse(fn, "element type %d: float16, bfloat16 or float8_e4m3", type);
+    if (type == F8 ? !known_type(y, false) : y != type) return refuse(fn, "results of type %d from operands of type %d", y, type);
+    if (((M + 63) / 64) * ((N + 63) / 64) > MOST) return refuse(fn, "result of %llu x %llu: more tiles than a launch holds", (unsigned long long)M, (unsigned long long)N);
+    return 0;
+}
+
+}  // namespace
+}  // namespace tops
+
+using namespace tops;
+
+extern "C" {
+
+int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum, float *scale, float *rstd, uint64_t rows,
+                          uint64_t columns, uint64_t ldx, uint64_t ldr, float eps, int32_t type, int32_t y_type) {
+    if (rows > MOST || columns > MOST) return refuse(__FUNCTION__, "dimension exceeds 2^31-1");
+    if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
+    if (y_type != type && y_type != F8) return refuse(__FUNCTION__, "results of type %d from rows of type %d", y_type, type);
+    if (rows == 0 || columns == 0) return 0;
+    if (!x || !weight || !y) return refuse(__FUNCTION__, "x, weight and y are needed");
+    if ((residual != nullptr) != (sum != nullptr)) return refuse(__FUNCTION__, "a residual and a place for the sum belong together");
+    if ((y_type == F8) != (scale != nullptr)) return refuse(__FUNCTION__, "8-bit results and a place for their scales belong together");
+    timed record(__FUNCTION__);
+    const norm_arguments a = {x, residual, weight, y, sum, scale, rstd, (long)rows, (long)columns, ldx ? (long)ldx : (long)columns, ldr ? (long)ldr : (long)columns, eps};
+    return norm(__FUNCTION__, type, y_type, a);
+}
+
+int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type) {
+    if (rows > MOST || columns > MOST) return refuse(__FUNCTION__, "dimension exceeds 2^31-1");
+    if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
+    if (rows == 0 || columns == 0) return 0;
+    if (!x || !q || !scale) return refuse(__FUNCTION__, "x, q and scale are needed");
+    timed record(__FUNCTION__);
+    const norm_arguments a = {x, nullptr, nullptr, q, nullptr, scale, nullptr, (long)rows, (long)columns, ldx ? (long)ldx : (long)columns, 0, 0.f};
+    return norm(__FUNCTION__, type, F8, a);
+}
+
+int tiramisu_hip_rms_norm_backward(const void *dy, const void *sum, const void *weight, const float *rstd, const void *dsum, void *dx, void *dweight,
+                                   uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t lds, uint64_t ldd, int32_t type) {
+    if (rows > MOST || columns > MOST) return refuse(__FUNCTION__, "dimension exceeds 2^31-1");
+    if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
+    if (columns == 0) return 0;
+    if (!dweight || !weight || (rows && (!dy || !sum || !rstd || !dx))) return refuse(__FUNCTION__, "dy, sum, weight, rstd, dx and dweight are needed");
+    timed record(__FUNCTION__);
+    const norm_backward_arguments a = {dy, sum, weight, dsum, rstd, dx, nullptr, (long)rows, (long)columns, ldy ? (long)ldy : (long)columns,
+                                       lds ? (long)lds : (long)columns, ldd ? (long)ldd : (long)columns, 0};
+    if (type == F32) launch_norm_backward<F32>(__FUNCTION__, a, dweight);
+    else if (type == F16) launch_norm_backward<F16>(__FUNCTION__, a, dweight);
+    else launch_norm_backward<BF16>(__FUNCTION__, a, dweight);
+    return 0;
+}
+
+int tiramisu_hip_linear(const void *x, const void *weight, const void *bias, const void *residual, const float *x_scale, const float *weight_scale, void *y,
+                        void *pre, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldw, uint64_t ldr, int32_t activation, int32_t type,
+                        int32_t y_type) {
+    if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, y_type)) return rc;
+    if (M == 0 || N == 0) return 0;
+    if (!y || (K && (!x || !weight))) return refuse(__FUNCTION__, "x, weight and y are needed");
+    if ((type == F8) != (x_scale != nullptr) || (type == F8) != (weight_scale != nullptr)) return refuse(__FUNCTION__, "8-bit operands and their scales belong together");
+    timed record(__FUNCTION__);
+    product_arguments p = product_of((long)M, (long)N, (long)K);
+    p.a = x;
+    p.lda = ldx ? (long)ldx : (long)K;
+    p.b = weight;
+    p.ldb = ldw ? (long)ldw : (long)K;
+    p.bias = bias;
+    p.residual = residual;
+    p.ldr = ldr ? (long)ldr : (long)N;
+    p.a_scale = x_scale;
+    p.b_scale = weight_scale;
+    p.y = y;
+    p.pre = pre;
+    p.activation = activation;
+    return forward(__FUNCTION__, type, y_type, LINEAR, p);
+}
+
+int tiramisu_hip_gated_linear(const void *x, const void *gate_weight, const void *up_weight, const float *x_scale, const float *gate_scale,
+                              const float *up_scale, void *h, void *gate, void *up, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldg,
+                              uint64_t ldu, int32_t activation, int32_t type, int32_t h_type) {
+    if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, h_type)) return rc;
+    if (M == 0 || N == 0) return 0;
+    if (!h || (K && (!x || !gate_weight || !up_weight))) return refuse(__FUNCTION__, "x, both weights and h are needed");
+    if ((gate != nullptr) != (up != nullptr)) return refuse(__FUNCTION__, "gate and up are kept together");
+    if ((type == F8) != (x_scale != nullptr) || (type == F8) != (gate_scale != nullptr) || (type == F8) != (up_scale != nullptr))
+        return refuse(__FUNCTION__, "8-bit operands and their scales belong together");
+    timed record(__FUNCTION__);
+    product_arguments p = product_of((long)M, (long)N, (long)K);
+    p.a = x;
+    p.lda = ldx ? (long)ldx : (long)K;
+    p.b = gate_weight;
+    p.ldb = ldg ? (long)ldg : (long)K;
+    p.b2 = up_weight;
+    p.ldb2 = ldu ? (long)ldu : (long)K;
+    p.a_scale = x_scale;
+    p.b_scale = gate_scale;
+    p.b2_scale = up_scale;
+    p.y = h;
+    p.pre = gate;
+    p.pre2 = up;
+    p.activation = activation;
+    return forward(__FUNCTION__, type, h_type, GATED, p);
+}
+
+int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weight, const void *pre, void *dx, void *dweight, void *dbias, uint64_t M,
+                                 uint64_t N, uint64_t K, uint64_t ldy, uint64_t ldx, uint64_t ldw, uint64_t ldp, int32_t activation, int32_t type) {
+    if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, type)) return rc;
+    if ((int64_t)N * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (unsigned long long)N, (long long)MOST_ROW_BYTES);
+    if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
+    if ((activation != NONE) != (pre != nullptr)) return refuse(__FUNCTION__, "an activation and the sums ahead of it belong together");
+    if ((M && N && !dy) || (M && K && dweight && !x) || (N && K && dx && !weight)) return refuse(__FUNCTION__, "dy, x and weight are needed");
+    timed record(__FUNCTION__);
+    const long m = (long)M, n = (long)N, k = (long)K;
+    operand dz = {dy, ldy ? (long)ldy : n};
+    // the gradient ahead of the activation; without one it is dy, moved only where the tiles cannot load it
+    if (n > 0 && (activation != NONE || dbias)) {
+        activation_backward_arguments a = {dy, pre, nullptr, nullptr, m, n, dz.ld, ldp ? (long)ldp : n, 0, 0, activation, 0};
+        if (activation != NONE) {
+            a.ldz = (n + 7) / 8 * 8;
+            a.dz = scratch(GRADIENT, (uint64_t)std::max(1L, m) * a.ldz * 2);
+            dz = {a.dz, a.ldz};
+        }
+        if (type == F16) launch_activation_backward<F16>(__FUNCTION__, a, dbias);
+        else launch_activation_backward<BF16>(__FUNCTION__, a, dbias);
+    }
+    if (!loadable(dz, 2, true) || !loadable(dz, 2, false)) dz = moved_where_needed({dz.p, dz.ld}, m, n, 2, true, GRADIENT);
+    if (dx) {
+        product_arguments p = product_of(m, k, n);
+        p.a = dz.p;
+        p.lda = dz.ld;
+        const operand w = moved_where_needed({weight, ldw ? (long)ldw : k}, n, k, 2, false, MOVED_B);
+        p.b = w.p;
+        p.ldb = w.ld;
+        p.y = dx;
+        if (const int rc = launch_product(__FUNCTION__, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
+    }
+    if (dweight) {
+        product_arguments p = product_of(n, k, m);
+        p.a = dz.p;
+        p.lda = dz.ld;
+        const operand xs = moved_where_needed({x, ldx ? (long)ldx : k}, m, k, 2, false, MOVED_A);
+        p.b = xs.p;
+        p.ldb = xs.ld;
+        p.y = dweight;
+        if (const int rc = launch_product(__FUNCTION__, type, WEIGHT_GRADIENT, LINEAR, type, p)) return rc;
+    }
+    return 0;
+}
+
+int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate, const void *up,
+                                       void *dx, void *dgate_weight, void *dup_weight, uint64_t M, uint64_t N, uint64_t K, uint64_t ldh, uint64_t ldx,
+                                       uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type) {
+    if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, type)) return rc;
+    if ((int64_t)(2 * N + 16) * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (unsigned long long)N, (long long)MOST_ROW_BYTES);
+    if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
+    if ((M && N && (!dh || !gate || !up)) || (M && K && N && !x) || (N && K && (!gate_weight || !up_weight))) return refuse(__FUNCTION__, "dh, x, both weights, gate and up are needed");
+    if ((dgate_weight != nullptr) != (dup_weight != nullptr)) return refuse(__FUNCTION__, "gradients of both weights, or of neither");
+    timed record(__FUNCTION__);
+    const long m = (long)M, n = (long)N, k = (long)K;
+    // [dgate | dup] in rows of 2 x `half` elements
+    const long half = (n + 7) / 8 * 8, ld = 2 * half;
+    char *d = (char *)scratch(GRADIENT, (uint64_t)std::max(1L, m) * std::max(1L, ld) * 2);
+    if (m > 0 && n > 0) {
+        const gated_backward_arguments a = {dh, gate, up, d, d + 2 * half, m, n, ldh ? (long)ldh : n, ld_gate ? (long)ld_gate : n, ld_up ? (long)ld_up : n, ld, activation};
+        const unsigned blocks = (unsigned)((half / 8 * m + 255) / 256);
+        if (type == F16) hipLaunchKernelGGL(gated_backward_kernel<F16>, dim3(blocks), dim3(256), 0, stream(), a);
+        else hipLaunchKernelGGL(gated_backward_kernel<BF16>, dim3(blocks), dim3(256), 0, stream(), a);
+        check(hipGetLastError(), __FUNCTION__);
+    }
+    if (dx) {
+        operand g = moved_where_needed({gate_weight, ldg ? (long)ldg : k}, n, k, 2, false, MOVED_B);
+        operand u = moved_where_needed({up_weight, ldu ? (long)ldu : k}, n, k, 2, false, MOVED_C);
+        product_arguments p = product_of(m, k, n);
+        p.a = d;
+        p.a_more = d + 2 * half;
+        p.lda = ld;
+        p.b = g.p;
+        p.ldb = g.ld;
+        p.b_more = u.p;
+        p.ldb_more = u.ld;
+        p.y = dx;
+        if (const int rc = launch_product(__FUNCTION__, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
+    }
+    if (dgate_weight && n > 0) {
+        // rows of the product: those of gate, up to `half` nothing, those of up
+        product_arguments p = product_of(half + n, k, m);
+        p.a = d;
+        p.lda = ld;
+        const operand xs = moved_where_needed({x, ldx ? (long)ldx : k}, m, k, 2, false, MOVED_A);
+        p.b = xs.p;
+        p.ldb = xs.ld;
+        p.y = dgate_weight;
+        p.y_below = dup_weight;
+        p.rows_above = (int)n;
+        p.split_row = (int)half;
+        if (const int rc = launch_product(__FUNCTION__, type, WEIGHT_GRADIENT, LINEAR, type, p)) return rc;
+    }
+    return 0;
+}
+
+}  // extern "C"

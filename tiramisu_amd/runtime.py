@@ -146,6 +146,14 @@ def wrappers():
         lib.tiramisu_hip_sgemm_static_scratch.argtypes = lib.tiramisu_hip_sgemm.argtypes
         lib.tiramisu_hip_dgemm.argtypes = [ctypes.c_void_p] * 3 + [u64] * 3 + [ctypes.c_double] * 2 + \
             [u64] * 6 + [ctypes.c_bool] * 2
+        p, u, i = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int32
+        lib.tiramisu_hip_rms_norm.argtypes = [p] * 7 + [u] * 4 + [ctypes.c_float, i, i]
+        lib.tiramisu_hip_rms_norm_backward.argtypes = [p] * 7 + [u] * 5 + [i]
+        lib.tiramisu_hip_quantize_rows.argtypes = [p] * 3 + [u] * 3 + [i]
+        lib.tiramisu_hip_linear.argtypes = [p] * 8 + [u] * 6 + [i] * 3
+        lib.tiramisu_hip_linear_backward.argtypes = [p] * 7 + [u] * 7 + [i] * 2
+        lib.tiramisu_hip_gated_linear.argtypes = [p] * 9 + [u] * 6 + [i] * 3
+        lib.tiramisu_hip_gated_linear_backward.argtypes = [p] * 9 + [u] * 9 + [i] * 2
         _wrappers = lib
     return _wrappers
 
