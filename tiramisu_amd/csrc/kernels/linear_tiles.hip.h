@@ -160,9 +160,11 @@ __device__ __forceinline__ f32x16 multiply(const fragment<E, AR> &rows, const fr
     }
 }
 
-// Adds the product of one pair of operands' rows from m0 and n0, K elements of k, to the accumulators.  b0, b1: B's operand (GATED: gate and up).
+// Adds the product of one pair of operands' rows from m0 and n0, K elements of k, to the accumulators.  b, b2: B's operand (GATED: gate and up).
+// (The operands are __restrict__ so that the compiler does not take a transposing read of LDS for one that may see a load still on its way there: it
+// waited for every load ahead of each of them, 205 us where 105 are enough.)
 template <class C>
-__device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const void *a, long lda, const void *b, long ldb, const void *b2, long ldb2, long M, long N,
+__device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const void *__restrict__ a, long lda, const void *__restrict__ b, long ldb, const void *__restrict__ b2, long ldb2, long M, long N,
                                            long m0, long n0, long k0, long K, lds_char *lds) {
     constexpr int TM = C::TM, TN = C::TN, ST = C::STAGES, E = C::E;
     constexpr int Q = E == F8 ? 2 : 4;                                     // matrix steps of a slice
@@ -308,7 +310,7 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const vo
 
 // ---- epilogues: 8 columns from n on of row m; `some`: how many of them exist
 template <int Y>
-__device__ __forceinline__ void finish_linear(const product_arguments &p, float (&z)[8], long m, long n, int some) {
+__device__ __forceinline__ void activate_linear(const product_arguments &p, float (&z)[8], long m, long n, int some) {
     typedef stored<Y> T;
     if (p.a_scale) {
         const float s = p.a_scale[m];
@@ -325,14 +327,27 @@ __device__ __forceinline__ void finish_linear(const product_arguments &p, float 
     }
     if (p.pre) store_some<Y>((T *)p.pre + m * p.N + n, some, z);
     activate(p.activation, z);
+}
+template <int Y>
+__device__ __forceinline__ void load_residual(const product_arguments &p, float (&r)[8], long m, long n, int some) {
+    load_some<Y>((const stored<Y> *)p.residual + m * p.ldr + n, some, r);
+}
+template <int Y>
+__device__ __forceinline__ void store_linear(const product_arguments &p, const float (&z)[8], long m, long n, int some) {
+    typedef stored<Y> T;
+    if (m < p.rows_above) store_some<Y>((T *)p.y + m * p.N + n, some, z);
+    else if (m >= p.split_row) store_some<Y>((T *)p.y_below + (m - p.split_row) * p.N + n, some, z);
+}
+template <int Y>
+__device__ __forceinline__ void finish_linear(const product_arguments &p, float (&z)[8], long m, long n, int some) {
+    activate_linear<Y>(p, z, m, n, some);
     if (p.residual) {
         float r[8];
-        load_some<Y>((const T *)p.residual + m * p.ldr + n, some, r);
+        load_residual<Y>(p, r, m, n, some);
 #pragma unroll
         for (int i = 0; i < 8; i++) z[i] += r[i];
     }
-    if (m < p.rows_above) store_some<Y>((T *)p.y + m * p.N + n, some, z);
-    else if (m >= p.split_row) store_some<Y>((T *)p.y_below + (m - p.split_row) * p.N + n, some, z);
+    store_linear<Y>(p, z, m, n, some);
 }
 template <int Y>
 __device__ __forceinline__ void finish_gated(const product_arguments &p, float (&g)[8], float (&u)[8], long m, long n, int some) {
@@ -400,41 +415,87 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
     const int r0 = lane / ACROSS, c0 = 8 * (lane % ACROSS);
     const long n = n0 + wn * SPAN + c0;
     const int some = (int)min(8L, p.N - n);
+    constexpr int PASSES = 32 / DOWN;
+    auto order_lanes = [] {                                               // what the lanes of a wavefront pass to each other
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
 #pragma unroll
     for (int i = 0; i < C::TM; i++) {
+        const long first = m0 + wm * C::WM + i * 32 + r0;                 // the lane's row of pass 0
+        const bool across = some > 0;
+        auto take = [&](int pass, int c, float (&v)[8]) {
+            const f32x4 a = *(lds_f32x4 *)(strip + (pass * DOWN + r0) * C::STRIP + c), b = *(lds_f32x4 *)(strip + (pass * DOWN + r0) * C::STRIP + c + 4);
+#pragma unroll
+            for (int e = 0; e < 4; e++) { v[e] = a[e]; v[4 + e] = b[e]; }
+        };
+        // the residual's pieces are on their way while the strip is turned
+        constexpr bool RESIDUAL = C::EPILOGUE == LINEAR && C::A_ROWS && C::B_ROWS;
+        float r[RESIDUAL ? PASSES : 1][8];
+        if constexpr (RESIDUAL)
+            if (p.residual && !p.partial) {
+#pragma unroll
+                for (int pass = 0; pass < PASSES; pass++)
+                    if (across && first + pass * DOWN < p.M) load_residual<Y>(p, r[pass], first + pass * DOWN, n, some);
+            }
 #pragma unroll
         for (int j = 0; j < C::TN; j++)
 #pragma unroll
             for (int g = 0; g < 4; g++)
                 *(lds_f32x4 *)(strip + l32 * C::STRIP + j * 32 + 8 * g + 4 * h) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        order_lanes();
+        if (p.partial) {
+#pragma unroll 1
+            for (int pass = 0; pass < PASSES; pass++) {
+                const long m = first + pass * DOWN;
+                if (!across || m >= p.M) continue;
+                constexpr long PARTS = C::EPILOGUE == GATED ? 2 : 1;
+                float *out = p.partial + ((long)blockIdx.y * PARTS * p.M + m) * p.N + n;
 #pragma unroll
-        for (int pass = 0; pass < 32 / DOWN; pass++) {
-            const int r = pass * DOWN + r0;
-            const long m = m0 + wm * C::WM + i * 32 + r;
-            float z[8], u[8];
-            auto take = [&](int c, float (&v)[8]) {
-                const f32x4 a = *(lds_f32x4 *)(strip + r * C::STRIP + c), b = *(lds_f32x4 *)(strip + r * C::STRIP + c + 4);
+                for (int part = 0; part < PARTS; part++) {
+                    float z[8];
+                    take(pass, part * SPAN + c0, z);
+                    store_some<F32>(out + part * (long)p.M * p.N, some, z);
+                }
+            }
+        } else if constexpr (C::EPILOGUE == GATED) {
+#pragma unroll 1
+            for (int pass = 0; pass < PASSES; pass++) {
+                float z[8], u[8];
+                take(pass, c0, z);
+                take(pass, SPAN + c0, u);
+                if (across && first + pass * DOWN < p.M) finish_gated<Y>(p, z, u, first + pass * DOWN, n, some);
+            }
+        } else {
+            // what takes many instructions is a loop that is not unrolled, in place; then the results
+            if constexpr (RESIDUAL)
+                if (p.a_scale || p.bias || p.pre || p.activation != NONE) {
+#pragma unroll 1
+                    for (int pass = 0; pass < PASSES; pass++) {
+                        if (!across || first + pass * DOWN >= p.M) continue;
+                        float z[8];
+                        take(pass, c0, z);
+                        activate_linear<Y>(p, z, first + pass * DOWN, n, some);
+                        lds_f32x4 *const back = (lds_f32x4 *)(strip + (pass * DOWN + r0) * C::STRIP + c0);
+                        back[0] = f32x4{z[0], z[1], z[2], z[3]};
+                        back[1] = f32x4{z[4], z[5], z[6], z[7]};
+                    }
+                }
 #pragma unroll
-                for (int e = 0; e < 4; e++) { v[e] = a[e]; v[4 + e] = b[e]; }
-            };
-            take(c0, z);
-            if constexpr (C::EPILOGUE == GATED) take(SPAN + c0, u);
-            if (m < p.M && some > 0) {
-                if (p.partial) {
-                    const long parts = C::EPILOGUE == GATED ? 2 : 1;
-                    float *out = p.partial + ((long)blockIdx.y * parts * p.M + m) * p.N + n;
-                    store_some<F32>(out, some, z);
-                    if constexpr (C::EPILOGUE == GATED) store_some<F32>(out + (long)p.M * p.N, some, u);
-                } else if constexpr (C::EPILOGUE == GATED) finish_gated<Y>(p, z, u, m, n, some);
-                else finish_linear<Y>(p, z, m, n, some);
+            for (int pass = 0; pass < PASSES; pass++) {
+                if (!across || first + pass * DOWN >= p.M) continue;
+                float z[8];
+                take(pass, c0, z);
+                if constexpr (RESIDUAL)
+                    if (p.residual) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) z[e] += r[pass][e];
+                    }
+                store_linear<Y>(p, z, first + pass * DOWN, n, some);
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        order_lanes();
     }
 #endif
 }
