@@ -50,13 +50,15 @@ struct product_arguments {
     int slices_per_split;
 };
 
-template <int E_, int BM_, int BN_, int WGM_, int WGN_, int STAGES_, bool A_ROWS_, bool B_ROWS_, int EPILOGUE_>
+template <int E_, int BM_, int BN_, int WGM_, int WGN_, int STAGES_, bool A_ROWS_, bool B_ROWS_, int EPILOGUE_, int F_>
 struct tile_config {
+    static constexpr int F = F_;                                           // rows of a fragment: matrix instructions of F x F
     static constexpr int E = E_, BM = BM_, BN = BN_, WGM = WGM_, WGN = WGN_, STAGES = STAGES_, EPILOGUE = EPILOGUE_;
     static constexpr bool A_ROWS = A_ROWS_, B_ROWS = B_ROWS_;              // k along the rows
     static constexpr int BYTES = E == F8 ? 1 : 2, BK = 128 / BYTES;
     static constexpr int NW = WGM * WGN, NT = 64 * NW;
-    static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 32, TN = WN / 32;
+    static constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / F, TN = WN / F;
+    static constexpr int STEP = F == 16 ? (E == F8 ? 128 : 64) : (E == F8 ? 64 : 32);     // bytes of a row in a matrix step
     static constexpr int A_STAGE = BM * 128, B_STAGE = BN * 128, STAGE = A_STAGE + B_STAGE;
     static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;               // loads of a wavefront for a slice
     static constexpr int STRIP = WN + 4;                                   // floats of a row in the epilogue's strip: 16-byte stores of 16 rows fill the banks
@@ -74,12 +76,14 @@ template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_
 typedef __attribute__((address_space(3))) char lds_char;
 
 // An operand's slices: what a lane loads, and where.
-template <int BYTES, int ROWS, bool K_ALONG_ROWS, int LOADS>
+template <int BYTES, int ROWS, bool K_ALONG_ROWS, int LOADS, int F>
 struct operand_loader {
     static constexpr int G = K_ALONG_ROWS ? 8 : ROWS / 8;                  // granules of a row in LDS
+    // Lanes that an LDS read serves together, 8 or 16 of a 16-byte read and 16 or 32 of a transposing one, meet distinct banks.
     static __device__ __forceinline__ int swizzle(int row) {
         if (K_ALONG_ROWS) return (row ^ (row >> 3)) & 7;
-        return G == 8 ? 2 * (row & 3) : ((row & 1) << 2) | ((row & 2) ? 10 : 0);
+        const int eighth = F == 16 ? (row >> 3) & 1 : 0;                   // (F == 16: such 32 lanes read k and k + 8)
+        return G == 8 ? 2 * ((row & 3) ^ eighth) : (((row & 1) << 2) | ((row & 2) ? 10 : 0)) ^ (eighth << 1);
     }
     const char *base;
     long left, step;                        // bytes from base to the operand's end; from slice to slice (k down the columns)
@@ -125,37 +129,53 @@ typedef int s32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-// A lane's share of an operand's 32 rows for one matrix step: 8 k of 16 bits, or 32 of 8 bits.
+// A lane's share of F rows of an operand for one matrix step: 8 k of 16 bits, or 32 of 8 bits.
 template <int E, bool K_ALONG_ROWS> struct fragment {
     u32x4 w[E == F8 ? 2 : 1];
     s16x4 half[2];                          // (k down the columns: as the transposing reads give them)
 };
+template <int F> struct block_sums;         // a lane's share of the sums of F x F
+template <> struct block_sums<16> { typedef f32x4 type; };
+template <> struct block_sums<32> { typedef f32x16 type; };
 
-// One LDS read of the fragment of the 32 rows from `row` on of the slice at `s`, step `step`; L: the operand's loader.
-template <class L, int E>
+// The 16 bytes of k of a matrix step that piece `part` of a lane's fragment holds: their granule within a slice.
+template <int E, int F>
+__device__ __forceinline__ int granule_of(int step, int part, int lane) {
+    const int group = lane / F, groups = 64 / F;
+    return E == F8 ? 2 * (groups * step + group) + part : groups * step + group;
+}
+// One LDS read of the fragment of the F rows from `row` on of the slice at `s`, step `step`; L: the operand's loader.
+template <class L, int F, int E>
 __device__ __forceinline__ void read_piece(fragment<E, true> &f, lds_char *s, int row, int step, int part, int lane) {
-    const int m = row + (lane & 31), h = lane >> 5, q = E == F8 ? 4 * step + 2 * h + part : 2 * step + h;
+    const int m = row + lane % F, q = granule_of<E, F>(step, part, lane);
     f.w[part] = *reinterpret_cast<const __attribute__((address_space(3))) u32x4 *>(s + (m * 8 + (q ^ L::swizzle(m))) * 16);
 }
-template <class L, int E>
+template <class L, int F, int E>
 __device__ __forceinline__ void read_piece(fragment<E, false> &f, lds_char *s, int row, int step, int part, int lane) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     const int l16 = lane & 15, group = lane >> 4;
-    const int k = 16 * step + 8 * (group >> 1) + (l16 >> 2) + 4 * part, m = row + 16 * (group & 1) + 4 * (l16 & 3);
+    const int k = F == 16 ? 32 * step + 8 * group + (l16 >> 2) + 4 * part : 16 * step + 8 * (group >> 1) + (l16 >> 2) + 4 * part;
+    const int m = row + (F == 16 ? 0 : 16 * (group & 1)) + 4 * (l16 & 3);
     f.half[part] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s + (k * L::G + ((m >> 3) ^ L::swizzle(k))) * 16 + (m & 7) * 2));
 }
 
-template <int E, bool AR, bool BR>
-__device__ __forceinline__ f32x16 multiply(const fragment<E, AR> &rows, const fragment<E, BR> &columns, f32x16 c) {
+// (16 x 16 blocks take less power than 32 x 32 ones on operands of random bits: from registers 2030 and 1800 TFLOP/s of bf16, 4350 and 4000 of e4m3;
+// on zeros, where power does not limit, 2430 and 2450, 4970 and 4970)
+template <int E, bool AR, bool BR, class S>
+__device__ __forceinline__ S multiply(const fragment<E, AR> &rows, const fragment<E, BR> &columns, S c) {
+    constexpr bool SMALL = sizeof(S) == 16;
     if constexpr (E == F8) {
         const s32x8 a = __builtin_shufflevector(__builtin_bit_cast(s32x4, rows.w[0]), __builtin_bit_cast(s32x4, rows.w[1]), 0, 1, 2, 3, 4, 5, 6, 7);
         const s32x8 b = __builtin_shufflevector(__builtin_bit_cast(s32x4, columns.w[0]), __builtin_bit_cast(s32x4, columns.w[1]), 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+        if constexpr (SMALL) return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
     } else {
         s16x8 a, b;
         if constexpr (AR) a = __builtin_bit_cast(s16x8, rows.w[0]); else a = __builtin_shufflevector(rows.half[0], rows.half[1], 0, 1, 2, 3, 4, 5, 6, 7);
         if constexpr (BR) b = __builtin_bit_cast(s16x8, columns.w[0]); else b = __builtin_shufflevector(columns.half[0], columns.half[1], 0, 1, 2, 3, 4, 5, 6, 7);
-        if constexpr (E == BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        if constexpr (E == BF16 && SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else if constexpr (E == BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        else if constexpr (SMALL) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
         else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
 }
@@ -164,19 +184,19 @@ __device__ __forceinline__ f32x16 multiply(const fragment<E, AR> &rows, const fr
 // (The operands are __restrict__ so that the compiler does not take a transposing read of LDS for one that may see a load still on its way there: it
 // waited for every load ahead of each of them, 205 us where 105 are enough.)
 template <class C>
-__device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const void *__restrict__ a, long lda, const void *__restrict__ b, long ldb, const void *__restrict__ b2, long ldb2, long M, long N,
+__device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc)[C::TM][C::TN], const void *__restrict__ a, long lda, const void *__restrict__ b, long ldb, const void *__restrict__ b2, long ldb2, long M, long N,
                                            long m0, long n0, long k0, long K, lds_char *lds) {
     constexpr int TM = C::TM, TN = C::TN, ST = C::STAGES, E = C::E;
-    constexpr int Q = E == F8 ? 2 : 4;                                     // matrix steps of a slice
+    constexpr int F = C::F, Q = 128 / C::STEP;                             // matrix steps of a slice
     constexpr int HALVES = C::EPILOGUE == GATED ? 2 : 1;
     constexpr int LB1 = C::LB / HALVES;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int wm = wave / C::WGN, wn = wave % C::WGN, h = lane >> 5;
+    const int wm = wave / C::WGN, wn = wave % C::WGN;
     static_assert(C::LB % HALVES == 0, "gate and up are loaded by the same wavefronts");
 
-    operand_loader<C::BYTES, C::BM, C::A_ROWS, C::LA> la;
+    operand_loader<C::BYTES, C::BM, C::A_ROWS, C::LA, F> la;
     // (GATED: rows of gate in the first half of B's stage, rows of up in the second)
-    operand_loader<C::BYTES, C::BN / HALVES, C::B_ROWS, LB1> lb[HALVES];
+    operand_loader<C::BYTES, C::BN / HALVES, C::B_ROWS, LB1, F> lb[HALVES];
     la.start(a, lda, m0, M, k0, K, wave, lane);
     lb[0].start(b, ldb, n0, N, k0, K, wave, lane);
     if constexpr (HALVES == 2) lb[1].start(b2, ldb2, n0, N, k0, K, wave, lane);
@@ -199,27 +219,27 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const vo
     constexpr int READS = TM * RA + TN * RB, MFMAS = TM * TN;
     // rows of B's stage that fragment j of the wavefront holds (GATED: the first half of the fragments gate, the others up, of the same columns)
     auto row_of = [&](int j) {
-        if (HALVES == 1) return wn * C::WN + j * 32;
+        if (HALVES == 1) return wn * C::WN + j * F;
         constexpr int HALF = HALVES == 2 ? TN / 2 : 1;
-        return (j >= HALF ? C::BN / 2 : 0) + wn * (C::WN / 2) + (j % HALF) * 32;
+        return (j >= HALF ? C::BN / 2 : 0) + wn * (C::WN / 2) + (j % HALF) * F;
     };
     // read r of a step, in the order in which the matrix instructions need them: A's first rows, all of B, the other rows of A
     auto read_one = [&](int stage, int step, int buf, int r) {
         lds_char *const s = lds + stage * C::STAGE;
         if (r < RA || r >= RA + TN * RB) {
             const int i = r < RA ? 0 : 1 + (r - RA - TN * RB) / RA, part = r < RA ? r : (r - RA - TN * RB) % RA;
-            read_piece<decltype(la)>(fa[buf][i], s, wm * C::WM + i * 32, step, part, lane);
+            read_piece<decltype(la), F>(fa[buf][i], s, wm * C::WM + i * F, step, part, lane);
         } else {
             const int j = (r - RA) / RB, part = (r - RA) % RB;
             // (GATED: the two halves are one block of rows, and the swizzle repeats every 64 of them)
-            read_piece<typename std::remove_reference<decltype(lb[0])>::type>(fb[buf][j], s + C::A_STAGE, row_of(j), step, part, lane);
+            read_piece<typename std::remove_reference<decltype(lb[0])>::type, F>(fb[buf][j], s + C::A_STAGE, row_of(j), step, part, lane);
         }
     };
     // the last slice: k behind the last is zero in both operands
     auto clear_behind = [&](auto &f, int left, int step) {                // left: bytes of k from the slice's first on
 #pragma unroll
         for (int part = 0; part < (E == F8 ? 2 : 1); part++) {
-            const int rest = left - 16 * (E == F8 ? 4 * step + 2 * h + part : 2 * step + h);
+            const int rest = left - 16 * granule_of<E, F>(step, part, lane);
 #pragma unroll
             for (int w = 0; w < 4; w++) f.w[part][w] &= rest >= 4 * w + 4 ? 0xffffffffu : rest <= 4 * w ? 0u : (1u << (8 * (rest - 4 * w))) - 1u;
         }
@@ -233,7 +253,7 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const vo
     if (KT <= 0) return;
     const int tail = (int)(K - (long)(KT - 1) * C::BK) * C::BYTES;        // bytes of k in the last slice
     constexpr int PER = C::LA + C::LB;
-    constexpr int PRE = MFMAS >= 16 ? 4 : MFMAS > 1 ? 1 : 0;              // matrix instructions of a slice's last step ahead of the barrier
+    constexpr int PRE = MFMAS >= 32 ? 8 : MFMAS >= 16 ? 4 : MFMAS > 1 ? 1 : 0;              // matrix instructions of a slice's last step ahead of the barrier
     static_assert((ST - 1) * PER <= 63, "the load counter holds 63");
 #pragma unroll
     for (int p = 0; p < ST; p++)
@@ -246,11 +266,12 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const vo
     asm volatile("" ::: "memory");
 #pragma unroll
     for (int r = 0; r < READS; r++) read_one(0, 0, 0, r);
-    auto slice = [&](int stage, int next, auto issue_c, auto more_c) {
+    // (`first`: which of the two sets of fragments holds the slice's first step)
+    auto slice = [&](int stage, int next, auto issue_c, auto more_c, auto first_c) {
         constexpr bool ISSUE = decltype(issue_c)::value, MORE = decltype(more_c)::value;
 #pragma unroll
         for (int q = 0; q < Q; q++) {
-            const int buf = q & 1;
+            const int buf = (q + decltype(first_c)::value) & 1;
             if (!MORE && tail != 128) {
                 if constexpr (C::A_ROWS) {
 #pragma unroll
@@ -299,9 +320,30 @@ __device__ __forceinline__ void accumulate(f32x16 (&acc)[C::TM][C::TN], const vo
     };
     int kt = 0, stage = 0;
     auto advance = [&]() { kt++; stage = stage + 1 == ST ? 0 : stage + 1; };
-    for (; kt + ST < KT; advance()) slice(stage, stage + 1 == ST ? 0 : stage + 1, std::true_type(), std::true_type());
-    for (; kt + 1 < KT; advance()) slice(stage, stage + 1 == ST ? 0 : stage + 1, std::false_type(), std::true_type());
-    slice(stage, 0, std::false_type(), std::false_type());
+    auto following = [&]() { return stage + 1 == ST ? 0 : stage + 1; };
+    constexpr auto set_0 = std::integral_constant<int, 0>();
+    if constexpr (Q % 2 == 0) {
+        for (; kt + ST < KT; advance()) slice(stage, following(), std::true_type(), std::true_type(), set_0);
+        for (; kt + 1 < KT; advance()) slice(stage, following(), std::false_type(), std::true_type(), set_0);
+    } else {
+        // one step a slice: slices alternate between the sets, two to a turn of the loop; the last few move theirs back
+        constexpr auto set_1 = std::integral_constant<int, 1>();
+        auto move_back = [&]() {
+#pragma unroll
+            for (int i = 0; i < TM; i++) fa[0][i] = fa[1][i];
+#pragma unroll
+            for (int j = 0; j < TN; j++) fb[0][j] = fb[1][j];
+        };
+        while (kt + ST + 1 < KT) {
+            slice(stage, following(), std::true_type(), std::true_type(), set_0);
+            advance();
+            slice(stage, following(), std::true_type(), std::true_type(), set_1);
+            advance();
+        }
+        for (; kt + ST < KT; advance()) { slice(stage, following(), std::true_type(), std::true_type(), set_0); move_back(); }
+        for (; kt + 1 < KT; advance()) { slice(stage, following(), std::false_type(), std::true_type(), set_0); move_back(); }
+    }
+    slice(stage, 0, std::false_type(), std::false_type(), set_0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -392,13 +434,14 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
     int row, column;
     tile_of(blockIdx.x, (p.M + C::BM - 1) / C::BM, (p.N + C::COLUMNS - 1) / C::COLUMNS, row, column);
     const long m0 = (long)row * C::BM, n0 = (long)column * C::COLUMNS;
-    f32x16 acc[C::TM][C::TN];
+    constexpr int F = C::F, REGISTERS = F * F / 64;
+    typename block_sums<F>::type acc[C::TM][C::TN];
 #pragma unroll
     for (int i = 0; i < C::TM; i++)
 #pragma unroll
         for (int j = 0; j < C::TN; j++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
+            for (int r = 0; r < REGISTERS; r++) acc[i][j][r] = 0.f;
     const long k0 = p.partial ? (long)blockIdx.y * p.slices_per_split * C::BK : 0;
     const long K = p.partial ? min((long)p.slices_per_split * C::BK, p.K - k0) : p.K;
     accumulate<C>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds);
@@ -407,7 +450,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
 
     // A wavefront's strips of 32 rows, through LDS of its own: stored by columns of the accumulators, read by rows.
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / C::WGN, wn = wave % C::WGN, l32 = lane & 31, h = lane >> 5;
+    const int wm = wave / C::WGN, wn = wave % C::WGN, at = lane % F, group = lane / F;
     __attribute__((address_space(3))) float *const strip = (__attribute__((address_space(3))) float *)lds + wave * 32 * C::STRIP;
     typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
     constexpr int SPAN = C::EPILOGUE == GATED ? C::WN / 2 : C::WN;         // columns of C of a wavefront
@@ -422,7 +465,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
 #pragma unroll
-    for (int i = 0; i < C::TM; i++) {
+    for (int i = 0; i < C::WM / 32; i++) {
         const long first = m0 + wm * C::WM + i * 32 + r0;                 // the lane's row of pass 0
         const bool across = some > 0;
         auto take = [&](int pass, int c, float (&v)[8]) {
@@ -440,10 +483,14 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
                     if (across && first + pass * DOWN < p.M) load_residual<Y>(p, r[pass], first + pass * DOWN, n, some);
             }
 #pragma unroll
-        for (int j = 0; j < C::TN; j++)
+        for (int b = 0; b < 32 / F; b++)
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-                *(lds_f32x4 *)(strip + l32 * C::STRIP + j * 32 + 8 * g + 4 * h) = f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            for (int j = 0; j < C::TN; j++)
+#pragma unroll
+                for (int g = 0; g < REGISTERS / 4; g++) {
+                    const auto &v = acc[i * (32 / F) + b][j];
+                    *(lds_f32x4 *)(strip + (b * F + at) * C::STRIP + j * F + 8 * g + 4 * group) = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+                }
         order_lanes();
         if (p.partial) {
 #pragma unroll 1

@@ -66,27 +66,38 @@ operand moved_where_needed(const operand &o, long rows, long columns, int bytes,
     return {out, to / bytes};
 }
 
-// ---- which tile, and how many workgroups share the k of one.  A launch is modelled as `fixed` microseconds, and per slice of 128 bytes of k `first` for
-// the first round of tiles over the compute units and `further` for each round after it; splitting adds a launch and the partial sums' bytes.
-struct tile_model { int edge; double fixed, first, further; };
-constexpr tile_model TILE_MODELS[] = {{256, 9.0, 1.1, 1.7}, {128, 3.9, 0.50, 0.48}, {64, 3.35, 0.264, 0.234}};
-struct tile_plan { int edge, splits, slices; };
+// ---- which tile, and how many workgroups share the k of one.  A launch is modelled in microseconds: `fixed`, for every slice of 128 bytes of k `first` for the first
+// round of tiles over the compute units (and `full` as far as it fills them), and for every further round `round` and `further` a slice.
+// Splitting k adds a launch and the partial sums' bytes at 4 TB/s.  Fitted to launches of 16 ... 4096 tiles of 8 ... 64 slices (tables of
+// 29 configurations; rms error 6 %); us with 256 x 256, 256 x 128, 128 x 128 and 64 x 64 tiles, bf16: 4096^3 102, 115, 149, 190; 4096 x 1024 x 4096 74, 48, 35, 50;
+// 1024^3 24, 15.5, 11, 7.0; 128 x 4096 x 4096 70, 45, 29, 18.
+struct tile_model { product_tile tile; int rows, columns; double fixed, first, full, round, further; };
+constexpr tile_model TILES_16_BITS[] = {{TILE_256, 256, 256, 9.0, 0.94, 0.5, 4.0, 1.44}, {TILE_256x128, 256, 128, 5.8, 0.6, 0.15, 7.0, 0.75},
+                                        {TILE_128, 128, 128, 4.8, 0.38, 0.09, 0.8, 0.58}, {TILE_64, 64, 64, 3.5, 0.2, 0.03, 0.7, 0.155}};
+constexpr tile_model TILES_8_BITS[] = {{TILE_256, 256, 256, 13.8, 0.8, 0.6, 9.0, 1.4}, {TILE_256x128, 256, 128, 9.6, 0.44, 0.24, 13.5, 0.69},
+                                       {TILE_128, 128, 128, 7.0, 0.26, 0.24, 4.7, 0.467}, {TILE_64, 64, 64, 4.8, 0.13, 0.02, 0.7, 0.19}};
+// (a gated layer's smallest tile is 64 x 128: 64 columns of gate and the same of up)
+constexpr tile_model GATED_64_16_BITS = {TILE_64, 64, 128, 3.9, 0.27, 0.08, 0.7, 0.31}, GATED_64_8_BITS = {TILE_64, 64, 128, 5.4, 0.13, 0.05, 0.7, 0.3};
+struct tile_plan { product_tile tile; int splits, slices; };
 tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
     const long slices = std::max(1L, (K * bytes + 127) / 128);
-    tile_plan best = {0, 1, 0};
+    tile_plan best = {TILE_64, 0, 0};
     double best_cost = 0;
-    for (const tile_model &t : TILE_MODELS) {
-        const long rows = t.edge, columns = gated ? std::max(t.edge / 2, 64) : t.edge, weight = gated && t.edge == 64 ? 2 : 1;
-        const long tiles = ((M + rows - 1) / rows) * ((N + columns - 1) / columns);
+    auto consider = [&](const tile_model &t) {
+        const long tiles = ((M + t.rows - 1) / t.rows) * ((N * (gated ? 2 : 1) + t.columns - 1) / t.columns);
         for (long splits = 1; splits <= 16 && splits <= slices; splits++) {
-            const long each = (slices + splits - 1) / splits, used = (slices + each - 1) / each;
-            if (used != splits) continue;
-            const double rounds = (double)((tiles * splits + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
-            double cost = t.fixed + (double)each * weight * (t.first + (rounds - 1) * t.further);
-            if (splits > 1) cost += 4.0 + (double)(gated ? 2 : 1) * M * N * 4 * 2 * splits / 4e6;
-            if (!best.edge || cost < best_cost) { best = {t.edge, (int)splits, (int)each}; best_cost = cost; }
+            const long each = (slices + splits - 1) / splits;
+            if ((slices + each - 1) / each != splits) continue;            // (the same slices to each as with fewer)
+            const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
+            double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
+            if (splits > 1) cost += 3.0 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 4e6;
+            if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each}; best_cost = cost; }
         }
-    }
+    };
+    for (const tile_model &t : TILES_16_BITS)
+        if (bytes == 2) consider(gated && t.tile == TILE_64 ? GATED_64_16_BITS : t);
+    for (const tile_model &t : TILES_8_BITS)
+        if (bytes == 1) consider(gated && t.tile == TILE_64 ? GATED_64_8_BITS : t);
     return best;
 }
 
@@ -99,9 +110,9 @@ int launch_product(const char *fn, int type, product_layout layout, int epilogue
     p.partial = nullptr;
     p.slices_per_split = plan.slices;
     if (plan.splits > 1) p.partial = (float *)scratch(PARTIAL, (uint64_t)plan.splits * (gated ? 2 : 1) * p.M * p.N * 4);
-    if (type == BF16) launch_tiles_BF16(plan.edge, layout, epilogue, y, p, plan.splits, stream());
-    else if (type == F16) launch_tiles_F16(plan.edge, layout, epilogue, y, p, plan.splits, stream());
-    else launch_tiles_F8(plan.edge, layout, epilogue, y, p, plan.splits, stream());
+    if (type == BF16) launch_tiles_BF16(plan.tile, layout, epilogue, y, p, plan.splits, stream());
+    else if (type == F16) launch_tiles_F16(plan.tile, layout, epilogue, y, p, plan.splits, stream());
+    else launch_tiles_F8(plan.tile, layout, epilogue, y, p, plan.splits, stream());
     if (plan.splits > 1) {
         const unsigned blocks = (unsigned)(((p.N + 7L) / 8 * p.M + 255) / 256);
         auto kernel = gated ? (y == BF16 ? finish_kernel<BF16, GATED> : finish_kernel<F16, GATED>) : (y == BF16 ? finish_kernel<BF16, LINEAR> : finish_kernel<F16, LINEAR>);
