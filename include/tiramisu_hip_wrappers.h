@@ -209,6 +209,15 @@ int tiramisu_hip_gated_linear(const void *x, const void *gate_weight, const void
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate,
                                        const void *up, void *dx, void *dgate_weight, void *dup_weight, uint64_t M, uint64_t N, uint64_t K, uint64_t ldh,
                                        uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
+/* Any of the functions above on a stream of the caller's (null: HIP's null stream, torch's default stream) instead of the thread's current one, for
+ * callers that pay for every argument they convert: its arguments in order, each in eight bytes, numbers and floats of 32 bits in the first
+ * four of them. */
+enum tiramisu_hip_operator_t {
+    TIRAMISU_HIP_OPERATOR_RMS_NORM = 0, TIRAMISU_HIP_OPERATOR_RMS_NORM_BACKWARD = 1, TIRAMISU_HIP_OPERATOR_QUANTIZE_ROWS = 2,
+    TIRAMISU_HIP_OPERATOR_LINEAR = 3, TIRAMISU_HIP_OPERATOR_LINEAR_BACKWARD = 4, TIRAMISU_HIP_OPERATOR_GATED_LINEAR = 5,
+    TIRAMISU_HIP_OPERATOR_GATED_LINEAR_BACKWARD = 6
+};
+int tiramisu_hip_operator(int32_t op, const uint64_t *arguments, void *stream);
 
 /* ---- per-launch timing.  Between profile_start and profile_stop every tiramisu_hip_launch
  *      (and GEMM library call), from any thread, is bracketed by two events on its current

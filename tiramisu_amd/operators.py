@@ -8,6 +8,7 @@ kernels run on torch's current stream of the tensors' device; nothing waits for 
 dimension), with one stride from row to row; others are refused, never copied silently.  Results are new, dense tensors.
 ValueError says what does not fit, RuntimeError that the runtime refused the call (its reason is on stderr).
 """
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -17,8 +18,22 @@ from . import runtime
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3}
 _HALVES = (torch.float16, torch.bfloat16)
-_NULL_STREAM = 1                  # HIP's handle of the null stream, torch's default stream (whose handle, 0, means the thread's own to the runtime)
+_NORM_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_PRODUCT_TYPES = _HALVES + (torch.float8_e4m3fn,)
+
+# The operators of the C ABI: number, and how their arguments are packed for tiramisu_hip_operator (a call of 16 converted arguments and three for the
+# stream cost 2 us more; a norm of one token 12.9 us a call then, of which 5 are the kernel)
+_RMS_NORM = 0, struct.Struct("=11Qf4x2Q").pack
+_RMS_NORM_BACKWARD = 1, struct.Struct("=13Q").pack
+_QUANTIZE_ROWS = 2, struct.Struct("=7Q").pack
+_LINEAR = 3, struct.Struct("=17Q").pack
+_LINEAR_BACKWARD = 4, struct.Struct("=16Q").pack
+_GATED_LINEAR = 5, struct.Struct("=18Q").pack
+_GATED_LINEAR_BACKWARD = 6, struct.Struct("=20Q").pack
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_entry = None                     # tiramisu_hip_operator, from the first call on
 
 
 class RmsNorm(NamedTuple):
@@ -132,21 +147,23 @@ def _activation(name):
     return ACTIVATIONS[name]
 
 
-def _call(entry, where, *args):
-    """One entry of the C ABI on torch's current stream of GPU `where`."""
-    w = runtime.wrappers()
-    if where != torch.cuda.current_device():
+def _call(operator, where, *args):
+    """One operator of the C ABI on torch's current stream of GPU `where`."""
+    global _entry
+    if _entry is None:
+        _entry = runtime.wrappers().tiramisu_hip_operator
+    number, pack = operator
+    if where != _device():
         with torch.cuda.device(where):
-            return _call(entry, where, *args)
+            return _call(operator, where, *args)
     stream = _raw_stream(where) if _raw_stream else torch.cuda.current_stream(where).cuda_stream
-    before = w.tiramisu_hip_get_stream()
-    w.tiramisu_hip_set_stream(stream or _NULL_STREAM)
-    try:
-        rc = getattr(w, entry)(*args)
-    finally:
-        w.tiramisu_hip_set_stream(before)
-    if rc != 0:
-        raise RuntimeError("%s refused the call" % entry)
+    if _entry(number, pack(*args), stream) != 0:
+        raise RuntimeError("the runtime refused the call")
+
+
+def _like(t, dtype):
+    """A new dense tensor of t's shape."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _eight_bit_scales(x, pairs):
@@ -161,35 +178,35 @@ def rms_norm(x, weight, residual=None, eps=1e-6, eight_bit=False, keep_rstd=Fals
     """sum = x + residual, y = sum / sqrt(mean(sum^2) + eps) * weight for each row, of the sum ahead of its rounding.  float32, float16 or
     bfloat16; with ``eight_bit`` y is float8_e4m3fn and stands for y * scale[row].  ``keep_rstd`` keeps 1 / length of each row, which the
     backward pass reads together with ``sum``."""
-    rows, ldx = _rows(x, "x", dtypes=(torch.bfloat16, torch.float16, torch.float32))
+    rows, ldx = _rows(x, "x", dtypes=_NORM_TYPES)
     columns, where = x.shape[-1], x.get_device()
     w = _vector(weight, "weight", columns, x.dtype, where)
-    r, ldr, total = None, 0, None
+    r, ldr, total = 0, 0, None
     if residual is not None:
         ldr = _rows(residual, "residual", shape=x.shape, dtypes=(x.dtype,))[1]
-        r, total = _pointer(residual, "residual", where), torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if eight_bit else x.dtype, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if eight_bit else None
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if keep_rstd else None
-    _call("tiramisu_hip_rms_norm", where, x.data_ptr(), r, w, y.data_ptr(), None if total is None else total.data_ptr(),
-          scale.data_ptr() if eight_bit else None, rstd.data_ptr() if keep_rstd else None, rows, columns, ldx, ldr, eps, _TYPES[x.dtype], _TYPES[y.dtype])
+        r, total = _pointer(residual, "residual", where), _like(x, x.dtype)
+    y = _like(x, torch.float8_e4m3fn if eight_bit else x.dtype)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if eight_bit else None
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32) if keep_rstd else None
+    _call(_RMS_NORM, where, x.data_ptr(), r, w, y.data_ptr(), 0 if total is None else total.data_ptr(),
+          scale.data_ptr() if eight_bit else 0, rstd.data_ptr() if keep_rstd else 0, rows, columns, ldx, ldr, eps, _TYPES[x.dtype], _TYPES[y.dtype])
     return RmsNorm(y, x if total is None else total, scale, rstd)
 
 
 def rms_norm_backward(dy, sum, weight, rstd, dsum=None):
     """Gradients of ``rms_norm`` from the gradient of y and, where the sum is used further on, the gradient ``dsum`` of the sum."""
-    rows, lds = _rows(sum, "sum", dtypes=(torch.bfloat16, torch.float16, torch.float32))
+    rows, lds = _rows(sum, "sum", dtypes=_NORM_TYPES)
     columns, where = sum.shape[-1], sum.get_device()
     ldy = _rows(dy, "dy", shape=sum.shape, dtypes=(sum.dtype,))[1]
     w = _vector(weight, "weight", columns, sum.dtype, where)
     lengths = _row_scale(rstd, "rstd", sum, rows, where)
-    d, ldd = None, 0
+    d, ldd = 0, 0
     if dsum is not None:
         ldd = _rows(dsum, "dsum", shape=sum.shape, dtypes=(sum.dtype,))[1]
         d = _pointer(dsum, "dsum", where)
-    dx = torch.empty(sum.shape, dtype=sum.dtype, device=sum.device)
-    dweight = torch.empty_like(weight)
-    _call("tiramisu_hip_rms_norm_backward", where, _pointer(dy, "dy", where), sum.data_ptr(), w, lengths, d, dx.data_ptr(), dweight.data_ptr(), rows, columns,
+    dx = _like(sum, sum.dtype)
+    dweight = weight.new_empty(columns)
+    _call(_RMS_NORM_BACKWARD, where, _pointer(dy, "dy", where), sum.data_ptr(), w, lengths, d, dx.data_ptr(), dweight.data_ptr(), rows, columns,
           ldy, lds, ldd, _TYPES[sum.dtype])
     return RmsNormGradients(dx, dweight)
 
@@ -197,10 +214,10 @@ def rms_norm_backward(dy, sum, weight, rstd, dsum=None):
 def quantize_rows(x):
     """x as float8_e4m3fn with a scale for each row, max|row| / 448 (1 for a row of zeros): weights once, activations where no norm
     precedes the product."""
-    rows, ldx = _rows(x, "x", dtypes=(torch.bfloat16, torch.float16, torch.float32))
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _call("tiramisu_hip_quantize_rows", x.get_device(), x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], ldx, _TYPES[x.dtype])
+    rows, ldx = _rows(x, "x", dtypes=_NORM_TYPES)
+    q = _like(x, torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _call(_QUANTIZE_ROWS, x.get_device(), x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], ldx, _TYPES[x.dtype])
     return EightBitRows(q, scale)
 
 
@@ -220,25 +237,25 @@ def linear(x, weight, bias=None, residual=None, activation="none", x_scale=None,
     """y = activation(x weight^T + bias) + residual.  x and weight are float16 or bfloat16, or float8_e4m3fn with ``x_scale`` (of each row
     of x) and ``weight_scale`` (of each output), then ``dtype`` (bfloat16) is the result's type.  bias and residual are of the result's
     type.  ``keep_pre`` keeps the sums ahead of the activation, which the backward pass reads."""
-    rows, ldx = _rows(x, "x", dtypes=_HALVES + (torch.float8_e4m3fn,))
+    rows, ldx = _rows(x, "x", dtypes=_PRODUCT_TYPES)
     k, where = x.shape[-1], x.get_device()
     ldw = _matrix(weight, "weight", None, k, x.dtype)
     n, out = weight.shape[0], _result_dtype(x, dtype)
     _eight_bit_scales(x, (("x_scale", x_scale), ("weight_scale", weight_scale)))
     shape = x.shape[:-1] + (n,)
-    xs = None if x_scale is None else _row_scale(x_scale, "x_scale", x, rows, where)
-    ws = None if weight_scale is None else _vector(weight_scale, "weight_scale", n, torch.float32, where)
-    b = None if bias is None else _vector(bias, "bias", n, out, where)
-    r, ldr = None, 0
+    xs = 0 if x_scale is None else _row_scale(x_scale, "x_scale", x, rows, where)
+    ws = 0 if weight_scale is None else _vector(weight_scale, "weight_scale", n, torch.float32, where)
+    b = 0 if bias is None else _vector(bias, "bias", n, out, where)
+    r, ldr = 0, 0
     if residual is not None:
         ldr = _rows(residual, "residual", shape=shape, dtypes=(out,))[1]
         r = _pointer(residual, "residual", where)
     if k == 0:
         rows = shape[:-1].numel()
     a = _activation(activation)
-    y = torch.empty(shape, dtype=out, device=x.device)
-    pre = torch.empty(shape, dtype=out, device=x.device) if keep_pre else None
-    _call("tiramisu_hip_linear", where, x.data_ptr(), _pointer(weight, "weight", where), b, r, xs, ws, y.data_ptr(), pre.data_ptr() if keep_pre else None,
+    y = x.new_empty(shape, dtype=out)
+    pre = x.new_empty(shape, dtype=out) if keep_pre else None
+    _call(_LINEAR, where, x.data_ptr(), _pointer(weight, "weight", where), b, r, xs, ws, y.data_ptr(), pre.data_ptr() if keep_pre else 0,
           rows, n, k, ldx, ldw, ldr, a, _TYPES[x.dtype], _TYPES[out])
     return Linear(y, pre)
 
@@ -258,11 +275,11 @@ def linear_backward(dy, x, weight, pre=None, activation="none", bias=False):
         raise ValueError("pre: an activation and the sums ahead of it belong together")
     if pre is not None:
         ldp = _rows(pre, "pre", shape=shape, dtypes=(x.dtype,))[1]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dweight = torch.empty((n, k), dtype=x.dtype, device=x.device)
-    dbias = torch.empty(n, dtype=x.dtype, device=x.device) if bias else None
-    _call("tiramisu_hip_linear_backward", where, _pointer(dy, "dy", where), x.data_ptr(), _pointer(weight, "weight", where), None if pre is None else _pointer(pre, "pre", where),
-          dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr() if bias else None, rows, n, k, ldy, ldx, ldw, ldp, a, _TYPES[x.dtype])
+    dx = _like(x, x.dtype)
+    dweight = x.new_empty((n, k), dtype=x.dtype)
+    dbias = x.new_empty(n, dtype=x.dtype) if bias else None
+    _call(_LINEAR_BACKWARD, where, _pointer(dy, "dy", where), x.data_ptr(), _pointer(weight, "weight", where), 0 if pre is None else _pointer(pre, "pre", where),
+          dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr() if bias else 0, rows, n, k, ldy, ldx, ldw, ldp, a, _TYPES[x.dtype])
     return LinearGradients(dx, dweight, dbias)
 
 
@@ -271,22 +288,22 @@ def linear_backward(dy, x, weight, pre=None, activation="none", bias=False):
 def gated_linear(x, gate_weight, up_weight, activation="silu", x_scale=None, gate_scale=None, up_scale=None, dtype=None, keep_pre=False):
     """h = activation(x gate_weight^T) * (x up_weight^T), types and scales as for ``linear``.  ``keep_pre`` keeps both projections, which
     the backward pass reads."""
-    rows, ldx = _rows(x, "x", dtypes=_HALVES + (torch.float8_e4m3fn,))
+    rows, ldx = _rows(x, "x", dtypes=_PRODUCT_TYPES)
     k, where = x.shape[-1], x.get_device()
     ldg = _matrix(gate_weight, "gate_weight", None, k, x.dtype)
     n, out = gate_weight.shape[0], _result_dtype(x, dtype)
     ldu = _matrix(up_weight, "up_weight", n, k, x.dtype)
     _eight_bit_scales(x, (("x_scale", x_scale), ("gate_scale", gate_scale), ("up_scale", up_scale)))
-    xs = None if x_scale is None else _row_scale(x_scale, "x_scale", x, rows, where)
-    gs = None if gate_scale is None else _vector(gate_scale, "gate_scale", n, torch.float32, where)
-    us = None if up_scale is None else _vector(up_scale, "up_scale", n, torch.float32, where)
+    xs = 0 if x_scale is None else _row_scale(x_scale, "x_scale", x, rows, where)
+    gs = 0 if gate_scale is None else _vector(gate_scale, "gate_scale", n, torch.float32, where)
+    us = 0 if up_scale is None else _vector(up_scale, "up_scale", n, torch.float32, where)
     a, shape = _activation(activation), x.shape[:-1] + (n,)
     if k == 0:
         rows = shape[:-1].numel()
-    h = torch.empty(shape, dtype=out, device=x.device)
-    gate, up = [torch.empty(shape, dtype=out, device=x.device) for _ in range(2)] if keep_pre else (None, None)
-    _call("tiramisu_hip_gated_linear", where, x.data_ptr(), _pointer(gate_weight, "gate_weight", where), _pointer(up_weight, "up_weight", where), xs, gs, us, h.data_ptr(),
-          gate.data_ptr() if keep_pre else None, up.data_ptr() if keep_pre else None, rows, n, k, ldx, ldg, ldu, a, _TYPES[x.dtype], _TYPES[out])
+    h = x.new_empty(shape, dtype=out)
+    gate, up = [x.new_empty(shape, dtype=out) for _ in range(2)] if keep_pre else (None, None)
+    _call(_GATED_LINEAR, where, x.data_ptr(), _pointer(gate_weight, "gate_weight", where), _pointer(up_weight, "up_weight", where), xs, gs, us, h.data_ptr(),
+          gate.data_ptr() if keep_pre else 0, up.data_ptr() if keep_pre else 0, rows, n, k, ldx, ldg, ldu, a, _TYPES[x.dtype], _TYPES[out])
     return GatedLinear(h, gate, up)
 
 
@@ -301,9 +318,9 @@ def gated_linear_backward(dh, x, gate_weight, up_weight, gate, up, activation="s
     rows = shape[:-1].numel()
     ldh, ld_gate, ld_up = [_rows(t, name, shape=shape, dtypes=(x.dtype,))[1] for name, t in (("dh", dh), ("gate", gate), ("up", up))]
     a = _activation(activation)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dg, du = [torch.empty((n, k), dtype=x.dtype, device=x.device) for _ in range(2)]
-    _call("tiramisu_hip_gated_linear_backward", where, _pointer(dh, "dh", where), x.data_ptr(), _pointer(gate_weight, "gate_weight", where), _pointer(up_weight, "up_weight", where),
+    dx = _like(x, x.dtype)
+    dg, du = [x.new_empty((n, k), dtype=x.dtype) for _ in range(2)]
+    _call(_GATED_LINEAR_BACKWARD, where, _pointer(dh, "dh", where), x.data_ptr(), _pointer(gate_weight, "gate_weight", where), _pointer(up_weight, "up_weight", where),
           _pointer(gate, "gate", where), _pointer(up, "up", where), dx.data_ptr(), dg.data_ptr(), du.data_ptr(), rows, n, k, ldh, ldx, ldg, ldu, ld_gate, ld_up, a,
           _TYPES[x.dtype])
     return GatedLinearGradients(dx, dg, du)
