@@ -75,7 +75,8 @@ def build_compiler(force=True):
 
 # The runtime's translation units: (object, source, what it is compiled with).  The matrix products' kernels are one unit for each type of operand.
 WRAPPER_UNITS = [("hip_wrappers", "hip_wrappers.hip", []), ("operators", "operators.hip", [])] + \
-    [("linear_tiles_" + e.lower(), "linear_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16", "F8")]
+    [("linear_tiles_" + e.lower(), "linear_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16")] + \
+    [("linear_tiles_f8", "linear_tiles.hip", ["-DTIRAMISU_OPERAND=F8", "-DTIRAMISU_OPERAND_HAS_NO_GRADIENTS"])]
 
 
 def build_wrappers(force=True):

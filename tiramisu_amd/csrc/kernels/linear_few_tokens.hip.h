@@ -113,8 +113,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
                 for (int i = 0; i < 4; i++) z[q][4 * four + i] += s[i];
             }
     }
-    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, z[0], z[1], m, n, some);
-    else finish_linear<Y>(p, z[0], m, n, some);
+    column_terms columns;
+    load_column_terms<Y>(p, columns, n, some);
+    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z[0], z[1], m, n, some);
+    else finish_linear<Y>(p, columns, z[0], m, n, some);
 }
 
 }  // namespace tops

@@ -351,23 +351,26 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
 }
 
 // ---- epilogues: 8 columns from n on of row m; `some`: how many of them exist
+// (what belongs to the columns is loaded once for all rows of a strip)
+struct column_terms { float bias[8], scale[8], scale_2[8]; };
 template <int Y>
-__device__ __forceinline__ void activate_linear(const product_arguments &p, float (&z)[8], long m, long n, int some) {
-    typedef stored<Y> T;
+__device__ __forceinline__ void load_column_terms(const product_arguments &p, column_terms &c, long n, int some) {
+    if (p.bias) load_some<Y>((const stored<Y> *)p.bias + n, some, c.bias);
+    if (p.b_scale) load_some<F32>(p.b_scale + n, some, c.scale);
+    if (p.b2_scale) load_some<F32>(p.b2_scale + n, some, c.scale_2);
+}
+template <int Y>
+__device__ __forceinline__ void activate_linear(const product_arguments &p, const column_terms &c, float (&z)[8], long m, long n, int some) {
     if (p.a_scale) {
         const float s = p.a_scale[m];
-        float c[8];
-        load_some<F32>(p.b_scale + n, some, c);
 #pragma unroll
-        for (int i = 0; i < 8; i++) z[i] *= s * c[i];
+        for (int i = 0; i < 8; i++) z[i] *= s * c.scale[i];
     }
     if (p.bias) {
-        float b[8];
-        load_some<Y>((const T *)p.bias + n, some, b);
 #pragma unroll
-        for (int i = 0; i < 8; i++) z[i] += b[i];
+        for (int i = 0; i < 8; i++) z[i] += c.bias[i];
     }
-    if (p.pre) store_some<Y>((T *)p.pre + m * p.N + n, some, z);
+    if (p.pre) store_some<Y>((stored<Y> *)p.pre + m * p.N + n, some, z);
     activate(p.activation, z);
 }
 template <int Y>
@@ -381,8 +384,8 @@ __device__ __forceinline__ void store_linear(const product_arguments &p, const f
     else if (m >= p.split_row) store_some<Y>((T *)p.y_below + (m - p.split_row) * p.N + n, some, z);
 }
 template <int Y>
-__device__ __forceinline__ void finish_linear(const product_arguments &p, float (&z)[8], long m, long n, int some) {
-    activate_linear<Y>(p, z, m, n, some);
+__device__ __forceinline__ void finish_linear(const product_arguments &p, const column_terms &c, float (&z)[8], long m, long n, int some) {
+    activate_linear<Y>(p, c, z, m, n, some);
     if (p.residual) {
         float r[8];
         load_residual<Y>(p, r, m, n, some);
@@ -392,15 +395,12 @@ __device__ __forceinline__ void finish_linear(const product_arguments &p, float 
     store_linear<Y>(p, z, m, n, some);
 }
 template <int Y>
-__device__ __forceinline__ void finish_gated(const product_arguments &p, float (&g)[8], float (&u)[8], long m, long n, int some) {
+__device__ __forceinline__ void finish_gated(const product_arguments &p, const column_terms &c, float (&g)[8], float (&u)[8], long m, long n, int some) {
     typedef stored<Y> T;
     if (p.a_scale) {
         const float s = p.a_scale[m];
-        float c[8], d[8];
-        load_some<F32>(p.b_scale + n, some, c);
-        load_some<F32>(p.b2_scale + n, some, d);
 #pragma unroll
-        for (int i = 0; i < 8; i++) { g[i] *= s * c[i]; u[i] *= s * d[i]; }
+        for (int i = 0; i < 8; i++) { g[i] *= s * c.scale[i]; u[i] *= s * c.scale_2[i]; }
     }
     if (p.pre) {
         store_some<Y>((T *)p.pre + m * p.N + n, some, g);
@@ -425,14 +425,12 @@ __device__ __forceinline__ void tile_of(int id, int rows, int columns, int &row,
     row = band * BAND + in - column * height;
 }
 
-// grid: (tiles, splits of k).  Y: type of bias, residual and outputs.
+#ifdef __HIP_DEVICE_COMPILE__               // (the host's compilation needs no body, and rejects a second one of the same configuration)
+// Tile `id` of the product, of part `split` of k.  Y: type of bias, residual and outputs.
 template <class C, int Y>
-__global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
-#ifdef __HIP_DEVICE_COMPILE__               // (a second instantiation of one configuration does not pass the host's compilation, which needs no body)
-    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
-    lds_char *const lds = (lds_char *)shared_bytes;
+__device__ __forceinline__ void compute_tile(const product_arguments &p, int id, int split, lds_char *lds) {
     int row, column;
-    tile_of(blockIdx.x, (p.M + C::BM - 1) / C::BM, (p.N + C::COLUMNS - 1) / C::COLUMNS, row, column);
+    tile_of(id, (p.M + C::BM - 1) / C::BM, (p.N + C::COLUMNS - 1) / C::COLUMNS, row, column);
     const long m0 = (long)row * C::BM, n0 = (long)column * C::COLUMNS;
     constexpr int F = C::F, REGISTERS = F * F / 64;
     typename block_sums<F>::type acc[C::TM][C::TN];
@@ -442,7 +440,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
         for (int j = 0; j < C::TN; j++)
 #pragma unroll
             for (int r = 0; r < REGISTERS; r++) acc[i][j][r] = 0.f;
-    const long k0 = p.partial ? (long)blockIdx.y * p.slices_per_split * C::BK : 0;
+    const long k0 = p.partial ? (long)split * p.slices_per_split * C::BK : 0;
     const long K = p.partial ? min((long)p.slices_per_split * C::BK, p.K - k0) : p.K;
     accumulate<C>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds);
     if constexpr (C::EPILOGUE == LINEAR && C::A_ROWS && !C::B_ROWS)        // (only the gradient of a gated layer's input has two)
@@ -459,6 +457,8 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
     const long n = n0 + wn * SPAN + c0;
     const int some = (int)min(8L, p.N - n);
     constexpr int PASSES = 32 / DOWN;
+    column_terms columns;
+    if (some > 0 && !p.partial) load_column_terms<Y>(p, columns, n, some);
     auto order_lanes = [] {                                               // what the lanes of a wavefront pass to each other
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -498,7 +498,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
                 const long m = first + pass * DOWN;
                 if (!across || m >= p.M) continue;
                 constexpr long PARTS = C::EPILOGUE == GATED ? 2 : 1;
-                float *out = p.partial + ((long)blockIdx.y * PARTS * p.M + m) * p.N + n;
+                float *out = p.partial + ((long)split * PARTS * p.M + m) * p.N + n;
 #pragma unroll
                 for (int part = 0; part < PARTS; part++) {
                     float z[8];
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
                 float z[8], u[8];
                 take(pass, c0, z);
                 take(pass, SPAN + c0, u);
-                if (across && first + pass * DOWN < p.M) finish_gated<Y>(p, z, u, first + pass * DOWN, n, some);
+                if (across && first + pass * DOWN < p.M) finish_gated<Y>(p, columns, z, u, first + pass * DOWN, n, some);
             }
         } else {
             // what takes many instructions is a loop that is not unrolled, in place; then the results
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
                         if (!across || first + pass * DOWN >= p.M) continue;
                         float z[8];
                         take(pass, c0, z);
-                        activate_linear<Y>(p, z, first + pass * DOWN, n, some);
+                        activate_linear<Y>(p, columns, z, first + pass * DOWN, n, some);
                         lds_f32x4 *const back = (lds_f32x4 *)(strip + (pass * DOWN + r0) * C::STRIP + c0);
                         back[0] = f32x4{z[0], z[1], z[2], z[3]};
                         back[1] = f32x4{z[4], z[5], z[6], z[7]};
@@ -544,6 +544,28 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
         }
         order_lanes();
     }
+}
+#endif
+
+// grid: (tiles, splits of k)
+template <class C, int Y>
+__global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    compute_tile<C, Y>(p, blockIdx.x, blockIdx.y, (lds_char *)shared_bytes);
+#endif
+}
+
+// Two products in one launch (both gradients of a layer), the second's tiles behind the first's: compute units that the last round of
+// the first leaves idle begin with the second.  `start`: the second's first workgroup, a multiple of the XCDs.
+template <class C, class D, int Y>
+__global__ __launch_bounds__(C::NT) void product_pair_kernel(product_arguments p, product_arguments q, int tiles, int start) {
+#ifdef __HIP_DEVICE_COMPILE__
+    static_assert(C::NT == D::NT, "one workgroup's size");
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    const int id = blockIdx.x;
+    if (id < tiles) compute_tile<C, Y>(p, id, 0, (lds_char *)shared_bytes);
+    else if (id >= start) compute_tile<D, Y>(q, id - start, 0, (lds_char *)shared_bytes);
 #endif
 }
 
@@ -570,8 +592,10 @@ __global__ __launch_bounds__(256) void finish_kernel(product_arguments p, int sp
             for (int i = 0; i < 8; i++) u[i] += v[i];
         }
     }
-    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, z, u, m, n, some);
-    else finish_linear<Y>(p, z, m, n, some);
+    column_terms columns;
+    load_column_terms<Y>(p, columns, n, some);
+    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z, u, m, n, some);
+    else finish_linear<Y>(p, columns, z, m, n, some);
 }
 
 }  // namespace tops

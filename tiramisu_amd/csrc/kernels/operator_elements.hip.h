@@ -117,10 +117,28 @@ __device__ __forceinline__ u32x4 load_guarded(const char *p, long left) {
 #pragma unroll
     for (int i = 0; i < 16 / BYTES; i++)
         if (i * BYTES < left) {
-            const uint32_t e = BYTES == 2 ? (uint32_t)*reinterpret_cast<const uint16_t *>(p + 2 * i) : (uint32_t)*reinterpret_cast<const uint8_t *>(p + i);
+            const uint32_t e = BYTES == 4 ? *reinterpret_cast<const uint32_t *>(p + 4 * i) : BYTES == 2 ? (uint32_t)*reinterpret_cast<const uint16_t *>(p + 2 * i)
+                                                                                           : (uint32_t)*reinterpret_cast<const uint8_t *>(p + i);
             w[i * BYTES / 4] |= e << (8 * (i * BYTES % 4));
         }
     return w;
+}
+
+// ... as fp32
+template <int E, int N>
+__device__ __forceinline__ void widen(u32x4 w, float (&v)[N]) {
+    static_assert(N == (E == F32 ? 4 : 8), "16 bytes");
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const uint32_t word = w[c];                          // (an element of a vector, given to the cast by itself, came out as another one)
+        if constexpr (E == F32) v[c] = __builtin_bit_cast(float, word);
+        else {
+            typedef stored<E> pair __attribute__((ext_vector_type(2)));
+            const pair e = __builtin_bit_cast(pair, word);
+            v[2 * c] = (float)e[0];
+            v[2 * c + 1] = (float)e[1];
+        }
+    }
 }
 
 // ---- activations and their slopes.  exp2 of a large argument is infinite and 1 / infinity zero: silu and the sigmoid of the tanh form
@@ -129,19 +147,18 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 __device__ __forceinline__ float gelu_tanh_argument(float z) { return 1.5957691216f * (z + 0.044715f * z * z * z); }   // 2 sqrt(2 / pi): 0.5 (1 + tanh a) = sigmoid(2 a)
 
 // The normal distribution's lower tail at -|z|, 0.5 erfc(|z| / sqrt 2) = exp(-z^2 / 2) R(t) with t = 1 / (1 + 0.31 |z|), and exp(-z^2 / 2).  R is t times a
-// polynomial of degree 7, fitted here to the smallest relative error (1.7e-7 up to |z| = 14, where the tail is below fp32's numbers): relative,
-// so that gelu of a large negative z, z times the tail, keeps its digits.  (The library's erff and the sum 1 + erf cost four times the instructions.)
+// polynomial of degree 5, fitted here to the smallest relative error (4.7e-6 up to |z| = 14, where the tail is below fp32's numbers; half a unit of
+// float16 is 2.4e-4): relative, so that gelu of a large negative z, z times the tail, keeps its digits.  gelu(z) = max(z, 0) - |z| tail.
+// (Epilogues are bound by these instructions: 3 million gelu cost 5 us with 17 of them and two of a quarter of the rate.)
 __device__ __forceinline__ float normal_tail(float z, float &bell) {
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.31f, fabsf(z), 1.f));
     bell = __builtin_amdgcn_exp2f(-0.72134752044f * z * z);
-    float r = 0.0358405643f;
-    r = __builtin_fmaf(r, t, -0.141600065f);
-    r = __builtin_fmaf(r, t, 0.155060586f);
-    r = __builtin_fmaf(r, t, -0.0148971602f);
-    r = __builtin_fmaf(r, t, 0.110107074f);
-    r = __builtin_fmaf(r, t, 0.10777195f);
-    r = __builtin_fmaf(r, t, 0.124060214f);
-    r = __builtin_fmaf(r, t, 0.123656918f);
+    float r = -0.0739265304f;
+    r = __builtin_fmaf(r, t, 0.180442905f);
+    r = __builtin_fmaf(r, t, 0.0157528392f);
+    r = __builtin_fmaf(r, t, 0.133425542f);
+    r = __builtin_fmaf(r, t, 0.120442332f);
+    r = __builtin_fmaf(r, t, 0.123860602f);
     return r * t * bell;
 }
 
@@ -154,8 +171,7 @@ __device__ __forceinline__ void activate(int a, float (&v)[N]) {
         if (a == RELU) v[i] = z < 0.f ? 0.f : z;
         else if (a == GELU) {
             float bell;
-            const float tail = normal_tail(z, bell);
-            v[i] = z * (z < 0.f ? tail : 1.f - tail);
+            v[i] = __builtin_fmaf(-fabsf(z), normal_tail(z, bell), fmaxf(z, 0.f));
         }
         else if (a == GELU_TANH) v[i] = z * sigmoid(gelu_tanh_argument(z));
         else v[i] = z * sigmoid(z);

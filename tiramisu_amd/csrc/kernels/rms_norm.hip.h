@@ -5,7 +5,7 @@
 // Each input is read once and each output written once: a row stays in the registers of its team (64, 256 or 1024 threads, PER
 // pieces of 16 bytes of the widest input each), which reduces it by lane exchanges and, where it is more than a wavefront, through LDS.  The norm
 // is of the unrounded sum.  Rows too long for that are read a second time.
-// Sums of the backward pass over rows are kept per team in registers, written once, and added by a second launch in a fixed
+// Sums of the backward pass over rows are kept per team in registers, written once a workgroup, and added by a second launch in a fixed
 // order: results do not depend on the order of workgroups.
 #ifndef TIRAMISU_AMD_RMS_NORM_HIP_H
 #define TIRAMISU_AMD_RMS_NORM_HIP_H
@@ -88,15 +88,11 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void rms_norm_kernel(norm_
     auto finish = [&](int p, float (&v)[N], float factor) {  // v: s; becomes y
         const long c = ((long)p * TEAM + t) * N;
         const int n = (int)min((long)N, a.columns - c);
-        if (n <= 0) {
-#pragma unroll
-            for (int i = 0; i < N; i++) v[i] = 0.f;
-            return;
-        }
+        if (!w || n <= 0) return;                            // (what lies behind the row is zero)
         float g[N];
-        if (w) load_some<E>(w + c, n, g);
+        load_some<E>(w + c, n, g);
 #pragma unroll
-        for (int i = 0; i < N; i++) v[i] = w ? v[i] * factor * g[i] : v[i];
+        for (int i = 0; i < N; i++) v[i] = v[i] * factor * g[i];
     };
     auto write_sum = [&](int p, float (&v)[N]) {
         const long c = ((long)p * TEAM + t) * N;
@@ -184,84 +180,102 @@ struct norm_backward_arguments {
     const void *dy, *sum, *weight, *dsum;   // dsum: may be null
     const float *rstd;
     void *dx;
-    float *partial;                         // [teams][columns]
+    float *partial;                         // [workgroups][columns]
     long rows, columns, ldy, lds, ldd;
-    int teams;
+    int parts;                              // (rows that no team holds: of the walk down the columns)
 };
 
-// Teams walk over the rows, team g taking rows g, g + teams, ...
+// Teams walk over the rows, team g taking rows g, g + teams, ....  Teams of one wavefront need no barrier on the way, and the eight of a workgroup add their
+// columns' sums in LDS before they are written (8192 x 2048 bf16: workgroups of one team of 256 threads, a barrier a row, 44.5 us).
 template <int E, int TEAM, int PER>
-__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void rms_norm_backward_kernel(norm_backward_arguments a) {
+constexpr int norm_backward_threads = TEAM == 64 ? 512 : TEAM;
+template <int E, int TEAM, int PER>
+__global__ __launch_bounds__((norm_backward_threads<E, TEAM, PER>)) void rms_norm_backward_kernel(norm_backward_arguments a) {
     constexpr int N = E == F32 ? 4 : 8;
-    constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+    constexpr int TEAMS = norm_backward_threads<E, TEAM, PER> / TEAM;
     __shared__ float slots[2][TEAM > 64 ? TEAM / 64 : 1];
     typedef stored<E> T;
     const int t = threadIdx.x % TEAM;
-    const long team = (long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
-    if (TEAMS > 1 && team >= a.teams) return;
+    const long team = (long)blockIdx.x * TEAMS + threadIdx.x / TEAM, teams = (long)gridDim.x * TEAMS;
     float dw[PER][N];
 #pragma unroll
     for (int p = 0; p < PER; p++)
 #pragma unroll
         for (int i = 0; i < N; i++) dw[p][i] = 0.f;
+    // (pieces stay as they are in memory, a quarter or half of what they are as fp32, so that more rows are on their way in a compute unit)
+    auto read = [&](const T *from, int p) {
+        const long c = ((long)p * TEAM + t) * N;
+        return load_guarded<sizeof(T)>((const char *)(from + c), (a.columns - c) * (long)sizeof(T));
+    };
+    u32x4 weights[PER];
+#pragma unroll
+    for (int p = 0; p < PER; p++) weights[p] = read((const T *)a.weight, p);
     int turn = 0;
-    for (long row = team; row < a.rows; row += a.teams, turn ^= 1) {
-        const T *dy = (const T *)a.dy + row * a.ldy, *s = (const T *)a.sum + row * a.lds, *w = (const T *)a.weight;
+    for (long row = team; row < a.rows; row += teams, turn ^= 1) {
+        const T *dy = (const T *)a.dy + row * a.ldy, *s = (const T *)a.sum + row * a.lds, *ds = a.dsum ? (const T *)a.dsum + row * a.ldd : nullptr;
         const float rstd = a.rstd[row];
-        float xhat[PER][N], g[PER][N];
+        u32x4 held_s[PER], held_dy[PER], held_ds[PER];
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            held_s[p] = read(s, p);
+            held_dy[p] = read(dy, p);
+        }
+#pragma unroll
+        for (int p = 0; p < PER; p++) held_ds[p] = ds ? read(ds, p) : u32x4{0, 0, 0, 0};
         float dot = 0.f;
 #pragma unroll
         for (int p = 0; p < PER; p++) {
-            const long c = ((long)p * TEAM + t) * N;
-            const int n = (int)min((long)N, a.columns - c);
-#pragma unroll
-            for (int i = 0; i < N; i++) xhat[p][i] = g[p][i] = 0.f;
-            if (n > 0) {
-                load_some<E>(s + c, n, xhat[p]);
-                load_some<E>(dy + c, n, g[p]);
-            }
-        }
-#pragma unroll
-        for (int p = 0; p < PER; p++) {
-            const long c = ((long)p * TEAM + t) * N;
-            const int n = (int)min((long)N, a.columns - c);
-            float f[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) f[i] = 0.f;
-            if (n > 0) load_some<E>(w + c, n, f);
+            float x[N], g[N], f[N];
+            widen<E>(held_s[p], x);
+            widen<E>(held_dy[p], g);
+            widen<E>(weights[p], f);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                xhat[p][i] *= rstd;
-                dw[p][i] += g[p][i] * xhat[p][i];
-                g[p][i] *= f[i];
-                dot += g[p][i] * xhat[p][i];
+                x[i] *= rstd;
+                dw[p][i] += g[i] * x[i];
+                dot += g[i] * f[i] * x[i];
             }
         }
         dot = team_reduce<TEAM, false>(dot, slots[turn]) / (float)a.columns;
         T *dx = (T *)a.dx + row * a.columns;
-        const T *ds = a.dsum ? (const T *)a.dsum + row * a.ldd : nullptr;
 #pragma unroll
         for (int p = 0; p < PER; p++) {
             const long c = ((long)p * TEAM + t) * N;
             const int n = (int)min((long)N, a.columns - c);
             if (n <= 0) continue;
-            float v[N];
+            float x[N], g[N], f[N], d[N];
+            widen<E>(held_s[p], x);
+            widen<E>(held_dy[p], g);
+            widen<E>(weights[p], f);
+            widen<E>(held_ds[p], d);
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = rstd * (g[p][i] - xhat[p][i] * dot);
-            if (ds) {
-                float d[N];
-                load_some<E>(ds + c, n, d);
-#pragma unroll
-                for (int i = 0; i < N; i++) v[i] += d[i];
-            }
-            store_some<E>(dx + c, n, v);
+            for (int i = 0; i < N; i++) d[i] += rstd * (g[i] * f[i] - x[i] * rstd * dot);
+            store_some<E>(dx + c, n, d);
         }
+    }
+    if constexpr (TEAMS > 1) {
+        // one wavefront after the other, in order
+        __shared__ float sums[PER][N][64];
+        const int wave = threadIdx.x / 64;
+        for (int turn_of = 0; turn_of < TEAMS; turn_of++) {
+            if (wave == turn_of) {
+#pragma unroll
+                for (int p = 0; p < PER; p++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        if (turn_of > 0) dw[p][i] += sums[p][i][t];
+                        if (turn_of < TEAMS - 1) sums[p][i][t] = dw[p][i];
+                    }
+            }
+            __syncthreads();
+        }
+        if (wave != TEAMS - 1) return;
     }
 #pragma unroll
     for (int p = 0; p < PER; p++) {
         const long c = ((long)p * TEAM + t) * N;
         const int n = (int)min((long)N, a.columns - c);
-        if (n > 0) store_some<F32>(a.partial + team * a.columns + c, n, dw[p]);
+        if (n > 0) store_some<F32>(a.partial + (long)blockIdx.x * a.columns + c, n, dw[p]);
     }
 }
 
@@ -289,7 +303,7 @@ __global__ __launch_bounds__(256) void rms_norm_backward_long_columns_kernel(nor
     const long c = (long)blockIdx.x * 256 + threadIdx.x;
     if (c >= a.columns) return;
     float sum = 0.f;
-    for (long row = blockIdx.y; row < a.rows; row += a.teams)
+    for (long row = blockIdx.y; row < a.rows; row += a.parts)
         sum += (float)((const T *)a.dy)[row * a.ldy + c] * ((float)((const T *)a.sum)[row * a.lds + c] * a.rstd[row]);
     a.partial[(long)blockIdx.y * a.columns + c] = sum;
 }

@@ -78,10 +78,10 @@ constexpr tile_model TILES_8_BITS[] = {{TILE_256, 256, 256, 13.8, 0.8, 0.6, 9.0,
                                        {TILE_128, 128, 128, 7.0, 0.26, 0.24, 4.7, 0.467}, {TILE_64, 64, 64, 4.8, 0.13, 0.02, 0.7, 0.19}};
 // (a gated layer's smallest tile is 64 x 128: 64 columns of gate and the same of up)
 constexpr tile_model GATED_64_16_BITS = {TILE_64, 64, 128, 3.9, 0.27, 0.08, 0.7, 0.31}, GATED_64_8_BITS = {TILE_64, 64, 128, 5.4, 0.13, 0.05, 0.7, 0.3};
-struct tile_plan { product_tile tile; int splits, slices; };
+struct tile_plan { product_tile tile; int splits, slices; double cost; };
 tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
     const long slices = std::max(1L, (K * bytes + 127) / 128);
-    tile_plan best = {TILE_64, 0, 0};
+    tile_plan best = {TILE_64, 0, 0, 0.0};
     double best_cost = 0;
     auto consider = [&](const tile_model &t) {
         const long tiles = ((M + t.rows - 1) / t.rows) * ((N * (gated ? 2 : 1) + t.columns - 1) / t.columns);
@@ -91,13 +91,46 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
             const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
             double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
             if (splits > 1) cost += 3.0 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 4e6;
-            if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each}; best_cost = cost; }
+            if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each, cost}; best_cost = cost; }
         }
     };
     for (const tile_model &t : TILES_16_BITS)
         if (bytes == 2) consider(gated && t.tile == TILE_64 ? GATED_64_16_BITS : t);
     for (const tile_model &t : TILES_8_BITS)
         if (bytes == 1) consider(gated && t.tile == TILE_64 ? GATED_64_8_BITS : t);
+    return best;
+}
+
+// Both gradients in one launch: tiles of the longer product first, then those of the other on compute units as they become free.  Modelled from the
+// same figures, against the two launches one after the other (about 2 us more than their sum).
+struct pair_plan { product_tile tile; bool together, q_first; };
+pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
+    pair_plan best = {TILE_64, false, false};
+    double best_cost = plan_for(M, N, K, 2, false).cost + plan_for(M2, N2, K2, 2, false).cost + 2.0;
+    for (const tile_model &t : TILES_16_BITS) {
+        auto tiles_of = [&](long m, long n) { return ((m + t.rows - 1) / t.rows) * ((n + t.columns - 1) / t.columns); };
+        const long units = ttarget::COMPUTE_UNITS, tiles[2] = {tiles_of(M, N), tiles_of(M2, N2)};
+        const double busy = std::min(1.0, (double)(tiles[0] + tiles[1]) / units);
+        double each[2];
+        for (int i = 0; i < 2; i++) each[i] = (double)(((i ? K2 : K) + 63) / 64) * (t.first + busy * t.full) + t.round;
+        const int a = each[0] >= each[1] ? 0 : 1, b = 1 - a;
+        // whole rounds of the first kind, its last tiles, and how many of the second are done when
+        const long rounds = tiles[a] / units, last = tiles[a] % units;
+        const double free_at[2] = {rounds * each[a], (rounds + (last > 0)) * each[a]};
+        double done = free_at[1];
+        for (long k = 0;; k++) {
+            // the earliest time at which the compute units free from either moment have finished all of the second
+            const double when[2] = {free_at[0] + k * each[b], free_at[1] + k * each[b]};
+            bool enough = false;
+            for (double w : when) {
+                const long finished = (units - last) * (long)((w - free_at[0]) / each[b] + 1e-6) + last * (w < free_at[1] ? 0 : (long)((w - free_at[1]) / each[b] + 1e-6));
+                if (finished >= tiles[b]) { done = std::max(free_at[1], w); enough = true; break; }
+            }
+            if (enough) break;
+        }
+        const double cost = t.fixed + done;
+        if (cost < best_cost) { best = {t.tile, true, a == 1}; best_cost = cost; }
+    }
     return best;
 }
 
@@ -120,6 +153,19 @@ int launch_product(const char *fn, int type, product_layout layout, int epilogue
         check(hipGetLastError(), fn);
     }
     return 0;
+}
+
+// p: gradient of the input, q: of the weights; what is not asked for has no place for its result
+int launch_gradients(const char *fn, int type, const product_arguments &p, const product_arguments &q) {
+    const bool both = p.y && q.y && p.M && p.N && q.M && q.N;
+    const pair_plan plan = both ? plan_for_pair(p.M, p.N, p.a_more ? 2L * p.K : p.K, q.M, q.N, q.K) : pair_plan();
+    if (both && plan.together) {
+        (type == BF16 ? launch_gradients_BF16 : launch_gradients_F16)(plan.tile, plan.q_first, p, q, stream());
+        return 0;
+    }
+    if (p.y)
+        if (const int rc = launch_product(fn, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
+    return q.y ? launch_product(fn, type, WEIGHT_GRADIENT, LINEAR, type, q) : 0;
 }
 
 // Rows of x for which the weights are streamed through registers (linear_few_tokens.hip.h).
@@ -172,6 +218,7 @@ void launch_norm(const char *fn, const norm_arguments &a) {
     auto go = [&](auto kernel, int threads, int rows) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((a.rows + rows - 1) / rows)), dim3(threads), 0, stream(), a);
     };
+    // (A wavefront to a row of up to 256 pieces, without a barrier, is no faster: 2000 x 1430 float16 10.5 us, with 256 threads 9.2.)
     if (pieces <= 64) go(rms_norm_kernel<E, Y, 64, 1, true>, 256, 4);
     else if (pieces <= 256) go(rms_norm_kernel<E, Y, 256, 1, true>, 256, 1);
     else if (pieces <= 512) go(rms_norm_kernel<E, Y, 256, 2, true>, 256, 1);
@@ -198,25 +245,27 @@ template <int E>
 void launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweight) {
     constexpr int N = E == F32 ? 4 : 8;
     const long pieces = (a.columns + N - 1) / N;
-    // teams: enough for every compute unit, few enough that their sums are little beside the rows
-    auto go = [&](auto kernel, int threads, int teams_each) {
-        a.teams = (int)std::max(1L, std::min(a.rows, 512L * teams_each));
-        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.teams * a.columns * 4);
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.teams + teams_each - 1) / teams_each)), dim3(threads), 0, stream(), a);
+    // workgroups: enough to cover the way to memory, few enough that their sums are little beside the rows
+    auto go = [&](auto kernel, int threads, int teams, long most) {
+        a.parts = (int)std::max(1L, std::min((a.rows + teams - 1) / teams, most));
+        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.parts * a.columns * 4);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)a.parts), dim3(threads), 0, stream(), a);
     };
-    if (pieces <= 64) go(rms_norm_backward_kernel<E, 64, 1>, 256, 4);
-    else if (pieces <= 256) go(rms_norm_backward_kernel<E, 256, 1>, 256, 1);
-    else if (pieces <= 512) go(rms_norm_backward_kernel<E, 256, 2>, 256, 1);
-    else if (pieces <= 1024) go(rms_norm_backward_kernel<E, 256, 4>, 256, 1);
-    else if (pieces <= 4096) go(rms_norm_backward_kernel<E, 1024, 4>, 1024, 1);
+    if (pieces <= 64) go(rms_norm_backward_kernel<E, 64, 1>, 512, 8, 512);
+    else if (pieces <= 128) go(rms_norm_backward_kernel<E, 64, 2>, 512, 8, 512);
+    else if (pieces <= 192) go(rms_norm_backward_kernel<E, 64, 3>, 512, 8, 512);
+    else if (pieces <= 256) go(rms_norm_backward_kernel<E, 64, 4>, 512, 8, 512);
+    else if (pieces <= 512) go(rms_norm_backward_kernel<E, 256, 2>, 256, 1, 768);
+    else if (pieces <= 1024) go(rms_norm_backward_kernel<E, 256, 4>, 256, 1, 512);
+    else if (pieces <= 2048) go(rms_norm_backward_kernel<E, 512, 4>, 512, 1, 256);
     else {
-        a.teams = (int)std::max(1L, std::min(a.rows, 64L));
-        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.teams * a.columns * 4);
+        a.parts = (int)std::max(1L, std::min(a.rows, 64L));
+        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.parts * a.columns * 4);
         if (a.rows > 0) hipLaunchKernelGGL(rms_norm_backward_long_rows_kernel<E>, dim3((unsigned)a.rows), dim3(1024), 0, stream(), a);
-        hipLaunchKernelGGL(rms_norm_backward_long_columns_kernel<E>, dim3((unsigned)((a.columns + 255) / 256), (unsigned)a.teams), dim3(256), 0, stream(), a);
+        hipLaunchKernelGGL(rms_norm_backward_long_columns_kernel<E>, dim3((unsigned)((a.columns + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream(), a);
     }
     check(hipGetLastError(), fn);
-    sum_parts<E>(fn, a.partial, a.teams, a.columns, dweight);
+    sum_parts<E>(fn, a.partial, a.parts, a.columns, dweight);
 }
 
 // dz and the bias's gradient; what is null is not computed
@@ -373,27 +422,22 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
         else launch_activation_backward<BF16>(__FUNCTION__, a, dbias);
     }
     if (!loadable(dz, 2, true) || !loadable(dz, 2, false)) dz = moved_where_needed({dz.p, dz.ld}, m, n, 2, true, GRADIENT);
+    product_arguments p = product_of(m, k, n), q = product_of(n, k, m);
+    p.a = q.a = dz.p;
+    p.lda = q.lda = dz.ld;
+    p.y = dx;
+    q.y = dweight;
     if (dx) {
-        product_arguments p = product_of(m, k, n);
-        p.a = dz.p;
-        p.lda = dz.ld;
         const operand w = moved_where_needed({weight, ldw ? (long)ldw : k}, n, k, 2, false, MOVED_B);
         p.b = w.p;
         p.ldb = w.ld;
-        p.y = dx;
-        if (const int rc = launch_product(__FUNCTION__, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
     }
     if (dweight) {
-        product_arguments p = product_of(n, k, m);
-        p.a = dz.p;
-        p.lda = dz.ld;
         const operand xs = moved_where_needed({x, ldx ? (long)ldx : k}, m, k, 2, false, MOVED_A);
-        p.b = xs.p;
-        p.ldb = xs.ld;
-        p.y = dweight;
-        if (const int rc = launch_product(__FUNCTION__, type, WEIGHT_GRADIENT, LINEAR, type, p)) return rc;
+        q.b = xs.p;
+        q.ldb = xs.ld;
     }
-    return 0;
+    return launch_gradients(__FUNCTION__, type, p, q);
 }
 
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate, const void *up,
@@ -416,35 +460,30 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
         else hipLaunchKernelGGL(gated_backward_kernel<BF16>, dim3(blocks), dim3(256), 0, stream(), a);
         check(hipGetLastError(), __FUNCTION__);
     }
+    product_arguments p = product_of(m, k, n), q = product_of(half + n, k, m);
+    p.a = q.a = d;
+    p.lda = q.lda = ld;
     if (dx) {
-        operand g = moved_where_needed({gate_weight, ldg ? (long)ldg : k}, n, k, 2, false, MOVED_B);
-        operand u = moved_where_needed({up_weight, ldu ? (long)ldu : k}, n, k, 2, false, MOVED_C);
-        product_arguments p = product_of(m, k, n);
-        p.a = d;
+        const operand g = moved_where_needed({gate_weight, ldg ? (long)ldg : k}, n, k, 2, false, MOVED_B);
+        const operand u = moved_where_needed({up_weight, ldu ? (long)ldu : k}, n, k, 2, false, MOVED_C);
         p.a_more = d + 2 * half;
-        p.lda = ld;
         p.b = g.p;
         p.ldb = g.ld;
         p.b_more = u.p;
         p.ldb_more = u.ld;
         p.y = dx;
-        if (const int rc = launch_product(__FUNCTION__, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
     }
     if (dgate_weight && n > 0) {
         // rows of the product: those of gate, up to `half` nothing, those of up
-        product_arguments p = product_of(half + n, k, m);
-        p.a = d;
-        p.lda = ld;
         const operand xs = moved_where_needed({x, ldx ? (long)ldx : k}, m, k, 2, false, MOVED_A);
-        p.b = xs.p;
-        p.ldb = xs.ld;
-        p.y = dgate_weight;
-        p.y_below = dup_weight;
-        p.rows_above = (int)n;
-        p.split_row = (int)half;
-        if (const int rc = launch_product(__FUNCTION__, type, WEIGHT_GRADIENT, LINEAR, type, p)) return rc;
+        q.b = xs.p;
+        q.ldb = xs.ld;
+        q.y = dgate_weight;
+        q.y_below = dup_weight;
+        q.rows_above = (int)n;
+        q.split_row = (int)half;
     }
-    return 0;
+    return launch_gradients(__FUNCTION__, type, p, q);
 }
 
 // Each argument in eight bytes, as tiramisu_hip_operator takes them
