@@ -385,10 +385,10 @@ __device__ __forceinline__ void store_linear(const product_arguments &p, const f
 }
 template <int Y>
 __device__ __forceinline__ void finish_linear(const product_arguments &p, const column_terms &c, float (&z)[8], long m, long n, int some) {
+    float r[8];
+    if (p.residual) load_residual<Y>(p, r, m, n, some);
     activate_linear<Y>(p, c, z, m, n, some);
     if (p.residual) {
-        float r[8];
-        load_residual<Y>(p, r, m, n, some);
 #pragma unroll
         for (int i = 0; i < 8; i++) z[i] += r[i];
     }
@@ -473,11 +473,11 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
 #pragma unroll
             for (int e = 0; e < 4; e++) { v[e] = a[e]; v[4 + e] = b[e]; }
         };
-        // the residual's pieces are on their way while the strip is turned
+        // the residual's pieces are on their way while the strip is turned, where nothing else is to be done
         constexpr bool RESIDUAL = C::EPILOGUE == LINEAR && C::A_ROWS && C::B_ROWS;
         float r[RESIDUAL ? PASSES : 1][8];
         if constexpr (RESIDUAL)
-            if (p.residual && !p.partial) {
+            if (p.residual && !p.partial && !(p.a_scale || p.bias || p.pre || p.activation != NONE)) {
 #pragma unroll
                 for (int pass = 0; pass < PASSES; pass++)
                     if (across && first + pass * DOWN < p.M) load_residual<Y>(p, r[pass], first + pass * DOWN, n, some);
@@ -515,31 +515,30 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
                 if (across && first + pass * DOWN < p.M) finish_gated<Y>(p, columns, z, u, first + pass * DOWN, n, some);
             }
         } else {
-            // what takes many instructions is a loop that is not unrolled, in place; then the results
-            if constexpr (RESIDUAL)
-                if (p.a_scale || p.bias || p.pre || p.activation != NONE) {
-#pragma unroll 1
-                    for (int pass = 0; pass < PASSES; pass++) {
-                        if (!across || first + pass * DOWN >= p.M) continue;
-                        float z[8];
-                        take(pass, c0, z);
-                        activate_linear<Y>(p, columns, z, first + pass * DOWN, n, some);
-                        lds_f32x4 *const back = (lds_f32x4 *)(strip + (pass * DOWN + r0) * C::STRIP + c0);
-                        back[0] = f32x4{z[0], z[1], z[2], z[3]};
-                        back[1] = f32x4{z[4], z[5], z[6], z[7]};
-                    }
+            bool plain = true;
+            if constexpr (RESIDUAL) plain = !(p.a_scale || p.bias || p.pre || p.activation != NONE);
+            if (plain) {
+#pragma unroll
+                for (int pass = 0; pass < PASSES; pass++) {
+                    if (!across || first + pass * DOWN >= p.M) continue;
+                    float z[8];
+                    take(pass, c0, z);
+                    if constexpr (RESIDUAL)
+                        if (p.residual) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) z[e] += r[pass][e];
+                        }
+                    store_linear<Y>(p, z, first + pass * DOWN, n, some);
                 }
-#pragma unroll
-            for (int pass = 0; pass < PASSES; pass++) {
-                if (!across || first + pass * DOWN >= p.M) continue;
-                float z[8];
-                take(pass, c0, z);
-                if constexpr (RESIDUAL)
-                    if (p.residual) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) z[e] += r[pass][e];
-                    }
-                store_linear<Y>(p, z, first + pass * DOWN, n, some);
+            } else {
+                // (many instructions: not unrolled)
+#pragma unroll 1
+                for (int pass = 0; pass < PASSES; pass++) {
+                    if (!across || first + pass * DOWN >= p.M) continue;
+                    float z[8];
+                    take(pass, c0, z);
+                    finish_linear<Y>(p, columns, z, first + pass * DOWN, n, some);
+                }
             }
         }
         order_lanes();

@@ -216,6 +216,8 @@ __global__ __launch_bounds__((norm_backward_threads<E, TEAM, PER>)) void rms_nor
         const float rstd = a.rstd[row];
         u32x4 held_s[PER], held_dy[PER], held_ds[PER];
 #pragma unroll
+        for (int p = 0; p < PER; p++) asm volatile("" : "+v"(weights[p]));     // (not kept as fp32 from row to row: 32 registers more)
+#pragma unroll
         for (int p = 0; p < PER; p++) {
             held_s[p] = read(s, p);
             held_dy[p] = read(dy, p);

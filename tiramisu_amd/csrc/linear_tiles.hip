@@ -46,13 +46,14 @@ void launch_pair(const product_arguments &p, const product_arguments &q, hipStre
 
 // Wavefronts, stages and matrix instructions of each tile.  Of those measured, the fastest for the launches that choose the tile; us for bf16 with 2 x 2
 // wavefronts and 32 x 32 blocks / as here: 256 x 256 (4096^3) 117 / 102 (4 x 2: 133, registers spilled); 256 x 128 (4096^3) 123 / 115; 128 x 128 in
-// one round (4096 x 1024 x 4096) 43 with two stages, 37.4 with four / 35.1; 64 x 64 (1024^3) 7.7 / 7.0.  8 bits: 256 x 256 (4096^3) 68 / 62, where 16 x 16 blocks
+// one round (4096 x 1024 x 4096) 43 with two stages, 37.4 with four / 35.1; 64 x 64 (1024^3) 7.7 / 7.0;
+// gated 64 x 128 (e4m3, 1000 x 1500 x 700) with 2 x 2 wavefronts 12.2, with 2 x 4 10.3.  8 bits: 256 x 256 (4096^3) 68 / 62, where 16 x 16 blocks
 // do not leave registers for two sets of fragments (150); 256 x 128 74 / 67; 128 x 128 (4096 x 1024 x 4096) 26 / 23; 64 x 64 (512 x 2048 x 2048) 8.2 / 7.0.
 template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
     typedef tile_config<E, 256, 256, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, E == F8 ? 32 : 16> tile_256;
     typedef tile_config<E, 256, 128, 4, 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_256x128;
     typedef tile_config<E, 128, 128, 4, 2, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128;
-    typedef tile_config<E, 64, EPILOGUE == GATED ? 128 : 64, 2, 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
+    typedef tile_config<E, 64, EPILOGUE == GATED ? 128 : 64, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
 };
 template <int E, int Y, bool A_ROWS, bool B_ROWS, int EPILOGUE>
 void launch_tile(product_tile tile, const product_arguments &p, int splits, hipStream_t stream) {

@@ -87,6 +87,7 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
         const long tiles = ((M + t.rows - 1) / t.rows) * ((N * (gated ? 2 : 1) + t.columns - 1) / t.columns);
         for (long splits = 1; splits <= 16 && splits <= slices; splits++) {
             const long each = (slices + splits - 1) / splits;
+            if (splits > 1 && tiles * splits > 2 * ttarget::COMPUTE_UNITS) break;
             if ((slices + each - 1) / each != splits) continue;            // (the same slices to each as with fewer)
             const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
             double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
@@ -117,17 +118,17 @@ pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
         // whole rounds of the first kind, its last tiles, and how many of the second are done when
         const long rounds = tiles[a] / units, last = tiles[a] % units;
         const double free_at[2] = {rounds * each[a], (rounds + (last > 0)) * each[a]};
-        double done = free_at[1];
-        for (long k = 0;; k++) {
-            // the earliest time at which the compute units free from either moment have finished all of the second
-            const double when[2] = {free_at[0] + k * each[b], free_at[1] + k * each[b]};
-            bool enough = false;
-            for (double w : when) {
-                const long finished = (units - last) * (long)((w - free_at[0]) / each[b] + 1e-6) + last * (w < free_at[1] ? 0 : (long)((w - free_at[1]) / each[b] + 1e-6));
-                if (finished >= tiles[b]) { done = std::max(free_at[1], w); enough = true; break; }
+        // the earliest moment, a whole number of the second kind's tiles behind either, at which all of them are finished
+        double done = 0;
+        for (int from = 0; from < 2; from++)
+            for (long k = 0;; k++) {
+                const double when = free_at[from] + k * each[b];
+                const auto finished_since = [&](double begin) { return when < begin ? 0L : (long)((when - begin) / each[b] + 1e-6); };
+                if ((units - last) * finished_since(free_at[0]) + last * finished_since(free_at[1]) < tiles[b]) continue;
+                done = from == 0 ? when : std::min(done, when);
+                break;
             }
-            if (enough) break;
-        }
+        done = std::max(done, free_at[1]);
         const double cost = t.fixed + done;
         if (cost < best_cost) { best = {t.tile, true, a == 1}; best_cost = cost; }
     }
@@ -253,8 +254,8 @@ void launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweig
     };
     if (pieces <= 64) go(rms_norm_backward_kernel<E, 64, 1>, 512, 8, 512);
     else if (pieces <= 128) go(rms_norm_backward_kernel<E, 64, 2>, 512, 8, 512);
-    else if (pieces <= 192) go(rms_norm_backward_kernel<E, 64, 3>, 512, 8, 512);
-    else if (pieces <= 256) go(rms_norm_backward_kernel<E, 64, 4>, 512, 8, 512);
+    else if (pieces <= 192) go(rms_norm_backward_kernel<E, 64, 3>, 512, 8, 256);
+    else if (pieces <= 256) go(rms_norm_backward_kernel<E, 64, 4>, 512, 8, 256);
     else if (pieces <= 512) go(rms_norm_backward_kernel<E, 256, 2>, 256, 1, 768);
     else if (pieces <= 1024) go(rms_norm_backward_kernel<E, 256, 4>, 256, 1, 512);
     else if (pieces <= 2048) go(rms_norm_backward_kernel<E, 512, 4>, 512, 1, 256);
