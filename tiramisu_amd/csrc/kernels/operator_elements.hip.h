@@ -162,19 +162,29 @@ __device__ __forceinline__ float normal_tail(float z, float &bell) {
     return r * t * bell;
 }
 
+__device__ __forceinline__ float activated(int a, float z) {
+    if (a == RELU) return z < 0.f ? 0.f : z;
+    if (a == GELU) {
+        float bell;
+        return __builtin_fmaf(-fabsf(z), normal_tail(z, bell), fmaxf(z, 0.f));
+    }
+    return z * sigmoid(a == GELU_TANH ? gelu_tanh_argument(z) : z);
+}
+// (the choice is made once for all elements, whose instructions then cover each other)
 template <int N>
 __device__ __forceinline__ void activate(int a, float (&v)[N]) {
-    if (a == NONE) return;
+    if (a == GELU) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float z = v[i];
-        if (a == RELU) v[i] = z < 0.f ? 0.f : z;
-        else if (a == GELU) {
-            float bell;
-            v[i] = __builtin_fmaf(-fabsf(z), normal_tail(z, bell), fmaxf(z, 0.f));
-        }
-        else if (a == GELU_TANH) v[i] = z * sigmoid(gelu_tanh_argument(z));
-        else v[i] = z * sigmoid(z);
+        for (int i = 0; i < N; i++) v[i] = activated(GELU, v[i]);
+    } else if (a == SILU) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = activated(SILU, v[i]);
+    } else if (a == GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = activated(GELU_TANH, v[i]);
+    } else if (a == RELU) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = activated(RELU, v[i]);
     }
 }
 
