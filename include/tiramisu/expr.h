@@ -209,6 +209,20 @@ expr cublas_gemm(const buffer &A, const buffer &B, buffer &C, expr M, expr N, ex
                  expr offsetA = expr(), expr offsetB = expr(), expr offsetC = expr(),
                  expr transposeA = expr(), expr transposeB = expr());
 
+/** Operators of a transformer's feed-forward sublayer as library calls on GPU buffers (this back-end's own; tiramisu_hip_wrappers.h
+  * says what they compute), used like cublas_gemm.  All buffers of a call hold one type: p_bfloat16 (rms_norm also p_float32), rows dense.
+  * A call that the runtime refuses ends the process. */
+enum class hip_activation { none = 0, relu = 1, gelu = 2, gelu_tanh = 3, silu = 4 };
+/** y = s / sqrt(mean(s^2) + eps) * weight of each row, s = x + residual where a residual is given, stored in \p sum then. */
+expr hip_rms_norm(const buffer &x, const buffer &weight, buffer &y, expr rows, expr columns, float eps = 1e-6f,
+                  const buffer *residual = nullptr, buffer *sum = nullptr);
+/** y = activation(x weight^T + bias) + residual; x is M x K, weight N x K, y and residual M x N. */
+expr hip_linear(const buffer &x, const buffer &weight, buffer &y, expr M, expr N, expr K,
+                hip_activation activation = hip_activation::none, const buffer *bias = nullptr, const buffer *residual = nullptr);
+/** h = activation(x gate_weight^T) * (x up_weight^T); both weights N x K. */
+expr hip_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, buffer &h, expr M, expr N, expr K,
+                      hip_activation activation = hip_activation::silu);
+
 std::string str_from_tiramisu_type_expr(expr_t t);
 std::string str_tiramisu_type_op(op_t o);
 

@@ -218,6 +218,10 @@ enum tiramisu_hip_operator_t {
     TIRAMISU_HIP_OPERATOR_GATED_LINEAR_BACKWARD = 6
 };
 int tiramisu_hip_operator(int32_t op, const uint64_t *arguments, void *stream);
+/* For generated code: no buffer in the place of one that may be left out, and what becomes of a refused call there -- the reference's failure
+ * model, the process ends with status 1 behind the operator's message. */
+float *tiramisu_hip_no_buffer(void);
+int tiramisu_hip_require(int32_t status);
 
 /* ---- per-launch timing.  Between profile_start and profile_stop every tiramisu_hip_launch
  *      (and GEMM library call), from any thread, is bracketed by two events on its current

@@ -401,4 +401,43 @@ expr cublas_gemm(const buffer &A, const buffer &B, buffer &C, expr M, expr N, ex
                 p_int32);
 }
 
+// ---- operators of the runtime
+namespace {
+
+expr u64_of(expr e) { return cast(p_uint64, e); }
+expr buffer_argument(const buffer *b) { return b ? expr(o_buffer, b->get_name()) : expr(o_call, "tiramisu_hip_no_buffer", {}, p_uint64); }
+expr element_of(const char *op, const buffer &like, std::initializer_list<const buffer *> others, bool with_float) {
+    const primitive_t t = like.get_elements_type();
+    if (t != p_bfloat16 && !(with_float && t == p_float32))
+        ERROR(std::string(op) + ": buffer " + like.get_name() + " holds " + str_from_tiramisu_type_primitive(t), true);
+    for (const buffer *b : others)
+        if (b && b->get_elements_type() != t) ERROR(std::string(op) + ": buffers " + like.get_name() + " and " + b->get_name() + " hold different types", true);
+    return expr((int32_t)(t == p_bfloat16 ? 2 : 0));
+}
+expr operator_call(const std::string &name, std::vector<expr> arguments) {
+    return expr(o_call, "tiramisu_hip_require", {expr(o_call, name, arguments, p_int32)}, p_int32);
+}
+
+}  // namespace
+
+expr hip_rms_norm(const buffer &x, const buffer &weight, buffer &y, expr rows, expr columns, float eps, const buffer *residual, buffer *sum) {
+    const expr type = element_of("hip_rms_norm", x, {&weight, &y, residual, sum}, true), dense = expr((uint64_t)0);
+    return operator_call("tiramisu_hip_rms_norm", {buffer_argument(&x), buffer_argument(residual), buffer_argument(&weight), buffer_argument(&y), buffer_argument(sum),
+                                                   buffer_argument(nullptr), buffer_argument(nullptr), u64_of(rows), u64_of(columns), dense, dense, expr(eps), type, type});
+}
+
+expr hip_linear(const buffer &x, const buffer &weight, buffer &y, expr M, expr N, expr K, hip_activation activation, const buffer *bias, const buffer *residual) {
+    const expr type = element_of("hip_linear", x, {&weight, &y, bias, residual}, false), dense = expr((uint64_t)0);
+    return operator_call("tiramisu_hip_linear", {buffer_argument(&x), buffer_argument(&weight), buffer_argument(bias), buffer_argument(residual), buffer_argument(nullptr),
+                                                 buffer_argument(nullptr), buffer_argument(&y), buffer_argument(nullptr), u64_of(M), u64_of(N), u64_of(K), dense, dense, dense,
+                                                 expr((int32_t)activation), type, type});
+}
+
+expr hip_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, buffer &h, expr M, expr N, expr K, hip_activation activation) {
+    const expr type = element_of("hip_gated_linear", x, {&gate_weight, &up_weight, &h}, false), dense = expr((uint64_t)0);
+    return operator_call("tiramisu_hip_gated_linear", {buffer_argument(&x), buffer_argument(&gate_weight), buffer_argument(&up_weight), buffer_argument(nullptr),
+                                                       buffer_argument(nullptr), buffer_argument(nullptr), buffer_argument(&h), buffer_argument(nullptr), buffer_argument(nullptr),
+                                                       u64_of(M), u64_of(N), u64_of(K), dense, dense, dense, expr((int32_t)activation), type, type});
+}
+
 }  // namespace tiramisu

@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <cstdlib>
 
 #include "../../include/tiramisu_hip_wrappers.h"
 #include "kernels/linear_few_tokens.hip.h"
@@ -531,6 +532,13 @@ int tiramisu_hip_operator(int32_t op, const uint64_t *arguments, void *stream) {
     }
     tiramisu_hip_set_stream(before);
     return rc;
+}
+
+float *tiramisu_hip_no_buffer(void) { return nullptr; }       // (a pointer that is also one to scales)
+
+int tiramisu_hip_require(int32_t status) {
+    if (status != 0) exit(1);
+    return 0;
 }
 
 }  // extern "C"
