@@ -78,19 +78,17 @@ class GatedLinearGradients(NamedTuple):
 
 # ---------------------------------------------------------------- checks
 
-def _rows(t, name, columns=None, shape=None, dtypes=None):
+def _rows(t, name, shape=None, dtypes=()):
     """(rows, elements from row to row) of a tensor on the GPU whose rows are dense."""
     if not isinstance(t, torch.Tensor):
         raise ValueError("%s is a tensor, not %s" % (name, type(t).__name__))
-    if dtypes is not None and t.dtype not in dtypes:
+    if t.dtype not in dtypes:
         raise ValueError("%s holds %s: %s are taken here" % (name, t.dtype, ", ".join(str(d) for d in dtypes)))
     if t.dim() < 1:
         raise ValueError("%s has no rows" % name)
     if shape is not None and t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, list(t.shape), list(shape)))
     width = t.shape[-1]
-    if columns is not None and width != columns:
-        raise ValueError("%s has rows of %d, not %d" % (name, width, columns))
     if not t.is_cuda:
         raise ValueError("%s lives on %s: operators run on the GPU" % (name, t.device))
     rows = t.numel() // width if width else 0
@@ -162,8 +160,26 @@ def _call(operator, where, *args):
 
 
 def _like(t, dtype):
-    """A new dense tensor of t's shape."""
+    """A new dense tensor of t's shape.  (The fewer arguments, the faster: 0.9 us as it is, 1.1 with both.)"""
+    if dtype is t.dtype and t.is_contiguous():
+        return torch.empty_like(t)
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
+def _new(t, shape, dtype):
+    """A new dense tensor on t's GPU."""
+    return t.new_empty(shape) if dtype is t.dtype else t.new_empty(shape, dtype=dtype)
+
+
+_float = {}                       # a tensor of 32-bit numbers on each GPU, for its new_empty (0.9 us; of another type than the tensor's 1.5)
+
+
+def _row_numbers(t, where):
+    """A new 32-bit number for each row of t."""
+    f = _float.get(where)
+    if f is None:
+        f = _float[where] = t.new_empty(1, dtype=torch.float32)
+    return f.new_empty(t.shape[:-1])
 
 
 def _eight_bit_scales(x, pairs):
@@ -186,8 +202,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6, eight_bit=False, keep_rstd=Fals
         ldr = _rows(residual, "residual", shape=x.shape, dtypes=(x.dtype,))[1]
         r, total = _pointer(residual, "residual", where), _like(x, x.dtype)
     y = _like(x, torch.float8_e4m3fn if eight_bit else x.dtype)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if eight_bit else None
-    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32) if keep_rstd else None
+    scale = _row_numbers(x, where) if eight_bit else None
+    rstd = _row_numbers(x, where) if keep_rstd else None
     _call(_RMS_NORM, where, x.data_ptr(), r, w, y.data_ptr(), 0 if total is None else total.data_ptr(),
           scale.data_ptr() if eight_bit else 0, rstd.data_ptr() if keep_rstd else 0, rows, columns, ldx, ldr, eps, _TYPES[x.dtype], _TYPES[y.dtype])
     return RmsNorm(y, x if total is None else total, scale, rstd)
@@ -216,7 +232,7 @@ def quantize_rows(x):
     precedes the product."""
     rows, ldx = _rows(x, "x", dtypes=_NORM_TYPES)
     q = _like(x, torch.float8_e4m3fn)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    scale = _row_numbers(x, x.get_device())
     _call(_QUANTIZE_ROWS, x.get_device(), x.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, x.shape[-1], ldx, _TYPES[x.dtype])
     return EightBitRows(q, scale)
 
@@ -253,8 +269,8 @@ def linear(x, weight, bias=None, residual=None, activation="none", x_scale=None,
     if k == 0:
         rows = shape[:-1].numel()
     a = _activation(activation)
-    y = x.new_empty(shape, dtype=out)
-    pre = x.new_empty(shape, dtype=out) if keep_pre else None
+    y = _new(x, shape, out)
+    pre = torch.empty_like(y) if keep_pre else None
     _call(_LINEAR, where, x.data_ptr(), _pointer(weight, "weight", where), b, r, xs, ws, y.data_ptr(), pre.data_ptr() if keep_pre else 0,
           rows, n, k, ldx, ldw, ldr, a, _TYPES[x.dtype], _TYPES[out])
     return Linear(y, pre)
@@ -276,8 +292,8 @@ def linear_backward(dy, x, weight, pre=None, activation="none", bias=False):
     if pre is not None:
         ldp = _rows(pre, "pre", shape=shape, dtypes=(x.dtype,))[1]
     dx = _like(x, x.dtype)
-    dweight = x.new_empty((n, k), dtype=x.dtype)
-    dbias = x.new_empty(n, dtype=x.dtype) if bias else None
+    dweight = _like(weight, x.dtype)
+    dbias = x.new_empty(n) if bias else None
     _call(_LINEAR_BACKWARD, where, _pointer(dy, "dy", where), x.data_ptr(), _pointer(weight, "weight", where), 0 if pre is None else _pointer(pre, "pre", where),
           dx.data_ptr(), dweight.data_ptr(), dbias.data_ptr() if bias else 0, rows, n, k, ldy, ldx, ldw, ldp, a, _TYPES[x.dtype])
     return LinearGradients(dx, dweight, dbias)
@@ -300,8 +316,8 @@ def gated_linear(x, gate_weight, up_weight, activation="silu", x_scale=None, gat
     a, shape = _activation(activation), x.shape[:-1] + (n,)
     if k == 0:
         rows = shape[:-1].numel()
-    h = x.new_empty(shape, dtype=out)
-    gate, up = [x.new_empty(shape, dtype=out) for _ in range(2)] if keep_pre else (None, None)
+    h = _new(x, shape, out)
+    gate, up = (torch.empty_like(h), torch.empty_like(h)) if keep_pre else (None, None)
     _call(_GATED_LINEAR, where, x.data_ptr(), _pointer(gate_weight, "gate_weight", where), _pointer(up_weight, "up_weight", where), xs, gs, us, h.data_ptr(),
           gate.data_ptr() if keep_pre else 0, up.data_ptr() if keep_pre else 0, rows, n, k, ldx, ldg, ldu, a, _TYPES[x.dtype], _TYPES[out])
     return GatedLinear(h, gate, up)
@@ -319,7 +335,7 @@ def gated_linear_backward(dh, x, gate_weight, up_weight, gate, up, activation="s
     ldh, ld_gate, ld_up = [_rows(t, name, shape=shape, dtypes=(x.dtype,))[1] for name, t in (("dh", dh), ("gate", gate), ("up", up))]
     a = _activation(activation)
     dx = _like(x, x.dtype)
-    dg, du = [x.new_empty((n, k), dtype=x.dtype) for _ in range(2)]
+    dg, du = _like(gate_weight, x.dtype), _like(up_weight, x.dtype)
     _call(_GATED_LINEAR_BACKWARD, where, _pointer(dh, "dh", where), x.data_ptr(), _pointer(gate_weight, "gate_weight", where), _pointer(up_weight, "up_weight", where),
           _pointer(gate, "gate", where), _pointer(up, "up", where), dx.data_ptr(), dg.data_ptr(), du.data_ptr(), rows, n, k, ldh, ldx, ldg, ldu, ld_gate, ld_up, a,
           _TYPES[x.dtype])
