@@ -143,6 +143,8 @@ void tiramisu_hip_parallel_for(int32_t first, int32_t last, void (*body)(int32_t
  * block out again while that work still runs. */
 int tiramisu_hip_set_stream(void *stream);
 void *tiramisu_hip_get_stream(void);
+/* The handle under which tiramisu_hip_set_stream takes the device's null stream (torch's default stream, whose own handle is NULL). */
+void *tiramisu_hip_null_stream(void);
 /* Waits for the device's null stream (other libraries' default stream), whatever the calling thread's current one. */
 int tiramisu_hip_null_stream_synchronize(void);
 /* Calls a generated function (extern "C" int f(halide_buffer_t *...)) of up to eight arguments, all in GPU memory.  `description` holds for
@@ -209,15 +211,6 @@ int tiramisu_hip_gated_linear(const void *x, const void *gate_weight, const void
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate,
                                        const void *up, void *dx, void *dgate_weight, void *dup_weight, uint64_t M, uint64_t N, uint64_t K, uint64_t ldh,
                                        uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
-/* Any of the functions above on a stream of the caller's (null: HIP's null stream, torch's default stream) instead of the thread's current one, for
- * callers that pay for every argument they convert: its arguments in order, each in eight bytes, numbers and floats of 32 bits in the first
- * four of them. */
-enum tiramisu_hip_operator_t {
-    TIRAMISU_HIP_OPERATOR_RMS_NORM = 0, TIRAMISU_HIP_OPERATOR_RMS_NORM_BACKWARD = 1, TIRAMISU_HIP_OPERATOR_QUANTIZE_ROWS = 2,
-    TIRAMISU_HIP_OPERATOR_LINEAR = 3, TIRAMISU_HIP_OPERATOR_LINEAR_BACKWARD = 4, TIRAMISU_HIP_OPERATOR_GATED_LINEAR = 5,
-    TIRAMISU_HIP_OPERATOR_GATED_LINEAR_BACKWARD = 6
-};
-int tiramisu_hip_operator(int32_t op, const uint64_t *arguments, void *stream);
 /* For generated code: no buffer in the place of one that may be left out, and what becomes of a refused call there -- the reference's failure
  * model, the process ends with status 1 behind the operator's message. */
 float *tiramisu_hip_no_buffer(void);

@@ -188,6 +188,26 @@ def build_python_module():
     return python_module()
 
 
+def torch_module():
+    import sysconfig
+    return os.path.join(PKG, "_torch_operators" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_torch_module():
+    """The extension behind ``tiramisu_amd.operators``: the runtime's operators on torch tensors."""
+    import sysconfig
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__))
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+                os.path.join(os.path.dirname(os.path.dirname(HIPCC)), "include")]
+    lib = os.path.join(root, "lib")
+    _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch.compiled_with_cxx11_abi(),
+          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"] + ["-I" + d for d in includes] +
+         ["-o", torch_module(), os.path.join(CSRC, "torch_operators.cpp"), "-L" + PKG, "-ltiramisu_hip_wrappers", "-L" + lib, "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python",
+          "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + lib])
+    return torch_module()
+
+
 def build_python_programs(verbose=False):
     """Run the Tiramisu programs written in Python (tests/python_programs/*.py): each generates its
     object and links lib<function>.so under tests/python_programs/build/."""
@@ -230,6 +250,7 @@ def build_all(force=True, verbose=False):
     build_compiler(force)
     build_wrappers(force)
     build_python_module()
+    build_torch_module()
     build_python_programs(verbose)
     for src in program_sources():
         if "CPU_ONLY_PROGRAM" in open(src).read():

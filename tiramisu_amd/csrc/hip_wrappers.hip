@@ -875,6 +875,8 @@ int tiramisu_hip_set_stream(void *stream) {
 
 void *tiramisu_hip_get_stream(void) { return (void *)current_stream; }
 
+void *tiramisu_hip_null_stream(void) { return (void *)hipStreamLegacy; }
+
 int tiramisu_hip_null_stream_synchronize(void) {
     check(hipStreamSynchronize(hipStreamLegacy), __FUNCTION__);
     return 0;

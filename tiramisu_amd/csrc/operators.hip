@@ -488,52 +488,6 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
     return launch_gradients(__FUNCTION__, type, p, q);
 }
 
-// Each argument in eight bytes, as tiramisu_hip_operator takes them
-namespace {
-union argument {
-    uint64_t number;
-    void *pointer;
-    float real;
-};
-}  // namespace
-
-int tiramisu_hip_operator(int32_t op, const uint64_t *arguments, void *stream) {
-    argument a[20];
-    static const int counts[] = {14, 13, 7, 17, 16, 18, 20};
-    if (op < 0 || op > 6 || !arguments) return refuse(__FUNCTION__, "operator %d is not known", op);
-    for (int i = 0; i < counts[op]; i++) a[i].number = arguments[i];
-    void *const before = tiramisu_hip_get_stream();
-    tiramisu_hip_set_stream(stream ? stream : (void *)hipStreamLegacy);
-    auto p = [&](int i) { return a[i].pointer; };
-    auto f = [&](int i) { return (float *)a[i].pointer; };
-    auto u = [&](int i) { return a[i].number; };
-    auto n = [&](int i) { return (int32_t)a[i].number; };
-    int rc = 1;
-    switch (op) {
-    case TIRAMISU_HIP_OPERATOR_RMS_NORM:
-        rc = tiramisu_hip_rms_norm(p(0), p(1), p(2), p(3), p(4), f(5), f(6), u(7), u(8), u(9), u(10), a[11].real, n(12), n(13));
-        break;
-    case TIRAMISU_HIP_OPERATOR_RMS_NORM_BACKWARD:
-        rc = tiramisu_hip_rms_norm_backward(p(0), p(1), p(2), f(3), p(4), p(5), p(6), u(7), u(8), u(9), u(10), u(11), n(12));
-        break;
-    case TIRAMISU_HIP_OPERATOR_QUANTIZE_ROWS: rc = tiramisu_hip_quantize_rows(p(0), p(1), f(2), u(3), u(4), u(5), n(6)); break;
-    case TIRAMISU_HIP_OPERATOR_LINEAR:
-        rc = tiramisu_hip_linear(p(0), p(1), p(2), p(3), f(4), f(5), p(6), p(7), u(8), u(9), u(10), u(11), u(12), u(13), n(14), n(15), n(16));
-        break;
-    case TIRAMISU_HIP_OPERATOR_LINEAR_BACKWARD:
-        rc = tiramisu_hip_linear_backward(p(0), p(1), p(2), p(3), p(4), p(5), p(6), u(7), u(8), u(9), u(10), u(11), u(12), u(13), n(14), n(15));
-        break;
-    case TIRAMISU_HIP_OPERATOR_GATED_LINEAR:
-        rc = tiramisu_hip_gated_linear(p(0), p(1), p(2), f(3), f(4), f(5), p(6), p(7), p(8), u(9), u(10), u(11), u(12), u(13), u(14), n(15), n(16), n(17));
-        break;
-    default:
-        rc = tiramisu_hip_gated_linear_backward(p(0), p(1), p(2), p(3), p(4), p(5), p(6), p(7), p(8), u(9), u(10), u(11), u(12), u(13), u(14), u(15), u(16), u(17),
-                                                n(18), n(19));
-    }
-    tiramisu_hip_set_stream(before);
-    return rc;
-}
-
 float *tiramisu_hip_no_buffer(void) { return nullptr; }       // (a pointer that is also one to scales)
 
 int tiramisu_hip_require(int32_t status) {

@@ -154,7 +154,6 @@ def wrappers():
         lib.tiramisu_hip_linear_backward.argtypes = [p] * 7 + [u] * 7 + [i] * 2
         lib.tiramisu_hip_gated_linear.argtypes = [p] * 9 + [u] * 6 + [i] * 3
         lib.tiramisu_hip_gated_linear_backward.argtypes = [p] * 9 + [u] * 9 + [i] * 2
-        lib.tiramisu_hip_operator.argtypes = [i, ctypes.c_char_p, p]
         _wrappers = lib
     return _wrappers
 
