@@ -2,8 +2,8 @@
 // are read once, straight into registers in the matrix instruction's layout.
 // A workgroup computes 16 columns of C (GATED: of gate and of up) for all rows: 16 rows of the weights against up to TILES x 16 rows of x with
 // v_mfma_f32_16x16x32, the weights as the instruction's rows.  k is dealt to the wavefronts in units of 128 bytes of a row (every
-// line of the weights is read by one wavefront, by two loads that follow each other), BATCH units of loads are in flight in each, and the
-// wavefronts' sums are added through LDS.  x is read by every workgroup, from the L2; rows behind the last read the last one again.
+// line of the weights is read by one wavefront, by two loads that follow each other), up to BATCH units of loads are in flight in each (one token, 4096 x 4096:
+// with 8 units 8.1 us, 5.4 TB/s behind the launch; with 4 8.7), and the wavefronts' sums are added through LDS.  x is read by every workgroup, from the L2; rows behind the last read the last one again.
 // Addresses may be any multiple of an element.
 #ifndef TIRAMISU_AMD_LINEAR_FEW_TOKENS_HIP_H
 #define TIRAMISU_AMD_LINEAR_FEW_TOKENS_HIP_H
@@ -30,7 +30,7 @@ __device__ __forceinline__ f32x4 multiply_16(u32x4 rows, u32x4 columns, f32x4 c)
 
 template <int E, int Y, int EPILOGUE, int TILES>
 __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_arguments p) {
-    constexpr int BYTES = E == F8 ? 1 : 2, PARTS = EPILOGUE == GATED ? 2 : 1, BATCH = TILES * PARTS >= 4 ? 2 : 4;
+    constexpr int BYTES = E == F8 ? 1 : 2, PARTS = EPILOGUE == GATED ? 2 : 1, BATCH = TILES * PARTS >= 4 ? 2 : TILES * PARTS == 2 ? 4 : 8;
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     __attribute__((address_space(3))) f32x4 *const sums = (__attribute__((address_space(3))) f32x4 *)shared_bytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -52,27 +52,35 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
 
     const int whole = (int)(bytes / 128), units = (int)((bytes + 127) / 128);
     int u = wave;
-    for (; u + (BATCH - 1) * FEW_WAVES < whole; u += BATCH * FEW_WAVES) {
-        u32x4 fw[BATCH][2][PARTS], fx[BATCH][2][TILES];
+    // as many units at a time as are left, by halves
+    auto take = [&](auto batch_c) {
+        constexpr int B = decltype(batch_c)::value;
+        for (; u + (B - 1) * FEW_WAVES < whole; u += B * FEW_WAVES) {
+            u32x4 fw[B][2][PARTS], fx[B][2][TILES];
 #pragma unroll
-        for (int b = 0; b < BATCH; b++)
+            for (int b = 0; b < B; b++)
 #pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const long at = (long)(u + b * FEW_WAVES) * 128 + 64 * half;
+                for (int half = 0; half < 2; half++) {
+                    const long at = (long)(u + b * FEW_WAVES) * 128 + 64 * half;
 #pragma unroll
-                for (int q = 0; q < PARTS; q++) fw[b][half][q] = *reinterpret_cast<const u32x4_any *>(w[q] + at);
+                    for (int q = 0; q < PARTS; q++) fw[b][half][q] = *reinterpret_cast<const u32x4_any *>(w[q] + at);
 #pragma unroll
-                for (int i = 0; i < TILES; i++) fx[b][half][i] = *reinterpret_cast<const u32x4_any *>(x[i] + at);
-            }
+                    for (int i = 0; i < TILES; i++) fx[b][half][i] = *reinterpret_cast<const u32x4_any *>(x[i] + at);
+                }
 #pragma unroll
-        for (int b = 0; b < BATCH; b++)
+            for (int b = 0; b < B; b++)
 #pragma unroll
-            for (int half = 0; half < 2; half++)
+                for (int half = 0; half < 2; half++)
 #pragma unroll
-                for (int q = 0; q < PARTS; q++)
+                    for (int q = 0; q < PARTS; q++)
 #pragma unroll
-                    for (int i = 0; i < TILES; i++) acc[q][i] = multiply_16<E>(fw[b][half][q], fx[b][half][i], acc[q][i]);
-    }
+                        for (int i = 0; i < TILES; i++) acc[q][i] = multiply_16<E>(fw[b][half][q], fx[b][half][i], acc[q][i]);
+        }
+    };
+    if constexpr (BATCH >= 8) take(std::integral_constant<int, 8>());
+    if constexpr (BATCH >= 4) take(std::integral_constant<int, 4>());
+    take(std::integral_constant<int, 2>());
+    take(std::integral_constant<int, 1>());
     for (; u < units; u += FEW_WAVES) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {

@@ -92,7 +92,7 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
             if ((slices + each - 1) / each != splits) continue;            // (the same slices to each as with fewer)
             const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
             double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
-            if (splits > 1) cost += 3.0 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 4e6;
+            if (splits > 1) cost += 5.5 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 4e6;
             if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each, cost}; best_cost = cost; }
         }
     };
@@ -170,8 +170,21 @@ int launch_gradients(const char *fn, int type, const product_arguments &p, const
     return q.y ? launch_product(fn, type, WEIGHT_GRADIENT, LINEAR, type, q) : 0;
 }
 
-// Rows of x for which the weights are streamed through registers (linear_few_tokens.hip.h).
+// Rows of x that the kernel of few tokens (linear_few_tokens.hip.h) takes at most, and what a call of it takes: the weights' bytes at what memory gives, or what a
+// compute unit takes in of weights and x for the workgroups it runs, the other hidden but for a part.  The tiles are held to the weights' bytes too, at
+// the rates they reached.  us as the kernel of few tokens / as tiles, for 1, 16 and 64 rows: bf16 4096 x 4096 8.7, 9.9, 20.6 / 11.2,
+// 11.7, 13.1; 8192 x 2048 9.1, 10.5, 20.7 / 10.8, 10.7, 11.2; 16384 x 4096 25, 37, 83 / 33, 33, 34; gated 4096 x 4096 14.3, 14.6, 24.6 / 16.3, 16.9, 19.5,
+// 8192 x 2048 15.1, 16.6, 25.8 / 13.1, 13.4, 14.0; e4m3 4096 x 4096 6.6, 7.6, 12.0 / 11.2, 11.0, 11.6, 16384 x 4096 17.7, 20.2, 38.3 / 12.8, 12.7, 14.0.
 constexpr long FEW_TOKENS = 64;
+double few_tokens_cost(long M, long N, long K, int bytes, bool gated) {
+    const double parts = gated ? 2 : 1, row = (double)K * bytes, rounds = (double)((N + 16L * ttarget::COMPUTE_UNITS - 1) / (16L * ttarget::COMPUTE_UNITS));
+    const double memory = parts * N * row / 5.4e6, unit = rounds * (16 * parts + M) * row / 39e3;
+    return 2.5 + std::max(memory, unit) + 0.1 * std::min(memory, unit) + (rounds - 1);
+}
+double tiles_cost(const tile_plan &plan, long N, long K, int bytes, bool gated, int moved) {
+    const double rate = !gated && bytes == 2 ? 4.4e6 : gated && N < 64L * ttarget::COMPUTE_UNITS / 2 ? 5.0e6 : 6.2e6;
+    return std::max(plan.cost, 3.0 + (gated ? 2.0 : 1.0) * N * K * bytes / rate) + 3.5 * moved;
+}
 
 template <int E, int Y, int EPILOGUE, int TILES>
 void launch_few(const char *fn, const product_arguments &p) {
@@ -196,11 +209,15 @@ void launch_few(const char *fn, int type, int y, const product_arguments &p) {
 // A forward product: few tokens, or tiles
 int forward(const char *fn, int type, int y, int epilogue, product_arguments p) {
     if (p.M == 0 || p.N == 0) return 0;
-    if (p.M <= FEW_TOKENS && p.K > 0) {
-        epilogue == GATED ? launch_few<GATED>(fn, type, y, p) : launch_few<LINEAR>(fn, type, y, p);
-        return 0;
-    }
     const int bytes = bytes_of(type);
+    const bool gated = epilogue == GATED;
+    if (p.M <= FEW_TOKENS && p.K > 0) {
+        const int moved = !loadable({p.a, p.lda}, bytes, true) + !loadable({p.b, p.ldb}, bytes, true) + (gated && !loadable({p.b2, p.ldb2}, bytes, true));
+        if (few_tokens_cost(p.M, p.N, p.K, bytes, gated) <= tiles_cost(plan_for(p.M, p.N, p.K, bytes, gated), p.N, p.K, bytes, gated, moved)) {
+            gated ? launch_few<GATED>(fn, type, y, p) : launch_few<LINEAR>(fn, type, y, p);
+            return 0;
+        }
+    }
     auto take = [&](const void *&q, long &ld, long rows, scratch_use use) {
         const operand o = moved_where_needed({q, ld}, rows, p.K, bytes, true, use);
         q = o.p;
@@ -208,7 +225,7 @@ int forward(const char *fn, int type, int y, int epilogue, product_arguments p) 
     };
     take(p.a, p.lda, p.M, MOVED_A);
     take(p.b, p.ldb, p.N, MOVED_B);
-    if (epilogue == GATED) take(p.b2, p.ldb2, p.N, MOVED_C);
+    if (gated) take(p.b2, p.ldb2, p.N, MOVED_C);
     return launch_product(fn, type, FORWARD, epilogue, y, p);
 }
 
