@@ -79,9 +79,11 @@ typedef __attribute__((address_space(3))) char lds_char;
 template <int BYTES, int ROWS, bool K_ALONG_ROWS, int LOADS, int F>
 struct operand_loader {
     static constexpr int G = K_ALONG_ROWS ? 8 : ROWS / 8;                  // granules of a row in LDS
-    // Lanes that an LDS read serves together, 8 or 16 of a 16-byte read and 16 or 32 of a transposing one, meet distinct banks.
+    // Lanes that an LDS read serves together meet distinct banks: of a 16-byte read they are 16 at a time, 0-3, 12-15, 20-23 and 24-27 the first of
+    // them, whose rows and granules F and the element's size decide (with the first form for all, 16-bit fragments of 16 rows took two cycles for
+    // one: half of the LDS's busy cycles); of a transposing one 16 or 32.
     static __device__ __forceinline__ int swizzle(int row) {
-        if (K_ALONG_ROWS) return (row ^ (row >> 3)) & 7;
+        if (K_ALONG_ROWS) return (F == 16 && BYTES == 2 ? row >> 1 : row ^ (row >> 3)) & 7;
         const int eighth = F == 16 ? (row >> 3) & 1 : 0;                   // (F == 16: such 32 lanes read k and k + 8)
         return G == 8 ? 2 * ((row & 3) ^ eighth) : (((row & 1) << 2) | ((row & 2) ? 10 : 0)) ^ (eighth << 1);
     }
