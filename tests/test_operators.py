@@ -516,6 +516,35 @@ def test_calls_in_a_graph():
 
 
 @pytest.mark.gpu
+def test_a_graph_recorded_without_a_call_before():
+    """Scratch (the activation's gradient, rows that are moved, sums of columns) is allocated while the stream records."""
+    g = generator(89)
+    x, w, dy, pre = normal((301, 77), torch.bfloat16, g), normal((95, 77), torch.bfloat16, g), normal((301, 95), torch.bfloat16, g), normal((301, 95), torch.bfloat16, g)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        got = operators.linear_backward(dy, x, w, pre=pre, activation="gelu", bias=True)
+    for seed in range(3):
+        dy.copy_(normal((301, 95), torch.bfloat16, generator(seed)))
+        graph.replay()
+        replayed = [t.clone() for t in got]
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(replayed, operators.linear_backward(dy, x, w, pre=pre, activation="gelu", bias=True)))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_holds():
+    """The last of 2^22 + 77 rows are those of a call of their own."""
+    rows = (1 << 22) + 77
+    x = normal((rows, 8), torch.bfloat16, generator(97))
+    w = x[0]
+    got, last = operators.rms_norm(x, w, residual=x, eight_bit=True), operators.rms_norm(x[-200:], w, residual=x[-200:], eight_bit=True)
+    assert torch.equal(got.y[-200:].float(), last.y.float()) and torch.equal(got.scale[-200:], last.scale) and torch.equal(got.sum[-200:], last.sum)
+    kept = operators.rms_norm(x, w, keep_rstd=True)
+    assert torch.equal(kept.rstd[-200:], operators.rms_norm(x[-200:], w, keep_rstd=True).rstd)
+
+
+@pytest.mark.gpu
 def test_launches_are_recorded_by_the_profile():
     x, w = normal((4, 64), torch.bfloat16, generator(79)), normal((64, 64), torch.bfloat16, generator(83))
     records = runtime.profile(lambda: (operators.rms_norm(x, w[0]), operators.linear(x, w), operators.gated_linear(x, w, w)))
@@ -584,5 +613,7 @@ def test_what_the_c_abi_refuses(capfd):
     assert w.tiramisu_hip_linear_backward(p, p, p, None, p, p, None, 4, 8, 8, 0, 0, 0, 0, 1, 2) == 1
     assert w.tiramisu_hip_linear_backward(p, p, p, None, p, p, None, 4, 8, 8, 0, 0, 0, 0, 0, 3) == 1
     assert w.tiramisu_hip_gated_linear_backward(p, p, p, p, p, p, p, p, None, 4, 8, 8, 0, 0, 0, 0, 0, 0, 4, 2) == 1
+    assert w.tiramisu_hip_linear(p, p, None, None, None, None, p, None, 1 << 29, 1 << 9, 8, 0, 0, 0, 0, 2, 2) == 1     # 2^26 tiles
+    assert w.tiramisu_hip_rms_norm(p, None, p, p, None, None, None, 4, 1 << 27, 0, 0, 1e-6, 2, 2) == 1
     messages = capfd.readouterr().err.strip().splitlines()
-    assert len(messages) == 18 and all(m.startswith("Error at tiramisu_hip_") for m in messages)
+    assert len(messages) == 20 and all(m.startswith("Error at tiramisu_hip_") for m in messages)

@@ -733,7 +733,11 @@ void *tiramisu_hip_kept_scratch(const void *site, uint64_t bytes, int32_t *fresh
             check(hipStreamSynchronize(current_stream), __FUNCTION__);
             check(hipFree(block.ptr), __FUNCTION__);
         }
+        // (allowed while the thread records a graph, like the allocations of other libraries: the block outlives the recording)
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        check(hipThreadExchangeStreamCaptureMode(&mode), __FUNCTION__);
         check(hipMalloc(&block.ptr, bytes), __FUNCTION__);
+        check(hipThreadExchangeStreamCaptureMode(&mode), __FUNCTION__);
         block.bytes = bytes;
         if (fresh) *fresh = 1;
     }

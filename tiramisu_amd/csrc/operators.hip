@@ -33,7 +33,11 @@ __attribute__((format(printf, 2, 3))) int refuse(const char *fn, const char *for
     return 1;
 }
 
-constexpr uint64_t MOST = 0x7fffffff;                    // rows and columns are counted in 31 bits
+constexpr uint64_t MOST = 0x3fffffff;                    // rows and columns are counted in 31 bits, with room for a tile
+constexpr int64_t MOST_ROWS_A_LAUNCH = 1 << 22;          // of a workgroup each: a launch holds 2^32 threads
+constexpr uint64_t MOST_TILES = (1 << 23) - 1;           // of 64 x 64: the same
+constexpr uint64_t MOST_COLUMNS = 1 << 26;               // of a norm: the same for the sums of its columns
+constexpr long MOST_FEW_COLUMNS = 1 << 26;               // of a product of few tokens
 constexpr int64_t MOST_ROW_BYTES = 1 << 22;              // of an operand with k along its rows: a tile's offsets stay below 2^31
 constexpr int64_t MOST_STEP = 1 << 23;                   // elements from k to k of one with k down its columns: the same
 
@@ -211,7 +215,7 @@ int forward(const char *fn, int type, int y, int epilogue, product_arguments p) 
     if (p.M == 0 || p.N == 0) return 0;
     const int bytes = bytes_of(type);
     const bool gated = epilogue == GATED;
-    if (p.M <= FEW_TOKENS && p.K > 0) {
+    if (p.M <= FEW_TOKENS && p.K > 0 && p.N <= MOST_FEW_COLUMNS) {
         const int moved = !loadable({p.a, p.lda}, bytes, true) + !loadable({p.b, p.ldb}, bytes, true) + (gated && !loadable({p.b2, p.ldb2}, bytes, true));
         if (few_tokens_cost(p.M, p.N, p.K, bytes, gated) <= tiles_cost(plan_for(p.M, p.N, p.K, bytes, gated), p.N, p.K, bytes, gated, moved)) {
             gated ? launch_few<GATED>(fn, type, y, p) : launch_few<LINEAR>(fn, type, y, p);
@@ -246,11 +250,23 @@ void launch_norm(const char *fn, const norm_arguments &a) {
     else go(rms_norm_kernel<E, Y, 1024, 1, false>, 1024, 1);
     check(hipGetLastError(), fn);
 }
-int norm(const char *fn, int type, int y, const norm_arguments &a) {
+int norm(const char *fn, int type, int y, norm_arguments a) {
     if (a.rows == 0 || a.columns == 0) return 0;
-    if (type == F32) y == F8 ? launch_norm<F32, F8>(fn, a) : launch_norm<F32, F32>(fn, a);
-    else if (type == F16) y == F8 ? launch_norm<F16, F8>(fn, a) : launch_norm<F16, F16>(fn, a);
-    else y == F8 ? launch_norm<BF16, F8>(fn, a) : launch_norm<BF16, BF16>(fn, a);
+    const long all = a.rows, step = bytes_of(type), step_y = bytes_of(y);
+    auto moved = [](auto *p, long bytes) { return p ? (decltype(p))((uintptr_t)p + bytes) : p; };
+    for (long first = 0; first < all; first += MOST_ROWS_A_LAUNCH) {
+        norm_arguments part = a;
+        part.rows = std::min(MOST_ROWS_A_LAUNCH, all - first);
+        part.x = moved(a.x, first * a.ldx * step);
+        part.residual = moved(a.residual, first * a.ldr * step);
+        part.y = moved(a.y, first * a.columns * step_y);
+        part.sum = moved(a.sum, first * a.columns * step);
+        part.scale = moved(a.scale, first * 4);
+        part.rstd = moved(a.rstd, first * 4);
+        if (type == F32) y == F8 ? launch_norm<F32, F8>(fn, part) : launch_norm<F32, F32>(fn, part);
+        else if (type == F16) y == F8 ? launch_norm<F16, F8>(fn, part) : launch_norm<F16, F16>(fn, part);
+        else y == F8 ? launch_norm<BF16, F8>(fn, part) : launch_norm<BF16, BF16>(fn, part);
+    }
     return 0;
 }
 
@@ -311,15 +327,18 @@ product_arguments product_of(long M, long N, long K) {
     return p;
 }
 
+int refuse_result(const char *fn, uint64_t rows, uint64_t columns) {
+    if (((rows + 63) / 64) * ((columns + 63) / 64) <= MOST_TILES) return 0;
+    return refuse(fn, "result of %llu x %llu: more tiles than a launch holds", (unsigned long long)rows, (unsigned long long)columns);
+}
 // What both products refuse alike
 int refuse_product(const char *fn, uint64_t M, uint64_t N, uint64_t K, int activation, int type, int y) {
-    if (M > MOST || N > MOST || K > MOST) return refuse(fn, "dimension exceeds 2^31-1");
+    if (M > MOST || N > MOST || K > MOST) return refuse(fn, "product of %llu x %llu x %llu: dimensions of at most 2^30 - 1", (unsigned long long)M, (unsigned long long)N, (unsigned long long)K);
     if ((int64_t)K * bytes_of(type) > MOST_ROW_BYTES) return refuse(fn, "K of %llu: rows of at most %lld bytes", (unsigned long long)K, (long long)MOST_ROW_BYTES);
     if (activation < NONE || activation > SILU) return refuse(fn, "activation %d is not known", activation);
     if (!known_type(type, false) && type != F8) return refuse(fn, "element type %d: float16, bfloat16 or float8_e4m3", type);
     if (type == F8 ? !known_type(y, false) : y != type) return refuse(fn, "results of type %d from operands of type %d", y, type);
-    if (((M + 63) / 64) * ((N + 63) / 64) > MOST) return refuse(fn, "result of %llu x %llu: more tiles than a launch holds", (unsigned long long)M, (unsigned long long)N);
-    return 0;
+    return refuse_result(fn, M, N);
 }
 
 }  // namespace
@@ -331,7 +350,7 @@ extern "C" {
 
 int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum, float *scale, float *rstd, uint64_t rows,
                           uint64_t columns, uint64_t ldx, uint64_t ldr, float eps, int32_t type, int32_t y_type) {
-    if (rows > MOST || columns > MOST) return refuse(__FUNCTION__, "dimension exceeds 2^31-1");
+    if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu: at most 2^30 - 1 of at most 2^26", (unsigned long long)rows, (unsigned long long)columns);
     if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
     if (y_type != type && y_type != F8) return refuse(__FUNCTION__, "results of type %d from rows of type %d", y_type, type);
     if (rows == 0 || columns == 0) return 0;
@@ -344,7 +363,7 @@ int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weigh
 }
 
 int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type) {
-    if (rows > MOST || columns > MOST) return refuse(__FUNCTION__, "dimension exceeds 2^31-1");
+    if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu: at most 2^30 - 1 of at most 2^26", (unsigned long long)rows, (unsigned long long)columns);
     if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
     if (rows == 0 || columns == 0) return 0;
     if (!x || !q || !scale) return refuse(__FUNCTION__, "x, q and scale are needed");
@@ -355,7 +374,7 @@ int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t ro
 
 int tiramisu_hip_rms_norm_backward(const void *dy, const void *sum, const void *weight, const float *rstd, const void *dsum, void *dx, void *dweight,
                                    uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t lds, uint64_t ldd, int32_t type) {
-    if (rows > MOST || columns > MOST) return refuse(__FUNCTION__, "dimension exceeds 2^31-1");
+    if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu: at most 2^30 - 1 of at most 2^26", (unsigned long long)rows, (unsigned long long)columns);
     if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
     if (columns == 0) return 0;
     if (!dweight || !weight || (rows && (!dy || !sum || !rstd || !dx))) return refuse(__FUNCTION__, "dy, sum, weight, rstd, dx and dweight are needed");
@@ -423,6 +442,7 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
                                  uint64_t N, uint64_t K, uint64_t ldy, uint64_t ldx, uint64_t ldw, uint64_t ldp, int32_t activation, int32_t type) {
     if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, type)) return rc;
     if ((int64_t)N * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (unsigned long long)N, (long long)MOST_ROW_BYTES);
+    if (refuse_result(__FUNCTION__, M, K) || refuse_result(__FUNCTION__, N, K)) return 1;
     if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
     if ((activation != NONE) != (pre != nullptr)) return refuse(__FUNCTION__, "an activation and the sums ahead of it belong together");
     if ((M && N && !dy) || (M && K && dweight && !x) || (N && K && dx && !weight)) return refuse(__FUNCTION__, "dy, x and weight are needed");
@@ -464,6 +484,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
                                        uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type) {
     if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, type)) return rc;
     if ((int64_t)(2 * N + 16) * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (unsigned long long)N, (long long)MOST_ROW_BYTES);
+    if (refuse_result(__FUNCTION__, M, K) || refuse_result(__FUNCTION__, 2 * N + 16, K)) return 1;
     if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
     if ((M && N && (!dh || !gate || !up)) || (M && K && N && !x) || (N && K && (!gate_weight || !up_weight))) return refuse(__FUNCTION__, "dh, x, both weights, gate and up are needed");
     if ((dgate_weight != nullptr) != (dup_weight != nullptr)) return refuse(__FUNCTION__, "gradients of both weights, or of neither");
