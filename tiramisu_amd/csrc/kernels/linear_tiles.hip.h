@@ -558,14 +558,16 @@ __global__ __launch_bounds__(C::NT) void product_kernel(product_arguments p) {
 }
 
 // Two products in one launch (both gradients of a layer), the second's tiles behind the first's: compute units that the last round of
-// the first leaves idle begin with the second.  `start`: the second's first workgroup, a multiple of the XCDs.
+// the first leaves idle begin with the second, and where it leaves some, with the sums of the bias's gradient.  `start`: the second's first workgroup, a
+// multiple of the XCDs; `end`: that of the sums.
 template <class C, class D, int Y>
-__global__ __launch_bounds__(C::NT) void product_pair_kernel(product_arguments p, product_arguments q, int tiles, int start) {
+__global__ __launch_bounds__(C::NT) void product_pair_kernel(product_arguments p, product_arguments q, column_sums sums, int tiles, int start, int end) {
 #ifdef __HIP_DEVICE_COMPILE__
     static_assert(C::NT == D::NT, "one workgroup's size");
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     const int id = blockIdx.x;
     if (id < tiles) compute_tile<C, Y>(p, id, 0, (lds_char *)shared_bytes);
+    else if (id >= end) sum_parts<Y, C::NT>(sums, id - end, (float *)shared_bytes);
     else if (id >= start) compute_tile<D, Y>(q, id - start, 0, (lds_char *)shared_bytes);
 #endif
 }

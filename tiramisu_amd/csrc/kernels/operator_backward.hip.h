@@ -16,6 +16,7 @@ struct activation_backward_arguments {
 
 // dz = dy activation'(pre), and its sums over the rows of a chunk (the bias's gradient; the chunks are added by sum_parts_kernel).
 // dz is rounded to the operands' 16 bits, as it is multiplied by matrix instructions of that type.
+// 4096 x 4096 bf16 with gelu: 21.4 us, 4.7 TB/s (one row at a time 24); 300 x 520 with one row to a thread 3.4 us less than with four.
 template <int E>
 __global__ __launch_bounds__(256) void activation_backward_kernel(activation_backward_arguments a) {
     __shared__ float s[256][9];
@@ -28,21 +29,33 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(activation_bac
 #pragma unroll
     for (int i = 0; i < 8; i++) sum[i] = 0.f;
     if (some > 0) {
-        for (long m = (long)blockIdx.y * a.rows + y; m < end; m += down) {
-            float v[8];
-            load_some<E>((const T *)a.dy + m * a.ldy + n, some, v);
-            if (a.pre) {
-                float z[8];
-                load_some<E>((const T *)a.pre + m * a.ldp + n, some, z);
+        // (ROWS rows are on their way at a time)
+        constexpr int ROWS = 4;
+        for (long m = (long)blockIdx.y * a.rows + y; m < end; m += ROWS * down) {
+            u32x4 held[ROWS], held_pre[ROWS];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float value;
-                    v[i] *= activation_slope(a.activation, z[i], value);
-                }
+            for (int r = 0; r < ROWS; r++) {
+                const long row = m + r * down, left = row < end ? 2 * some : 0;
+                held[r] = load_guarded<2>((const char *)((const T *)a.dy + row * a.ldy + n), left);
+                if (a.pre) held_pre[r] = load_guarded<2>((const char *)((const T *)a.pre + row * a.ldp + n), left);
             }
-            if (a.dz) store_some<E>((T *)a.dz + m * a.ldz + n, some, v);
 #pragma unroll
-            for (int i = 0; i < 8; i++) sum[i] += v[i];
+            for (int r = 0; r < ROWS; r++) {
+                const long row = m + r * down;
+                if (row >= end) break;
+                float v[8];
+                widen<E>(held[r], v);
+                if (a.pre) {
+                    float z[8], slope[8], value[8];
+                    widen<E>(held_pre[r], z);
+                    activation_slopes(a.activation, z, slope, value);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[i] *= slope[i];
+                }
+                if (a.dz) store_some<E>((T *)a.dz + row * a.ldz + n, some, v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) sum[i] += v[i];
+            }
         }
     }
     if (!a.partial) return;
@@ -63,7 +76,7 @@ struct gated_backward_arguments {
     int activation;
 };
 
-// dgate = dh up activation'(gate), dup = dh activation(gate)
+// dgate = dh up activation'(gate), dup = dh activation(gate): 16 bits as they are multiplied.  4096 x 4096 bf16: 30 us, 5.6 TB/s.
 template <int E>
 __global__ __launch_bounds__(256) void gated_backward_kernel(gated_backward_arguments a) {
     const long across = (a.N + 7) / 8, id = (long)blockIdx.x * 256 + threadIdx.x;
@@ -75,12 +88,12 @@ __global__ __launch_bounds__(256) void gated_backward_kernel(gated_backward_argu
     load_some<E>((const T *)a.dh + m * a.ldh + n, some, d);
     load_some<E>((const T *)a.gate + m * a.ldg + n, some, g);
     load_some<E>((const T *)a.up + m * a.ldu + n, some, u);
+    float slope[8], value[8];
+    activation_slopes(a.activation, g, slope, value);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        float value;
-        const float slope = activation_slope(a.activation, g[i], value);
-        g[i] = d[i] * u[i] * slope;
-        u[i] = d[i] * value;
+        g[i] = d[i] * u[i] * slope[i];
+        u[i] = d[i] * value[i];
     }
     store_some<E>((T *)a.dgate + m * a.ldd + n, some, g);
     store_some<E>((T *)a.dup + m * a.ldd + n, some, u);

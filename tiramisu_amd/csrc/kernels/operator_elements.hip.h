@@ -211,6 +211,45 @@ __device__ __forceinline__ float activation_slope(int a, float z, float &value) 
     value = z;
     return 1.f;
 }
+template <int N>
+__device__ __forceinline__ void activation_slopes(int a, const float (&z)[N], float (&slope)[N], float (&value)[N]) {
+    auto all = [&](int known) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < N; i++) slope[i] = activation_slope(known, z[i], value[i]);
+    };
+    if (a == GELU) all(GELU);
+    else if (a == SILU) all(SILU);
+    else if (a == GELU_TANH) all(GELU_TANH);
+    else if (a == RELU) all(RELU);
+    else all(NONE);
+}
+
+// out[c] = sum over `parts` rows of partial[][c], in a fixed order: 32 columns to a workgroup, THREADS / 32 threads down each.  `s`: 33 floats for each of these.
+struct column_sums {
+    const float *partial;                   // [parts][columns]
+    void *out;
+    long columns;
+    int parts;                              // 0: no sums
+};
+constexpr int SUM_COLUMNS = 32;
+template <int E, int THREADS, typename FLOATS>
+__device__ __forceinline__ void sum_parts(const column_sums &a, int id, FLOATS *s) {
+    constexpr int DOWN = THREADS / SUM_COLUMNS;
+    const int x = threadIdx.x % SUM_COLUMNS, y = threadIdx.x / SUM_COLUMNS;
+    const long first = (long)id * SUM_COLUMNS, c = first + x;
+    float v = 0.f;
+    if (c < a.columns) {
+#pragma unroll 8
+        for (int p = y; p < a.parts; p += DOWN) v += a.partial[(long)p * a.columns + c];
+    }
+    s[y * (SUM_COLUMNS + 1) + x] = v;
+    __syncthreads();
+    const int column = threadIdx.x / DOWN, part = threadIdx.x % DOWN;
+    v = s[part * (SUM_COLUMNS + 1) + column];
+#pragma unroll
+    for (int o = DOWN / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    if (part == 0 && first + column < a.columns) store_one<E>((stored<E> *)a.out + first + column, v);
+}
 
 }  // namespace tops
 #endif

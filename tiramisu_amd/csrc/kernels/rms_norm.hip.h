@@ -310,24 +310,10 @@ __global__ __launch_bounds__(256) void rms_norm_backward_long_columns_kernel(nor
     a.partial[(long)blockIdx.y * a.columns + c] = sum;
 }
 
-// out[c] = sum over `parts` rows of partial[][c], in a fixed order: 32 columns to a workgroup, 32 threads down each.
 template <int E>
-__global__ __launch_bounds__(1024) void sum_parts_kernel(const float *partial, int parts, long columns, stored<E> *out) {
-    __shared__ float s[32][33];
-    const int x = threadIdx.x & 31, yy = threadIdx.x >> 5;
-    const long c = (long)blockIdx.x * 32 + x;
-    float v = 0.f;
-    if (c < columns) {
-#pragma unroll 8
-        for (int p = yy; p < parts; p += 32) v += partial[(long)p * columns + c];
-    }
-    s[yy][x] = v;
-    __syncthreads();
-    v = s[x][yy];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    const long out_c = (long)blockIdx.x * 32 + yy;
-    if (x == 0 && out_c < columns) store_one<E>(out + out_c, v);
+__global__ __launch_bounds__(1024) void sum_parts_kernel(column_sums a) {
+    __shared__ float s[1024 + 32];
+    sum_parts<E, 1024>(a, blockIdx.x, s);
 }
 
 }  // namespace tops

@@ -34,13 +34,14 @@ void launch(const product_arguments &p, int splits, hipStream_t stream) {
 }
 
 template <class C, class D, int Y>
-void launch_pair(const product_arguments &p, const product_arguments &q, hipStream_t stream) {
+void launch_pair(const product_arguments &p, const product_arguments &q, const column_sums &sums, hipStream_t stream) {
     auto kernel = product_pair_kernel<C, D, Y>;
     constexpr int LDS = C::LDS_BYTES > D::LDS_BYTES ? C::LDS_BYTES : D::LDS_BYTES;
     static std::atomic<unsigned long long> asked{0};
     allow_lds((const void *)kernel, LDS, asked);
-    const int tiles = tiles_of<C>(p), start = (tiles + XCDS - 1) / XCDS * XCDS;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(start + tiles_of<D>(q))), dim3(C::NT), LDS, stream, p, q, tiles, start);
+    const int tiles = tiles_of<C>(p), start = (tiles + XCDS - 1) / XCDS * XCDS, end = start + tiles_of<D>(q);
+    const int of_sums = sums.parts ? (int)((sums.columns + SUM_COLUMNS - 1) / SUM_COLUMNS) : 0;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(end + of_sums)), dim3(C::NT), LDS, stream, p, q, sums, tiles, start, end);
     tiramisu_runtime::check(hipGetLastError(), "tiramisu_hip_linear");
 }
 
@@ -66,11 +67,11 @@ void launch_tile(product_tile tile, const product_arguments &p, int splits, hipS
 
 // (P, Q: how the operands of the two products lie)
 template <int E, class P, class Q>
-void launch_pair_of(product_tile tile, const product_arguments &p, const product_arguments &q, hipStream_t stream) {
-    if (tile == TILE_256) launch_pair<typename P::tile_256, typename Q::tile_256, E>(p, q, stream);
-    else if (tile == TILE_256x128) launch_pair<typename P::tile_256x128, typename Q::tile_256x128, E>(p, q, stream);
-    else if (tile == TILE_128) launch_pair<typename P::tile_128, typename Q::tile_128, E>(p, q, stream);
-    else launch_pair<typename P::tile_64, typename Q::tile_64, E>(p, q, stream);
+void launch_pair_of(product_tile tile, const product_arguments &p, const product_arguments &q, const column_sums &sums, hipStream_t stream) {
+    if (tile == TILE_256) launch_pair<typename P::tile_256, typename Q::tile_256, E>(p, q, sums, stream);
+    else if (tile == TILE_256x128) launch_pair<typename P::tile_256x128, typename Q::tile_256x128, E>(p, q, sums, stream);
+    else if (tile == TILE_128) launch_pair<typename P::tile_128, typename Q::tile_128, E>(p, q, sums, stream);
+    else launch_pair<typename P::tile_64, typename Q::tile_64, E>(p, q, sums, stream);
 }
 
 }  // namespace
@@ -89,12 +90,12 @@ void NAME_OF(launch_tiles_, TIRAMISU_OPERAND)(product_tile tile, product_layout 
 }
 
 #ifndef TIRAMISU_OPERAND_HAS_NO_GRADIENTS
-void NAME_OF(launch_gradients_, TIRAMISU_OPERAND)(product_tile tile, bool q_first, const product_arguments &p, const product_arguments &q, hipStream_t stream) {
+void NAME_OF(launch_gradients_, TIRAMISU_OPERAND)(product_tile tile, bool q_first, const product_arguments &p, const product_arguments &q, const column_sums &sums, hipStream_t stream) {
     constexpr int E = TIRAMISU_OPERAND;
     typedef tiles_for<E, true, false, LINEAR> of_input;
     typedef tiles_for<E, false, false, LINEAR> of_weights;
-    if (q_first) launch_pair_of<E, of_weights, of_input>(tile, q, p, stream);
-    else launch_pair_of<E, of_input, of_weights>(tile, p, q, stream);
+    if (q_first) launch_pair_of<E, of_weights, of_input>(tile, q, p, sums, stream);
+    else launch_pair_of<E, of_input, of_weights>(tile, p, q, sums, stream);
 }
 #endif
 

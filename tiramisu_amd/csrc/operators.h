@@ -7,6 +7,7 @@
 namespace tops {
 
 struct product_arguments;
+struct column_sums;
 
 // How a product's operands lie: k along the rows of both (forward), of A alone (gradient of the input), of neither (gradient of the weights).
 enum product_layout { FORWARD, INPUT_GRADIENT, WEIGHT_GRADIENT };
@@ -19,9 +20,11 @@ void launch_tiles_F16(product_tile, product_layout, int epilogue, int y, const p
 void launch_tiles_BF16(product_tile, product_layout, int epilogue, int y, const product_arguments &, int splits, hipStream_t stream);
 void launch_tiles_F8(product_tile, product_layout, int epilogue, int y, const product_arguments &, int splits, hipStream_t stream);
 
-// The gradient of the input (p) and of the weights (q) in one launch, on the same tiles; `q_first`: the longer one begins.
-void launch_gradients_F16(product_tile, bool q_first, const product_arguments &p, const product_arguments &q, hipStream_t stream);
-void launch_gradients_BF16(product_tile, bool q_first, const product_arguments &p, const product_arguments &q, hipStream_t stream);
+// The gradient of the input (p) and of the weights (q) in one launch, on the same tiles; `q_first`: the longer one begins; and behind them `sums`.
+void launch_gradients_F16(product_tile, bool q_first, const product_arguments &p, const product_arguments &q, const column_sums &sums,
+                          hipStream_t stream);
+void launch_gradients_BF16(product_tile, bool q_first, const product_arguments &p, const product_arguments &q, const column_sums &sums,
+                          hipStream_t stream);
 
 }  // namespace tops
 

@@ -35,8 +35,9 @@ __attribute__((format(printf, 2, 3))) int refuse(const char *fn, const char *for
 
 constexpr uint64_t MOST = 0x3fffffff;                    // rows and columns are counted in 31 bits, with room for a tile
 constexpr int64_t MOST_ROWS_A_LAUNCH = 1 << 22;          // of a workgroup each: a launch holds 2^32 threads
+constexpr int64_t MOST_PIECES_A_LAUNCH = 1LL << 31;      // of a thread each
 constexpr uint64_t MOST_TILES = (1 << 23) - 1;           // of 64 x 64: the same
-constexpr uint64_t MOST_COLUMNS = 1 << 26;               // of a norm: the same for the sums of its columns
+constexpr uint64_t MOST_COLUMNS = 1 << 26;               // of a norm: the same for the sums of the columns
 constexpr long MOST_FEW_COLUMNS = 1 << 26;               // of a product of few tokens
 constexpr int64_t MOST_ROW_BYTES = 1 << 22;              // of an operand with k along its rows: a tile's offsets stay below 2^31
 constexpr int64_t MOST_STEP = 1 << 23;                   // elements from k to k of one with k down its columns: the same
@@ -46,7 +47,7 @@ int bytes_of(int type) { return type == F32 ? 4 : type == F8 ? 1 : 2; }
 
 // ---- scratch.  A block for each use and power of two of bytes: a block, once given, stays where it is until
 // tiramisu_hip_release_cached_memory(), so that launches recorded into a graph keep theirs.
-enum scratch_use { GRADIENT, PARTIAL, MOVED_A, MOVED_B, MOVED_C, MOVED_D, COLUMN_SUMS, SCRATCH_USES };
+enum scratch_use { GRADIENT, PARTIAL, MOVED_A, MOVED_B, MOVED_C, COLUMN_SUMS, SCRATCH_USES };
 void *scratch(scratch_use use, uint64_t bytes) {
     static char sites[SCRATCH_USES][64];
     int log2 = 16;
@@ -64,9 +65,13 @@ operand moved_where_needed(const operand &o, long rows, long columns, int bytes,
     if (rows <= 0 || columns <= 0 || loadable(o, bytes, k_along_rows)) return o;
     const long to = (columns * bytes + 15) / 16 * 16;
     char *out = (char *)scratch(use, (uint64_t)(to * rows));
-    const unsigned blocks = (unsigned)((to / 16 * rows + 255) / 256);
-    if (bytes == 1) hipLaunchKernelGGL(move_rows_kernel<1>, dim3(blocks), dim3(256), 0, stream(), (const char *)o.p, out, rows, columns * bytes, o.ld * bytes, to);
-    else hipLaunchKernelGGL(move_rows_kernel<2>, dim3(blocks), dim3(256), 0, stream(), (const char *)o.p, out, rows, columns * bytes, o.ld * bytes, to);
+    for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / (to / 16)); first < rows; first += most) {
+        const long n = std::min(most, rows - first);
+        const unsigned blocks = (unsigned)((to / 16 * n + 255) / 256);
+        const char *in = (const char *)o.p + first * o.ld * bytes;
+        if (bytes == 1) hipLaunchKernelGGL(move_rows_kernel<1>, dim3(blocks), dim3(256), 0, stream(), in, out + first * to, n, columns * bytes, o.ld * bytes, to);
+        else hipLaunchKernelGGL(move_rows_kernel<2>, dim3(blocks), dim3(256), 0, stream(), in, out + first * to, n, columns * bytes, o.ld * bytes, to);
+    }
     check(hipGetLastError(), "tiramisu_hip_linear");
     return {out, to / bytes};
 }
@@ -116,6 +121,7 @@ pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
     for (const tile_model &t : TILES_16_BITS) {
         auto tiles_of = [&](long m, long n) { return ((m + t.rows - 1) / t.rows) * ((n + t.columns - 1) / t.columns); };
         const long units = ttarget::COMPUTE_UNITS, tiles[2] = {tiles_of(M, N), tiles_of(M2, N2)};
+        if (tiles[0] + tiles[1] > (long)MOST_TILES / 2) continue;          // (workgroups of up to 512 threads, and those of sums)
         const double busy = std::min(1.0, (double)(tiles[0] + tiles[1]) / units);
         double each[2];
         for (int i = 0; i < 2; i++) each[i] = (double)(((i ? K2 : K) + 63) / 64) * (t.first + busy * t.full) + t.round;
@@ -161,14 +167,22 @@ int launch_product(const char *fn, int type, product_layout layout, int epilogue
     return 0;
 }
 
-// p: gradient of the input, q: of the weights; what is not asked for has no place for its result
-int launch_gradients(const char *fn, int type, const product_arguments &p, const product_arguments &q) {
+template <int E>
+void launch_sums(const char *fn, const column_sums &a) {
+    hipLaunchKernelGGL(sum_parts_kernel<E>, dim3((unsigned)((a.columns + SUM_COLUMNS - 1) / SUM_COLUMNS)), dim3(1024), 0, stream(), a);
+    check(hipGetLastError(), fn);
+}
+
+// p: gradient of the input, q: of the weights; what is not asked for has no place for its result.  sums: the bias's gradient, which the one launch of both
+// gradients takes along (4096 x 4096 x 1024: 64 us; as a launch of their own ahead of it 63 and 4.7).
+int launch_gradients(const char *fn, int type, const product_arguments &p, const product_arguments &q, const column_sums &sums) {
     const bool both = p.y && q.y && p.M && p.N && q.M && q.N;
     const pair_plan plan = both ? plan_for_pair(p.M, p.N, p.a_more ? 2L * p.K : p.K, q.M, q.N, q.K) : pair_plan();
     if (both && plan.together) {
-        (type == BF16 ? launch_gradients_BF16 : launch_gradients_F16)(plan.tile, plan.q_first, p, q, stream());
+        (type == BF16 ? launch_gradients_BF16 : launch_gradients_F16)(plan.tile, plan.q_first, p, q, sums, stream());
         return 0;
     }
+    if (sums.parts) type == BF16 ? launch_sums<BF16>(fn, sums) : launch_sums<F16>(fn, sums);
     if (p.y)
         if (const int rc = launch_product(fn, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
     return q.y ? launch_product(fn, type, WEIGHT_GRADIENT, LINEAR, type, q) : 0;
@@ -271,12 +285,6 @@ int norm(const char *fn, int type, int y, norm_arguments a) {
 }
 
 template <int E>
-void sum_parts(const char *fn, const float *partial, int parts, long columns, void *out) {
-    hipLaunchKernelGGL(sum_parts_kernel<E>, dim3((unsigned)((columns + 31) / 32)), dim3(1024), 0, stream(), partial, parts, columns, (stored<E> *)out);
-    check(hipGetLastError(), fn);
-}
-
-template <int E>
 void launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweight) {
     constexpr int N = E == F32 ? 4 : 8;
     const long pieces = (a.columns + N - 1) / N;
@@ -300,22 +308,23 @@ void launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweig
         hipLaunchKernelGGL(rms_norm_backward_long_columns_kernel<E>, dim3((unsigned)((a.columns + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream(), a);
     }
     check(hipGetLastError(), fn);
-    sum_parts<E>(fn, a.partial, a.parts, a.columns, dweight);
+    launch_sums<E>(fn, {a.partial, dweight, a.columns, a.parts});
 }
 
-// dz and the bias's gradient; what is null is not computed
+// dz, and what the bias's gradient is the sums of; what is null is not computed
 template <int E>
-void launch_activation_backward(const char *fn, activation_backward_arguments a, void *dbias) {
+column_sums launch_activation_backward(const char *fn, activation_backward_arguments a, void *dbias) {
     a.across = 1;
     while (a.across < 64 && a.across * 8 < a.N) a.across *= 2;
     const long columns = (a.N + 8L * a.across - 1) / (8L * a.across), down = 256 / a.across;
-    const long chunks = std::max(1L, std::min((a.M + 4 * down - 1) / (4 * down), std::max(1L, 1024 / columns)));
+    // workgroups: one row to a thread where there are few, and few enough that their sums are little beside the rows
+    const long chunks = std::max(1L, std::min((a.M + down - 1) / down, std::min(256L, std::max(1L, 1024 / columns))));
     a.rows = std::max(1L, (a.M + chunks - 1) / chunks);
     const int used = (int)std::max(1L, (a.M + a.rows - 1) / a.rows);
     a.partial = dbias ? (float *)scratch(COLUMN_SUMS, (uint64_t)used * a.N * 4) : nullptr;
     hipLaunchKernelGGL(activation_backward_kernel<E>, dim3((unsigned)columns, (unsigned)used), dim3(256), 0, stream(), a);
     check(hipGetLastError(), fn);
-    if (dbias) sum_parts<E>(fn, a.partial, used, a.N, dbias);
+    return {a.partial, dbias, a.N, dbias ? used : 0};
 }
 
 product_arguments product_of(long M, long N, long K) {
@@ -449,6 +458,7 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
     timed record(__FUNCTION__);
     const long m = (long)M, n = (long)N, k = (long)K;
     operand dz = {dy, ldy ? (long)ldy : n};
+    column_sums sums = {};
     // the gradient ahead of the activation; without one it is dy, moved only where the tiles cannot load it
     if (n > 0 && (activation != NONE || dbias)) {
         activation_backward_arguments a = {dy, pre, nullptr, nullptr, m, n, dz.ld, ldp ? (long)ldp : n, 0, 0, activation, 0};
@@ -457,8 +467,7 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
             a.dz = scratch(GRADIENT, (uint64_t)std::max(1L, m) * a.ldz * 2);
             dz = {a.dz, a.ldz};
         }
-        if (type == F16) launch_activation_backward<F16>(__FUNCTION__, a, dbias);
-        else launch_activation_backward<BF16>(__FUNCTION__, a, dbias);
+        sums = type == F16 ? launch_activation_backward<F16>(__FUNCTION__, a, dbias) : launch_activation_backward<BF16>(__FUNCTION__, a, dbias);
     }
     if (!loadable(dz, 2, true) || !loadable(dz, 2, false)) dz = moved_where_needed({dz.p, dz.ld}, m, n, 2, true, GRADIENT);
     product_arguments p = product_of(m, k, n), q = product_of(n, k, m);
@@ -476,7 +485,7 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
         q.b = xs.p;
         q.ldb = xs.ld;
     }
-    return launch_gradients(__FUNCTION__, type, p, q);
+    return launch_gradients(__FUNCTION__, type, p, q, sums);
 }
 
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate, const void *up,
@@ -523,7 +532,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
         q.rows_above = (int)n;
         q.split_row = (int)half;
     }
-    return launch_gradients(__FUNCTION__, type, p, q);
+    return launch_gradients(__FUNCTION__, type, p, q, {});
 }
 
 float *tiramisu_hip_no_buffer(void) { return nullptr; }       // (a pointer that is also one to scales)
