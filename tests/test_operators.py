@@ -516,6 +516,20 @@ def test_calls_in_a_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES + [F8])
+@pytest.mark.parametrize("M,N,K", [(1030, 1990, 130), (1500, 1000, 77), (960, 1700, 512)])
+def test_linear_of_some_two_hundred_tiles(M, N, K, dtype):
+    test_linear(M, N, K, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("M,N,K", [(1030, 130, 990), (1000, 700, 500), (77, 1100, 1500)])
+def test_linear_backward_of_some_two_hundred_tiles(M, N, K, dtype):
+    test_linear_backward(M, N, K, dtype)
+
+
+@pytest.mark.gpu
 def test_a_graph_recorded_without_a_call_before():
     """Scratch (the activation's gradient, rows that are moved, sums of columns) is allocated while the stream records."""
     g = generator(89)

@@ -54,6 +54,7 @@ template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
     typedef tile_config<E, 256, 256, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, E == F8 ? 32 : 16> tile_256;
     typedef tile_config<E, 256, 128, 4, 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_256x128;
     typedef tile_config<E, 128, 128, 4, 2, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128;
+    typedef tile_config<E, 128, EPILOGUE == GATED ? 128 : 64, 4, 2, EPILOGUE == GATED ? 4 : 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128x64;      // (gated: the one before)
     typedef tile_config<E, 64, EPILOGUE == GATED ? 128 : 64, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
 };
 template <int E, int Y, bool A_ROWS, bool B_ROWS, int EPILOGUE>
@@ -62,6 +63,7 @@ void launch_tile(product_tile tile, const product_arguments &p, int splits, hipS
     if (tile == TILE_256) launch<typename T::tile_256, Y>(p, splits, stream);
     else if (tile == TILE_256x128) launch<typename T::tile_256x128, Y>(p, splits, stream);
     else if (tile == TILE_128) launch<typename T::tile_128, Y>(p, splits, stream);
+    else if (tile == TILE_128x64) launch<typename T::tile_128x64, Y>(p, splits, stream);
     else launch<typename T::tile_64, Y>(p, splits, stream);
 }
 
@@ -71,6 +73,7 @@ void launch_pair_of(product_tile tile, const product_arguments &p, const product
     if (tile == TILE_256) launch_pair<typename P::tile_256, typename Q::tile_256, E>(p, q, sums, stream);
     else if (tile == TILE_256x128) launch_pair<typename P::tile_256x128, typename Q::tile_256x128, E>(p, q, sums, stream);
     else if (tile == TILE_128) launch_pair<typename P::tile_128, typename Q::tile_128, E>(p, q, sums, stream);
+    else if (tile == TILE_128x64) launch_pair<typename P::tile_128x64, typename Q::tile_128x64, E>(p, q, sums, stream);
     else launch_pair<typename P::tile_64, typename Q::tile_64, E>(p, q, sums, stream);
 }
 

@@ -13,7 +13,7 @@ struct column_sums;
 enum product_layout { FORWARD, INPUT_GRADIENT, WEIGHT_GRADIENT };
 
 // The tiles, by rows and columns of the product (a gated layer's columns count twice).
-enum product_tile { TILE_256, TILE_256x128, TILE_128, TILE_64 };
+enum product_tile { TILE_256, TILE_256x128, TILE_128, TILE_128x64, TILE_64 };
 
 // Launches on `stream`; splits > 1: partial sums to arguments.partial, without the epilogue.  y: element type of the outputs.
 void launch_tiles_F16(product_tile, product_layout, int epilogue, int y, const product_arguments &, int splits, hipStream_t stream);

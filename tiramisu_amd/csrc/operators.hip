@@ -78,22 +78,26 @@ operand moved_where_needed(const operand &o, long rows, long columns, int bytes,
 
 // ---- which tile, and how many workgroups share the k of one.  A launch is modelled in microseconds: `fixed`, for every slice of 128 bytes of k `first` for the first
 // round of tiles over the compute units (and `full` as far as it fills them), and for every further round `round` and `further` a slice.
-// Splitting k adds a launch and the partial sums' bytes at 4 TB/s.  Fitted to launches of 16 ... 4096 tiles of 8 ... 64 slices (tables of
+// Splitting k adds a launch and the partial sums' bytes, which caches hold, at 8 TB/s.  Fitted to launches of 16 ... 4096 tiles of 8 ... 64 slices (tables of
 // 29 configurations; rms error 6 %); us with 256 x 256, 256 x 128, 128 x 128 and 64 x 64 tiles, bf16: 4096^3 102, 115, 149, 190; 4096 x 1024 x 4096 74, 48, 35, 50;
-// 1024^3 24, 15.5, 11, 7.0; 128 x 4096 x 4096 70, 45, 29, 18.
-struct tile_model { product_tile tile; int rows, columns; double fixed, first, full, round, further; };
-constexpr tile_model TILES_16_BITS[] = {{TILE_256, 256, 256, 9.0, 0.94, 0.5, 4.0, 1.44}, {TILE_256x128, 256, 128, 5.8, 0.6, 0.15, 7.0, 0.75},
-                                        {TILE_128, 128, 128, 4.8, 0.38, 0.09, 0.8, 0.58}, {TILE_64, 64, 64, 3.5, 0.2, 0.03, 0.7, 0.155}};
-constexpr tile_model TILES_8_BITS[] = {{TILE_256, 256, 256, 13.8, 0.8, 0.6, 9.0, 1.4}, {TILE_256x128, 256, 128, 9.6, 0.44, 0.24, 13.5, 0.69},
-                                       {TILE_128, 128, 128, 7.0, 0.26, 0.24, 4.7, 0.467}, {TILE_64, 64, 64, 4.8, 0.13, 0.02, 0.7, 0.19}};
+// 1024^3 24, 15.5, 11, 7.0; 128 x 4096 x 4096 70, 45, 29, 18.  128 x 64 tiles lie between (128 x 128, 128 x 64, 64 x 64): 1024 x 2048 x 1024 bf16 10.3, 8.2, 9.4,
+// 512 x 4096 x 2048 16.3, 12.9, 16.0, 2000 x 1500 x 1000 12.8, 15.8, 17.8; e4m3 9.2, 7.0, 7.2, 11.5, 8.8, 10.7 and 11.0, 11.0, 11.3.
+struct tile_model { product_tile tile; int rows, columns; double fixed, first, full, round, further, pair_round, pair_slice; };
+constexpr tile_model TILES_16_BITS[] = {{TILE_256, 256, 256, 9.0, 0.94, 0.5, 4.0, 1.44, 4.0, 1.44}, {TILE_256x128, 256, 128, 5.8, 0.6, 0.15, 7.0, 0.75, 3.0, 0.75},
+                                        {TILE_128, 128, 128, 4.8, 0.38, 0.09, 0.8, 0.58, 0.8, 0.58}, {TILE_128x64, 128, 64, 4.0, 0.24, 0.03, 0.8, 0.32, 0.8, 0.32},
+                                        {TILE_64, 64, 64, 3.5, 0.2, 0.03, 0.7, 0.155, 0.7, 0.18}};
+constexpr tile_model TILES_8_BITS[] = {{TILE_256, 256, 256, 13.8, 0.8, 0.6, 9.0, 1.4, 0, 0}, {TILE_256x128, 256, 128, 9.6, 0.44, 0.24, 13.5, 0.69, 0, 0},
+                                       {TILE_128, 128, 128, 7.0, 0.26, 0.24, 4.7, 0.467, 0, 0}, {TILE_128x64, 128, 64, 5.2, 0.15, 0.07, 0.9, 0.4, 0, 0},
+                                       {TILE_64, 64, 64, 4.8, 0.13, 0.02, 0.7, 0.19, 0, 0}};
 // (a gated layer's smallest tile is 64 x 128: 64 columns of gate and the same of up)
-constexpr tile_model GATED_64_16_BITS = {TILE_64, 64, 128, 3.9, 0.27, 0.08, 0.7, 0.31}, GATED_64_8_BITS = {TILE_64, 64, 128, 5.4, 0.13, 0.05, 0.7, 0.3};
+constexpr tile_model GATED_64_16_BITS = {TILE_64, 64, 128, 3.9, 0.27, 0.08, 0.7, 0.31, 0, 0}, GATED_64_8_BITS = {TILE_64, 64, 128, 5.4, 0.13, 0.05, 0.7, 0.3, 0, 0};
 struct tile_plan { product_tile tile; int splits, slices; double cost; };
 tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
     const long slices = std::max(1L, (K * bytes + 127) / 128);
     tile_plan best = {TILE_64, 0, 0, 0.0};
     double best_cost = 0;
     auto consider = [&](const tile_model &t) {
+        if (gated && t.tile == TILE_128x64) return;
         const long tiles = ((M + t.rows - 1) / t.rows) * ((N * (gated ? 2 : 1) + t.columns - 1) / t.columns);
         for (long splits = 1; splits <= 16 && splits <= slices; splits++) {
             const long each = (slices + splits - 1) / splits;
@@ -101,7 +105,7 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
             if ((slices + each - 1) / each != splits) continue;            // (the same slices to each as with fewer)
             const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
             double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
-            if (splits > 1) cost += 5.5 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 4e6;
+            if (splits > 1) cost += 4.0 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 8e6;
             if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each, cost}; best_cost = cost; }
         }
     };
@@ -112,8 +116,11 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
     return best;
 }
 
-// Both gradients in one launch: tiles of the longer product first, then those of the other on compute units as they become free.  Modelled from the
-// same figures, against the two launches one after the other (about 2 us more than their sum).
+// Both gradients in one launch: tiles of the longer product first, then those of the other on compute units as they become free.  Modelled like one
+// product, with `pair_slice` and `pair_round` for tiles of more than a round (slices of the two kinds take their time together; over 23 pairs the choices are 2 %
+// behind the best ones in the mean), against the two launches one after the other (about 2 us more than their sum).  us as 256 x 256, 256 x 128, 128 x 128,
+// 128 x 64, 64 x 64 tiles and apart: 4096 x 4096 x 1024 86, 62, 77, 85, 107, 73; 1024 x 4096 x 1024 73, 44, 31, 27, 31, 35; 2048^3 47, 34, 41, 46, 56, 44;
+// 1000 x 700 x 500 25, 16, 11, 9.4, 7.8, 13.5.
 struct pair_plan { product_tile tile; bool together, q_first; };
 pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
     pair_plan best = {TILE_64, false, false};
@@ -124,7 +131,8 @@ pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
         if (tiles[0] + tiles[1] > (long)MOST_TILES / 2) continue;          // (workgroups of up to 512 threads, and those of sums)
         const double busy = std::min(1.0, (double)(tiles[0] + tiles[1]) / units);
         double each[2];
-        for (int i = 0; i < 2; i++) each[i] = (double)(((i ? K2 : K) + 63) / 64) * (t.first + busy * t.full) + t.round;
+        const double slice = tiles[0] + tiles[1] <= units ? t.first + busy * t.full : t.pair_slice;
+        for (int i = 0; i < 2; i++) each[i] = (double)(((i ? K2 : K) + 63) / 64) * slice + t.pair_round;
         const int a = each[0] >= each[1] ? 0 : 1, b = 1 - a;
         // whole rounds of the first kind, its last tiles, and how many of the second are done when
         const long rounds = tiles[a] / units, last = tiles[a] % units;
