@@ -78,7 +78,7 @@ operand moved_where_needed(const operand &o, long rows, long columns, int bytes,
 
 // ---- which tile, and how many workgroups share the k of one.  A launch is modelled in microseconds: `fixed`, for every slice of 128 bytes of k `first` for the first
 // round of tiles over the compute units (and `full` as far as it fills them), and for every further round `round` and `further` a slice.
-// Splitting k adds a launch and the partial sums' bytes, which caches hold, at 8 TB/s.  Fitted to launches of 16 ... 4096 tiles of 8 ... 64 slices (tables of
+// Splitting k adds a launch and the partial sums' bytes, which caches hold in part, at 5 TB/s.  Fitted to launches of 16 ... 4096 tiles of 8 ... 64 slices (tables of
 // 29 configurations; rms error 6 %); us with 256 x 256, 256 x 128, 128 x 128 and 64 x 64 tiles, bf16: 4096^3 102, 115, 149, 190; 4096 x 1024 x 4096 74, 48, 35, 50;
 // 1024^3 24, 15.5, 11, 7.0; 128 x 4096 x 4096 70, 45, 29, 18.  128 x 64 tiles lie between (128 x 128, 128 x 64, 64 x 64): 1024 x 2048 x 1024 bf16 10.3, 8.2, 9.4,
 // 512 x 4096 x 2048 16.3, 12.9, 16.0, 2000 x 1500 x 1000 12.8, 15.8, 17.8; e4m3 9.2, 7.0, 7.2, 11.5, 8.8, 10.7 and 11.0, 11.0, 11.3.
@@ -105,7 +105,7 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
             if ((slices + each - 1) / each != splits) continue;            // (the same slices to each as with fewer)
             const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
             double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
-            if (splits > 1) cost += 4.0 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 8e6;
+            if (splits > 1) cost += 5.5 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 5e6;
             if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each, cost}; best_cost = cost; }
         }
     };
