@@ -50,6 +50,20 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
 #pragma unroll
         for (int i = 0; i < TILES; i++) acc[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // what the epilogue of 8 columns of row m reads, ahead of the product
+    const int id = threadIdx.x, m = id >> 1, c0 = 8 * (id & 1);
+    const long n = n0 + c0;
+    const int some = (int)min(8L, p.N - n);
+    const bool mine = m < p.M && m < 16 * TILES && some > 0;
+    column_pieces pieces;
+    u32x4 residual = {0, 0, 0, 0};
+    float scale = 1.f;
+    if (mine) {
+        load_column_pieces(p, pieces, n, some);
+        if (EPILOGUE == LINEAR && p.residual) residual = load_guarded<2>((const char *)p.residual + 2 * ((long)m * p.ldr + n), 2 * some);
+        if (E == F8) scale = p.a_scale[m];
+    }
+
     const int whole = (int)(bytes / 128), units = (int)((bytes + 127) / 128);
     int u = wave;
     // as many units at a time as are left, by halves
@@ -103,10 +117,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
 #pragma unroll
         for (int i = 0; i < TILES; i++) sums[((wave * PARTS + q) * TILES + i) * 64 + lane] = acc[q][i];
     __syncthreads();
-    const int id = threadIdx.x, m = id >> 1, c0 = 8 * (id & 1);            // 8 columns of row m
-    const long n = n0 + c0;
-    const int some = (int)min(8L, p.N - n);
-    if (m >= p.M || m >= 16 * TILES || some <= 0) return;
+    if (!mine) return;
     float z[PARTS][8];
 #pragma unroll
     for (int q = 0; q < PARTS; q++) {
@@ -122,9 +133,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
             }
     }
     column_terms columns;
-    load_column_terms<Y>(p, columns, n, some);
-    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z[0], z[1], m, n, some);
-    else finish_linear<Y>(p, columns, z[0], m, n, some);
+    widen_column_pieces<Y>(p, pieces, columns);
+    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z[0], z[1], scale, m, n, some);
+    else {
+        float r[8];
+        widen<Y>(residual, r);
+        finish_linear<Y>(p, columns, z[0], r, scale, m, n, some);
+    }
 }
 
 }  // namespace tops

@@ -359,27 +359,30 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
 }
 
 // ---- epilogues: 8 columns from n on of row m; `some`: how many of them exist
-// (what belongs to the columns is loaded once for all rows of a strip)
+// (what belongs to the columns is loaded once for all rows; bias: as it lies in memory)
+struct column_pieces { u32x4 bias; float scale[8], scale_2[8]; };
 struct column_terms { float bias[8], scale[8], scale_2[8]; };
-template <int Y>
-__device__ __forceinline__ void load_column_terms(const product_arguments &p, column_terms &c, long n, int some) {
-    if (p.bias) load_some<Y>((const stored<Y> *)p.bias + n, some, c.bias);
+__device__ __forceinline__ void load_column_pieces(const product_arguments &p, column_pieces &c, long n, int some) {
+    if (p.bias) c.bias = load_guarded<2>((const char *)p.bias + 2 * n, 2 * some);
     if (p.b_scale) load_some<F32>(p.b_scale + n, some, c.scale);
     if (p.b2_scale) load_some<F32>(p.b2_scale + n, some, c.scale_2);
 }
 template <int Y>
-__device__ __forceinline__ void activate_linear(const product_arguments &p, const column_terms &c, float (&z)[8], long m, long n, int some) {
-    if (p.a_scale) {
-        const float s = p.a_scale[m];
+__device__ __forceinline__ void widen_column_pieces(const product_arguments &p, const column_pieces &from, column_terms &c) {
+    if (p.bias) widen<Y>(from.bias, c.bias);
 #pragma unroll
-        for (int i = 0; i < 8; i++) z[i] *= s * c.scale[i];
+    for (int i = 0; i < 8; i++) { c.scale[i] = from.scale[i]; c.scale_2[i] = from.scale_2[i]; }
+}
+// z: the product's sums; row_scale: of row m of a
+__device__ __forceinline__ void scale_linear(const product_arguments &p, const column_terms &c, float (&z)[8], float row_scale) {
+    if (p.a_scale) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] *= row_scale * c.scale[i];
     }
     if (p.bias) {
 #pragma unroll
         for (int i = 0; i < 8; i++) z[i] += c.bias[i];
     }
-    if (p.pre) store_some<Y>((stored<Y> *)p.pre + m * p.N + n, some, z);
-    activate(p.activation, z);
 }
 template <int Y>
 __device__ __forceinline__ void load_residual(const product_arguments &p, float (&r)[8], long m, long n, int some) {
@@ -392,10 +395,11 @@ __device__ __forceinline__ void store_linear(const product_arguments &p, const f
     else if (m >= p.split_row) store_some<Y>((T *)p.y_below + (m - p.split_row) * p.N + n, some, z);
 }
 template <int Y>
-__device__ __forceinline__ void finish_linear(const product_arguments &p, const column_terms &c, float (&z)[8], long m, long n, int some) {
-    float r[8];
-    if (p.residual) load_residual<Y>(p, r, m, n, some);
-    activate_linear<Y>(p, c, z, m, n, some);
+__device__ __forceinline__ void finish_linear(const product_arguments &p, const column_terms &c, float (&z)[8], const float (&r)[8], float row_scale, long m, long n,
+                                              int some) {
+    scale_linear(p, c, z, row_scale);
+    if (p.pre) store_some<Y>((stored<Y> *)p.pre + m * p.N + n, some, z);
+    activate(p.activation, z);
     if (p.residual) {
 #pragma unroll
         for (int i = 0; i < 8; i++) z[i] += r[i];
@@ -403,12 +407,11 @@ __device__ __forceinline__ void finish_linear(const product_arguments &p, const 
     store_linear<Y>(p, z, m, n, some);
 }
 template <int Y>
-__device__ __forceinline__ void finish_gated(const product_arguments &p, const column_terms &c, float (&g)[8], float (&u)[8], long m, long n, int some) {
+__device__ __forceinline__ void finish_gated(const product_arguments &p, const column_terms &c, float (&g)[8], float (&u)[8], float row_scale, long m, long n, int some) {
     typedef stored<Y> T;
     if (p.a_scale) {
-        const float s = p.a_scale[m];
 #pragma unroll
-        for (int i = 0; i < 8; i++) { g[i] *= s * c.scale[i]; u[i] *= s * c.scale_2[i]; }
+        for (int i = 0; i < 8; i++) { g[i] *= row_scale * c.scale[i]; u[i] *= row_scale * c.scale_2[i]; }
     }
     if (p.pre) {
         store_some<Y>((T *)p.pre + m * p.N + n, some, g);
@@ -448,32 +451,50 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
         for (int j = 0; j < C::TN; j++)
 #pragma unroll
             for (int r = 0; r < REGISTERS; r++) acc[i][j][r] = 0.f;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WGN, wn = wave % C::WGN;
+    constexpr int SPAN = C::EPILOGUE == GATED ? C::WN / 2 : C::WN;         // columns of C of a wavefront
+    constexpr int ACROSS = SPAN / 8, DOWN = 64 / ACROSS;                   // lanes along a row, rows of one pass
+    constexpr int PASSES = 32 / DOWN, STRIPS = C::WM / 32;
+    const int r0 = lane / ACROSS, c0 = 8 * (lane % ACROSS);
+    const long n = n0 + wn * SPAN + c0;
+    const int some = (int)min(8L, p.N - n);
+    // Bias and scales, where there are registers for them ahead of the product, which then covers their way from memory (e4m3, loaded behind the product /
+    // ahead of it: 1024 x 4096 x 1024 9.8 / 8.6 us, 3000 x 700 x 2000 12.8 / 11.9, 1024 x 2048 x 1024 6.8 / 6.3).  A lane holds the scales of rows lane % 32 of the strips.
+    constexpr bool TERMS = C::A_ROWS && C::B_ROWS, EARLY = C::TM * C::TN * REGISTERS <= 64;
+    column_pieces pieces;
+    float row_scales[STRIPS];
+    auto load_terms = [&] {
+        if (!TERMS || p.partial) return;
+        if (some > 0) load_column_pieces(p, pieces, n, some);
+        if constexpr (C::E == F8)
+#pragma unroll
+            for (int i = 0; i < STRIPS; i++) {
+                const long m = m0 + wm * C::WM + i * 32 + lane % 32;
+                row_scales[i] = p.a_scale[min(m, p.M - 1L)];
+            }
+    };
+    if constexpr (EARLY) load_terms();
     const long k0 = p.partial ? (long)split * p.slices_per_split * C::BK : 0;
     const long K = p.partial ? min((long)p.slices_per_split * C::BK, p.K - k0) : p.K;
     accumulate<C>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds);
     if constexpr (C::EPILOGUE == LINEAR && C::A_ROWS && !C::B_ROWS)        // (only the gradient of a gated layer's input has two)
         if (p.a_more) accumulate<C>(acc, p.a_more, p.lda, p.b_more, p.ldb_more, nullptr, 0, p.M, p.N, m0, n0, k0, K, lds);
 
+    if constexpr (!EARLY) load_terms();
+    column_terms columns;
+    if (TERMS && some > 0 && !p.partial) widen_column_pieces<Y>(p, pieces, columns);
+
     // A wavefront's strips of 32 rows, through LDS of its own: stored by columns of the accumulators, read by rows.
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / C::WGN, wn = wave % C::WGN, at = lane % F, group = lane / F;
+    const int at = lane % F, group = lane / F;
     __attribute__((address_space(3))) float *const strip = (__attribute__((address_space(3))) float *)lds + wave * 32 * C::STRIP;
     typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-    constexpr int SPAN = C::EPILOGUE == GATED ? C::WN / 2 : C::WN;         // columns of C of a wavefront
-    constexpr int ACROSS = SPAN / 8, DOWN = 64 / ACROSS;                   // lanes along a row, rows of one pass
-    const int r0 = lane / ACROSS, c0 = 8 * (lane % ACROSS);
-    const long n = n0 + wn * SPAN + c0;
-    const int some = (int)min(8L, p.N - n);
-    constexpr int PASSES = 32 / DOWN;
-    column_terms columns;
-    if (some > 0 && !p.partial) load_column_terms<Y>(p, columns, n, some);
     auto order_lanes = [] {                                               // what the lanes of a wavefront pass to each other
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
 #pragma unroll
-    for (int i = 0; i < C::WM / 32; i++) {
+    for (int i = 0; i < STRIPS; i++) {
         const long first = m0 + wm * C::WM + i * 32 + r0;                 // the lane's row of pass 0
         const bool across = some > 0;
         auto take = [&](int pass, int c, float (&v)[8]) {
@@ -485,7 +506,7 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
         constexpr bool RESIDUAL = C::EPILOGUE == LINEAR && C::A_ROWS && C::B_ROWS;
         float r[RESIDUAL ? PASSES : 1][8];
         if constexpr (RESIDUAL)
-            if (p.residual && !p.partial && !(p.a_scale || p.bias || p.pre || p.activation != NONE)) {
+            if (p.residual && !p.partial && !(p.pre || p.activation != NONE)) {
 #pragma unroll
                 for (int pass = 0; pass < PASSES; pass++)
                     if (across && first + pass * DOWN < p.M) load_residual<Y>(p, r[pass], first + pass * DOWN, n, some);
@@ -500,6 +521,7 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
                     *(lds_f32x4 *)(strip + (b * F + at) * C::STRIP + j * F + 8 * g + 4 * group) = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
                 }
         order_lanes();
+        auto row_scale = [&](int pass) { return C::E == F8 ? __shfl(row_scales[i], pass * DOWN + r0) : 1.f; };       // (by all lanes)
         if (p.partial) {
 #pragma unroll 1
             for (int pass = 0; pass < PASSES; pass++) {
@@ -520,32 +542,38 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
                 float z[8], u[8];
                 take(pass, c0, z);
                 take(pass, SPAN + c0, u);
-                if (across && first + pass * DOWN < p.M) finish_gated<Y>(p, columns, z, u, first + pass * DOWN, n, some);
+                const float scale = row_scale(pass);
+                if (across && first + pass * DOWN < p.M) finish_gated<Y>(p, columns, z, u, scale, first + pass * DOWN, n, some);
             }
         } else {
             bool plain = true;
-            if constexpr (RESIDUAL) plain = !(p.a_scale || p.bias || p.pre || p.activation != NONE);
+            if constexpr (RESIDUAL) plain = !(p.pre || p.activation != NONE);
             if (plain) {
 #pragma unroll
                 for (int pass = 0; pass < PASSES; pass++) {
+                    const float scale = row_scale(pass);
                     if (!across || first + pass * DOWN >= p.M) continue;
                     float z[8];
                     take(pass, c0, z);
-                    if constexpr (RESIDUAL)
+                    if constexpr (RESIDUAL) {
+                        scale_linear(p, columns, z, scale);
                         if (p.residual) {
 #pragma unroll
                             for (int e = 0; e < 8; e++) z[e] += r[pass][e];
                         }
+                    }
                     store_linear<Y>(p, z, first + pass * DOWN, n, some);
                 }
             } else {
                 // (many instructions: not unrolled)
 #pragma unroll 1
                 for (int pass = 0; pass < PASSES; pass++) {
+                    const float scale = row_scale(pass);
                     if (!across || first + pass * DOWN >= p.M) continue;
-                    float z[8];
+                    float z[8], r[8];
+                    if (p.residual) load_residual<Y>(p, r, first + pass * DOWN, n, some);
                     take(pass, c0, z);
-                    finish_linear<Y>(p, columns, z, first + pass * DOWN, n, some);
+                    finish_linear<Y>(p, columns, z, r, scale, first + pass * DOWN, n, some);
                 }
             }
         }
@@ -601,10 +629,16 @@ __global__ __launch_bounds__(256) void finish_kernel(product_arguments p, int sp
             for (int i = 0; i < 8; i++) u[i] += v[i];
         }
     }
+    column_pieces pieces;
     column_terms columns;
-    load_column_terms<Y>(p, columns, n, some);
-    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z, u, m, n, some);
-    else finish_linear<Y>(p, columns, z, m, n, some);
+    load_column_pieces(p, pieces, n, some);
+    widen_column_pieces<Y>(p, pieces, columns);
+    const float scale = p.a_scale ? p.a_scale[m] : 1.f;
+    if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z, u, scale, m, n, some);
+    else {
+        if (p.residual) load_residual<Y>(p, u, m, n, some);
+        finish_linear<Y>(p, columns, z, u, scale, m, n, some);
+    }
 }
 
 }  // namespace tops
