@@ -81,7 +81,7 @@ int tiramisu_hip_batch_begin(void);
 int tiramisu_hip_batch_end(void);
 
 /* The scratch block that deep reductions of tiramisu_hip_sgemm use on the calling thread's current stream (partial
- * tiles and per-tile counters), or NULL before the first such call: one block per (host thread, stream), so that
+ * tiles and per-tile counters), or NULL before the first such call: one block per (host thread, stream, GPU), so that
  * calls of one thread on two streams may overlap.  No counterpart in the reference; for tests and diagnostics. */
 void *tiramisu_hip_sgemm_workspace(void);
 
@@ -89,7 +89,7 @@ void *tiramisu_hip_sgemm_workspace(void);
  *      frees everything on every call. ---- */
 /* Scratch that a generated function keeps from one call to the next (the third plane of a time-tiled stencil, the
  * hand-over area of the windowed convolution): one block per requesting site (generated code passes the address of
- * a static of its own), host thread and stream, at least `bytes` large, allocated at the first request and handed
+ * a static of its own), host thread, stream and GPU, at least `bytes` large, allocated at the first request and handed
  * out again at every later one.  *fresh (may be NULL) is 1 when this call allocated the block -- its contents are
  * undefined then -- and 0 when it is the block of the call before. */
 void *tiramisu_hip_kept_scratch(const void *site, uint64_t bytes, int32_t *fresh);
@@ -154,7 +154,7 @@ int tiramisu_hip_null_stream_synchronize(void);
 int tiramisu_hip_call(void *function, int32_t arguments, const uint64_t *pointers, const int32_t *description, void *stream);
 /* A new stream that does not synchronise with the default stream (default priority), for callers that overlap
  * calls; destroy waits for the stream's work and, if it is the calling thread's current stream, restores the
- * per-thread default stream.  Scratch blocks that the runtime keeps per (thread, stream) stay allocated until
+ * per-thread default stream.  Scratch blocks that the runtime keeps per (thread, stream, GPU) stay allocated until
  * tiramisu_hip_release_cached_memory. */
 void *tiramisu_hip_stream_create(void);
 int tiramisu_hip_stream_destroy(void *stream);
@@ -170,7 +170,7 @@ int tiramisu_hip_device_count(void);
  *      overlap inputs.  Weights are [outputs][inputs].  Operands may begin at any element; rows that the
  *      matrix kernels cannot load in place (odd strides of 16-bit elements) are moved to scratch first.  Sums are kept in 32 bits and rounded once.
  *      Types and activations are the numbers below.  Arguments that do not fit together are refused: a message on stderr,
- *      return value 1, nothing launched.  Scratch is kept per thread and stream like tiramisu_hip_sgemm's, and stays where it is until
+ *      return value 1, nothing launched.  Scratch is kept per thread, stream and GPU like tiramisu_hip_sgemm's, and stays where it is until
  *      tiramisu_hip_release_cached_memory(): a call recorded into a graph uses at every replay the scratch of the stream it was recorded on,
  *      so work on that stream and replays elsewhere have to wait for each other. ---- */
 enum tiramisu_hip_element_t { TIRAMISU_HIP_FLOAT32 = 0, TIRAMISU_HIP_FLOAT16 = 1, TIRAMISU_HIP_BFLOAT16 = 2, TIRAMISU_HIP_FLOAT8_E4M3 = 3 };

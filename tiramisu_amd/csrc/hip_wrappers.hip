@@ -13,8 +13,10 @@
 #include <cstdlib>
 #include <map>
 #include <mutex>
+#include <set>
 #include <string>
 #include <thread>
+#include <tuple>
 #include <vector>
 
 #include "../../include/tiramisu_hip_wrappers.h"
@@ -388,17 +390,30 @@ void dispatch_splitk(const splitk_plan &p, bool tA, bool tB, bool edge, const fl
 #undef SPLITK_CASE
 }
 
-// Scratch of the allocating entry point: one block per host thread and stream (a call works on the thread's
+// Scratch of the allocating entry point: one block per host thread, stream and GPU (a call works on the thread's
 // current stream, and two calls of one thread on two streams may run at the same time: they must not share partial
 // tiles and counters), grown on demand, kept until the process ends.
 struct splitk_block { void *ptr = nullptr; uint64_t bytes = 0; };
-// (the per-thread default stream is one handle that names a different stream in every thread, hence the thread in the key)
-typedef std::pair<std::thread::id, hipStream_t> thread_and_stream;
-thread_and_stream here() { return {std::this_thread::get_id(), current_stream}; }
+// (the per-thread default stream is one handle that names a different stream in every thread, and the null stream's one that names a different
+// stream on every GPU, hence the thread and the GPU in the key)
+struct place {
+    std::thread::id thread;
+    hipStream_t stream;
+    int device;
+    bool operator<(const place &o) const { return std::tie(thread, stream, device) < std::tie(o.thread, o.stream, o.device); }
+};
+place here() {
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) {           // (without a GPU nothing is kept)
+        (void)hipGetLastError();
+        device = -1;
+    }
+    return {std::this_thread::get_id(), current_stream, device};
+}
 std::mutex kept_mutex;                                                    // guards the two maps below
-std::map<thread_and_stream, splitk_block> splitk_workspaces;
-// Scratch that generated functions keep between their calls (tiramisu_hip_kept_scratch): by requesting site, thread and stream.
-std::map<std::pair<const void *, thread_and_stream>, splitk_block> kept_scratch;
+std::map<place, splitk_block> splitk_workspaces;
+// Scratch that generated functions keep between their calls (tiramisu_hip_kept_scratch): by requesting site, thread, stream and GPU.
+std::map<std::pair<const void *, place>, splitk_block> kept_scratch;
 constexpr uint64_t SPLITK_WORKSPACE_LIMIT = (uint64_t)256 << 20;
 
 // Scratch of the entry point that allocates nothing: lives in the code object, one copy per device.
@@ -749,6 +764,15 @@ uint64_t tiramisu_hip_release_cached_memory(void) {
     uint64_t released = 0;
     {
         std::lock_guard<std::mutex> g(kept_mutex);
+        // (blocks of other GPUs wait for those)
+        int device = 0;
+        check(hipGetDevice(&device), __FUNCTION__);
+        std::set<int> others;
+        for (auto &kv : splitk_workspaces) others.insert(kv.first.device);
+        for (auto &kv : kept_scratch) others.insert(kv.first.second.device);
+        others.erase(device);
+        for (int other : others) { check(hipSetDevice(other), __FUNCTION__); check(hipDeviceSynchronize(), __FUNCTION__); }
+        if (!others.empty()) check(hipSetDevice(device), __FUNCTION__);
         for (auto &kv : splitk_workspaces) if (kv.second.ptr) { check(hipFree(kv.second.ptr), __FUNCTION__); released += kv.second.bytes; }
         for (auto &kv : kept_scratch) if (kv.second.ptr) { check(hipFree(kv.second.ptr), __FUNCTION__); released += kv.second.bytes; }
         splitk_workspaces.clear();

@@ -1,5 +1,5 @@
 // Entry points of the transformer operators (include/tiramisu_hip_wrappers.h): what they refuse, which kernel a call goes to, and the launches.
-// Every launch goes to the calling thread's stream; scratch is the runtime's (tiramisu_hip_kept_scratch), kept per thread and stream.
+// Every launch goes to the calling thread's stream; scratch is the runtime's (tiramisu_hip_kept_scratch), kept per thread, stream and GPU.
 #include "operators.h"
 
 #include <algorithm>
