@@ -169,10 +169,11 @@ int tiramisu_hip_device_count(void);
  *      Matrices are row-major with their columns dense and `ld...` elements from row to row (0: dense rows too); results are dense and must not
  *      overlap inputs.  Weights are [outputs][inputs].  Operands may begin at any element; rows that the
  *      matrix kernels cannot load in place (odd strides of 16-bit elements) are moved to scratch first.  Sums are kept in 32 bits and rounded once.
- *      Types and activations are the numbers below.  Arguments that do not fit together are refused: a message on stderr,
- *      return value 1, nothing launched.  Scratch is kept per thread, stream and GPU like tiramisu_hip_sgemm's, and stays where it is until
- *      tiramisu_hip_release_cached_memory(): a call recorded into a graph uses at every replay the scratch of the stream it was recorded on,
- *      so work on that stream and replays elsewhere have to wait for each other. ---- */
+ *      Types and activations are the numbers below.  Arguments that do not fit together, and calls whose scratch cannot be had, are refused: a message
+ *      on stderr, return value 1, nothing launched.  Scratch (gradients ahead of an activation, partial sums, moved rows) is one block for each thread, stream
+ *      and GPU, as large as the largest call there needed, until tiramisu_hip_release_cached_memory().  A call recorded into a graph uses at every replay the
+ *      block that it was recorded with, which stays where it is: work on the stream of the recording, replays elsewhere and replays of
+ *      other graphs recorded there have to wait for each other. ---- */
 enum tiramisu_hip_element_t { TIRAMISU_HIP_FLOAT32 = 0, TIRAMISU_HIP_FLOAT16 = 1, TIRAMISU_HIP_BFLOAT16 = 2, TIRAMISU_HIP_FLOAT8_E4M3 = 3 };
 enum tiramisu_hip_activation_t {
     TIRAMISU_HIP_NONE = 0, TIRAMISU_HIP_RELU = 1, TIRAMISU_HIP_GELU = 2 /* erf */, TIRAMISU_HIP_GELU_TANH = 3, TIRAMISU_HIP_SILU = 4

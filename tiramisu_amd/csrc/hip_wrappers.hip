@@ -138,6 +138,16 @@ std::mutex pool_mutex;
 std::map<uint64_t, std::vector<void *>> pool_free;   // idle blocks by size
 std::map<void *, uint64_t> pool_live;                  // blocks handed out
 uint64_t pool_idle_bytes = 0;
+// Idle blocks go back to HIP; returns their bytes
+uint64_t release_idle_blocks() {
+    std::lock_guard<std::mutex> g(pool_mutex);
+    uint64_t released = 0;
+    for (auto &kv : pool_free)
+        for (void *q : kv.second) { check(hipFree(q), "tiramisu_hip_malloc"); released += kv.first; }
+    pool_free.clear();
+    pool_idle_bytes = 0;
+    return released;
+}
 uint64_t pool_limit() {
     static const uint64_t limit = [] {
         const char *e = std::getenv("TIRAMISU_HIP_POOL_BYTES");
@@ -410,11 +420,15 @@ place here() {
     }
     return {std::this_thread::get_id(), current_stream, device};
 }
-std::mutex kept_mutex;                                                    // guards the two maps below
+std::mutex kept_mutex;                                                    // guards the maps below
 std::map<place, splitk_block> splitk_workspaces;
 // Scratch that generated functions keep between their calls (tiramisu_hip_kept_scratch): by requesting site, thread, stream and GPU.
 std::map<std::pair<const void *, place>, splitk_block> kept_scratch;
 constexpr uint64_t SPLITK_WORKSPACE_LIMIT = (uint64_t)256 << 20;
+// Scratch of the operators (operators.h: operator_scratch).  `before`: smaller blocks that a recorded graph still uses.
+struct operator_block { void *ptr = nullptr; uint64_t bytes = 0; bool recorded = false; };
+struct operator_blocks { operator_block now; std::vector<operator_block> before; };
+std::map<place, operator_blocks> operator_memory;
 
 // Scratch of the entry point that allocates nothing: lives in the code object, one copy per device.
 constexpr uint64_t STATIC_SCRATCH_BYTES = ((uint64_t)4 << 20) + SPLITK_COUNTER_BYTES;
@@ -486,6 +500,51 @@ timed::~timed() {
     if (stop) ::check(hipEventRecord(stop, current_stream), "tiramisu_hip_profile");
 }
 
+void *operator_scratch(uint64_t bytes) {
+    constexpr const char *function = "tiramisu_hip_kept_scratch";
+    // (the null stream records nothing, and may not be asked while another one does)
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (current_stream != hipStreamLegacy && hipStreamIsCapturing(current_stream, &status) != hipSuccess) {
+        (void)hipGetLastError();
+        status = hipStreamCaptureStatusNone;
+    }
+    const bool recording = status != hipStreamCaptureStatusNone;
+    std::lock_guard<std::mutex> g(kept_mutex);
+    operator_blocks &blocks = operator_memory[here()];
+    if (blocks.now.bytes < bytes) {
+        // eighths of a power of two: little is held beyond what the largest call needs, and sizes that creep up seldom allocate
+        uint64_t step = 8192;
+        while (8 * step < bytes) step *= 2;
+        const uint64_t size = (bytes + step - 1) / step * step;
+        // (memory may be had while a graph is recorded, like the allocations of other libraries; none is given back then)
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+        ::check(hipThreadExchangeStreamCaptureMode(&mode), function);
+        if (blocks.now.ptr && !blocks.now.recorded && !recording) {
+            ::check(hipStreamSynchronize(current_stream), function);
+            ::check(hipFree(blocks.now.ptr), function);
+            blocks.now = operator_block();
+        }
+        void *p = nullptr;
+        hipError_t e = hipMalloc(&p, size);
+        if (e == hipErrorOutOfMemory && !recording) {
+            (void)hipGetLastError();
+            release_idle_blocks();
+            e = hipMalloc(&p, size);
+        }
+        ::check(hipThreadExchangeStreamCaptureMode(&mode), function);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            return nullptr;
+        }
+        if (blocks.now.ptr) blocks.before.push_back(blocks.now);
+        blocks.now.ptr = p;
+        blocks.now.bytes = size;
+        blocks.now.recorded = false;
+    }
+    blocks.now.recorded |= recording;
+    return blocks.now.ptr;
+}
+
 }  // namespace tiramisu_runtime
 
 extern "C" {
@@ -511,13 +570,7 @@ void *tiramisu_hip_malloc(uint64_t size) {
     if (e == hipErrorOutOfMemory) {
         // give the idle blocks back to HIP and try once more
         (void)hipGetLastError();
-        {
-            std::lock_guard<std::mutex> g(pool_mutex);
-            for (auto &kv : pool_free)
-                for (void *q : kv.second) check(hipFree(q), __FUNCTION__);
-            pool_free.clear();
-            pool_idle_bytes = 0;
-        }
+        release_idle_blocks();
         e = hipMalloc(&p, size);
     }
     check(e, __FUNCTION__);
@@ -770,20 +823,21 @@ uint64_t tiramisu_hip_release_cached_memory(void) {
         std::set<int> others;
         for (auto &kv : splitk_workspaces) others.insert(kv.first.device);
         for (auto &kv : kept_scratch) others.insert(kv.first.second.device);
+        for (auto &kv : operator_memory) others.insert(kv.first.device);
         others.erase(device);
         for (int other : others) { check(hipSetDevice(other), __FUNCTION__); check(hipDeviceSynchronize(), __FUNCTION__); }
         if (!others.empty()) check(hipSetDevice(device), __FUNCTION__);
         for (auto &kv : splitk_workspaces) if (kv.second.ptr) { check(hipFree(kv.second.ptr), __FUNCTION__); released += kv.second.bytes; }
         for (auto &kv : kept_scratch) if (kv.second.ptr) { check(hipFree(kv.second.ptr), __FUNCTION__); released += kv.second.bytes; }
+        for (auto &kv : operator_memory) {
+            kv.second.before.push_back(kv.second.now);
+            for (const operator_block &b : kv.second.before) if (b.ptr) { check(hipFree(b.ptr), __FUNCTION__); released += b.bytes; }
+        }
         splitk_workspaces.clear();
         kept_scratch.clear();
+        operator_memory.clear();
     }
-    std::lock_guard<std::mutex> g(pool_mutex);
-    for (auto &kv : pool_free)
-        for (void *q : kv.second) { check(hipFree(q), __FUNCTION__); released += kv.first; }
-    pool_free.clear();
-    pool_idle_bytes = 0;
-    return released;
+    return released + release_idle_blocks();
 }
 
 uint64_t tiramisu_hip_cached_memory_bytes(void) {
@@ -792,6 +846,10 @@ uint64_t tiramisu_hip_cached_memory_bytes(void) {
         std::lock_guard<std::mutex> g(kept_mutex);
         for (auto &kv : splitk_workspaces) held += kv.second.bytes;
         for (auto &kv : kept_scratch) held += kv.second.bytes;
+        for (auto &kv : operator_memory) {
+            held += kv.second.now.bytes;
+            for (const operator_block &b : kv.second.before) held += b.bytes;
+        }
     }
     std::lock_guard<std::mutex> g(pool_mutex);
     return held + pool_idle_bytes;

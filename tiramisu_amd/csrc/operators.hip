@@ -1,5 +1,6 @@
 // Entry points of the transformer operators (include/tiramisu_hip_wrappers.h): what they refuse, which kernel a call goes to, and the launches.
-// Every launch goes to the calling thread's stream; scratch is the runtime's (tiramisu_hip_kept_scratch), kept per thread, stream and GPU.
+// Every launch goes to the calling thread's stream.  A call plans all of its launches first, then asks for the scratch that they need, as one block, and
+// launches only when it has it.
 #include "operators.h"
 
 #include <algorithm>
@@ -45,15 +46,26 @@ constexpr int64_t MOST_STEP = 1 << 23;                   // elements from k to k
 bool known_type(int type, bool with_f32) { return type == F16 || type == BF16 || (with_f32 && type == F32); }
 int bytes_of(int type) { return type == F32 ? 4 : type == F8 ? 1 : 2; }
 
-// ---- scratch.  A block for each use and power of two of bytes: a block, once given, stays where it is until
-// tiramisu_hip_release_cached_memory(), so that launches recorded into a graph keep theirs.
-enum scratch_use { GRADIENT, PARTIAL, MOVED_A, MOVED_B, MOVED_C, COLUMN_SUMS, SCRATCH_USES };
-void *scratch(scratch_use use, uint64_t bytes) {
-    static char sites[SCRATCH_USES][64];
-    int log2 = 16;
-    while ((1ull << log2) < bytes) log2++;
-    return tiramisu_hip_kept_scratch(&sites[use][log2], 1ull << log2, nullptr);
-}
+// ---- scratch of one call: places are given out while its launches are planned, and become addresses when the block is taken.
+class call_scratch {
+public:
+    static constexpr uint64_t NOWHERE = ~0ull;
+    uint64_t want(uint64_t bytes) {
+        const uint64_t place = total;
+        total += (bytes + 255) / 256 * 256;
+        return place;
+    }
+    // 0, or 1 and a message where the memory cannot be had
+    int take(const char *fn) {
+        if (total == 0 || (base = (char *)tiramisu_runtime::operator_scratch(total))) return 0;
+        return refuse(fn, "no memory for %llu bytes of scratch", (unsigned long long)total);
+    }
+    void *at(uint64_t place) const { return place == NOWHERE ? nullptr : base + place; }
+
+private:
+    uint64_t total = 0;
+    char *base = nullptr;
+};
 
 // ---- operands as the tiles can load them: rows that begin at multiples of 4 bytes, and strides within the limits above.  Others are
 // moved to scratch, rows at multiples of 16 bytes.
@@ -61,19 +73,35 @@ struct operand { const void *p; long ld; };
 bool loadable(const operand &o, int bytes, bool k_along_rows) {
     return (uintptr_t)o.p % 4 == 0 && (o.ld * bytes) % 4 == 0 && (k_along_rows ? o.ld * bytes <= MOST_ROW_BYTES : o.ld <= MOST_STEP);
 }
-operand moved_where_needed(const operand &o, long rows, long columns, int bytes, bool k_along_rows, scratch_use use) {
-    if (rows <= 0 || columns <= 0 || loadable(o, bytes, k_along_rows)) return o;
+struct placed_operand {
+    operand from;
+    long rows, columns;
+    int bytes;
+    uint64_t place;                         // NOWHERE: stays where it is
+    long ld;
+};
+placed_operand place_operand(const operand &o, long rows, long columns, int bytes, bool k_along_rows, call_scratch &s) {
+    placed_operand q = {o, rows, columns, bytes, call_scratch::NOWHERE, o.ld};
+    if (rows <= 0 || columns <= 0 || loadable(o, bytes, k_along_rows)) return q;
     const long to = (columns * bytes + 15) / 16 * 16;
-    char *out = (char *)scratch(use, (uint64_t)(to * rows));
-    for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / (to / 16)); first < rows; first += most) {
-        const long n = std::min(most, rows - first);
+    q.ld = to / bytes;
+    q.place = s.want((uint64_t)to * (uint64_t)rows);
+    return q;
+}
+// its address, and the launch that moves it there
+const void *settle(const char *fn, const placed_operand &q, const call_scratch &s) {
+    if (q.place == call_scratch::NOWHERE) return q.from.p;
+    const long to = q.ld * q.bytes;
+    char *out = (char *)s.at(q.place);
+    for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / (to / 16)); first < q.rows; first += most) {
+        const long n = std::min(most, q.rows - first);
         const unsigned blocks = (unsigned)((to / 16 * n + 255) / 256);
-        const char *in = (const char *)o.p + first * o.ld * bytes;
-        if (bytes == 1) hipLaunchKernelGGL(move_rows_kernel<1>, dim3(blocks), dim3(256), 0, stream(), in, out + first * to, n, columns * bytes, o.ld * bytes, to);
-        else hipLaunchKernelGGL(move_rows_kernel<2>, dim3(blocks), dim3(256), 0, stream(), in, out + first * to, n, columns * bytes, o.ld * bytes, to);
+        const char *in = (const char *)q.from.p + first * q.from.ld * q.bytes;
+        auto kernel = q.bytes == 1 ? move_rows_kernel<1> : move_rows_kernel<2>;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream(), in, out + first * to, n, q.columns * q.bytes, q.from.ld * q.bytes, to);
     }
-    check(hipGetLastError(), "tiramisu_hip_linear");
-    return {out, to / bytes};
+    check(hipGetLastError(), fn);
+    return out;
 }
 
 // ---- which tile, and how many workgroups share the k of one.  A launch is modelled in microseconds: `fixed`, for every slice of 128 bytes of k `first` for the first
@@ -154,25 +182,41 @@ pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
     return best;
 }
 
-int launch_product(const char *fn, int type, product_layout layout, int epilogue, int y, product_arguments p) {
-    if (p.M == 0 || p.N == 0) return 0;
+// A product as it will be launched; its operands' addresses and `a_more` may still be missing.  `pairs`: 2 where a second pair of operands will be added.
+struct planned_product {
+    int type, epilogue, y;
+    product_layout layout;
+    product_arguments p;
+    tile_plan plan;
+    uint64_t partial;
+};
+planned_product plan_product(int type, product_layout layout, int epilogue, int y, const product_arguments &p, int pairs, call_scratch &s) {
+    planned_product q = {type, epilogue, y, layout, p, {TILE_64, 1, 0, 0.0}, call_scratch::NOWHERE};
+    if (p.M == 0 || p.N == 0) return q;
     const bool gated = epilogue == GATED;
-    const long work = p.a_more ? 2L * p.K : p.K;
-    tile_plan plan = plan_for(p.M, p.N, work, bytes_of(type), gated);
-    if (p.a_more && plan.splits > 1) plan.slices = (plan.slices + 1) / 2, plan.splits = (int)std::max(1L, ((long)p.K + 64L * plan.slices - 1) / (64L * plan.slices));
-    p.partial = nullptr;
-    p.slices_per_split = plan.slices;
-    if (plan.splits > 1) p.partial = (float *)scratch(PARTIAL, (uint64_t)plan.splits * (gated ? 2 : 1) * p.M * p.N * 4);
-    if (type == BF16) launch_tiles_BF16(plan.tile, layout, epilogue, y, p, plan.splits, stream());
-    else if (type == F16) launch_tiles_F16(plan.tile, layout, epilogue, y, p, plan.splits, stream());
-    else launch_tiles_F8(plan.tile, layout, epilogue, y, p, plan.splits, stream());
-    if (plan.splits > 1) {
+    q.plan = plan_for(p.M, p.N, (long)pairs * p.K, bytes_of(type), gated);
+    if (pairs == 2 && q.plan.splits > 1) {
+        // (the slices are those of both pairs, and each workgroup takes its part of either)
+        q.plan.slices = (q.plan.slices + 1) / 2;
+        q.plan.splits = (int)std::max(1L, ((long)p.K + 64L * q.plan.slices - 1) / (64L * q.plan.slices));
+    }
+    q.p.slices_per_split = q.plan.slices;
+    if (q.plan.splits > 1) q.partial = s.want((uint64_t)q.plan.splits * (gated ? 2 : 1) * p.M * p.N * 4);
+    return q;
+}
+void launch_product(const char *fn, planned_product &q, const call_scratch &s) {
+    product_arguments &p = q.p;
+    if (p.M == 0 || p.N == 0) return;
+    p.partial = (float *)s.at(q.partial);
+    if (q.type == BF16) launch_tiles_BF16(q.plan.tile, q.layout, q.epilogue, q.y, p, q.plan.splits, stream());
+    else if (q.type == F16) launch_tiles_F16(q.plan.tile, q.layout, q.epilogue, q.y, p, q.plan.splits, stream());
+    else launch_tiles_F8(q.plan.tile, q.layout, q.epilogue, q.y, p, q.plan.splits, stream());
+    if (q.plan.splits > 1) {
         const unsigned blocks = (unsigned)(((p.N + 7L) / 8 * p.M + 255) / 256);
-        auto kernel = gated ? (y == BF16 ? finish_kernel<BF16, GATED> : finish_kernel<F16, GATED>) : (y == BF16 ? finish_kernel<BF16, LINEAR> : finish_kernel<F16, LINEAR>);
-        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream(), p, plan.splits);
+        auto kernel = q.epilogue == GATED ? (q.y == BF16 ? finish_kernel<BF16, GATED> : finish_kernel<F16, GATED>) : (q.y == BF16 ? finish_kernel<BF16, LINEAR> : finish_kernel<F16, LINEAR>);
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream(), p, q.plan.splits);
         check(hipGetLastError(), fn);
     }
-    return 0;
 }
 
 template <int E>
@@ -183,17 +227,30 @@ void launch_sums(const char *fn, const column_sums &a) {
 
 // p: gradient of the input, q: of the weights; what is not asked for has no place for its result.  sums: the bias's gradient, which the one launch of both
 // gradients takes along (4096 x 4096 x 1024: 64 us; as a launch of their own ahead of it 63 and 4.7).
-int launch_gradients(const char *fn, int type, const product_arguments &p, const product_arguments &q, const column_sums &sums) {
-    const bool both = p.y && q.y && p.M && p.N && q.M && q.N;
-    const pair_plan plan = both ? plan_for_pair(p.M, p.N, p.a_more ? 2L * p.K : p.K, q.M, q.N, q.K) : pair_plan();
-    if (both && plan.together) {
-        (type == BF16 ? launch_gradients_BF16 : launch_gradients_F16)(plan.tile, plan.q_first, p, q, sums, stream());
+struct planned_gradients {
+    int type;
+    pair_plan pair;
+    planned_product p, q;
+};
+planned_gradients plan_gradients(int type, const product_arguments &p, int pairs, const product_arguments &q, call_scratch &s) {
+    planned_gradients g = {type, {TILE_64, false, false}, {}, {}};
+    g.p.p = p;
+    g.q.p = q;
+    if (p.y && q.y && p.M && p.N && q.M && q.N) g.pair = plan_for_pair(p.M, p.N, (long)pairs * p.K, q.M, q.N, q.K);
+    if (g.pair.together) return g;
+    if (p.y) g.p = plan_product(type, INPUT_GRADIENT, LINEAR, type, p, pairs, s);
+    if (q.y) g.q = plan_product(type, WEIGHT_GRADIENT, LINEAR, type, q, 1, s);
+    return g;
+}
+int launch_gradients(const char *fn, planned_gradients &g, const column_sums &sums, const call_scratch &s) {
+    if (g.pair.together) {
+        (g.type == BF16 ? launch_gradients_BF16 : launch_gradients_F16)(g.pair.tile, g.pair.q_first, g.p.p, g.q.p, sums, stream());
         return 0;
     }
-    if (sums.parts) type == BF16 ? launch_sums<BF16>(fn, sums) : launch_sums<F16>(fn, sums);
-    if (p.y)
-        if (const int rc = launch_product(fn, type, INPUT_GRADIENT, LINEAR, type, p)) return rc;
-    return q.y ? launch_product(fn, type, WEIGHT_GRADIENT, LINEAR, type, q) : 0;
+    if (sums.parts) g.type == BF16 ? launch_sums<BF16>(fn, sums) : launch_sums<F16>(fn, sums);
+    if (g.p.p.y) launch_product(fn, g.p, s);
+    if (g.q.p.y) launch_product(fn, g.q, s);
+    return 0;
 }
 
 // Rows of x that the kernel of few tokens (linear_few_tokens.hip.h) takes at most, and what a call of it takes: the weights' bytes at what memory gives, or what a
@@ -244,15 +301,19 @@ int forward(const char *fn, int type, int y, int epilogue, product_arguments p) 
             return 0;
         }
     }
-    auto take = [&](const void *&q, long &ld, long rows, scratch_use use) {
-        const operand o = moved_where_needed({q, ld}, rows, p.K, bytes, true, use);
-        q = o.p;
-        ld = o.ld;
-    };
-    take(p.a, p.lda, p.M, MOVED_A);
-    take(p.b, p.ldb, p.N, MOVED_B);
-    if (gated) take(p.b2, p.ldb2, p.N, MOVED_C);
-    return launch_product(fn, type, FORWARD, epilogue, y, p);
+    call_scratch s;
+    const placed_operand a = place_operand({p.a, p.lda}, p.M, p.K, bytes, true, s), b = place_operand({p.b, p.ldb}, p.N, p.K, bytes, true, s),
+                         b2 = place_operand({p.b2, p.ldb2}, gated ? p.N : 0, p.K, bytes, true, s);
+    p.lda = a.ld;
+    p.ldb = b.ld;
+    p.ldb2 = b2.ld;
+    planned_product q = plan_product(type, FORWARD, epilogue, y, p, 1, s);
+    if (s.take(fn)) return 1;
+    q.p.a = settle(fn, a, s);
+    q.p.b = settle(fn, b, s);
+    q.p.b2 = settle(fn, b2, s);
+    launch_product(fn, q, s);
+    return 0;
 }
 
 // ---- rows
@@ -293,46 +354,63 @@ int norm(const char *fn, int type, int y, norm_arguments a) {
 }
 
 template <int E>
-void launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweight) {
+int launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweight) {
     constexpr int N = E == F32 ? 4 : 8;
     const long pieces = (a.columns + N - 1) / N;
+    call_scratch s;
+    auto sums_of = [&](long parts) {
+        a.parts = (int)std::max(1L, parts);
+        const uint64_t place = s.want((uint64_t)a.parts * a.columns * 4);
+        if (s.take(fn)) return false;
+        a.partial = (float *)s.at(place);
+        return true;
+    };
     // workgroups: enough to cover the way to memory, few enough that their sums are little beside the rows
     auto go = [&](auto kernel, int threads, int teams, long most) {
-        a.parts = (int)std::max(1L, std::min((a.rows + teams - 1) / teams, most));
-        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.parts * a.columns * 4);
+        if (!sums_of(std::min((a.rows + teams - 1) / teams, most))) return false;
         hipLaunchKernelGGL(kernel, dim3((unsigned)a.parts), dim3(threads), 0, stream(), a);
+        return true;
     };
-    if (pieces <= 64) go(rms_norm_backward_kernel<E, 64, 1>, 512, 8, 512);
-    else if (pieces <= 128) go(rms_norm_backward_kernel<E, 64, 2>, 512, 8, 512);
-    else if (pieces <= 192) go(rms_norm_backward_kernel<E, 64, 3>, 512, 8, 256);
-    else if (pieces <= 256) go(rms_norm_backward_kernel<E, 64, 4>, 512, 8, 256);
-    else if (pieces <= 512) go(rms_norm_backward_kernel<E, 256, 2>, 256, 1, 768);
-    else if (pieces <= 1024) go(rms_norm_backward_kernel<E, 256, 4>, 256, 1, 512);
-    else if (pieces <= 2048) go(rms_norm_backward_kernel<E, 512, 4>, 512, 1, 256);
-    else {
-        a.parts = (int)std::max(1L, std::min(a.rows, 64L));
-        a.partial = (float *)scratch(COLUMN_SUMS, (uint64_t)a.parts * a.columns * 4);
+    auto go_long = [&] {
+        if (!sums_of(std::min(a.rows, 64L))) return false;
         if (a.rows > 0) hipLaunchKernelGGL(rms_norm_backward_long_rows_kernel<E>, dim3((unsigned)a.rows), dim3(1024), 0, stream(), a);
         hipLaunchKernelGGL(rms_norm_backward_long_columns_kernel<E>, dim3((unsigned)((a.columns + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream(), a);
-    }
+        return true;
+    };
+    const bool launched = pieces <= 64    ? go(rms_norm_backward_kernel<E, 64, 1>, 512, 8, 512)
+                          : pieces <= 128  ? go(rms_norm_backward_kernel<E, 64, 2>, 512, 8, 512)
+                          : pieces <= 192  ? go(rms_norm_backward_kernel<E, 64, 3>, 512, 8, 256)
+                          : pieces <= 256  ? go(rms_norm_backward_kernel<E, 64, 4>, 512, 8, 256)
+                          : pieces <= 512  ? go(rms_norm_backward_kernel<E, 256, 2>, 256, 1, 768)
+                          : pieces <= 1024 ? go(rms_norm_backward_kernel<E, 256, 4>, 256, 1, 512)
+                          : pieces <= 2048 ? go(rms_norm_backward_kernel<E, 512, 4>, 512, 1, 256)
+                                           : go_long();
+    if (!launched) return 1;
     check(hipGetLastError(), fn);
     launch_sums<E>(fn, {a.partial, dweight, a.columns, a.parts});
+    return 0;
 }
 
+// How the launch of dz is divided: `across` threads along a row and columns of workgroups, rows of a chunk and chunks
+struct activation_backward_plan { int across; long columns, rows; int chunks; };
+activation_backward_plan plan_activation_backward(long M, long N) {
+    activation_backward_plan plan = {1, 0, 0, 0};
+    while (plan.across < 64 && plan.across * 8 < N) plan.across *= 2;
+    plan.columns = (N + 8L * plan.across - 1) / (8L * plan.across);
+    // workgroups: one row to a thread where there are few, and few enough that their sums are little beside the rows
+    const long down = 256 / plan.across, chunks = std::max(1L, std::min((M + down - 1) / down, std::min(256L, std::max(1L, 1024 / plan.columns))));
+    plan.rows = std::max(1L, (M + chunks - 1) / chunks);
+    plan.chunks = (int)std::max(1L, (M + plan.rows - 1) / plan.rows);
+    return plan;
+}
 // dz, and what the bias's gradient is the sums of; what is null is not computed
 template <int E>
-column_sums launch_activation_backward(const char *fn, activation_backward_arguments a, void *dbias) {
-    a.across = 1;
-    while (a.across < 64 && a.across * 8 < a.N) a.across *= 2;
-    const long columns = (a.N + 8L * a.across - 1) / (8L * a.across), down = 256 / a.across;
-    // workgroups: one row to a thread where there are few, and few enough that their sums are little beside the rows
-    const long chunks = std::max(1L, std::min((a.M + down - 1) / down, std::min(256L, std::max(1L, 1024 / columns))));
-    a.rows = std::max(1L, (a.M + chunks - 1) / chunks);
-    const int used = (int)std::max(1L, (a.M + a.rows - 1) / a.rows);
-    a.partial = dbias ? (float *)scratch(COLUMN_SUMS, (uint64_t)used * a.N * 4) : nullptr;
-    hipLaunchKernelGGL(activation_backward_kernel<E>, dim3((unsigned)columns, (unsigned)used), dim3(256), 0, stream(), a);
+column_sums launch_activation_backward(const char *fn, activation_backward_arguments a, const activation_backward_plan &plan, void *dbias) {
+    a.across = plan.across;
+    a.rows = plan.rows;
+    hipLaunchKernelGGL(activation_backward_kernel<E>, dim3((unsigned)plan.columns, (unsigned)plan.chunks), dim3(256), 0, stream(), a);
     check(hipGetLastError(), fn);
-    return {a.partial, dbias, a.N, dbias ? used : 0};
+    return {a.partial, dbias, a.N, dbias ? plan.chunks : 0};
 }
 
 product_arguments product_of(long M, long N, long K) {
@@ -398,10 +476,7 @@ int tiramisu_hip_rms_norm_backward(const void *dy, const void *sum, const void *
     timed record(__FUNCTION__);
     const norm_backward_arguments a = {dy, sum, weight, dsum, rstd, dx, nullptr, (long)rows, (long)columns, ldy ? (long)ldy : (long)columns,
                                        lds ? (long)lds : (long)columns, ldd ? (long)ldd : (long)columns, 0};
-    if (type == F32) launch_norm_backward<F32>(__FUNCTION__, a, dweight);
-    else if (type == F16) launch_norm_backward<F16>(__FUNCTION__, a, dweight);
-    else launch_norm_backward<BF16>(__FUNCTION__, a, dweight);
-    return 0;
+    return type == F32 ? launch_norm_backward<F32>(__FUNCTION__, a, dweight) : type == F16 ? launch_norm_backward<F16>(__FUNCTION__, a, dweight) : launch_norm_backward<BF16>(__FUNCTION__, a, dweight);
 }
 
 int tiramisu_hip_linear(const void *x, const void *weight, const void *bias, const void *residual, const float *x_scale, const float *weight_scale, void *y,
@@ -465,35 +540,32 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
     if ((M && N && !dy) || (M && K && dweight && !x) || (N && K && dx && !weight)) return refuse(__FUNCTION__, "dy, x and weight are needed");
     timed record(__FUNCTION__);
     const long m = (long)M, n = (long)N, k = (long)K;
-    operand dz = {dy, ldy ? (long)ldy : n};
-    column_sums sums = {};
+    const bool activated = activation != NONE && n > 0, elementwise = n > 0 && (activated || dbias);
+    call_scratch s;
     // the gradient ahead of the activation; without one it is dy, moved only where the tiles cannot load it
-    if (n > 0 && (activation != NONE || dbias)) {
-        activation_backward_arguments a = {dy, pre, nullptr, nullptr, m, n, dz.ld, ldp ? (long)ldp : n, 0, 0, activation, 0};
-        if (activation != NONE) {
-            a.ldz = (n + 7) / 8 * 8;
-            a.dz = scratch(GRADIENT, (uint64_t)std::max(1L, m) * a.ldz * 2);
-            dz = {a.dz, a.ldz};
-        }
-        sums = type == F16 ? launch_activation_backward<F16>(__FUNCTION__, a, dbias) : launch_activation_backward<BF16>(__FUNCTION__, a, dbias);
-    }
-    if (!loadable(dz, 2, true) || !loadable(dz, 2, false)) dz = moved_where_needed({dz.p, dz.ld}, m, n, 2, true, GRADIENT);
+    const long ldz = (n + 7) / 8 * 8;
+    const uint64_t gradient = activated ? s.want((uint64_t)std::max(1L, m) * ldz * 2) : call_scratch::NOWHERE;
+    const placed_operand moved_dy = place_operand({dy, ldy ? (long)ldy : n}, activated ? 0 : m, n, 2, true, s);
+    const activation_backward_plan rows = elementwise ? plan_activation_backward(m, n) : activation_backward_plan();
+    const uint64_t partial = elementwise && dbias ? s.want((uint64_t)rows.chunks * n * 4) : call_scratch::NOWHERE;
+    const placed_operand w = place_operand({weight, ldw ? (long)ldw : k}, dx ? n : 0, k, 2, false, s), xs = place_operand({x, ldx ? (long)ldx : k}, dweight ? m : 0, k, 2, false, s);
     product_arguments p = product_of(m, k, n), q = product_of(n, k, m);
-    p.a = q.a = dz.p;
-    p.lda = q.lda = dz.ld;
+    p.lda = q.lda = activated ? ldz : moved_dy.ld;
+    p.ldb = w.ld;
+    q.ldb = xs.ld;
     p.y = dx;
     q.y = dweight;
-    if (dx) {
-        const operand w = moved_where_needed({weight, ldw ? (long)ldw : k}, n, k, 2, false, MOVED_B);
-        p.b = w.p;
-        p.ldb = w.ld;
+    planned_gradients g = plan_gradients(type, p, 1, q, s);
+    if (s.take(__FUNCTION__)) return 1;
+    column_sums sums = {};
+    if (elementwise) {
+        const activation_backward_arguments a = {dy, activated ? pre : nullptr, s.at(gradient), (float *)s.at(partial), m, n, ldy ? (long)ldy : n, ldp ? (long)ldp : n, ldz, 0, activation, 0};
+        sums = type == F16 ? launch_activation_backward<F16>(__FUNCTION__, a, rows, dbias) : launch_activation_backward<BF16>(__FUNCTION__, a, rows, dbias);
     }
-    if (dweight) {
-        const operand xs = moved_where_needed({x, ldx ? (long)ldx : k}, m, k, 2, false, MOVED_A);
-        q.b = xs.p;
-        q.ldb = xs.ld;
-    }
-    return launch_gradients(__FUNCTION__, type, p, q, sums);
+    g.p.p.a = g.q.p.a = activated ? s.at(gradient) : settle(__FUNCTION__, moved_dy, s);
+    g.p.p.b = settle(__FUNCTION__, w, s);
+    g.q.p.b = settle(__FUNCTION__, xs, s);
+    return launch_gradients(__FUNCTION__, g, sums, s);
 }
 
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate, const void *up,
@@ -509,7 +581,26 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
     const long m = (long)M, n = (long)N, k = (long)K;
     // [dgate | dup] in rows of 2 x `half` elements
     const long half = (n + 7) / 8 * 8, ld = 2 * half;
-    char *d = (char *)scratch(GRADIENT, (uint64_t)std::max(1L, m) * std::max(1L, ld) * 2);
+    call_scratch s;
+    const uint64_t gradient = s.want((uint64_t)std::max(1L, m) * std::max(1L, ld) * 2);
+    const placed_operand wg = place_operand({gate_weight, ldg ? (long)ldg : k}, dx ? n : 0, k, 2, false, s), wu = place_operand({up_weight, ldu ? (long)ldu : k}, dx ? n : 0, k, 2, false, s),
+                         xs = place_operand({x, ldx ? (long)ldx : k}, dgate_weight && n > 0 ? m : 0, k, 2, false, s);
+    product_arguments p = product_of(m, k, n), q = product_of(half + n, k, m);
+    p.lda = q.lda = ld;
+    p.ldb = wg.ld;
+    p.ldb_more = wu.ld;
+    p.y = dx;
+    if (dgate_weight && n > 0) {
+        // rows of the product: those of gate, up to `half` nothing, those of up
+        q.ldb = xs.ld;
+        q.y = dgate_weight;
+        q.y_below = dup_weight;
+        q.rows_above = (int)n;
+        q.split_row = (int)half;
+    }
+    planned_gradients g = plan_gradients(type, p, 2, q, s);
+    if (s.take(__FUNCTION__)) return 1;
+    char *d = (char *)s.at(gradient);
     if (m > 0 && n > 0) {
         const gated_backward_arguments a = {dh, gate, up, d, d + 2 * half, m, n, ldh ? (long)ldh : n, ld_gate ? (long)ld_gate : n, ld_up ? (long)ld_up : n, ld, activation};
         const unsigned blocks = (unsigned)((half / 8 * m + 255) / 256);
@@ -517,30 +608,12 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
         else hipLaunchKernelGGL(gated_backward_kernel<BF16>, dim3(blocks), dim3(256), 0, stream(), a);
         check(hipGetLastError(), __FUNCTION__);
     }
-    product_arguments p = product_of(m, k, n), q = product_of(half + n, k, m);
-    p.a = q.a = d;
-    p.lda = q.lda = ld;
-    if (dx) {
-        const operand g = moved_where_needed({gate_weight, ldg ? (long)ldg : k}, n, k, 2, false, MOVED_B);
-        const operand u = moved_where_needed({up_weight, ldu ? (long)ldu : k}, n, k, 2, false, MOVED_C);
-        p.a_more = d + 2 * half;
-        p.b = g.p;
-        p.ldb = g.ld;
-        p.b_more = u.p;
-        p.ldb_more = u.ld;
-        p.y = dx;
-    }
-    if (dgate_weight && n > 0) {
-        // rows of the product: those of gate, up to `half` nothing, those of up
-        const operand xs = moved_where_needed({x, ldx ? (long)ldx : k}, m, k, 2, false, MOVED_A);
-        q.b = xs.p;
-        q.ldb = xs.ld;
-        q.y = dgate_weight;
-        q.y_below = dup_weight;
-        q.rows_above = (int)n;
-        q.split_row = (int)half;
-    }
-    return launch_gradients(__FUNCTION__, type, p, q, {});
+    g.p.p.a = g.q.p.a = d;
+    g.p.p.a_more = d + 2 * half;
+    g.p.p.b = settle(__FUNCTION__, wg, s);
+    g.p.p.b_more = settle(__FUNCTION__, wu, s);
+    g.q.p.b = settle(__FUNCTION__, xs, s);
+    return launch_gradients(__FUNCTION__, g, {}, s);
 }
 
 float *tiramisu_hip_no_buffer(void) { return nullptr; }       // (a pointer that is also one to scales)
