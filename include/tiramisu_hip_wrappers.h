@@ -173,7 +173,7 @@ int tiramisu_hip_device_count(void);
  *      on stderr, return value 1, nothing launched.  Scratch (gradients ahead of an activation, partial sums, moved rows) is one block for each thread, stream
  *      and GPU, as large as the largest call there needed, until tiramisu_hip_release_cached_memory().  A call recorded into a graph uses at every replay the
  *      block that it was recorded with, which stays where it is: work on the stream of the recording, replays elsewhere and replays of
- *      other graphs recorded there have to wait for each other. ---- */
+ *      other graphs recorded there have to wait for each other.  A source of scratch of one's own (below) is free of that. ---- */
 enum tiramisu_hip_element_t { TIRAMISU_HIP_FLOAT32 = 0, TIRAMISU_HIP_FLOAT16 = 1, TIRAMISU_HIP_BFLOAT16 = 2, TIRAMISU_HIP_FLOAT8_E4M3 = 3 };
 enum tiramisu_hip_activation_t {
     TIRAMISU_HIP_NONE = 0, TIRAMISU_HIP_RELU = 1, TIRAMISU_HIP_GELU = 2 /* erf */, TIRAMISU_HIP_GELU_TANH = 3, TIRAMISU_HIP_SILU = 4
@@ -213,6 +213,11 @@ int tiramisu_hip_gated_linear(const void *x, const void *gate_weight, const void
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate,
                                        const void *up, void *dx, void *dgate_weight, void *dup_weight, uint64_t M, uint64_t N, uint64_t K, uint64_t ldh,
                                        uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
+/* Where the calling thread's operator calls take their scratch from, exchanged with *source.  `take` is called once at most by a call, before it launches
+ * anything, and returns GPU memory of at least `bytes` at a multiple of 256 which is the call's until what it puts on the thread's stream has run (for a call
+ * recorded into a graph: until the graph is gone), or NULL, which refuses the call.  It must not throw.  take = NULL: the runtime's blocks, where every thread begins. */
+struct tiramisu_hip_scratch_source { void *(*take)(uint64_t bytes, void *context); void *context; };
+int tiramisu_hip_exchange_scratch_source(struct tiramisu_hip_scratch_source *source);
 /* For generated code: no buffer in the place of one that may be left out, and what becomes of a refused call there -- the reference's failure
  * model, the process ends with status 1 behind the operator's message. */
 float *tiramisu_hip_no_buffer(void);

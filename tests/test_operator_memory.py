@@ -1,5 +1,9 @@
 """Where the operators' scratch and the memory that the runtime keeps between calls come from (include/tiramisu_hip_wrappers.h)."""
+import pytest
+import torch
+
 import host_runtime
+from tiramisu_amd import operators, runtime
 
 
 def test_kept_memory_belongs_to_a_gpu():
@@ -85,3 +89,102 @@ held = hip.recording_held()
 calls[2](4096)
 print(recorded > small, held >= recorded + 1024 * 4096, recorded + 4096 * 4096 <= hip.recording_held() < held + 4096 * 4096 * 1.2)
 """) == "True True True\n"
+
+
+def test_scratch_from_a_source_of_the_callers():
+    """Asked once a call, with as much as the call needs; the runtime keeps nothing then, and a source that has nothing refuses the call."""
+    assert host_runtime.printed(CALLS + """
+class Source(ctypes.Structure):
+    _fields_ = [("take", ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_uint64, ctypes.c_void_p)), ("context", ctypes.c_void_p)]
+asked = []
+def give(bytes, context):
+    asked.append(bytes)
+    return context
+ours = Source(Source._fields_[0][1](give), 1 << 40)
+held = Source(ours.take, ours.context)
+w.tiramisu_hip_exchange_scratch_source(ctypes.byref(held))
+print(bool(held.take), [call() for call in calls], len(asked), min(asked) > 0, hip.recording_held())
+print(asked[0] >= 4096 * 1024 * 2, asked[2] >= 4096 * 2048 * 2, asked[6] >= 5120 * 514 * 2)
+none = Source(ours.take, None)
+w.tiramisu_hip_exchange_scratch_source(ctypes.byref(none))
+launches()
+print([call() for call in calls], launches())
+w.tiramisu_hip_exchange_scratch_source(ctypes.byref(held))
+print([call() for call in calls], len(asked), hip.recording_held() > 0)
+""") == """False [0, 0, 0, 0, 0, 0, 0, 0] 8 True 0
+True True True
+[1, 1, 1, 1, 1, 1, 1, 1] []
+[0, 0, 0, 0, 0, 0, 0, 0] 16 True
+"""
+
+
+def scratch_inputs(M, N, K, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return [torch.randn(shape, device="cuda", generator=g).bfloat16() for shape in ((M, N), (M, K), (N, K), (M, N))]
+
+
+@pytest.mark.gpu
+def test_scratch_of_tensors_is_torchs():
+    """The runtime keeps nothing of calls on tensors, and a later tensor may have the memory."""
+    w = runtime.wrappers()
+    w.tiramisu_hip_release_cached_memory()
+    dy, x, weight, pre = scratch_inputs(301, 1000, 77, 1)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = operators.linear_backward(dy, x, weight, pre=pre, activation="gelu", bias=True)
+    assert w.tiramisu_hip_cached_memory_bytes() == 0
+    results = sum((t.numel() * 2 + 511) // 512 * 512 for t in got)
+    assert torch.cuda.memory_allocated() == before + results and torch.cuda.max_memory_allocated() >= before + results + 301 * 1000 * 2
+
+
+@pytest.mark.gpu
+def test_no_memory_is_an_exception():
+    """Scratch that torch has no memory for: torch's exception, and the same call runs where there is some."""
+    torch.cuda.empty_cache()
+    # (each an allocation of its own, so that no freed part of a larger one is left for the scratch of 512 MiB)
+    dy, x, weight, pre = [torch.randn(shape, device="cuda", dtype=torch.bfloat16) for shape in ((1 << 16, 4096), (1 << 16, 64), (4096, 64), (1 << 16, 4096))]
+    expected = operators.linear_backward(dy, x, weight, pre=pre, activation="silu")
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    try:
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (256 << 20)) / torch.cuda.get_device_properties(0).total_memory)
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            operators.linear_backward(dy, x, weight, pre=pre, activation="silu")
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    for got, was in zip(operators.linear_backward(dy, x, weight, pre=pre, activation="silu")[:2], expected):
+        assert torch.equal(got, was)
+
+
+@pytest.mark.gpu
+def test_graphs_of_one_recording_stream_replay_beside_each_other():
+    """Two graphs, recorded one after the other on the stream that torch records on, replayed at the same time on two streams: each has scratch of its own."""
+    shapes = [(900, 1003, 512), (700, 1203, 512)]
+    inputs = [scratch_inputs(*shape, seed) for seed, shape in enumerate(shapes)]
+
+    def call(dy, x, weight, pre):
+        return operators.linear_backward(dy, x, weight, pre=pre, activation="gelu", bias=True)
+
+    expected = [call(*t) for t in inputs]
+    graphs, results = [], []
+    for t in inputs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            results.append(call(*t))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for r in results:
+            for t in r:
+                t.zero_()
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for got, was in zip(results, expected):
+            assert all(torch.equal(u, v) for u, v in zip(got, was))
+        call(*inputs[turn % 2])

@@ -429,6 +429,7 @@ constexpr uint64_t SPLITK_WORKSPACE_LIMIT = (uint64_t)256 << 20;
 struct operator_block { void *ptr = nullptr; uint64_t bytes = 0; bool recorded = false; };
 struct operator_blocks { operator_block now; std::vector<operator_block> before; };
 std::map<place, operator_blocks> operator_memory;
+thread_local tiramisu_hip_scratch_source scratch_source = {nullptr, nullptr};
 
 // Scratch of the entry point that allocates nothing: lives in the code object, one copy per device.
 constexpr uint64_t STATIC_SCRATCH_BYTES = ((uint64_t)4 << 20) + SPLITK_COUNTER_BYTES;
@@ -501,6 +502,7 @@ timed::~timed() {
 }
 
 void *operator_scratch(uint64_t bytes) {
+    if (scratch_source.take) return scratch_source.take(bytes, scratch_source.context);
     constexpr const char *function = "tiramisu_hip_kept_scratch";
     // (the null stream records nothing, and may not be asked while another one does)
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -810,6 +812,11 @@ void *tiramisu_hip_kept_scratch(const void *site, uint64_t bytes, int32_t *fresh
         if (fresh) *fresh = 1;
     }
     return block.ptr;
+}
+
+int tiramisu_hip_exchange_scratch_source(tiramisu_hip_scratch_source *source) {
+    std::swap(scratch_source, *source);
+    return 0;
 }
 
 uint64_t tiramisu_hip_release_cached_memory(void) {

@@ -43,8 +43,9 @@ public:
 private:
     hipEvent_t stop;
 };
-// Scratch of one operator call on the thread's stream, at least `bytes` large; null where the memory cannot be had.  The next call there gets the same block or
-// a larger one, in the stream's order; a block that a call was given while its stream recorded a graph stays where it is.
+// Scratch of one operator call on the thread's stream, at least `bytes` large; null where the memory cannot be had.  It comes from the thread's source where
+// it has one (tiramisu_hip_exchange_scratch_source).  Else the next call there gets the same block or a larger one, in the stream's order; a block that
+// a call was given while its stream recorded a graph stays where it is.
 void *operator_scratch(uint64_t bytes);
 
 }  // namespace tiramisu_runtime

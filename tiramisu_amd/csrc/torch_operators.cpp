@@ -8,6 +8,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <exception>
 #include <initializer_list>
 #include <string>
 #include <utility>
@@ -158,22 +159,44 @@ PyObject *tuple_of(std::initializer_list<Tensor> tensors) {                 // u
 }
 void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// The thread's stream of the runtime while a call lasts: torch's current one of the tensors' GPU, which is the current device meanwhile.
+// The thread's stream of the runtime while a call lasts, torch's current one of the tensors' GPU, which is the current device meanwhile; and its scratch,
+// torch's memory: in the stream's order like any tensor's, a recording's own in a graph, and an exception of torch's where there is none left.
 class on_stream_of {
 public:
-    explicit on_stream_of(const Tensor &x) : guard(x.device()), before(tiramisu_hip_get_stream()) {
+    explicit on_stream_of(const Tensor &x) : guard(x.device()), before(tiramisu_hip_get_stream()), like(x) {
         void *const handle = (void *)c10::hip::getCurrentHIPStream(x.get_device()).stream();
         // torch's default stream is HIP's null stream; its handle, null, means the thread's own stream to the runtime
         tiramisu_hip_set_stream(handle ? handle : tiramisu_hip_null_stream());
+        tiramisu_hip_exchange_scratch_source(&source);
     }
-    ~on_stream_of() { tiramisu_hip_set_stream(before); }
+    ~on_stream_of() {
+        tiramisu_hip_exchange_scratch_source(&source);
+        tiramisu_hip_set_stream(before);
+    }
     on_stream_of(const on_stream_of &) = delete;
+    void accepted(int status) const {
+        if (failure) std::rethrow_exception(failure);
+        TORCH_CHECK(status == 0, "the runtime refused the call (its reason is on stderr)");
+    }
 
 private:
+    static void *take(uint64_t bytes, void *self) {
+        on_stream_of &call = *(on_stream_of *)self;
+        try {
+            call.scratch = at::empty({(int64_t)bytes}, call.like.options().dtype(at::kByte).requires_grad(false));
+            return call.scratch.data_ptr();
+        } catch (...) {
+            call.failure = std::current_exception();
+            return nullptr;
+        }
+    }
     c10::DeviceGuard guard;
     void *before;
+    const Tensor &like;
+    Tensor scratch;
+    std::exception_ptr failure;
+    tiramisu_hip_scratch_source source = {take, this};
 };
-void accepted(int status) { TORCH_CHECK(status == 0, "the runtime refused the call (its reason is on stderr)"); }
 void count(Py_ssize_t n, Py_ssize_t expected) { TORCH_CHECK_TYPE(n == expected, expected, " arguments, not ", n); }
 
 // ---- the operators
@@ -195,8 +218,8 @@ PyObject *rms_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     {
         on_stream_of stream(x);
         // (a residual of no rows may have no address)
-        accepted(tiramisu_hip_rms_norm(r.p, residual.p, weight, address(y), residual.p ? address(sum) : nullptr, (float *)address(scale), (float *)address(rstd), r.rows, r.width, r.step,
-                                       residual.step, (float)eps, element_of(type), element_of(y.scalar_type())));
+        stream.accepted(tiramisu_hip_rms_norm(r.p, residual.p, weight, address(y), residual.p ? address(sum) : nullptr, (float *)address(scale), (float *)address(rstd), r.rows, r.width, r.step,
+                                              residual.step, (float)eps, element_of(type), element_of(y.scalar_type())));
     }
     return tuple_of({y, sum, scale, rstd});
     END_HANDLE_TH_ERRORS
@@ -217,7 +240,7 @@ PyObject *rms_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor dx = new_like(sum, s.width, type), dweight = new_of(sum, {s.width});
     {
         on_stream_of stream(sum);
-        accepted(tiramisu_hip_rms_norm_backward(dy.p, s.p, weight, rstd, dsum.p, address(dx), address(dweight), s.rows, s.width, dy.step, s.step, dsum.step, element_of(type)));
+        stream.accepted(tiramisu_hip_rms_norm_backward(dy.p, s.p, weight, rstd, dsum.p, address(dx), address(dweight), s.rows, s.width, dy.step, s.step, dsum.step, element_of(type)));
     }
     return tuple_of({dx, dweight});
     END_HANDLE_TH_ERRORS
@@ -232,7 +255,7 @@ PyObject *quantize_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor q = new_like(x, r.width, EIGHT), scale = new_of_rows(x);
     {
         on_stream_of stream(x);
-        accepted(tiramisu_hip_quantize_rows(r.p, address(q), (float *)address(scale), r.rows, r.width, r.step, element_of(x.scalar_type())));
+        stream.accepted(tiramisu_hip_quantize_rows(r.p, address(q), (float *)address(scale), r.rows, r.width, r.step, element_of(x.scalar_type())));
     }
     return tuple_of({q, scale});
     END_HANDLE_TH_ERRORS
@@ -257,8 +280,8 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor y = new_like(x, outputs, type), pre = PyObject_IsTrue(a[8]) == 1 ? new_like(x, outputs, type) : Tensor();
     {
         on_stream_of stream(x);
-        accepted(tiramisu_hip_linear(r.p, weight.p, bias, residual.p, x_scale, weight_scale, address(y), address(pre), tokens, outputs, r.width, r.step, weight.step, residual.step,
-                                     activation_of(a[4]), element_of(x.scalar_type()), element_of(type)));
+        stream.accepted(tiramisu_hip_linear(r.p, weight.p, bias, residual.p, x_scale, weight_scale, address(y), address(pre), tokens, outputs, r.width, r.step, weight.step, residual.step,
+                                            activation_of(a[4]), element_of(x.scalar_type()), element_of(type)));
     }
     return tuple_of({y, pre});
     END_HANDLE_TH_ERRORS
@@ -283,8 +306,8 @@ PyObject *linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
     {
         on_stream_of stream(x);
         // (pre of no tokens has no address, and there is nothing to do with it)
-        accepted(tiramisu_hip_linear_backward(dy.p, r.p, weight.p, pre.p, address(dx), address(dweight), address(dbias), tokens, outputs, r.width, dy.step, r.step, weight.step, pre.step,
-                                              pre.p ? activation : 0, element_of(type)));
+        stream.accepted(tiramisu_hip_linear_backward(dy.p, r.p, weight.p, pre.p, address(dx), address(dweight), address(dbias), tokens, outputs, r.width, dy.step, r.step, weight.step, pre.step,
+                                                     pre.p ? activation : 0, element_of(type)));
     }
     return tuple_of({dx, dweight, dbias});
     END_HANDLE_TH_ERRORS
@@ -308,8 +331,8 @@ PyObject *gated_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor h = new_like(x, outputs, type), gate = keep ? new_like(x, outputs, type) : Tensor(), up = keep ? new_like(x, outputs, type) : Tensor();
     {
         on_stream_of stream(x);
-        accepted(tiramisu_hip_gated_linear(r.p, gate_weight.p, up_weight.p, x_scale, gate_scale, up_scale, address(h), address(gate), address(up), tokens, outputs, r.width, r.step,
-                                           gate_weight.step, up_weight.step, activation_of(a[3]), element_of(x.scalar_type()), element_of(type)));
+        stream.accepted(tiramisu_hip_gated_linear(r.p, gate_weight.p, up_weight.p, x_scale, gate_scale, up_scale, address(h), address(gate), address(up), tokens, outputs, r.width, r.step,
+                                                  gate_weight.step, up_weight.step, activation_of(a[3]), element_of(x.scalar_type()), element_of(type)));
     }
     return tuple_of({h, gate, up});
     END_HANDLE_TH_ERRORS
@@ -328,8 +351,8 @@ PyObject *gated_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Tensor dx = new_like(x, r.width, type), dgate = new_of(x, {outputs, r.width}), dup = new_of(x, {outputs, r.width});
     {
         on_stream_of stream(x);
-        accepted(tiramisu_hip_gated_linear_backward(dh.p, r.p, gate_weight.p, up_weight.p, gate.p, up.p, address(dx), address(dgate), address(dup), tokens_of(x), outputs, r.width, dh.step,
-                                                    r.step, gate_weight.step, up_weight.step, gate.step, up.step, activation_of(a[6]), element_of(type)));
+        stream.accepted(tiramisu_hip_gated_linear_backward(dh.p, r.p, gate_weight.p, up_weight.p, gate.p, up.p, address(dx), address(dgate), address(dup), tokens_of(x), outputs, r.width, dh.step,
+                                                           r.step, gate_weight.step, up_weight.step, gate.step, up.step, activation_of(a[6]), element_of(type)));
     }
     return tuple_of({dx, dgate, dup});
     END_HANDLE_TH_ERRORS

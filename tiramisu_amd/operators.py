@@ -7,7 +7,9 @@ kernels run on torch's current stream of the tensors' device; nothing waits for 
 functions of their own.  Leading dimensions are tokens: x of shape
 [..., K] gives a result of shape [..., N].  Weights are [outputs, inputs].  Tensors need dense rows (stride 1 in the last
 dimension), with one stride from row to row; others are refused, never copied silently.  Results are new, dense tensors.
-ValueError says what does not fit, RuntimeError that the runtime refused the call (its reason is on stderr).
+ValueError says what does not fit, RuntimeError that the runtime refused the call (its reason is on stderr), torch's out-of-memory error that there is no
+memory for results or scratch.  Scratch is torch's memory too: it is back with torch's allocator behind the call, and in a recorded graph it belongs to the graph, so
+graphs may be replayed beside each other.
 """
 import os
 from typing import NamedTuple, Optional
