@@ -142,18 +142,22 @@ def test_scratch_of_tensors_is_torchs():
 @pytest.mark.gpu
 def test_no_memory_is_an_exception():
     """Scratch that torch has no memory for: torch's exception, and the same call runs where there is some."""
-    torch.cuda.empty_cache()
-    # (each an allocation of its own, so that no freed part of a larger one is left for the scratch of 512 MiB)
     dy, x, weight, pre = [torch.randn(shape, device="cuda", dtype=torch.bfloat16) for shape in ((1 << 16, 4096), (1 << 16, 64), (4096, 64), (1 << 16, 4096))]
     expected = operators.linear_backward(dy, x, weight, pre=pre, activation="silu")
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
+    held = []
     try:
-        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (256 << 20)) / torch.cuda.get_device_properties(0).total_memory)
+        # room for the results, 9 MiB, but not for 520 MiB of scratch: what is left within torch's own blocks is taken
+        torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (64 << 20)) / torch.cuda.get_device_properties(0).total_memory)
         with pytest.raises(torch.cuda.OutOfMemoryError):
+            while True:
+                held.append(torch.empty(256 << 20, dtype=torch.uint8, device="cuda"))
+        with pytest.raises(torch.cuda.OutOfMemoryError, match="520.00 MiB"):
             operators.linear_backward(dy, x, weight, pre=pre, activation="silu")
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
+        held.clear()
     for got, was in zip(operators.linear_backward(dy, x, weight, pre=pre, activation="silu")[:2], expected):
         assert torch.equal(got, was)
 
