@@ -427,6 +427,21 @@ def test_infinities_reach_their_own_rows_and_columns_only():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("activation", list(operators.ACTIVATIONS))
+@pytest.mark.parametrize("M,N,K", [(3, 40, 100), (130, 140, 100), (100, 64, 4100)])
+def test_activation_of_an_infinite_sum(M, N, K, activation):
+    """Every activation of plus infinity is that: few tokens, tiles, and sums that were split; the other rows are what they are without it."""
+    g = generator(101)
+    x, w, up = [normal(shape, torch.bfloat16, g).abs() for shape in ((M, K), (N, K), (N, K))]
+    clean = operators.linear(x, w, activation=activation).y
+    x[1, K // 2] = math.inf
+    got, h = operators.linear(x, w, activation=activation, keep_pre=True), operators.gated_linear(x, w, up, activation=activation).h
+    rows = [i for i in range(M) if i != 1]
+    assert bool((got.pre[1] == math.inf).all()) and bool((got.y[1] == math.inf).all()) and bool((h[1] == math.inf).all())
+    assert torch.equal(got.y[rows], clean[rows])
+
+
+@pytest.mark.gpu
 def test_no_tokens_and_no_terms():
     x = torch.empty((0, 64), device="cuda", dtype=torch.bfloat16)
     w = normal((40, 64), torch.bfloat16, generator(59))

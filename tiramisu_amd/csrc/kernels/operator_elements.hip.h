@@ -148,7 +148,8 @@ __device__ __forceinline__ float gelu_tanh_argument(float z) { return 1.59576912
 
 // The normal distribution's lower tail at -|z|, 0.5 erfc(|z| / sqrt 2) = exp(-z^2 / 2) R(t) with t = 1 / (1 + 0.31 |z|), and exp(-z^2 / 2).  R is t times a
 // polynomial of degree 5, fitted here to the smallest relative error (4.7e-6 up to |z| = 14, where the tail is below fp32's numbers; half a unit of
-// float16 is 2.4e-4): relative, so that gelu of a large negative z, z times the tail, keeps its digits.  gelu(z) = max(z, 0) - |z| tail.
+// float16 is 2.4e-4): relative, so that gelu of a large negative z, z times the tail, keeps its digits.  gelu(z) = max(z, 0) - |z| tail; the tail is zero
+// from z = 16 on, and must not meet an infinite z there.
 // (Epilogues are bound by these instructions: 3 million gelu cost 5 us with 17 of them and two of a quarter of the rate.)
 __device__ __forceinline__ float normal_tail(float z, float &bell) {
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.31f, fabsf(z), 1.f));
@@ -166,7 +167,7 @@ __device__ __forceinline__ float activated(int a, float z) {
     if (a == RELU) return z < 0.f ? 0.f : z;
     if (a == GELU) {
         float bell;
-        return __builtin_fmaf(-fabsf(z), normal_tail(z, bell), fmaxf(z, 0.f));
+        return __builtin_fmaf(-fabsf(fminf(z, 16.f)), normal_tail(z, bell), fmaxf(z, 0.f));
     }
     return z * sigmoid(a == GELU_TANH ? gelu_tanh_argument(z) : z);
 }
