@@ -427,6 +427,25 @@ def test_infinities_reach_their_own_rows_and_columns_only():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_norm_of_rows_without_elements(dtype):
+    """Their scale is that of a row of zeros, their length is NaN like the mean of nothing: what is returned is written, whatever the memory held."""
+    stale = [torch.full((5,), 7.0, device="cuda") for _ in range(8)]
+    del stale                                  # (what the results' memory held)
+    x, w = torch.empty((5, 0), dtype=dtype, device="cuda"), torch.empty((0,), dtype=dtype, device="cuda")
+    q = operators.quantize_rows(x)
+    assert q.q.shape == (5, 0) and bool((q.scale == 1).all())
+    for residual in (None, x):
+        got = operators.rms_norm(x, w, residual=residual, eight_bit=True, keep_rstd=True)
+        assert got.y.shape == got.sum.shape == (5, 0) and bool((got.scale == 1).all()) and bool(torch.isnan(got.rstd).all())
+    assert bool(torch.isnan(operators.rms_norm(x.view(5, 1, 0), w, keep_rstd=True).rstd).all())
+    back = operators.rms_norm_backward(x, x, w, got.rstd)
+    assert back.dx.shape == (5, 0) and back.dweight.shape == (0,)
+    with pytest.raises(ValueError, match="rstd"):
+        operators.rms_norm_backward(x, x, w, got.rstd[:0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("activation", list(operators.ACTIVATIONS))
 @pytest.mark.parametrize("M,N,K", [(3, 40, 100), (130, 140, 100), (100, 64, 4100)])
 def test_activation_of_an_infinite_sum(M, N, K, activation):

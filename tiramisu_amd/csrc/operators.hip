@@ -334,7 +334,6 @@ void launch_norm(const char *fn, const norm_arguments &a) {
     check(hipGetLastError(), fn);
 }
 int norm(const char *fn, int type, int y, norm_arguments a) {
-    if (a.rows == 0 || a.columns == 0) return 0;
     const long all = a.rows, step = bytes_of(type), step_y = bytes_of(y);
     auto moved = [](auto *p, long bytes) { return p ? (decltype(p))((uintptr_t)p + bytes) : p; };
     for (long first = 0; first < all; first += MOST_ROWS_A_LAUNCH) {
@@ -448,10 +447,14 @@ int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weigh
     if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu: at most 2^30 - 1 of at most 2^26", (unsigned long long)rows, (unsigned long long)columns);
     if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
     if (y_type != type && y_type != F8) return refuse(__FUNCTION__, "results of type %d from rows of type %d", y_type, type);
-    if (rows == 0 || columns == 0) return 0;
-    if (!x || !weight || !y) return refuse(__FUNCTION__, "x, weight and y are needed");
+    if (rows == 0) return 0;
+    if (columns && (!x || !weight || !y)) return refuse(__FUNCTION__, "x, weight and y are needed");
     if ((residual != nullptr) != (sum != nullptr)) return refuse(__FUNCTION__, "a residual and a place for the sum belong together");
     if ((y_type == F8) != (scale != nullptr)) return refuse(__FUNCTION__, "8-bit results and a place for their scales belong together");
+    if (columns == 0) {
+        if (!scale && !rstd) return 0;
+        weight = scale ? scale : rstd;                       // (of no elements, and not read)
+    }
     timed record(__FUNCTION__);
     const norm_arguments a = {x, residual, weight, y, sum, scale, rstd, (long)rows, (long)columns, ldx ? (long)ldx : (long)columns, ldr ? (long)ldr : (long)columns, eps};
     return norm(__FUNCTION__, type, y_type, a);
@@ -460,8 +463,8 @@ int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weigh
 int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type) {
     if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu: at most 2^30 - 1 of at most 2^26", (unsigned long long)rows, (unsigned long long)columns);
     if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
-    if (rows == 0 || columns == 0) return 0;
-    if (!x || !q || !scale) return refuse(__FUNCTION__, "x, q and scale are needed");
+    if (rows == 0) return 0;
+    if ((columns && (!x || !q)) || !scale) return refuse(__FUNCTION__, "x, q and scale are needed");
     timed record(__FUNCTION__);
     const norm_arguments a = {x, nullptr, nullptr, q, nullptr, scale, nullptr, (long)rows, (long)columns, ldx ? (long)ldx : (long)columns, 0, 0.f};
     return norm(__FUNCTION__, type, F8, a);

@@ -71,7 +71,9 @@ device_rows rows_of(const Tensor &t, const char *name, std::initializer_list<Sca
     TORCH_CHECK_VALUE(t.is_cuda(), name, " lives on ", t.device(), ": operators run on the GPU");
     TORCH_CHECK_VALUE(!like || t.device() == like->device(), name, " lives on another GPU");
     const int64_t width = t.size(dims - 1);
-    device_rows r = {width ? t.numel() / width : 0, width, width, t.data_ptr()};
+    int64_t rows = 1;
+    for (int64_t d = 0; d + 1 < dims; d++) rows *= t.size(d);
+    device_rows r = {rows, width, width, t.data_ptr()};
     if (t.is_contiguous()) return r;
     TORCH_CHECK_VALUE(t.stride(dims - 1) == 1 || width <= 1, name, ": the elements of a row are not next to each other");
     // dimensions of one row do not count, the others follow each other
