@@ -181,14 +181,14 @@ enum tiramisu_hip_activation_t {
 
 /* sum = x + residual (both or neither; else x itself), rstd = 1 / sqrt(mean(sum^2) + eps) of each row, y = sum rstd weight, of the
  * sum ahead of its rounding.  x, residual, weight, sum: `type` (float32, float16, bfloat16); y: the same, or y_type float8_e4m3:
- * y / scale with scale = max|y| / 448 of each row (1 for a row of zeros or of no elements).  rstd may be null; of a row of no elements it is NaN, like its mean. */
+ * y / scale with scale = max|y| / 448 of each row (1 where that is zero, and for a row of no elements).  rstd may be null; of a row of no elements it is NaN, like its mean. */
 int tiramisu_hip_rms_norm(const void *x, const void *residual, const void *weight, void *y, void *sum, float *scale, float *rstd,
                           uint64_t rows, uint64_t columns, uint64_t ldx, uint64_t ldr, float eps, int32_t type, int32_t y_type);
 /* dx = rstd (g - sum rstd^2 mean(g sum)) + dsum with g = dy weight; dweight = sum over the rows of dy sum rstd.  dsum (the
  * gradient that arrives at the sum itself) may be null.  dx is the gradient of x and of the residual.  Deterministic. */
 int tiramisu_hip_rms_norm_backward(const void *dy, const void *sum, const void *weight, const float *rstd, const void *dsum, void *dx,
                                    void *dweight, uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t lds, uint64_t ldd, int32_t type);
-/* q = x / scale in float8_e4m3, scale = max|x| / 448 of each row (1 for a row of zeros or of no elements). */
+/* q = x / scale in float8_e4m3, scale = max|x| / 448 of each row (1 where that is zero, and for a row of no elements). */
 int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type);
 
 /* z = x weight^T [x_scale of the row, weight_scale of the column] + bias; pre = z; y = activation(z) + residual.  x is M x K, weight N x K, both of

@@ -427,6 +427,24 @@ def test_infinities_reach_their_own_rows_and_columns_only():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("columns", [7, 300, 40000])
+def test_rows_of_the_smallest_numbers_to_8_bits(columns):
+    """Numbers below half of 448 times the smallest one have a scale of zero in 32 bits: such rows become zeros with scale 1, not NaN.  Somewhat larger ones keep a scale of few bits."""
+    least = 2.0 ** -149
+    x = torch.zeros((5, columns), device="cuda")
+    x[0, 1], x[1, ::2], x[2, 3], x[3, :], x[4, 2] = least, 100 * least, 223 * least, 400 * least, -1e-40
+    q, scale = operators.quantize_rows(x)
+    assert [float(s) / least for s in scale[3:4]] == [1.0] and bool((scale[:3] == 1).all())
+    values = q.float().double() * scale.double()[:, None]
+    assert bool(torch.isfinite(values).all()) and not bool(values[:3].any()) and torch.equal(values == 0, (x == 0) | (scale[:, None] == 1))
+    # (400: between 384 and 416 in e4m3; 1e-40: within half a step of its 4 bits, and half a unit of the scale's 8)
+    assert bool(((values[3] - 400 * least).abs() <= 16 * least).all()) and abs(float(values[4, 2]) + 1e-40) <= 1e-40 * (2.0 ** -4 + 2.0 ** -7)
+    w = torch.ones(columns, device="cuda")
+    got = operators.rms_norm(x, w, eps=1.0, eight_bit=True)
+    assert torch.equal(got.y.float(), q.float()) and torch.equal(got.scale, scale)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_norm_of_rows_without_elements(dtype):
     """Their scale is that of a row of zeros, their length is NaN like the mean of nothing: what is returned is written, whatever the memory held."""

@@ -145,7 +145,8 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void rms_norm_kernel(norm_
             }
         }
         most = team_reduce<TEAM, true>(most, slots[1]);
-        most = most == 0.f ? 1.f : most / E4M3_MOST;         // the scale; a row of zeros has 1
+        most = most / E4M3_MOST;                             // the scale
+        if (most == 0.f) most = 1.f;                         // of a row of zeros, or of numbers so small that their scale would be zero
         if (t == 0) a.scale[row] = most;
     }
     auto write = [&](int p, float (&v)[N]) {

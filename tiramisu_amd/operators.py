@@ -100,7 +100,7 @@ def rms_norm_backward(dy, sum, weight, rstd, dsum=None):
 
 
 def quantize_rows(x):
-    """x as float8_e4m3fn with a scale for each row, max|row| / 448 (1 for a row of zeros or of no elements): weights once, activations where no norm
+    """x as float8_e4m3fn with a scale for each row, max|row| / 448 (1 where that is zero, and for a row of no elements): weights once, activations where no norm
     precedes the product."""
     return EightBitRows(*_operators.quantize_rows(x))
 
