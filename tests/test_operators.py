@@ -634,6 +634,25 @@ def test_what_is_refused_without_a_gpu():
 
 
 @pytest.mark.gpu
+def test_gradients_are_not_dropped_silently():
+    """A tensor that requires a gradient is refused while gradients are recorded, in any place; otherwise it is a tensor like others."""
+    g = generator(103)
+    x, w, h = normal((4, 64), torch.bfloat16, g), normal((8, 64), torch.bfloat16, g), normal((4, 8), torch.bfloat16, g)
+    p, rstd = torch.nn.Parameter(w), torch.ones(4, device="cuda")
+    calls = [lambda w: operators.linear(x, w).y, lambda w: operators.gated_linear(x, w, w).h, lambda w: operators.rms_norm(x, w[0]).y, lambda w: operators.quantize_rows(w).scale,
+             lambda w: operators.linear(x, p.detach(), residual=h, bias=w[:, 0].contiguous()).y, lambda w: operators.rms_norm(x, p.detach()[0], residual=w[:4]).sum,
+             lambda w: operators.linear_backward(h, x, w).dx, lambda w: operators.rms_norm_backward(x, x, w[0], rstd).dx]
+    for call in calls:
+        with pytest.raises(ValueError, match="requires a gradient"):
+            call(p)
+        plain = call(w)
+        for without in (torch.no_grad(), torch.inference_mode()):
+            with without:
+                assert torch.equal(call(p), plain)
+        assert not plain.requires_grad
+
+
+@pytest.mark.gpu
 def test_what_is_refused():
     x, w = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((8, 64), dtype=torch.bfloat16, device="cuda")
     h = torch.zeros((4, 8), dtype=torch.bfloat16, device="cuda")

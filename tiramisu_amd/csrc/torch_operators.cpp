@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/Allocator.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -53,7 +54,11 @@ std::string names_of(std::initializer_list<ScalarType> types) {
 // ---- arguments
 Tensor tensor_of(PyObject *o, const char *name) {
     TORCH_CHECK_VALUE(THPVariable_Check(o), name, " is a tensor, not ", Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
+    const Tensor &t = THPVariable_Unpack(o);
+    // (a result without a graph would say nothing of the gradient that it loses)
+    TORCH_CHECK_VALUE(!t.requires_grad() || !c10::GradMode::is_enabled(), name, " requires a gradient, which operators do not record: call them under torch.no_grad(), and their "
+                      "backward functions");
+    return t;
 }
 bool given(PyObject *o) { return o != Py_None; }
 

@@ -4,7 +4,7 @@ kernel; each with its backward pass, on 16-bit operands or (forward) 8-bit ones 
 
 These functions check their arguments, allocate the results and call the runtime's C ABI (include/tiramisu_hip_wrappers.h), whose
 kernels run on torch's current stream of the tensors' device; nothing waits for them.  They record nothing for autograd: the backward passes are
-functions of their own.  Leading dimensions are tokens: x of shape
+functions of their own, and tensors that require a gradient are taken where none is recorded (torch.no_grad()).  Leading dimensions are tokens: x of shape
 [..., K] gives a result of shape [..., N].  Weights are [outputs, inputs].  Tensors need dense rows (stride 1 in the last
 dimension), with one stride from row to row; others are refused, never copied silently.  Results are new, dense tensors.
 ValueError says what does not fit, RuntimeError that the runtime refused the call (its reason is on stderr), torch's out-of-memory error that there is no
