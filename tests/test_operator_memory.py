@@ -192,3 +192,23 @@ def test_graphs_of_one_recording_stream_replay_beside_each_other():
         for got, was in zip(results, expected):
             assert all(torch.equal(u, v) for u, v in zip(got, was))
         call(*inputs[turn % 2])
+
+
+def test_launches_hold_fewer_than_2_to_the_32_threads():
+    """Rows of a workgroup of 1024 threads each, just more than one launch holds: several launches, which together are all of the rows'."""
+    out = host_runtime.printed("""
+p = 1 << 20
+rows = (1 << 22) + 5
+def rows_of(kernel):
+    found = [b for k, b, t in launches() if kernel in k]
+    return len(found), sum(found)
+for type, columns in ((2, 8200), (0, 4100), (2, 40000)):
+    assert w.tiramisu_hip_quantize_rows(p, p, p, rows, columns, 0, type) == 0
+    print(rows_of("rms_norm_kernel"))
+assert w.tiramisu_hip_rms_norm(p, p, p, p, p, None, p, rows - 5, 8200, 0, 0, 1e-6, 2, 2) == 0
+print(rows_of("rms_norm_kernel"))
+assert w.tiramisu_hip_rms_norm_backward(p, p, p, p, p, p, p, rows, 40000, 0, 0, 0, 2) == 0
+print(rows_of("long_rows"))
+""")
+    rows = (1 << 22) + 5
+    assert out == ("(2, %d)\n" % rows) * 3 + "(2, %d)\n" % (rows - 5) + "(2, %d)\n" % rows

@@ -187,6 +187,7 @@ struct norm_backward_arguments {
     float *partial;                         // [workgroups][columns]
     long rows, columns, ldy, lds, ldd;
     int parts;                              // (rows that no team holds: of the walk down the columns)
+    long first;                             // (... and the launch's first row)
 };
 
 // Teams walk over the rows, team g taking rows g, g + teams, ....  Teams of one wavefront need no barrier on the way, and the eight of a workgroup add their
@@ -290,7 +291,7 @@ template <int E>
 __global__ __launch_bounds__(1024) void rms_norm_backward_long_rows_kernel(norm_backward_arguments a) {
     __shared__ float slots[16];
     typedef stored<E> T;
-    const long row = blockIdx.x;
+    const long row = a.first + blockIdx.x;
     const T *dy = (const T *)a.dy + row * a.ldy, *s = (const T *)a.sum + row * a.lds, *w = (const T *)a.weight;
     const T *ds = a.dsum ? (const T *)a.dsum + row * a.ldd : nullptr;
     const float rstd = a.rstd[row];

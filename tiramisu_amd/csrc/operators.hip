@@ -35,7 +35,7 @@ __attribute__((format(printf, 2, 3))) int refuse(const char *fn, const char *for
 }
 
 constexpr uint64_t MOST = 0x3fffffff;                    // rows and columns are counted in 31 bits, with room for a tile
-constexpr int64_t MOST_ROWS_A_LAUNCH = 1 << 22;          // of a workgroup each: a launch holds 2^32 threads
+constexpr int64_t MOST_ROWS_A_LAUNCH = (1 << 22) - 4;    // of a workgroup of up to 1024 threads each: a launch holds fewer than 2^32 threads
 constexpr int64_t MOST_PIECES_A_LAUNCH = 1LL << 31;      // of a thread each
 constexpr uint64_t MOST_TILES = (1 << 23) - 1;           // of 64 x 64: the same
 constexpr uint64_t MOST_COLUMNS = 1 << 26;               // of a norm: the same for the sums of the columns
@@ -372,7 +372,8 @@ int launch_norm_backward(const char *fn, norm_backward_arguments a, void *dweigh
     };
     auto go_long = [&] {
         if (!sums_of(std::min(a.rows, 64L))) return false;
-        if (a.rows > 0) hipLaunchKernelGGL(rms_norm_backward_long_rows_kernel<E>, dim3((unsigned)a.rows), dim3(1024), 0, stream(), a);
+        for (a.first = 0; a.first < a.rows; a.first += MOST_ROWS_A_LAUNCH)
+            hipLaunchKernelGGL(rms_norm_backward_long_rows_kernel<E>, dim3((unsigned)std::min(MOST_ROWS_A_LAUNCH, a.rows - a.first)), dim3(1024), 0, stream(), a);
         hipLaunchKernelGGL(rms_norm_backward_long_columns_kernel<E>, dim3((unsigned)((a.columns + 255) / 256), (unsigned)a.parts), dim3(256), 0, stream(), a);
         return true;
     };
@@ -478,7 +479,7 @@ int tiramisu_hip_rms_norm_backward(const void *dy, const void *sum, const void *
     if (!dweight || !weight || (rows && (!dy || !sum || !rstd || !dx))) return refuse(__FUNCTION__, "dy, sum, weight, rstd, dx and dweight are needed");
     timed record(__FUNCTION__);
     const norm_backward_arguments a = {dy, sum, weight, dsum, rstd, dx, nullptr, (long)rows, (long)columns, ldy ? (long)ldy : (long)columns,
-                                       lds ? (long)lds : (long)columns, ldd ? (long)ldd : (long)columns, 0};
+                                       lds ? (long)lds : (long)columns, ldd ? (long)ldd : (long)columns, 0, 0};
     return type == F32 ? launch_norm_backward<F32>(__FUNCTION__, a, dweight) : type == F16 ? launch_norm_backward<F16>(__FUNCTION__, a, dweight) : launch_norm_backward<BF16>(__FUNCTION__, a, dweight);
 }
 
