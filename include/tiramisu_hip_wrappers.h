@@ -166,8 +166,8 @@ int tiramisu_hip_device_count(void);
 
 /* ---- operators of a transformer's feed-forward sublayer on this build's own kernels, forward and backward (the reference has
  *      nothing of the kind).  All pointers are GPU memory; all launches go to the calling thread's stream and nothing waits.
- *      Matrices are row-major with their columns dense and `ld...` elements from row to row (0: dense rows too); results are dense and must not
- *      overlap inputs.  Weights are [outputs][inputs].  Operands may begin at any element; rows that the
+ *      Matrices are row-major with their columns dense and `ld...` elements from row to row (0: dense rows too; gradients refuse rows of operands that
+ *      overlap); results are dense and must not overlap inputs.  Weights are [outputs][inputs].  Operands may begin at any element; rows that the
  *      matrix kernels cannot load in place (odd strides of 16-bit elements) are moved to scratch first.  Sums are kept in 32 bits and rounded once.
  *      Types and activations are the numbers below.  Arguments that do not fit together, and calls whose scratch cannot be had, are refused: a message
  *      on stderr, return value 1, nothing launched.  Scratch (gradients ahead of an activation, partial sums, moved rows) is one block for each thread, stream

@@ -212,3 +212,15 @@ print(rows_of("long_rows"))
 """)
     rows = (1 << 22) + 5
     assert out == ("(2, %d)\n" % rows) * 3 + "(2, %d)\n" % (rows - 5) + "(2, %d)\n" % rows
+
+
+def test_gradients_of_overlapping_rows_are_refused():
+    """dx and dweight read their operands down the columns, up to an end behind the last row: rows closer together than they are long have none."""
+    out, r = host_runtime.run("""
+p = 1 << 20
+print([w.tiramisu_hip_linear_backward(p, p, p, None, p, p, None, 70, 40, 50, *strides, 0, 0, 2) for strides in ((39, 0, 0), (0, 49, 0), (0, 0, 1), (40, 50, 50))])
+print([w.tiramisu_hip_gated_linear_backward(p, p, p, p, p, p, p, p, p, 70, 40, 50, 0, *strides, 0, 0, 4, 2) for strides in ((49, 0, 0), (0, 49, 0), (0, 0, 49), (50, 51, 52))])
+print(w.tiramisu_hip_linear_backward(p, p, p, None, p, p, None, 1, 40, 50, 1, 1, 0, 0, 0, 2))
+""")
+    assert r.returncode == 0 and out == "[1, 1, 1, 0]\n[1, 1, 1, 0]\n0\n", r.stderr
+    assert r.stderr.count(" apart") == 6

@@ -426,6 +426,11 @@ int refuse_result(const char *fn, uint64_t rows, uint64_t columns) {
     if (((rows + 63) / 64) * ((columns + 63) / 64) <= MOST_TILES) return 0;
     return refuse(fn, "result of %llu x %llu: more tiles than a launch holds", (unsigned long long)rows, (unsigned long long)columns);
 }
+// An operand whose rows overlap has no end behind its last row that the tiles could stop at where k runs down its columns.
+int refuse_overlap(const char *fn, const char *name, uint64_t rows, uint64_t columns, uint64_t ld) {
+    if (rows <= 1 || ld == 0 || ld >= columns) return 0;
+    return refuse(fn, "%s: rows of %llu are %llu apart", name, (unsigned long long)columns, (unsigned long long)ld);
+}
 // What both products refuse alike
 int refuse_product(const char *fn, uint64_t M, uint64_t N, uint64_t K, int activation, int type, int y) {
     if (M > MOST || N > MOST || K > MOST) return refuse(fn, "product of %llu x %llu x %llu: dimensions of at most 2^30 - 1", (unsigned long long)M, (unsigned long long)N, (unsigned long long)K);
@@ -540,6 +545,7 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
     if ((int64_t)N * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (unsigned long long)N, (long long)MOST_ROW_BYTES);
     if (refuse_result(__FUNCTION__, M, K) || refuse_result(__FUNCTION__, N, K)) return 1;
     if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
+    if (refuse_overlap(__FUNCTION__, "dy", M, N, ldy) || refuse_overlap(__FUNCTION__, "x", M, K, ldx) || refuse_overlap(__FUNCTION__, "weight", N, K, ldw)) return 1;
     if ((activation != NONE) != (pre != nullptr)) return refuse(__FUNCTION__, "an activation and the sums ahead of it belong together");
     if ((M && N && !dy) || (M && K && dweight && !x) || (N && K && dx && !weight)) return refuse(__FUNCTION__, "dy, x and weight are needed");
     timed record(__FUNCTION__);
@@ -579,6 +585,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
     if ((int64_t)(2 * N + 16) * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (unsigned long long)N, (long long)MOST_ROW_BYTES);
     if (refuse_result(__FUNCTION__, M, K) || refuse_result(__FUNCTION__, 2 * N + 16, K)) return 1;
     if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
+    if (refuse_overlap(__FUNCTION__, "x", M, K, ldx) || refuse_overlap(__FUNCTION__, "gate_weight", N, K, ldg) || refuse_overlap(__FUNCTION__, "up_weight", N, K, ldu)) return 1;
     if ((M && N && (!dh || !gate || !up)) || (M && K && N && !x) || (N && K && (!gate_weight || !up_weight))) return refuse(__FUNCTION__, "dh, x, both weights, gate and up are needed");
     if ((dgate_weight != nullptr) != (dup_weight != nullptr)) return refuse(__FUNCTION__, "gradients of both weights, or of neither");
     timed record(__FUNCTION__);
