@@ -197,7 +197,7 @@ int tiramisu_hip_quantize_rows(const void *x, void *q, float *scale, uint64_t ro
 int tiramisu_hip_linear(const void *x, const void *weight, const void *bias, const void *residual, const float *x_scale,
                         const float *weight_scale, void *y, void *pre, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldw,
                         uint64_t ldr, int32_t activation, int32_t type, int32_t y_type);
-/* dz = dy activation'(pre), dx = dz weight, dweight = dz^T x, dbias = sum over the rows of dz (the residual's gradient is dy).  Of
+/* dz = dy activation'(pre) (relu's slope at 0 is 0), dx = dz weight, dweight = dz^T x, dbias = sum over the rows of dz (the residual's gradient is dy).  Of
  * float16 or bfloat16 throughout; dz is rounded to that type ahead of the products.  dx, dweight, dbias may be null; pre is null where
  * the activation is none. */
 int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weight, const void *pre, void *dx, void *dweight, void *dbias,
