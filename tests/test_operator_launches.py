@@ -16,20 +16,22 @@ HALVES = [torch.bfloat16, torch.float16]
 LINEAR_16 = {
     "few": (9, 93, 330), "few, 32": (31, 61, 166), "few, 64": (53, 45, 234),
     "y 64x64": (143, 9, 46), "y 64x64 split": (65, 9, 2918), "y 128x64": (135, 5677, 44), "y 128x64 split": (2267, 9, 4028), "y 128x128": (3965, 513, 32),
-    "y 256x128": (3311, 1369, 34), "y 256x256": (3661, 3551, 146),
+    "y 256x128": (3311, 1369, 34), "y 256x256": (3661, 3551, 146), "y 128x128 split": (145, 2743, 5258), "y 256x128 split": (6931, 69, 11422), "y 256x256 split": (521, 3609, 11362),
 }
 LINEAR_8 = {
     "few": (9, 93, 332), "few, 32": (31, 61, 164), "few, 64": (53, 45, 236),
     "y 64x64": (143, 9, 44), "y 128x64": (147, 5807, 36), "y 128x128": (331, 5645, 644), "y 256x128": (1655, 3815, 292), "y 256x256": (2805, 4937, 284),
+    "y 64x64 split": (1, 9, 28264), "y 128x64 split": (2823, 9, 10444), "y 256x128 split": (5011, 427, 12796),
 }
 GATED_16 = {
     "few": (9, 93, 330), "few, 32": (31, 61, 166), "few, 64": (53, 45, 234),
     "y 64x128": (79, 9, 36), "y 64x128 split": (15, 9, 3982), "y 128x128": (131, 5649, 34), "y 128x128 split": (3527, 9, 2834), "y 256x128": (1655, 2059, 34),
-    "y 256x256": (1113, 5619, 136),
+    "y 256x256": (1113, 5619, 136), "y 256x128 split": (9391, 9, 3784), "y 256x256 split": (141, 6435, 12082),
 }
 GATED_8 = {
     "few": (9, 93, 332), "few, 32": (31, 61, 164), "few, 64": (53, 45, 236),
     "y 64x128": (67, 9, 36), "y 128x128": (1633, 635, 1232), "y 256x128": (981, 3487, 560), "y 256x256": (2771, 2693, 420),
+    "y 64x128 split": (1, 11, 12400), "y 256x128 split": (6315, 149, 12104),
 }
 LINEAR_BACKWARD = {
     "dx and dw 64x64": (1, 11, 34), "dw and dx 64x64": (67, 9, 34), "dx and dw 128x64": (65, 133, 3436), "dw and dx 128x64": (143, 65, 3758), "dx and dw 128x128": (327, 365, 2830),
@@ -38,6 +40,9 @@ LINEAR_BACKWARD = {
     "dx 64x64, dw 64x64 split": (3733, 11, 34), "dx 64x64 split, dw 64x64": (1, 3991, 34), "dx 64x64 split, dw 128x64": (1, 6079, 132), "dx 64x64 split, dw 128x128": (1, 5897, 344),
     "dx 64x64 split, dw 256x128": (1, 5517, 850), "dx 128x64 split, dw 64x64": (1155, 5751, 66), "dx 128x64, dw 128x128": (1191, 1685, 1474), "dx 128x128, dw 128x64": (1715, 1043, 1770),
     "dx 128x128, dw 256x128": (957, 1233, 3718), "dx 128x64, dw 256x256": (315, 3707, 4058), "dx 256x128, dw 128x128": (1419, 987, 3986), "dx 256x256, dw 128x64": (3327, 419, 4038),
+    "dx 128x128 split, dw 128x128": (73, 10085, 4168), "dx 256x128 split, dw 128x128": (151, 14655, 2786), "dx 256x256 split, dw 256x256": (823, 14315, 2882),
+    "dx 128x128, dw 128x64 split": (9009, 71, 1156), "dx 256x256, dw 128x128 split": (8139, 67, 5974), "dx 256x256, dw 256x128 split": (8231, 129, 5790),
+    "dx 256x256, dw 256x256 split": (17381, 519, 3916),
 }
 GATED_BACKWARD = {
     "dx and dw 64x64": (1, 9, 50), "dw and dx 64x64": (81, 11, 32), "dx and dw 128x64": (71, 53, 4164), "dw and dx 128x64": (135, 33, 3824), "dx and dw 128x128": (249, 147, 3976),
@@ -46,7 +51,8 @@ GATED_BACKWARD = {
     "dx 64x64, dw 64x64 split": (3901, 9, 34), "dx 64x64 split, dw 64x64": (1, 1881, 42), "dx 64x64 split, dw 256x128": (1, 3627, 532), "dx 128x64 split, dw 128x64 split": (4157, 4759, 36),
     "dx 128x64 split, dw 128x128": (65, 4897, 1022), "dx 128x64 split, dw 256x256": (181, 5537, 1274), "dx 128x64, dw 128x128": (1523, 1345, 1194), "dx 128x128 split, dw 128x128": (129, 5591, 3114),
     "dx 128x128, dw 128x64": (1479, 519, 1724), "dx 256x128 split, dw 256x256": (1195, 4197, 1744), "dx 256x128, dw 64x64": (2581, 409, 2358), "dx 256x256, dw 128x128": (3979, 547, 3256),
-    "dx 256x256, dw 256x128": (3191, 687, 3902),
+    "dx 256x256, dw 256x128": (3191, 687, 3902), "dx 256x256 split, dw 256x256": (131, 9765, 8252), "dx 128x128, dw 128x128 split": (17879, 1369, 66),
+    "dx 128x128, dw 256x128 split": (20999, 2103, 74), "dx 256x256, dw 256x256 split": (15271, 305, 4314),
 }
 # rows, columns: what definitions.test_norm_backward leaves out, and rows that teams take several of
 NORM_BACKWARD = [(40, 400), (600, 1001), (5000, 2001), (900, 3999)]
