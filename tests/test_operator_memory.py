@@ -21,6 +21,22 @@ print(first != second, again == second, at() == first)
 """) == "True True True\n"
 
 
+def test_idle_blocks_of_the_pool_belong_to_a_gpu():
+    """A block that was freed on one GPU is handed out there only."""
+    assert host_runtime.printed("""
+first = w.tiramisu_hip_malloc(1 << 20)
+w.tiramisu_hip_free(first)
+hip.hipSetDevice(1)
+second = w.tiramisu_hip_malloc(1 << 20)
+hip.hipSetDevice(0)
+print(second != first, w.tiramisu_hip_malloc(1 << 20) == first)
+w.tiramisu_hip_free(second)
+print(w.tiramisu_hip_malloc(1 << 20) != second, w.tiramisu_hip_cached_memory_bytes() == 1 << 20)
+hip.hipSetDevice(1)
+print(w.tiramisu_hip_malloc(1 << 20) == second, w.tiramisu_hip_release_cached_memory())
+""") == "True True\nTrue True\nTrue 0\n"
+
+
 # Calls that need scratch for each of its uses, on addresses that are no memory: the gradient ahead of an activation, columns' sums, both projections' gradients,
 # sums of a product whose k is split, rows that begin at odd elements.
 CALLS = """

@@ -135,15 +135,16 @@ thread_local bool in_parallel_iteration = false;
 
 // ---- pooled device memory (see tiramisu_hip_malloc)
 std::mutex pool_mutex;
-std::map<uint64_t, std::vector<void *>> pool_free;   // idle blocks by size
-std::map<void *, uint64_t> pool_live;                  // blocks handed out
+typedef std::pair<int, uint64_t> pooled_size;           // of a GPU's memory
+std::map<pooled_size, std::vector<void *>> pool_free;  // idle blocks
+std::map<void *, pooled_size> pool_live;               // blocks handed out
 uint64_t pool_idle_bytes = 0;
 // Idle blocks go back to HIP; returns their bytes
 uint64_t release_idle_blocks() {
     std::lock_guard<std::mutex> g(pool_mutex);
     uint64_t released = 0;
     for (auto &kv : pool_free)
-        for (void *q : kv.second) { check(hipFree(q), "tiramisu_hip_malloc"); released += kv.first; }
+        for (void *q : kv.second) { check(hipFree(q), "tiramisu_hip_malloc"); released += kv.first.second; }
     pool_free.clear();
     pool_idle_bytes = 0;
     return released;
@@ -553,17 +554,18 @@ extern "C" {
 
 // Device memory is pooled: generated functions allocate their temporaries on entry and free
 // them on exit, every call (the reference pays cudaMalloc / cudaFree each time,
-// tiramisu_cuda_wrappers.cpp:55-68).  A freed block is kept, by size, for the next request of that
-// size; blocks beyond TIRAMISU_HIP_POOL_BYTES (default 16 GiB; 0 turns pooling off) go back to HIP.
+// tiramisu_cuda_wrappers.cpp:55-68).  A freed block is kept, by GPU and size, for the next request of that
+// size there; blocks beyond TIRAMISU_HIP_POOL_BYTES (default 16 GiB; 0 turns pooling off) go back to HIP.
 void *tiramisu_hip_malloc(uint64_t size) {
+    const pooled_size kind(here().device, size);
     {
         std::lock_guard<std::mutex> g(pool_mutex);
-        auto it = pool_free.find(size);
+        auto it = pool_free.find(kind);
         if (it != pool_free.end() && !it->second.empty()) {
             void *p = it->second.back();
             it->second.pop_back();
             pool_idle_bytes -= size;
-            pool_live[p] = size;
+            pool_live[p] = kind;
             return p;
         }
     }
@@ -577,21 +579,21 @@ void *tiramisu_hip_malloc(uint64_t size) {
     }
     check(e, __FUNCTION__);
     std::lock_guard<std::mutex> g(pool_mutex);
-    pool_live[p] = size;
+    pool_live[p] = kind;
     return p;
 }
 
 int tiramisu_hip_free(void *ptr) {
     if (!ptr) return 0;
-    uint64_t size = 0;
+    pooled_size kind;
     bool keep = false;
     {
         std::lock_guard<std::mutex> g(pool_mutex);
         auto it = pool_live.find(ptr);
         if (it != pool_live.end()) {
-            size = it->second;
+            kind = it->second;
             pool_live.erase(it);
-            keep = pool_idle_bytes + size <= pool_limit();
+            keep = pool_idle_bytes + kind.second <= pool_limit();
         }
     }
     if (!keep) {
@@ -602,8 +604,8 @@ int tiramisu_hip_free(void *ptr) {
     // streams that tiramisu_hip_parallel_for has already synchronised)
     check(hipStreamSynchronize(current_stream), __FUNCTION__);
     std::lock_guard<std::mutex> g(pool_mutex);
-    pool_free[size].push_back(ptr);
-    pool_idle_bytes += size;
+    pool_free[kind].push_back(ptr);
+    pool_idle_bytes += kind.second;
     return 0;
 }
 
