@@ -27,7 +27,7 @@
 // 4096 with both projections kept 420 - 440 us, 1250 - 1310; e4m3 4096^3 62 - 69 us, 2000 - 2200 TFLOP/s, matrix cores busy 45 % of the time: slices come
 // into a compute unit's LDS at about 40 bytes a nanosecond, and 256 x 256 is the largest tile whose sums fit the registers.  Slices of 64 bytes in a
 // deeper ring are no faster (bf16 103 us, e4m3 64), nor are rows padded to other strides.  Small products are one round of tiles: launch, first slices and
-// epilogue stand one after the other (2000 x 1500 x 1000 17.1 us with gelu and the sums kept, 11.8 without).
+// epilogue stand one after the other (2000 x 1500 x 1000 f16 17.3 us a call with gelu and the sums kept, 16.3 with gelu, 14.7 without).
 #ifndef TIRAMISU_AMD_LINEAR_TILES_HIP_H
 #define TIRAMISU_AMD_LINEAR_TILES_HIP_H
 #include <type_traits>

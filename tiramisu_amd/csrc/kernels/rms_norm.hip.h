@@ -5,8 +5,8 @@
 // Each input is read once and each output written once: a row stays in the registers of its team (64, 256 or 1024 threads, PER
 // pieces of 16 bytes of the widest input each), which reduces it by lane exchanges and, where it is more than a wavefront, through LDS.  The norm
 // is of the unrounded sum.  Rows too long for that are read a second time.
-// Bound by the bytes: 16384 x 4096 bf16 with a residual 96 us, 5.6 TB/s (a copy of 4 GiB: 4.9); 8192 x 2048 backward 29.5 us, 4.5 TB/s, of which the sums'
-// launch is 4.8.  Few rows are bound by the launch: one of 4096 to 8 bits 4.9 us, of which an empty kernel is 2.8.  Tried and not faster: weights
+// Bound by the bytes: 16384 x 4096 bf16 with a residual 96 us, 5.6 TB/s (the fastest copy of 4 GiB: 5.5), to 8 bits 91, 5.1 TB/s, without a norm 51, 4.0;
+// 8192 x 2048 backward 29.5 us, 4.5 TB/s, of which the sums' launch is 4.7.  Few rows are bound by the launch: one of 4096 to 8 bits 4.8 us, of which an empty kernel is 2.8.  Tried and not faster: weights
 // loaded ahead of the reduction (100 us), a wavefront to a row forward.
 // Sums of the backward pass over rows are kept per team in registers, written once a workgroup, and added by a second launch in a fixed
 // order: results do not depend on the order of workgroups.
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void rms_norm_kernel(norm_
         const int n = (int)min((long)N, a.columns - c);
         if (n <= 0) return;
         if constexpr (Y == F8) {
-            // (a scale below the normal numbers is rounded coarsely: what then lies beyond the format's largest number is set to it)
+            // (a scale below the normal numbers is rounded coarsely: what then lies beyond the format's largest number is set to it; one that would be zero is 1)
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 v[i] /= most;
