@@ -213,6 +213,52 @@ int tiramisu_hip_gated_linear(const void *x, const void *gate_weight, const void
 int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate,
                                        const void *up, void *dx, void *dgate_weight, void *dup_weight, uint64_t M, uint64_t N, uint64_t K, uint64_t ldh,
                                        uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
+/* ---- operators of a feed-forward sublayer with experts, and of 4-bit weights: the rules above, the numbers of types and activations below them.
+ *      Rows grouped by expert: `offsets` (groups + 1 of them, rising, in GPU memory; the host never reads them) say where each group's S places begin and end;
+ *      places behind the last group's are rows of zeros in results, and give nothing to gradients.  `rows` (may be null: x holds the S places' rows, T = S) picks
+ *      the row of x, of T, for each place; numbers that are none of x's give rows of zeros.  Group g's weight is N x K, all of them one below the other. ---- */
+
+/* The k largest of each token's `count` logits (ties to the lowest index, NaN above everything, minus infinity never), and their weights: softmax
+ * over the chosen ones (normalise) or over all.  A place that no expert is left for has expert -1 and weight 0.  Places by expert, in order of token and rank: offsets
+ * [count + 1], rows [tokens k] (token of a place; -1 behind the last), places [tokens][k] (of each choice; -1 for none).  logits: float32, float16, bfloat16; at most 1024 experts,
+ * 16 choices, 2^24 tokens. */
+int tiramisu_hip_route(const void *logits, int32_t *experts, float *weights, int32_t *offsets, int32_t *rows, int32_t *places, uint64_t tokens, uint64_t count, uint64_t k,
+                       uint64_t ldl, int32_t normalise, int32_t type);
+/* dlogits (dense, of their type) from the weights' gradient and the experts that were chosen (-1 and other numbers that are no expert: none). */
+int tiramisu_hip_route_backward(const float *dweights, const void *logits, const int32_t *experts, void *dlogits, uint64_t tokens, uint64_t count, uint64_t k, uint64_t ldl,
+                                int32_t normalise, int32_t type);
+/* y[s] = x[rows[s]] weight[g]^T, scaled like tiramisu_hip_linear (x_scale of x's T rows, weight_scale [groups][N]).  At most 1024 groups. */
+int tiramisu_hip_grouped_linear(const void *x, const void *weight, const int32_t *offsets, const int32_t *rows, const float *x_scale, const float *weight_scale, void *y,
+                                uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldw, int32_t type, int32_t y_type);
+/* dx[s] = dy[s] weight[g] (of each place: the gradient of a row of x that several places picked is their sum), dweight[g] = sum over the group of dy[s]^T x[rows[s]], zeros
+ * for a group without places.  Either may be null. */
+int tiramisu_hip_grouped_linear_backward(const void *dy, const void *x, const void *weight, const int32_t *offsets, const int32_t *rows, void *dx, void *dweight, uint64_t S,
+                                         uint64_t T, uint64_t groups, uint64_t N, uint64_t K, uint64_t ldy, uint64_t ldx, uint64_t ldw, int32_t type);
+/* tiramisu_hip_gated_linear for grouped rows: h, and gate and up where both are given, of S places. */
+int tiramisu_hip_grouped_gated_linear(const void *x, const void *gate_weight, const void *up_weight, const int32_t *offsets, const int32_t *rows, const float *x_scale,
+                                      const float *gate_scale, const float *up_scale, void *h, void *gate, void *up, uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K,
+                                      uint64_t ldx, uint64_t ldg, uint64_t ldu, int32_t activation, int32_t type, int32_t h_type);
+/* ... and its gradients; dx of each place.  dgate and dup are rounded to `type` ahead of the products. */
+int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate, const void *up, const int32_t *offsets,
+                                               const int32_t *rows, void *dx, void *dgate_weight, void *dup_weight, uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K,
+                                               uint64_t ldh, uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
+/* y[t] = residual[t] + sum over j < k of weights[t][j] x[places[t][j]]; places outside of x's `rows` count as none.  weights (null: ones) in 32 bits, residual may be null;
+ * the rest float16 or bfloat16. */
+int tiramisu_hip_combine_rows(const void *x, const int32_t *places, const float *weights, const void *residual, void *y, uint64_t tokens, uint64_t k, uint64_t rows, uint64_t columns,
+                              uint64_t ldx, uint64_t ldr, int32_t type);
+/* dx[places[t][j]] = weights[t][j] dy[t] (each row is in `places` once at most), zeros where owners (the token of each row: tiramisu_hip_route's rows) name no token;
+ * dweights[t][j] = dy[t] . x[places[t][j]].  Either may be null. */
+int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int32_t *places, const int32_t *owners, const float *weights, void *dx, float *dweights, uint64_t tokens,
+                                       uint64_t k, uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t ldx, int32_t type);
+/* Rows in 4 bits: e2m1 values (0, 1/2, 1, 3/2, 2, 3, 4, 6 and their negatives), two to a byte with the first in the low half, (columns + 1) / 2 bytes a row, and for each 32 of a row the
+ * power of two, as its exponent and 127 (e8m0), that is the smallest by which the largest of them is at most 6; 1 for zeros, 255 (NaN) where one is not finite.  Dense results. */
+int tiramisu_hip_quantize_groups(const void *x, void *q, uint8_t *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type);
+/* tiramisu_hip_linear and tiramisu_hip_gated_linear with weights in 4 bits; ldq, ldg, ldu, lds, ldgs, ldus: bytes from row to row of values and scales.  x, bias, residual and results
+ * are float16 or bfloat16; weights are multiplied as numbers of that type, which bfloat16 holds exactly and float16 within its range. */
+int tiramisu_hip_four_bit_linear(const void *x, const void *q, const uint8_t *scale, const void *bias, const void *residual, void *y, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx,
+                                 uint64_t ldq, uint64_t lds, uint64_t ldr, int32_t activation, int32_t type);
+int tiramisu_hip_four_bit_gated_linear(const void *x, const void *gate_q, const void *up_q, const uint8_t *gate_scale, const uint8_t *up_scale, void *h, uint64_t M, uint64_t N,
+                                       uint64_t K, uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ldgs, uint64_t ldus, int32_t activation, int32_t type);
 /* Where the calling thread's operator calls take their scratch from, exchanged with *source.  `take` is called once at most by a call, before it launches
  * anything, and returns GPU memory of at least `bytes` at a multiple of 256 which is the call's until what it puts on the thread's stream has run (for a call
  * recorded into a graph: until the graph is gone), or NULL, which refuses the call.  It must not throw.  take = NULL: the runtime's blocks, where every thread begins. */

@@ -74,15 +74,16 @@ def build_compiler(force=True):
 
 
 # The runtime's translation units: (object, source, what it is compiled with).  The matrix products' kernels are one unit for each type of operand.
-WRAPPER_UNITS = [("hip_wrappers", "hip_wrappers.hip", []), ("operators", "operators.hip", [])] + \
+WRAPPER_UNITS = [("hip_wrappers", "hip_wrappers.hip", []), ("operators", "operators.hip", []), ("expert_operators", "expert_operators.hip", [])] + \
     [("linear_tiles_" + e.lower(), "linear_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16")] + \
-    [("linear_tiles_f8", "linear_tiles.hip", ["-DTIRAMISU_OPERAND=F8", "-DTIRAMISU_OPERAND_HAS_NO_GRADIENTS"])]
+    [("linear_tiles_f8", "linear_tiles.hip", ["-DTIRAMISU_OPERAND=F8", "-DTIRAMISU_OPERAND_HAS_NO_GRADIENTS"])] + \
+    [("grouped_tiles_" + e.lower(), "grouped_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16", "F8")]
 
 
 def build_wrappers(force=True):
     kdir = os.path.join(CSRC, "kernels")
     deps = sorted({os.path.join(CSRC, source) for _, source, _ in WRAPPER_UNITS}) + \
-        [os.path.join(CSRC, "operators.h"), os.path.join(INCLUDE, "tiramisu_hip_wrappers.h")] + [os.path.join(kdir, h) for h in os.listdir(kdir)]
+        [os.path.join(CSRC, h) for h in ("operators.h", "operator_calls.h", "grouped_operators.h")] + [os.path.join(INCLUDE, "tiramisu_hip_wrappers.h")] + [os.path.join(kdir, h) for h in os.listdir(kdir)]
     out = wrappers_library()
     if not force and _newer(out, deps):
         return out

@@ -1,0 +1,550 @@
+// Entry points of the operators of a feed-forward sublayer with experts and of 4-bit weights (include/tiramisu_hip_wrappers.h): what they refuse, which kernel a
+// call goes to, and the launches.  As in operators.hip: all launches of a call are planned first, then its scratch is asked for, as one block.
+#include "operator_calls.h"
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/tiramisu_hip_wrappers.h"
+#include "grouped_operators.h"
+#include "kernels/combine.hip.h"
+#include "kernels/four_bit.hip.h"
+#include "kernels/operator_backward.hip.h"
+#include "kernels/route.hip.h"
+#include "kernels/target_gfx950.h"
+
+using namespace tops;
+using tiramisu_runtime::check;
+using tiramisu_runtime::stream;
+using tiramisu_runtime::timed;
+
+namespace {
+
+typedef unsigned long long ull;
+
+// ---- route
+using troute::ROUTE_THREADS;
+using troute::route_arguments;
+using troute::route_backward_arguments;
+
+// (lanes of a token and values of a lane, by the number of experts)
+template <class F>
+void by_experts(int experts, F f) {
+    if (experts <= 16) f(std::integral_constant<int, 16>(), std::integral_constant<int, 1>());
+    else if (experts <= 32) f(std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
+    else if (experts <= 64) f(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
+    else if (experts <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
+    else if (experts <= 256) f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    else f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+}
+
+constexpr long ROUTE_FEW = 256;             // tokens that one workgroup routes
+template <int E>
+int route(const char *fn, route_arguments a) {
+    const size_t lds = troute::route_lds_bytes(a.experts);
+    if (a.tokens <= ROUTE_FEW) {
+        by_experts(a.experts, [&](auto lanes, auto values) {
+            hipLaunchKernelGGL((troute::route_few_kernel<E, decltype(lanes)::value, decltype(values)::value>), dim3(1), dim3(ROUTE_THREADS), lds, stream(), a);
+        });
+        check(hipGetLastError(), fn);
+        return 0;
+    }
+    a.block = (int)std::max(32L, (a.tokens + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
+    const unsigned blocks = (unsigned)((a.tokens + a.block - 1) / a.block);
+    call_scratch s;
+    const uint64_t counts = s.want((uint64_t)blocks * a.experts * 4);
+    if (s.take(fn)) return 1;
+    a.counts = (int *)s.at(counts);
+    by_experts(a.experts, [&](auto lanes, auto values) {
+        hipLaunchKernelGGL((troute::route_choose_kernel<E, decltype(lanes)::value, decltype(values)::value>), dim3(blocks), dim3(ROUTE_THREADS), lds, stream(), a);
+    });
+    hipLaunchKernelGGL(troute::route_place_kernel, dim3(blocks), dim3(ROUTE_THREADS), lds, stream(), a);
+    check(hipGetLastError(), fn);
+    return 0;
+}
+template <int E>
+void route_backward(const char *fn, const route_backward_arguments &a) {
+    by_experts(a.experts, [&](auto lanes, auto values) {
+        constexpr int TOKENS = 256 / decltype(lanes)::value;
+        hipLaunchKernelGGL((troute::route_backward_kernel<E, decltype(lanes)::value, decltype(values)::value>), dim3((unsigned)((a.tokens + TOKENS - 1) / TOKENS)), dim3(256), 0, stream(), a);
+    });
+    check(hipGetLastError(), fn);
+}
+int refuse_route(const char *fn, uint64_t tokens, uint64_t experts, uint64_t k, int type) {
+    if (!known_type(type, true)) return refuse(fn, "element type %d: float32, float16 or bfloat16", type);
+    if (experts < 1 || experts > troute::MOST_EXPERTS) return refuse(fn, "%llu experts: 1 to %d", (ull)experts, troute::MOST_EXPERTS);
+    if (k < 1 || k > experts || k > troute::MOST_CHOSEN) return refuse(fn, "%llu of %llu experts: 1 to all of them, and to %d", (ull)k, (ull)experts, troute::MOST_CHOSEN);
+    if (tokens > (1 << 24)) return refuse(fn, "%llu tokens: at most 2^24", (ull)tokens);
+    return 0;
+}
+
+// ---- products of grouped rows
+using tgroups::grouped_arguments;
+
+constexpr uint64_t MOST_GROUPS = 1024;
+int refuse_grouped(const char *fn, uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K, int activation, int type, int y) {
+    if (groups < 1 || groups > MOST_GROUPS) return refuse(fn, "%llu groups: 1 to %llu", (ull)groups, (ull)MOST_GROUPS);
+    if (S > MOST || T > MOST) return refuse(fn, "%llu rows of %llu: at most 2^30 - 1", (ull)S, (ull)T);
+    if (const int rc = refuse_product(fn, std::min<uint64_t>(S, 64), N, K, activation, type, y)) return rc;
+    if ((uint64_t)tgroups::most_row_tiles((long)S, (long)groups, 64) * ((N + 63) / 64) > MOST_TILES) return refuse(fn, "%llu rows of %llu in %llu groups: more tiles than a launch holds", (ull)S, (ull)N, (ull)groups);
+    return 0;
+}
+
+product_tile grouped_tile(const grouped_arguments &a, long slices, int bytes, bool gated) {
+    const double active = (double)std::min(a.groups, a.rows), each = a.rows / active;
+    product_tile best = TILE_64;
+    double best_cost = 0;
+    const struct { product_tile tile; int rows, columns; } known[] = {{TILE_256, 256, 256}, {TILE_256x128, 256, 128}, {TILE_128, 128, 128}, {TILE_64, 64, gated ? 128 : 64}};
+    for (const auto &t : known) {
+        // (a group's last tile is half full where it has several)
+        const double down = active * std::max(1.0, each / t.rows + 0.5);
+        const long across = ((gated ? 2L : 1L) * a.p.N + t.columns - 1) / t.columns;
+        const double cost = tile_launch_cost(t.tile, std::max(1L, (long)(down * across)), std::max(1L, slices), bytes, gated);
+        if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
+    }
+    return best;
+}
+product_tile weights_tile(const grouped_arguments &a, int bytes) {
+    product_tile best = TILE_64;
+    double best_cost = 0;
+    const struct { product_tile tile; int rows, columns; } known[] = {{TILE_256, 256, 256}, {TILE_256x128, 256, 128}, {TILE_128, 128, 128}, {TILE_64, 64, 64}};
+    for (const auto &t : known) {
+        const long tiles = (a.p.M + t.rows - 1L) / t.rows * ((a.p.N + t.columns - 1L) / t.columns) * a.groups;
+        const double cost = tile_launch_cost(t.tile, std::max(1L, tiles), std::max(1L, (long)a.rows / a.groups * bytes / 128), bytes, false);
+        if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
+    }
+    return best;
+}
+
+void launch_tiles(int type, product_tile tile, product_layout layout, int epilogue, int y, const grouped_arguments &a) {
+    if (type == BF16) tgroups::launch_grouped_BF16(tile, layout, epilogue, y, a, stream());
+    else if (type == F16) tgroups::launch_grouped_F16(tile, layout, epilogue, y, a, stream());
+    else tgroups::launch_grouped_F8(tile, layout, epilogue, y, a, stream());
+}
+
+template <int E, int Y, int EPILOGUE>
+void launch_few(const char *fn, const grouped_arguments &a) {
+    const int active = std::min(a.groups, a.rows);
+    const dim3 grid((unsigned)((a.p.N + FEW_ROWS - 1L) / FEW_ROWS), (unsigned)active + 1);
+    hipLaunchKernelGGL((tgroups::grouped_few_kernel<E, Y, EPILOGUE, 1>), grid, dim3(64 * FEW_WAVES), few_lds_bytes(1, EPILOGUE == GATED), stream(), a);
+    check(hipGetLastError(), fn);
+}
+template <int EPILOGUE>
+void launch_few(const char *fn, int type, int y, const grouped_arguments &a) {
+    if (type == BF16) launch_few<BF16, BF16, EPILOGUE>(fn, a);
+    else if (type == F16) launch_few<F16, F16, EPILOGUE>(fn, a);
+    else if (y == BF16) launch_few<F8, BF16, EPILOGUE>(fn, a);
+    else launch_few<F8, F16, EPILOGUE>(fn, a);
+}
+
+// Rows of x as a product takes them: picked by it where it can, else moved, in the groups' order
+struct planned_rows {
+    const void *x;
+    const int *index;
+    long ldx, rows, tokens, columns;
+    int bytes;
+    uint64_t place;
+    long ld;
+};
+planned_rows plan_rows(const void *x, const int *index, long ldx, long rows, long tokens, long columns, int bytes, call_scratch &s) {
+    planned_rows q = {x, index, ldx, rows, tokens, columns, bytes, call_scratch::NOWHERE, (columns * bytes + 15) / 16 * 16 / bytes};
+    if (rows > 0 && columns > 0) q.place = s.want((uint64_t)q.ld * bytes * rows);
+    return q;
+}
+const void *settle_rows(const char *fn, const planned_rows &q, const call_scratch &s) {
+    if (q.place == call_scratch::NOWHERE) return q.x;
+    char *out = (char *)s.at(q.place);
+    const long to = q.ld * q.bytes;
+    for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / (to / 16)); first < q.rows; first += most) {
+        const long n = std::min(most, q.rows - first);
+        auto kernel = q.bytes == 1 ? tgroups::pick_rows_kernel<1> : tgroups::pick_rows_kernel<2>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((to / 16 * n + 255) / 256)), dim3(256), 0, stream(), (const char *)q.x, out + first * to, q.index + first, n, q.tokens, q.columns * q.bytes,
+                           q.ldx * q.bytes, to);
+    }
+    check(hipGetLastError(), fn);
+    return out;
+}
+
+// Rows that a group has in the mean, up to which its weights' bytes bound it and wavefronts that load them straight into registers are faster than tiles.
+constexpr long FEW_ROWS_OF_A_GROUP = 8;
+
+int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_arguments a, const int *rows, long tokens) {
+    if (a.rows == 0 || a.p.N == 0) return 0;
+    const int bytes = bytes_of(type);
+    const bool gated = epilogue == GATED;
+    const long K = a.p.K, all = (long)a.groups * a.p.N;
+    a.picked = {rows, rows ? tokens : a.rows};
+    a.b_step = (long)a.p.N * a.p.ldb;
+    a.b2_step = (long)a.p.N * a.p.ldb2;
+    if (K > 0 && a.p.N <= MOST_FEW_COLUMNS && a.rows <= FEW_ROWS_OF_A_GROUP * std::min(a.groups, a.rows)) {
+        gated ? launch_few<GATED>(fn, type, y, a) : launch_few<LINEAR>(fn, type, y, a);
+        return 0;
+    }
+    call_scratch s;
+    const operand x = {a.p.a, a.p.lda};
+    // (rows are picked at offsets of 31 bits)
+    const bool pick = rows && loadable(x, bytes, true) && ((tokens - 1) * a.p.lda + K) * bytes < 0x7ffffff0L && tokens > 0;
+    planned_rows moved = {};
+    placed_operand in_order = {};
+    moved.place = in_order.place = call_scratch::NOWHERE;
+    if (rows && !pick) moved = plan_rows(a.p.a, rows, a.p.lda, a.rows, tokens, K, bytes, s);
+    else if (!rows) in_order = place_operand(x, a.rows, K, bytes, true, s);
+    const uint64_t scales = rows && !pick && a.p.a_scale ? s.want((uint64_t)a.rows * 4) : call_scratch::NOWHERE;
+    const placed_operand b = place_operand({a.p.b, a.p.ldb}, all, K, bytes, true, s), b2 = place_operand({a.p.b2, a.p.ldb2}, gated ? all : 0, K, bytes, true, s);
+    if (s.take(fn)) return 1;
+    if (rows && !pick) {
+        a.p.a = settle_rows(fn, moved, s);
+        a.p.lda = moved.ld;
+        a.picked = {nullptr, a.rows};
+        if (a.p.a_scale) {
+            hipLaunchKernelGGL(tgroups::pick_scales_kernel, dim3((unsigned)((a.rows + 255L) / 256)), dim3(256), 0, stream(), a.p.a_scale, (float *)s.at(scales), rows, (long)a.rows, tokens);
+            check(hipGetLastError(), fn);
+            a.p.a_scale = (const float *)s.at(scales);
+        }
+    } else if (!rows) {
+        a.p.a = settle(fn, in_order, s);
+        a.p.lda = in_order.ld;
+    }
+    a.p.b = settle(fn, b, s);
+    a.p.b2 = settle(fn, b2, s);
+    a.p.ldb = b.ld;
+    a.p.ldb2 = b2.ld;
+    a.b_step = (long)a.p.N * b.ld;
+    a.b2_step = (long)a.p.N * b2.ld;
+    launch_tiles(type, grouped_tile(a, (K * bytes + 127) / 128, bytes, gated), FORWARD, epilogue, y, a);
+    return 0;
+}
+
+grouped_arguments grouped_of(uint64_t S, uint64_t groups, uint64_t N, uint64_t K, const int32_t *offsets) {
+    grouped_arguments a = {};
+    a.p = product_of((long)S, (long)N, (long)K);
+    a.offsets = offsets;
+    a.groups = (int)groups;
+    a.rows = (int)S;
+    return a;
+}
+
+// ---- 4-bit weights
+using tfour::four_bit_arguments;
+
+// Tokens up to which the weights' bytes bound the product, and which go in parts of 64; with more the weights are widened ahead of a product on tiles.
+constexpr long FOUR_BIT_FEW = 128;
+
+template <int E, int EPILOGUE, int TILES>
+void launch_four_few(const char *fn, const four_bit_arguments &a) {
+    const dim3 grid((unsigned)((a.p.N + FEW_ROWS - 1L) / FEW_ROWS), (unsigned)((a.p.M + 16 * TILES - 1) / (16 * TILES)));
+    hipLaunchKernelGGL((tfour::four_bit_few_kernel<E, EPILOGUE, TILES>), grid, dim3(64 * FEW_WAVES), few_lds_bytes(TILES, EPILOGUE == GATED), stream(), a);
+    check(hipGetLastError(), fn);
+}
+template <int E, int EPILOGUE>
+void launch_four_few(const char *fn, const four_bit_arguments &a) {
+    if (a.p.M <= 16) launch_four_few<E, EPILOGUE, 1>(fn, a);
+    else if (a.p.M <= 32) launch_four_few<E, EPILOGUE, 2>(fn, a);
+    else launch_four_few<E, EPILOGUE, 4>(fn, a);
+}
+template <int E>
+int four_bit(const char *fn, int epilogue, four_bit_arguments a) {
+    if (a.p.M == 0 || a.p.N == 0) return 0;
+    const bool gated = epilogue == GATED;
+    if (a.p.K > 0 && a.p.M <= FOUR_BIT_FEW && a.p.N <= MOST_FEW_COLUMNS) {
+        gated ? launch_four_few<E, GATED>(fn, a) : launch_four_few<E, LINEAR>(fn, a);
+        return 0;
+    }
+    call_scratch s;
+    const long N = a.p.N, K = a.p.K, to = (K + 7) / 8 * 8, groups = (K + tfour::GROUP - 1) / tfour::GROUP;
+    const uint64_t wide[2] = {s.want((uint64_t)to * N * 2), gated ? s.want((uint64_t)to * N * 2) : call_scratch::NOWHERE};
+    product_arguments p = a.p;
+    p.b = p.b2 = nullptr;
+    p.ldb = p.ldb2 = to;
+    planned_forward f = plan_forward(E, E, epilogue, p, s);
+    if (s.take(fn)) return 1;
+    f.b.from.p = s.at(wide[0]);
+    f.b2.from.p = s.at(wide[1]);
+    for (int i = 0; i < (gated ? 2 : 1) && K > 0; i++)
+        for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / groups); first < N; first += most) {
+            const long n = std::min(most, N - first), ldq = i ? a.p.ldb2 : a.p.ldb, lds = i ? a.lds_2 : a.lds;
+            hipLaunchKernelGGL((tfour::widen_rows_kernel<E>), dim3((unsigned)((groups * n + 255) / 256)), dim3(256), 0, stream(), (const char *)(i ? a.p.b2 : a.p.b) + first * ldq,
+                               (i ? a.scale_2 : a.scale) + first * lds, ldq, lds, n, K, (char *)s.at(wide[i]) + first * to * 2, to);
+        }
+    check(hipGetLastError(), fn);
+    launch_forward(fn, f, s);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tiramisu_hip_route(const void *logits, int32_t *experts, float *weights, int32_t *offsets, int32_t *rows, int32_t *places, uint64_t tokens, uint64_t count, uint64_t k,
+                       uint64_t ldl, int32_t normalise, int32_t type) {
+    if (const int rc = refuse_route(__FUNCTION__, tokens, count, k, type)) return rc;
+    if (!offsets || (tokens && (!logits || !experts || !weights || !rows || !places))) return refuse(__FUNCTION__, "logits and a place for every result are needed");
+    timed record(__FUNCTION__);
+    const route_arguments a = {logits, ldl ? (long)ldl : (long)count, (long)tokens, (int)count, (int)k, normalise != 0, experts, weights, offsets, rows, places, nullptr, 0};
+    return type == F32 ? route<F32>(__FUNCTION__, a) : type == F16 ? route<F16>(__FUNCTION__, a) : route<BF16>(__FUNCTION__, a);
+}
+
+int tiramisu_hip_route_backward(const float *dweights, const void *logits, const int32_t *experts, void *dlogits, uint64_t tokens, uint64_t count, uint64_t k, uint64_t ldl,
+                                int32_t normalise, int32_t type) {
+    if (const int rc = refuse_route(__FUNCTION__, tokens, count, k, type)) return rc;
+    if (tokens == 0) return 0;
+    if (!dweights || !logits || !experts || !dlogits) return refuse(__FUNCTION__, "dweights, logits, experts and dlogits are needed");
+    timed record(__FUNCTION__);
+    const route_backward_arguments a = {dweights, logits, experts, dlogits, ldl ? (long)ldl : (long)count, (long)tokens, (int)count, (int)k, normalise != 0};
+    type == F32 ? route_backward<F32>(__FUNCTION__, a) : type == F16 ? route_backward<F16>(__FUNCTION__, a) : route_backward<BF16>(__FUNCTION__, a);
+    return 0;
+}
+
+int tiramisu_hip_grouped_linear(const void *x, const void *weight, const int32_t *offsets, const int32_t *rows, const float *x_scale, const float *weight_scale, void *y,
+                                uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K, uint64_t ldx, uint64_t ldw, int32_t type, int32_t y_type) {
+    if (const int rc = refuse_grouped(__FUNCTION__, S, T, groups, N, K, NONE, type, y_type)) return rc;
+    if (S == 0 || N == 0) return 0;
+    if (!offsets || !y || (K && ((T && !x) || !weight))) return refuse(__FUNCTION__, "x, weight, offsets and y are needed");
+    if (!rows && T != S) return refuse(__FUNCTION__, "%llu rows of x for %llu places", (ull)T, (ull)S);
+    if ((type == F8) != (x_scale != nullptr) || (type == F8) != (weight_scale != nullptr)) return refuse(__FUNCTION__, "8-bit operands and their scales belong together");
+    timed record(__FUNCTION__);
+    grouped_arguments a = grouped_of(S, groups, N, K, offsets);
+    a.p.a = x;
+    a.p.lda = ldx ? (long)ldx : (long)K;
+    a.p.b = weight;
+    a.p.ldb = ldw ? (long)ldw : (long)K;
+    a.p.a_scale = x_scale;
+    a.p.b_scale = weight_scale;
+    a.p.y = y;
+    return grouped_forward(__FUNCTION__, type, y_type, LINEAR, a, rows, (long)T);
+}
+
+int tiramisu_hip_grouped_gated_linear(const void *x, const void *gate_weight, const void *up_weight, const int32_t *offsets, const int32_t *rows, const float *x_scale,
+                                      const float *gate_scale, const float *up_scale, void *h, void *gate, void *up, uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K,
+                                      uint64_t ldx, uint64_t ldg, uint64_t ldu, int32_t activation, int32_t type, int32_t h_type) {
+    if (const int rc = refuse_grouped(__FUNCTION__, S, T, groups, 2 * N, K, activation, type, h_type)) return rc;
+    if (S == 0 || N == 0) return 0;
+    if (!offsets || !h || (K && ((T && !x) || !gate_weight || !up_weight))) return refuse(__FUNCTION__, "x, both weights, offsets and h are needed");
+    if (!rows && T != S) return refuse(__FUNCTION__, "%llu rows of x for %llu places", (ull)T, (ull)S);
+    if ((gate != nullptr) != (up != nullptr)) return refuse(__FUNCTION__, "gate and up are kept together");
+    if ((type == F8) != (x_scale != nullptr) || (type == F8) != (gate_scale != nullptr) || (type == F8) != (up_scale != nullptr))
+        return refuse(__FUNCTION__, "8-bit operands and their scales belong together");
+    timed record(__FUNCTION__);
+    grouped_arguments a = grouped_of(S, groups, N, K, offsets);
+    a.p.a = x;
+    a.p.lda = ldx ? (long)ldx : (long)K;
+    a.p.b = gate_weight;
+    a.p.ldb = ldg ? (long)ldg : (long)K;
+    a.p.b2 = up_weight;
+    a.p.ldb2 = ldu ? (long)ldu : (long)K;
+    a.p.a_scale = x_scale;
+    a.p.b_scale = gate_scale;
+    a.p.b2_scale = up_scale;
+    a.p.y = h;
+    a.p.pre = gate;
+    a.p.pre2 = up;
+    a.p.activation = activation;
+    return grouped_forward(__FUNCTION__, type, h_type, GATED, a, rows, (long)T);
+}
+
+int tiramisu_hip_grouped_linear_backward(const void *dy, const void *x, const void *weight, const int32_t *offsets, const int32_t *rows, void *dx, void *dweight, uint64_t S,
+                                         uint64_t T, uint64_t groups, uint64_t N, uint64_t K, uint64_t ldy, uint64_t ldx, uint64_t ldw, int32_t type) {
+    if (const int rc = refuse_grouped(__FUNCTION__, S, T, groups, std::max(N, K), K, NONE, type, type)) return rc;
+    if ((int64_t)N * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (ull)N, (long long)MOST_ROW_BYTES);
+    if (refuse_result(__FUNCTION__, N * groups + 64 * groups, K)) return 1;
+    if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
+    if (!rows && T != S) return refuse(__FUNCTION__, "%llu rows of x for %llu places", (ull)T, (ull)S);
+    if (refuse_overlap(__FUNCTION__, "dy", S, N, ldy) || refuse_overlap(__FUNCTION__, "x", T, K, ldx) || refuse_overlap(__FUNCTION__, "weight", N * groups, K, ldw)) return 1;
+    if (!offsets || (S && N && !dy) || (T && S && K && dweight && !x) || (N && K && dx && !weight)) return refuse(__FUNCTION__, "dy, x, weight and offsets are needed");
+    if (K == 0) return 0;
+    timed record(__FUNCTION__);
+    call_scratch s;
+    const placed_operand d = place_operand({dy, ldy ? (long)ldy : (long)N}, (long)S, (long)N, 2, true, s);
+    const placed_operand w = place_operand({weight, ldw ? (long)ldw : (long)K}, dx && S ? (long)(N * groups) : 0, (long)K, 2, false, s);
+    const bool gradient = dweight && N > 0;
+    const planned_rows picked = plan_rows(x, rows, ldx ? (long)ldx : (long)K, gradient && rows ? (long)S : 0, (long)T, (long)K, 2, s);
+    const placed_operand xs = place_operand({x, ldx ? (long)ldx : (long)K}, gradient && !rows ? (long)S : 0, (long)K, 2, false, s);
+    if (s.take(__FUNCTION__)) return 1;
+    const void *at = settle(__FUNCTION__, d, s);
+    if (dx && S > 0) {
+        grouped_arguments a = grouped_of(S, groups, K, N, offsets);
+        a.p.a = at;
+        a.p.lda = d.ld;
+        a.p.b = settle(__FUNCTION__, w, s);
+        a.p.ldb = w.ld;
+        a.b_step = (long)N * w.ld;
+        a.p.y = dx;
+        launch_tiles(type, grouped_tile(a, ((long)N + 63) / 64, 2, false), INPUT_GRADIENT, LINEAR, type, a);
+    }
+    if (gradient) {
+        grouped_arguments a = grouped_of(N, groups, K, 0, offsets);
+        a.rows = (int)S;
+        a.p.a = at;
+        a.p.lda = d.ld;
+        a.p.b = rows ? settle_rows(__FUNCTION__, picked, s) : settle(__FUNCTION__, xs, s);
+        a.p.ldb = rows ? picked.ld : xs.ld;
+        a.p.y = dweight;
+        a.y_step = (long)N * (long)K;
+        launch_tiles(type, weights_tile(a, 2), WEIGHT_GRADIENT, LINEAR, type, a);
+    }
+    return 0;
+}
+
+int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, const void *gate_weight, const void *up_weight, const void *gate, const void *up, const int32_t *offsets,
+                                               const int32_t *rows, void *dx, void *dgate_weight, void *dup_weight, uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K,
+                                               uint64_t ldh, uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type) {
+    if (const int rc = refuse_grouped(__FUNCTION__, S, T, groups, std::max(N, K), K, activation, type, type)) return rc;
+    if ((int64_t)(2 * N + 16) * 2 > MOST_ROW_BYTES) return refuse(__FUNCTION__, "N of %llu: rows of at most %lld bytes", (ull)N, (long long)MOST_ROW_BYTES);
+    if (refuse_result(__FUNCTION__, (2 * N + 80) * groups, K)) return 1;
+    if (type == F8) return refuse(__FUNCTION__, "gradients are of float16 or bfloat16 operands");
+    if (!rows && T != S) return refuse(__FUNCTION__, "%llu rows of x for %llu places", (ull)T, (ull)S);
+    if (refuse_overlap(__FUNCTION__, "x", T, K, ldx) || refuse_overlap(__FUNCTION__, "gate_weight", N * groups, K, ldg) || refuse_overlap(__FUNCTION__, "up_weight", N * groups, K, ldu)) return 1;
+    if (!offsets || (S && N && (!dh || !gate || !up)) || (T && S && K && N && dgate_weight && !x) || (N && K && dx && (!gate_weight || !up_weight)))
+        return refuse(__FUNCTION__, "dh, x, both weights, gate, up and offsets are needed");
+    if ((dgate_weight != nullptr) != (dup_weight != nullptr)) return refuse(__FUNCTION__, "gradients of both weights, or of neither");
+    if (K == 0) return 0;
+    timed record(__FUNCTION__);
+    const long m = (long)S, n = (long)N, k = (long)K, half = (n + 7) / 8 * 8, ld = 2 * half;        // [dgate | dup] in rows of 2 x `half` elements
+    call_scratch s;
+    const uint64_t gradient = s.want((uint64_t)std::max(1L, m) * std::max(1L, ld) * 2);
+    const long of_weights = dx && m ? n * (long)groups : 0;
+    const placed_operand wg = place_operand({gate_weight, ldg ? (long)ldg : k}, of_weights, k, 2, false, s), wu = place_operand({up_weight, ldu ? (long)ldu : k}, of_weights, k, 2, false, s);
+    const bool weights = dgate_weight && n > 0;
+    const planned_rows picked = plan_rows(x, rows, ldx ? (long)ldx : k, weights && rows ? m : 0, (long)T, k, 2, s);
+    const placed_operand xs = place_operand({x, ldx ? (long)ldx : k}, weights && !rows ? m : 0, k, 2, false, s);
+    if (s.take(__FUNCTION__)) return 1;
+    char *const d = (char *)s.at(gradient);
+    if (m > 0 && n > 0) launch_gated_gradients(__FUNCTION__, type, {dh, gate, up, d, d + 2 * half, m, n, ldh ? (long)ldh : n, ld_gate ? (long)ld_gate : n, ld_up ? (long)ld_up : n, ld, activation});
+    if (dx && m > 0) {
+        grouped_arguments a = grouped_of(S, groups, K, N, offsets);
+        a.p.a = d;
+        a.p.a_more = d + 2 * half;
+        a.p.lda = ld;
+        a.p.b = settle(__FUNCTION__, wg, s);
+        a.p.b_more = settle(__FUNCTION__, wu, s);
+        a.p.ldb = wg.ld;
+        a.p.ldb_more = wu.ld;
+        a.b_step = n * wg.ld;
+        a.b2_step = n * wu.ld;
+        a.p.y = dx;
+        launch_tiles(type, grouped_tile(a, 2 * ((n + 63) / 64), 2, false), INPUT_GRADIENT, LINEAR, type, a);
+    }
+    if (weights) {
+        // rows of the product: those of gate, up to `half` nothing, those of up
+        grouped_arguments a = grouped_of((uint64_t)(half + n), groups, K, 0, offsets);
+        a.rows = (int)m;
+        a.p.rows_above = (int)n;
+        a.p.split_row = (int)half;
+        a.p.a = d;
+        a.p.lda = ld;
+        a.p.b = rows ? settle_rows(__FUNCTION__, picked, s) : settle(__FUNCTION__, xs, s);
+        a.p.ldb = rows ? picked.ld : xs.ld;
+        a.p.y = dgate_weight;
+        a.p.y_below = dup_weight;
+        a.y_step = n * k;
+        launch_tiles(type, weights_tile(a, 2), WEIGHT_GRADIENT, LINEAR, type, a);
+    }
+    return 0;
+}
+
+int tiramisu_hip_combine_rows(const void *x, const int32_t *places, const float *weights, const void *residual, void *y, uint64_t tokens, uint64_t k, uint64_t rows, uint64_t columns,
+                              uint64_t ldx, uint64_t ldr, int32_t type) {
+    if (tokens > MOST || rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu tokens of %llu columns: at most 2^30 - 1 of at most 2^26", (ull)tokens, (ull)columns);
+    if (k > 1024) return refuse(__FUNCTION__, "%llu rows of a token: at most 1024", (ull)k);
+    if (!known_type(type, false)) return refuse(__FUNCTION__, "element type %d: float16 or bfloat16", type);
+    if (tokens == 0 || columns == 0) return 0;
+    if (!y || (k && !places) || (k && rows && !x)) return refuse(__FUNCTION__, "x, places and y are needed");
+    timed record(__FUNCTION__);
+    const long n = (long)columns, across = (n + 7) / 8, most = std::max(1L, MOST_PIECES_A_LAUNCH / across);
+    for (long first = 0; first < (long)tokens; first += most) {
+        const long t = std::min(most, (long)tokens - first), step = ldr ? (long)ldr : n;
+        const tcombine::combine_arguments a = {x, residual ? (const char *)residual + first * step * 2 : nullptr, places + first * (long)k, weights ? weights + first * (long)k : nullptr,
+                                               (char *)y + first * n * 2, t, (long)rows, n, ldx ? (long)ldx : n, step, (int)k};
+        auto kernel = type == F16 ? tcombine::combine_kernel<F16> : tcombine::combine_kernel<BF16>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((across * t + 255) / 256)), dim3(256), 0, stream(), a);
+        check(hipGetLastError(), __FUNCTION__);
+    }
+    return 0;
+}
+
+int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int32_t *places, const int32_t *owners, const float *weights, void *dx, float *dweights, uint64_t tokens,
+                                       uint64_t k, uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t ldx, int32_t type) {
+    if (tokens > (1 << 23) || rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu tokens of %llu columns: at most 2^23 of at most 2^26", (ull)tokens, (ull)columns);
+    if (k > 1024) return refuse(__FUNCTION__, "%llu rows of a token: at most 1024", (ull)k);
+    if (!known_type(type, false)) return refuse(__FUNCTION__, "element type %d: float16 or bfloat16", type);
+    if ((tokens && columns && k && (!dy || !places)) || (rows && columns && dx && !owners) || (rows && columns && dweights && !x)) return refuse(__FUNCTION__, "dy, x, places and owners are needed");
+    if (dweights && !weights) return refuse(__FUNCTION__, "a gradient of weights that are not given");
+    timed record(__FUNCTION__);
+    const long n = (long)columns;
+    const bool team = n >= 1024;
+    const long token_blocks = k == 0 ? 0 : team ? (long)tokens : ((long)tokens + 3) / 4, blocks = token_blocks + (dx && n ? ((long)rows + 255) / 256 : 0);
+    if (blocks == 0) return 0;
+    const tcombine::combine_backward_arguments a = {dy, x, places, owners, weights, n ? dx : nullptr, dweights, (long)tokens, (long)rows, n, ldy ? (long)ldy : n, ldx ? (long)ldx : n, (int)k, token_blocks};
+    auto kernel = type == F16 ? (team ? tcombine::combine_backward_kernel<F16, 256> : tcombine::combine_backward_kernel<F16, 64>)
+                              : (team ? tcombine::combine_backward_kernel<BF16, 256> : tcombine::combine_backward_kernel<BF16, 64>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), a);
+    check(hipGetLastError(), __FUNCTION__);
+    return 0;
+}
+
+int tiramisu_hip_quantize_groups(const void *x, void *q, uint8_t *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type) {
+    if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu: at most 2^30 - 1 of at most 2^26", (ull)rows, (ull)columns);
+    if (!known_type(type, true)) return refuse(__FUNCTION__, "element type %d: float32, float16 or bfloat16", type);
+    if (rows == 0 || columns == 0) return 0;
+    if (!x || !q || !scale) return refuse(__FUNCTION__, "x, q and scale are needed");
+    timed record(__FUNCTION__);
+    const long n = (long)columns, step = ldx ? (long)ldx : n, groups = (n + tfour::GROUP - 1) / tfour::GROUP, most = std::max(1L, MOST_PIECES_A_LAUNCH / groups);
+    auto kernel = type == F32 ? tfour::quantize_groups_kernel<F32> : type == F16 ? tfour::quantize_groups_kernel<F16> : tfour::quantize_groups_kernel<BF16>;
+    for (long first = 0; first < (long)rows; first += most) {
+        const long m = std::min(most, (long)rows - first);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((groups * m + 255) / 256)), dim3(256), 0, stream(), (const void *)((const char *)x + first * step * bytes_of(type)), step, m, n,
+                           (char *)q + first * ((n + 1) / 2), scale + first * groups);
+        check(hipGetLastError(), __FUNCTION__);
+    }
+    return 0;
+}
+
+int tiramisu_hip_four_bit_linear(const void *x, const void *q, const uint8_t *scale, const void *bias, const void *residual, void *y, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx,
+                                 uint64_t ldq, uint64_t lds, uint64_t ldr, int32_t activation, int32_t type) {
+    if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, type)) return rc;
+    if (type == F8) return refuse(__FUNCTION__, "4-bit weights are multiplied with float16 or bfloat16");
+    if (M == 0 || N == 0) return 0;
+    if (!y || (K && (!x || !q || !scale))) return refuse(__FUNCTION__, "x, the weight, its scales and y are needed");
+    timed record(__FUNCTION__);
+    four_bit_arguments a = {};
+    a.p = product_of((long)M, (long)N, (long)K);
+    a.p.a = x;
+    a.p.lda = ldx ? (long)ldx : (long)K;
+    a.p.b = q;
+    a.p.ldb = ldq ? (long)ldq : (long)(K + 1) / 2;
+    a.scale = scale;
+    a.lds = lds ? (long)lds : (long)(K + tfour::GROUP - 1) / tfour::GROUP;
+    a.p.bias = bias;
+    a.p.residual = residual;
+    a.p.ldr = ldr ? (long)ldr : (long)N;
+    a.p.y = y;
+    a.p.activation = activation;
+    return type == F16 ? four_bit<F16>(__FUNCTION__, LINEAR, a) : four_bit<BF16>(__FUNCTION__, LINEAR, a);
+}
+
+int tiramisu_hip_four_bit_gated_linear(const void *x, const void *gate_q, const void *up_q, const uint8_t *gate_scale, const uint8_t *up_scale, void *h, uint64_t M, uint64_t N,
+                                       uint64_t K, uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ldgs, uint64_t ldus, int32_t activation, int32_t type) {
+    if (const int rc = refuse_product(__FUNCTION__, M, N, K, activation, type, type)) return rc;
+    if (type == F8) return refuse(__FUNCTION__, "4-bit weights are multiplied with float16 or bfloat16");
+    if (M == 0 || N == 0) return 0;
+    if (!h || (K && (!x || !gate_q || !up_q || !gate_scale || !up_scale))) return refuse(__FUNCTION__, "x, both weights, their scales and h are needed");
+    timed record(__FUNCTION__);
+    const long dense = (long)(K + 1) / 2, groups = (long)(K + tfour::GROUP - 1) / tfour::GROUP;
+    four_bit_arguments a = {};
+    a.p = product_of((long)M, (long)N, (long)K);
+    a.p.a = x;
+    a.p.lda = ldx ? (long)ldx : (long)K;
+    a.p.b = gate_q;
+    a.p.ldb = ldg ? (long)ldg : dense;
+    a.p.b2 = up_q;
+    a.p.ldb2 = ldu ? (long)ldu : dense;
+    a.scale = gate_scale;
+    a.scale_2 = up_scale;
+    a.lds = ldgs ? (long)ldgs : groups;
+    a.lds_2 = ldus ? (long)ldus : groups;
+    a.p.y = h;
+    a.p.activation = activation;
+    return type == F16 ? four_bit<F16>(__FUNCTION__, GATED, a) : four_bit<BF16>(__FUNCTION__, GATED, a);
+}
+
+}  // extern "C"

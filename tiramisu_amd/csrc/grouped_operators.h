@@ -1,0 +1,19 @@
+// What expert_operators.hip (the entry points) and grouped_tiles.hip (the kernels on tiles, compiled once for each operand type) share.
+#ifndef TIRAMISU_AMD_GROUPED_OPERATORS_H
+#define TIRAMISU_AMD_GROUPED_OPERATORS_H
+#include "operators.h"
+
+#include "kernels/grouped_products.hip.h"
+
+namespace tgroups {
+
+// Tiles of `height` rows that the rows of so many groups, and those behind them, can need at most
+inline long most_row_tiles(long rows, long groups, long height) { return rows / height + (groups + 1 < rows ? groups + 1 : rows); }
+
+// y: element type of the results
+void launch_grouped_F16(product_tile, product_layout, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+void launch_grouped_BF16(product_tile, product_layout, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+void launch_grouped_F8(product_tile, product_layout, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+
+}  // namespace tgroups
+#endif

@@ -1,0 +1,65 @@
+// The kernels of grouped_products.hip.h on tiles, for operands of one type (TIRAMISU_OPERAND: F16, BF16 or F8; compiled once for each), and the choice among
+// them by the tile, how the operands lie and the epilogue.
+#include "grouped_operators.h"
+
+#include <atomic>
+
+namespace tgroups {
+namespace {
+
+using tiramisu_runtime::check;
+
+// more LDS than a launch gets unasked: asked for once on every device
+void allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &asked) {
+    int device = 0;
+    check(hipGetDevice(&device), "tiramisu_hip_grouped_linear");
+    const unsigned long long bit = 1ull << (device & 63);
+    if (asked.load() & bit) return;
+    check(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), "tiramisu_hip_grouped_linear");
+    asked.fetch_or(bit);
+}
+
+template <class C, int Y>
+void launch(const grouped_arguments &a, hipStream_t stream) {
+    const long across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
+    const long tiles = C::A_ROWS ? most_row_tiles(a.rows, a.groups, C::BM) * across : (a.p.M + C::BM - 1L) / C::BM * across * a.groups;
+    void (*kernel)(grouped_arguments);
+    if constexpr (C::A_ROWS) kernel = grouped_rows_kernel<C, Y>;
+    else kernel = grouped_weights_kernel<C, Y>;
+    static std::atomic<unsigned long long> asked{0};
+    allow_lds((const void *)kernel, C::LDS_BYTES, asked);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), C::LDS_BYTES, stream, a);
+    check(hipGetLastError(), "tiramisu_hip_grouped_linear");
+}
+
+template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
+    typedef tile_config<E, 256, 256, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, E == F8 ? 32 : 16> tile_256;
+    typedef tile_config<E, 256, 128, 4, 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_256x128;
+    typedef tile_config<E, 128, 128, 4, 2, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128;
+    typedef tile_config<E, 64, EPILOGUE == GATED ? 128 : 64, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
+};
+template <int E, int Y, bool A_ROWS, bool B_ROWS, int EPILOGUE>
+void launch_tile(product_tile tile, const grouped_arguments &a, hipStream_t stream) {
+    typedef tiles_for<E, A_ROWS, B_ROWS, EPILOGUE> T;
+    if (tile == TILE_256) launch<typename T::tile_256, Y>(a, stream);
+    else if (tile == TILE_256x128) launch<typename T::tile_256x128, Y>(a, stream);
+    else if (tile == TILE_128) launch<typename T::tile_128, Y>(a, stream);
+    else launch<typename T::tile_64, Y>(a, stream);
+}
+
+}  // namespace
+
+#define JOIN_NAMES(name, element) name##element
+#define NAME_OF(name, element) JOIN_NAMES(name, element)
+void NAME_OF(launch_grouped_, TIRAMISU_OPERAND)(product_tile tile, product_layout layout, int epilogue, int y, const grouped_arguments &a, hipStream_t stream) {
+    constexpr int E = TIRAMISU_OPERAND;
+    if constexpr (E == F8) {                // with k along the rows, to either 16-bit type
+        if (epilogue == GATED) y == BF16 ? launch_tile<E, BF16, true, true, GATED>(tile, a, stream) : launch_tile<E, F16, true, true, GATED>(tile, a, stream);
+        else y == BF16 ? launch_tile<E, BF16, true, true, LINEAR>(tile, a, stream) : launch_tile<E, F16, true, true, LINEAR>(tile, a, stream);
+    } else if (epilogue == GATED) launch_tile<E, E, true, true, GATED>(tile, a, stream);
+    else if (layout == FORWARD) launch_tile<E, E, true, true, LINEAR>(tile, a, stream);
+    else if (layout == INPUT_GRADIENT) launch_tile<E, E, true, false, LINEAR>(tile, a, stream);
+    else launch_tile<E, E, false, false, LINEAR>(tile, a, stream);
+}
+
+}  // namespace tgroups

@@ -1,0 +1,212 @@
+// Matrix products of rows that are grouped, every group with a weight of its own: y[s] = x[s] W[g]^T for offsets[g] <= s < offsets[g + 1], and its gradients, on the
+// tiles of linear_tiles.hip.h and the wavefronts of linear_few_tokens.hip.h.  How many rows a group has stands in GPU memory and the host never asks: a launch
+// has as many workgroups as the groups could need at most, every workgroup looks up which tile of which group is its own, and those left over end at once.
+//
+// Looking up is a sum over the groups' tiles, 64 groups at a time across the lanes of a wavefront, and each wavefront does it for itself: no barrier, no
+// launch ahead that would plan, and no table.  Rows behind the last group's are rows of zeros: one more group, whose product has no terms.
+// Offsets are bounded by the number of rows before they are used, so that no offsets whatever lead outside of the operands.
+#ifndef TIRAMISU_AMD_GROUPED_PRODUCTS_HIP_H
+#define TIRAMISU_AMD_GROUPED_PRODUCTS_HIP_H
+#include "linear_few_tokens.hip.h"
+
+namespace tgroups {
+
+using namespace tops;
+
+struct grouped_arguments {
+    product_arguments p;                    // addresses of the first group's; M: rows in all (gradient of the weights: rows of a group's result)
+    const int *offsets;                     // groups + 1
+    int groups, rows;                       // rows in all
+    picked_rows picked;                     // forward: x's rows (index null: x holds the grouped rows themselves)
+    long b_step, b2_step;                   // elements from group to group of the weights (input's gradient, gated: b2 is the second pair's)
+    long y_step;                            // gradient of the weights: elements from group to group of the result
+};
+
+struct group_span { int first, rows; };
+__device__ __forceinline__ group_span span_of(const int *offsets, int g, int all) {
+    const int first = min(max(offsets[g], 0), all), end = min(max(offsets[g + 1], first), all);
+    return {first, end - first};
+}
+__device__ __forceinline__ int sum_up_to(int v, int lane) {                // over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int from = __shfl_up(v, o);
+        if (lane >= o) v += from;
+    }
+    return v;
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Consecutive workgroups go to the eight XCDs in turn: every XCD gets a run of consecutive tiles (as in tile_of).
+__device__ __forceinline__ int tile_in_runs(int id, int tiles) {
+    const int x = id % XCDS, each = tiles / XCDS, rest = tiles % XCDS;
+    return x * each + min(x, rest) + id / XCDS;
+}
+// Tile t of a product of `rows` x `columns` tiles: down BAND rows of tiles before a column on (as in tile_of)
+__device__ __forceinline__ void tile_in_bands(int t, int rows, int columns, int &row, int &column) {
+    constexpr int BAND = 4;
+    const int band = t / (BAND * columns), in = t - band * BAND * columns, height = min(rows - band * BAND, BAND);
+    column = in / height;
+    row = band * BAND + in - column * height;
+}
+
+// Whose tile workgroup `id` computes, of tiles that are HEIGHT rows high and `across` to a row: group < 0: nobody's; group == groups: the rows' behind the groups.
+struct found_tile { int group, first, rows, tile; };
+template <int HEIGHT>
+__device__ __forceinline__ found_tile find_tile(const int *offsets, int groups, int all, int across, int id, int lane) {
+    const int chunks = (groups + 63) / 64, last = uniform(min(max(offsets[groups], 0), all));
+    auto of_lane = [&](int chunk) {
+        const int g = chunk * 64 + lane;
+        return g < groups ? span_of(offsets, g, all) : group_span{0, 0};
+    };
+    auto tiles_of = [&](const group_span &s) { return (s.rows + HEIGHT - 1) / HEIGHT * across; };
+    group_span s = of_lane(0);
+    int tiles = tiles_of(s), upto = sum_up_to(tiles, lane), total = __builtin_amdgcn_readlane(upto, 63);
+    for (int c = 1; c < chunks; c++) total += __builtin_amdgcn_readlane(sum_up_to(tiles_of(of_lane(c)), lane), 63);
+    const int everything = total + (all - last + HEIGHT - 1) / HEIGHT * across;
+    if (id >= everything) return {-1, 0, 0, 0};
+    int t = tile_in_runs(id, everything);
+    if (t >= total) return {groups, last, all - last, t - total};
+    int c = 0;
+    for (int here; t >= (here = __builtin_amdgcn_readlane(upto, 63)) && c + 1 < chunks;) {
+        t -= here;
+        s = of_lane(++c);
+        tiles = tiles_of(s);
+        upto = sum_up_to(tiles, lane);
+    }
+    const int owner = __builtin_ctzll(__ballot(upto > t) | 1ull << 63);
+    return {c * 64 + owner, __builtin_amdgcn_readlane(s.first, owner), __builtin_amdgcn_readlane(s.rows, owner),
+            t - (__builtin_amdgcn_readlane(upto, owner) - __builtin_amdgcn_readlane(tiles, owner))};
+}
+
+// The product of one group's rows, from `first` on: forward and gradient of the input.  BYTES: of an operand's element, YB: of a result's.
+template <int BYTES>
+__device__ __forceinline__ product_arguments product_of_rows(const grouped_arguments &a, int group, int first, int rows, picked_rows &picked) {
+    product_arguments p = a.p;
+    picked = a.picked;
+    const long f = first;
+    if (picked.index) picked.index += f;
+    else {
+        p.a = (const char *)p.a + f * p.lda * BYTES;
+        picked.all = rows;
+        if (p.a_scale) p.a_scale += f;
+    }
+    if (p.a_more) p.a_more = (const char *)p.a_more + f * p.lda * BYTES;
+    p.y = (char *)p.y + f * p.N * 2;
+    if (p.pre) {
+        p.pre = (char *)p.pre + f * p.N * 2;
+        p.pre2 = (char *)p.pre2 + f * p.N * 2;
+    }
+    p.M = p.rows_above = p.split_row = rows;
+    if (group >= a.groups) {                               // rows of zeros
+        p.K = 0;
+        p.a_scale = nullptr;
+        return p;
+    }
+    const long g = group;
+    p.b = (const char *)p.b + g * a.b_step * BYTES;
+    if (p.b2) p.b2 = (const char *)p.b2 + g * a.b2_step * BYTES;
+    if (p.b_more) p.b_more = (const char *)p.b_more + g * a.b2_step * BYTES;
+    if (p.b_scale) p.b_scale += g * p.N;
+    if (p.b2_scale) p.b2_scale += g * p.N;
+    return p;
+}
+
+template <class C, int Y>
+__global__ __launch_bounds__(C::NT) void grouped_rows_kernel(grouped_arguments a) {
+#ifdef __HIP_DEVICE_COMPILE__
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    const int across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
+    const found_tile f = find_tile<C::BM>(a.offsets, a.groups, a.rows, across, blockIdx.x, threadIdx.x & 63);
+    const int group = uniform(f.group), rows = uniform(f.rows);
+    if (group < 0) return;
+    picked_rows picked;
+    const product_arguments p = product_of_rows<C::BYTES>(a, group, uniform(f.first), rows, picked);
+    int row, column;
+    tile_in_bands(uniform(f.tile), (rows + C::BM - 1) / C::BM, across, row, column);
+    compute_tile_at<C, Y, C::A_ROWS && C::B_ROWS>(p, row, column, 0, (lds_char *)shared_bytes, picked);
+#endif
+}
+
+// The gradient of the weights: a.p.M x a.p.N of every group, its rows the terms.  A group without rows has zeros.
+template <class C, int Y>
+__global__ __launch_bounds__(C::NT) void grouped_weights_kernel(grouped_arguments a) {
+#ifdef __HIP_DEVICE_COMPILE__
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    const int down = (a.p.M + C::BM - 1) / C::BM, across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
+    const int t = tile_in_runs(blockIdx.x, down * across * a.groups), group = t / (down * across);
+    const group_span s = span_of(a.offsets, group, a.rows);
+    product_arguments p = a.p;
+    const long first = uniform(s.first), g = group;
+    p.K = uniform(s.rows);
+    p.a = (const char *)p.a + first * p.lda * C::BYTES;
+    p.b = (const char *)p.b + first * p.ldb * C::BYTES;
+    p.y = (char *)p.y + g * a.y_step * 2;
+    if (p.y_below) p.y_below = (char *)p.y_below + g * a.y_step * 2;
+    int row, column;
+    tile_in_bands(t - group * down * across, down, across, row, column);
+    compute_tile_at<C, Y>(p, row, column, 0, (lds_char *)shared_bytes);
+#endif
+}
+
+// Few rows to a group: bound by the bytes of the weights of the groups that have rows.  grid: (columns in sixteens, groups that may have rows and one): workgroups
+// of the last row of the grid write the rows behind the groups.  A group's weights are read once for each TILES x 16 of its rows.
+template <int E, int Y, int EPILOGUE, int TILES>
+__global__ __launch_bounds__(64 * FEW_WAVES) void grouped_few_kernel(grouped_arguments a) {
+    constexpr int BYTES = E == F8 ? 1 : 2;
+    const int lane = threadIdx.x & 63, wanted = blockIdx.y;
+    const long n0 = (long)blockIdx.x * FEW_ROWS;
+    if (wanted == (int)gridDim.y - 1) {
+        const int last = min(max(a.offsets[a.groups], 0), a.rows), some = (int)min((long)FEW_ROWS, a.p.N - n0);
+        for (long i = threadIdx.x; i < (long)(a.rows - last) * FEW_ROWS; i += 64 * FEW_WAVES) {
+            const long at = (last + i / FEW_ROWS) * a.p.N + n0 + i % FEW_ROWS;
+            if (i % FEW_ROWS >= some) continue;
+            ((uint16_t *)a.p.y)[at] = 0;
+            if (a.p.pre) ((uint16_t *)a.p.pre)[at] = ((uint16_t *)a.p.pre2)[at] = 0;
+        }
+        return;
+    }
+    int group = -1, first = 0, rows = 0;
+    for (int c = 0, seen = 0; c * 64 < a.groups && group < 0; c++) {
+        const int g = c * 64 + lane;
+        const group_span s = g < a.groups ? span_of(a.offsets, g, a.rows) : group_span{0, 0};
+        const unsigned long long some = __ballot(s.rows > 0);
+        const int before = __popcll(some & ((1ull << lane) - 1));
+        const unsigned long long mine = __ballot(s.rows > 0 && seen + before == wanted);
+        if (mine) {
+            const int owner = __builtin_ctzll(mine);
+            group = c * 64 + owner;
+            first = __builtin_amdgcn_readlane(s.first, owner);
+            rows = __builtin_amdgcn_readlane(s.rows, owner);
+        }
+        seen += __popcll(some);
+    }
+    if (group < 0) return;
+    for (int from = 0; from < rows; from += 16 * TILES) {
+        if (from > 0) __syncthreads();                     // (the sums of the rows before have been read)
+        picked_rows picked;
+        const product_arguments p = product_of_rows<BYTES>(a, group, first + from, min(rows - from, 16 * TILES), picked);
+        few_tokens<E, Y, EPILOGUE, TILES, true>(p, n0, picked);
+    }
+}
+
+// Rows that an index picks, `across` pieces of 16 bytes each, to rows `to` bytes apart: where the tiles cannot pick them themselves.  One that is none of x's is zero.
+template <int BYTES>
+__global__ __launch_bounds__(256) void pick_rows_kernel(const char *in, char *out, const int *index, long rows, long all, long bytes, long from, long to) {
+    const long across = to / 16, id = (long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= across * rows) return;
+    const long m = id / across, c = 16 * (id - m * across), row = index[m];
+    u32x4 w = {0, 0, 0, 0};
+    if (row >= 0 && row < all) w = load_guarded<BYTES>(in + row * from + c, bytes - c);
+    *reinterpret_cast<u32x4 *>(out + m * to + c) = w;
+}
+// ... and their scales
+static __global__ __launch_bounds__(256) void pick_scales_kernel(const float *in, float *out, const int *index, long rows, long all) {
+    const long m = (long)blockIdx.x * 256 + threadIdx.x;
+    if (m >= rows) return;
+    const long row = index[m];
+    out[m] = row >= 0 && row < all ? in[row] : 1.f;
+}
+
+}  // namespace tgroups
+#endif

@@ -28,21 +28,30 @@ __device__ __forceinline__ f32x4 multiply_16(u32x4 rows, u32x4 columns, f32x4 c)
     }
 }
 
-template <int E, int Y, int EPILOGUE, int TILES>
-__global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_arguments p) {
+// The 16 columns from n0 on.  PICKED: rows of x may be picked by an index; one that is none of x's gives a row of zeros.
+template <int E, int Y, int EPILOGUE, int TILES, bool PICKED = false>
+__device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, picked_rows picked = {nullptr, 0}) {
     constexpr int BYTES = E == F8 ? 1 : 2, PARTS = EPILOGUE == GATED ? 2 : 1, BATCH = TILES * PARTS >= 4 ? 2 : TILES * PARTS == 2 ? 4 : 8;
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     __attribute__((address_space(3))) f32x4 *const sums = (__attribute__((address_space(3))) f32x4 *)shared_bytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int l16 = lane & 15, group = lane >> 4;
-    const long n0 = (long)blockIdx.x * FEW_ROWS, bytes = (long)p.K * BYTES;
+    const long bytes = (long)p.K * BYTES;
 
     const char *w[PARTS], *x[TILES];
     const long weight_row = min(n0 + l16, (long)p.N - 1);
     w[0] = (const char *)p.b + weight_row * p.ldb * BYTES + 16 * group;
     if constexpr (PARTS == 2) w[1] = (const char *)p.b2 + weight_row * p.ldb2 * BYTES + 16 * group;
 #pragma unroll
-    for (int i = 0; i < TILES; i++) x[i] = (const char *)p.a + (long)min(16 * i + l16, p.M - 1) * p.lda * BYTES + 16 * group;
+    for (int i = 0; i < TILES; i++) {
+        long row = min(16 * i + l16, p.M - 1);
+        if constexpr (PICKED)
+            if (picked.index) row = picked.index[row];
+        x[i] = (const char *)p.a + row * p.lda * BYTES + 16 * group;
+        // (none of x's: any readable row; its results are not used)
+        if constexpr (PICKED)
+            if (picked.index && (row < 0 || row >= picked.all)) x[i] = w[0];
+    }
 
     f32x4 acc[PARTS][TILES];
 #pragma unroll
@@ -58,10 +67,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
     column_pieces pieces;
     u32x4 residual = {0, 0, 0, 0};
     float scale = 1.f;
+    bool there = true;
     if (mine) {
         load_column_pieces(p, pieces, n, some);
         if (EPILOGUE == LINEAR && p.residual) residual = load_guarded<2>((const char *)p.residual + 2 * ((long)m * p.ldr + n), 2 * some);
-        if (E == F8) scale = p.a_scale[m];
+        if constexpr (PICKED) {
+            const int from = picked.index ? picked.index[m] : m;
+            there = !picked.index || (from >= 0 && from < picked.all);
+            if (E == F8 && there) scale = p.a_scale[from];
+        } else if (E == F8) scale = p.a_scale[m];
     }
 
     const int whole = (int)(bytes / 128), units = (int)((bytes + 127) / 128);
@@ -132,6 +146,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
                 for (int i = 0; i < 4; i++) z[q][4 * four + i] += s[i];
             }
     }
+    if constexpr (PICKED)
+        if (!there) {
+#pragma unroll
+            for (int q = 0; q < PARTS; q++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) z[q][i] = 0.f;
+        }
     column_terms columns;
     widen_column_pieces<Y>(p, pieces, columns);
     if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z[0], z[1], scale, m, n, some);
@@ -140,6 +161,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_argu
         widen<Y>(residual, r);
         finish_linear<Y>(p, columns, z[0], r, scale, m, n, some);
     }
+}
+
+template <int E, int Y, int EPILOGUE, int TILES>
+__global__ __launch_bounds__(64 * FEW_WAVES) void few_tokens_kernel(product_arguments p) {
+    few_tokens<E, Y, EPILOGUE, TILES>(p, (long)blockIdx.x * FEW_ROWS);
 }
 
 }  // namespace tops

@@ -116,6 +116,20 @@ struct operand_loader {
             offset[v] = (int)(row * ld * BYTES) + q * 16;
         }
     }
+    // The same for rows that an index picks out of an operand of `all` rows (below 2^31 bytes): row i is index[i], i < some; others read as zero.
+    __device__ __forceinline__ void start_picked(const void *p, long ld, const int *index, int some, long all, long k0, long k, int wave, int lane) {
+        static_assert(K_ALONG_ROWS, "rows are picked where k runs along them");
+        base = (const char *)p + k0 * BYTES;
+        left = ((all - 1) * ld + k) * BYTES;
+        step = 0;
+        along = 0;
+#pragma unroll
+        for (int v = 0; v < LOADS; v++) {
+            const int g = (wave * LOADS + v) * 64 + lane, row = g / G, q = (g % G) ^ swizzle(row);
+            const int from = row < some ? index[row] : -1;
+            offset[v] = from >= 0 && from < all ? (int)(from * ld * BYTES) + q * 16 : (int)0x80000000;      // (behind any descriptor's end)
+        }
+    }
     // (a dword that begins inside an operand and ends outside reads as zero: the end is moved to a whole one)
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor() const {
         const long n = (left + 3) & ~3L;
@@ -191,9 +205,11 @@ __device__ __forceinline__ S multiply(const fragment<E, AR> &rows, const fragmen
 // Adds the product of one pair of operands' rows from m0 and n0, K elements of k, to the accumulators.  b, b2: B's operand (GATED: gate and up).
 // (The operands are __restrict__ so that the compiler does not take a transposing read of LDS for one that may see a load still on its way there: it
 // waited for every load ahead of each of them, 205 us where 105 are enough.)
-template <class C>
+// picked: rows of A that an index picks, see compute_tile_at.
+struct picked_rows { const int *index; long all; };       // index: of the product's row 0 (null: rows follow each other); all: rows of the operand
+template <class C, bool PICKED = false>
 __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc)[C::TM][C::TN], const void *__restrict__ a, long lda, const void *__restrict__ b, long ldb, const void *__restrict__ b2, long ldb2, long M, long N,
-                                           long m0, long n0, long k0, long K, lds_char *lds) {
+                                           long m0, long n0, long k0, long K, lds_char *lds, picked_rows picked = {nullptr, 0}) {
     constexpr int TM = C::TM, TN = C::TN, ST = C::STAGES, E = C::E;
     constexpr int F = C::F, Q = 128 / C::STEP;                             // matrix steps of a slice
     constexpr int HALVES = C::EPILOGUE == GATED ? 2 : 1;
@@ -205,7 +221,13 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
     operand_loader<C::BYTES, C::BM, C::A_ROWS, C::LA, F> la;
     // (GATED: rows of gate in the first half of B's stage, rows of up in the second)
     operand_loader<C::BYTES, C::BN / HALVES, C::B_ROWS, LB1, F> lb[HALVES];
-    la.start(a, lda, m0, M, k0, K, wave, lane);
+    bool in_order = true;
+    if constexpr (PICKED)
+        if (picked.index) {
+            la.start_picked(a, lda, picked.index + m0, (int)min(M - m0, (long)C::BM), picked.all, k0, K, wave, lane);
+            in_order = false;
+        }
+    if (in_order) la.start(a, lda, m0, M, k0, K, wave, lane);
     lb[0].start(b, ldb, n0, N, k0, K, wave, lane);
     if constexpr (HALVES == 2) lb[1].start(b2, ldb2, n0, N, k0, K, wave, lane);
 
@@ -437,11 +459,10 @@ __device__ __forceinline__ void tile_of(int id, int rows, int columns, int &row,
 }
 
 #ifdef __HIP_DEVICE_COMPILE__               // (the host's compilation needs no body, and rejects a second one of the same configuration)
-// Tile `id` of the product, of part `split` of k.  Y: type of bias, residual and outputs.
-template <class C, int Y>
-__device__ __forceinline__ void compute_tile(const product_arguments &p, int id, int split, lds_char *lds) {
-    int row, column;
-    tile_of(id, (p.M + C::BM - 1) / C::BM, (p.N + C::COLUMNS - 1) / C::COLUMNS, row, column);
+// The tile of the product in this row and column of tiles, of part `split` of k.  Y: type of bias, residual and outputs.  PICKED: rows of A may be
+// picked by an index, and their scales with them.
+template <class C, int Y, bool PICKED = false>
+__device__ __forceinline__ void compute_tile_at(const product_arguments &p, int row, int column, int split, lds_char *lds, picked_rows picked = {nullptr, 0}) {
     const long m0 = (long)row * C::BM, n0 = (long)column * C::COLUMNS;
     constexpr int F = C::F, REGISTERS = F * F / 64;
     typename block_sums<F>::type acc[C::TM][C::TN];
@@ -470,13 +491,16 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
 #pragma unroll
             for (int i = 0; i < STRIPS; i++) {
                 const long m = m0 + wm * C::WM + i * 32 + lane % 32;
-                row_scales[i] = p.a_scale[min(m, p.M - 1L)];
+                if constexpr (PICKED) {
+                    const int from = !p.a_scale ? -1 : picked.index ? (m < p.M ? picked.index[m] : -1) : (int)min(m, p.M - 1L);
+                    row_scales[i] = from >= 0 && from < picked.all ? p.a_scale[from] : 1.f;
+                } else row_scales[i] = p.a_scale[min(m, p.M - 1L)];
             }
     };
     if constexpr (EARLY) load_terms();
     const long k0 = p.partial ? (long)split * p.slices_per_split * C::BK : 0;
     const long K = p.partial ? min((long)p.slices_per_split * C::BK, p.K - k0) : p.K;
-    accumulate<C>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds);
+    accumulate<C, PICKED>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds, picked);
     if constexpr (C::EPILOGUE == LINEAR && C::A_ROWS && !C::B_ROWS)        // (only the gradient of a gated layer's input has two)
         if (p.a_more) accumulate<C>(acc, p.a_more, p.lda, p.b_more, p.ldb_more, nullptr, 0, p.M, p.N, m0, n0, k0, K, lds);
 
@@ -579,6 +603,13 @@ __device__ __forceinline__ void compute_tile(const product_arguments &p, int id,
         }
         order_lanes();
     }
+}
+// Tile `id` of the product
+template <class C, int Y>
+__device__ __forceinline__ void compute_tile(const product_arguments &p, int id, int split, lds_char *lds) {
+    int row, column;
+    tile_of(id, (p.M + C::BM - 1) / C::BM, (p.N + C::COLUMNS - 1) / C::COLUMNS, row, column);
+    compute_tile_at<C, Y>(p, row, column, split, lds);
 }
 #endif
 

@@ -1,13 +1,10 @@
 // Entry points of the transformer operators (include/tiramisu_hip_wrappers.h): what they refuse, which kernel a call goes to, and the launches.
 // Every launch goes to the calling thread's stream.  A call plans all of its launches first, then asks for the scratch that they need, as one block, and
 // launches only when it has it.
-#include "operators.h"
+#include "operator_calls.h"
 
 #include <algorithm>
-#include <atomic>
-#include <cstdarg>
 #include <cstdint>
-#include <cstdio>
 #include <cstdlib>
 
 #include "../../include/tiramisu_hip_wrappers.h"
@@ -18,77 +15,11 @@
 #include "kernels/target_gfx950.h"
 
 namespace tops {
-namespace {
 
 using tiramisu_runtime::check;
 using tiramisu_runtime::stream;
 using tiramisu_runtime::timed;
 
-__attribute__((format(printf, 2, 3))) int refuse(const char *fn, const char *format, ...) {
-    fprintf(stderr, "Error at %s: ", fn);
-    va_list args;
-    va_start(args, format);
-    vfprintf(stderr, format, args);
-    va_end(args);
-    fprintf(stderr, "\n");
-    return 1;
-}
-
-constexpr uint64_t MOST = 0x3fffffff;                    // rows and columns are counted in 31 bits, with room for a tile
-constexpr int64_t MOST_ROWS_A_LAUNCH = (1 << 22) - 4;    // of a workgroup of up to 1024 threads each: a launch holds fewer than 2^32 threads
-constexpr int64_t MOST_PIECES_A_LAUNCH = 1LL << 31;      // of a thread each
-constexpr uint64_t MOST_TILES = (1 << 23) - 1;           // of 64 x 64: the same
-constexpr uint64_t MOST_COLUMNS = 1 << 26;               // of a norm: the same for the sums of the columns
-constexpr long MOST_FEW_COLUMNS = 1 << 26;               // of a product of few tokens
-constexpr int64_t MOST_ROW_BYTES = 1 << 22;              // of an operand with k along its rows: a tile's offsets stay below 2^31
-constexpr int64_t MOST_STEP = 1 << 23;                   // elements from k to k of one with k down its columns: the same
-
-bool known_type(int type, bool with_f32) { return type == F16 || type == BF16 || (with_f32 && type == F32); }
-int bytes_of(int type) { return type == F32 ? 4 : type == F8 ? 1 : 2; }
-
-// ---- scratch of one call: places are given out while its launches are planned, and become addresses when the block is taken.
-class call_scratch {
-public:
-    static constexpr uint64_t NOWHERE = ~0ull;
-    uint64_t want(uint64_t bytes) {
-        const uint64_t place = total;
-        total += (bytes + 255) / 256 * 256;
-        return place;
-    }
-    // 0, or 1 and a message where the memory cannot be had
-    int take(const char *fn) {
-        if (total == 0 || (base = (char *)tiramisu_runtime::operator_scratch(total))) return 0;
-        return refuse(fn, "no memory for %llu bytes of scratch", (unsigned long long)total);
-    }
-    void *at(uint64_t place) const { return place == NOWHERE ? nullptr : base + place; }
-
-private:
-    uint64_t total = 0;
-    char *base = nullptr;
-};
-
-// ---- operands as the tiles can load them: rows that begin at multiples of 4 bytes, and strides within the limits above.  Others are
-// moved to scratch, rows at multiples of 16 bytes.
-struct operand { const void *p; long ld; };
-bool loadable(const operand &o, int bytes, bool k_along_rows) {
-    return (uintptr_t)o.p % 4 == 0 && (o.ld * bytes) % 4 == 0 && (k_along_rows ? o.ld * bytes <= MOST_ROW_BYTES : o.ld <= MOST_STEP);
-}
-struct placed_operand {
-    operand from;
-    long rows, columns;
-    int bytes;
-    uint64_t place;                         // NOWHERE: stays where it is
-    long ld;
-};
-placed_operand place_operand(const operand &o, long rows, long columns, int bytes, bool k_along_rows, call_scratch &s) {
-    placed_operand q = {o, rows, columns, bytes, call_scratch::NOWHERE, o.ld};
-    if (rows <= 0 || columns <= 0 || loadable(o, bytes, k_along_rows)) return q;
-    const long to = (columns * bytes + 15) / 16 * 16;
-    q.ld = to / bytes;
-    q.place = s.want((uint64_t)to * (uint64_t)rows);
-    return q;
-}
-// its address, and the launch that moves it there
 const void *settle(const char *fn, const placed_operand &q, const call_scratch &s) {
     if (q.place == call_scratch::NOWHERE) return q.from.p;
     const long to = q.ld * q.bytes;
@@ -103,6 +34,8 @@ const void *settle(const char *fn, const placed_operand &q, const call_scratch &
     check(hipGetLastError(), fn);
     return out;
 }
+
+namespace {
 
 // ---- which tile, and how many workgroups share the k of one.  A launch is modelled in microseconds: `fixed`, for every slice of 128 bytes of k `first` for the first
 // round of tiles over the compute units (and `full` as far as it fills them), and for every further round `round` and `further` a slice.
@@ -119,7 +52,10 @@ constexpr tile_model TILES_8_BITS[] = {{TILE_256, 256, 256, 13.8, 0.8, 0.6, 9.0,
                                        {TILE_64, 64, 64, 4.8, 0.13, 0.02, 0.7, 0.19, 0, 0}};
 // (a gated layer's smallest tile is 64 x 128: 64 columns of gate and the same of up)
 constexpr tile_model GATED_64_16_BITS = {TILE_64, 64, 128, 3.9, 0.27, 0.08, 0.7, 0.31, 0, 0}, GATED_64_8_BITS = {TILE_64, 64, 128, 5.4, 0.13, 0.05, 0.7, 0.3, 0, 0};
-struct tile_plan { product_tile tile; int splits, slices; double cost; };
+double modelled(const tile_model &t, long tiles, long slices) {
+    const double busy = (double)tiles / ttarget::COMPUTE_UNITS, more = (double)((tiles - 1) / ttarget::COMPUTE_UNITS);
+    return t.fixed + (double)slices * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)slices * t.further);
+}
 tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
     const long slices = std::max(1L, (K * bytes + 127) / 128);
     tile_plan best = {TILE_64, 0, 0, 0.0};
@@ -131,8 +67,7 @@ tile_plan plan_for(long M, long N, long K, int bytes, bool gated) {
             const long each = (slices + splits - 1) / splits;
             if (splits > 1 && tiles * splits > 2 * ttarget::COMPUTE_UNITS) break;
             if ((slices + each - 1) / each != splits) continue;            // (the same slices to each as with fewer)
-            const double busy = (double)(tiles * splits) / ttarget::COMPUTE_UNITS, more = (double)((tiles * splits - 1) / ttarget::COMPUTE_UNITS);
-            double cost = t.fixed + (double)each * (t.first + std::min(1.0, busy) * t.full) + more * (t.round + (double)each * t.further);
+            double cost = modelled(t, tiles * splits, each);
             if (splits > 1) cost += 5.5 + (gated ? 2.0 : 1.0) * M * N * 4 * 2 * splits / 5e6;
             if (!best.splits || cost < best_cost) { best = {t.tile, (int)splits, (int)each, cost}; best_cost = cost; }
         }
@@ -182,14 +117,6 @@ pair_plan plan_for_pair(long M, long N, long K, long M2, long N2, long K2) {
     return best;
 }
 
-// A product as it will be launched; its operands' addresses and `a_more` may still be missing.  `pairs`: 2 where a second pair of operands will be added.
-struct planned_product {
-    int type, epilogue, y;
-    product_layout layout;
-    product_arguments p;
-    tile_plan plan;
-    uint64_t partial;
-};
 planned_product plan_product(int type, product_layout layout, int epilogue, int y, const product_arguments &p, int pairs, call_scratch &s) {
     planned_product q = {type, epilogue, y, layout, p, {TILE_64, 1, 0, 0.0}, call_scratch::NOWHERE};
     if (p.M == 0 || p.N == 0) return q;
@@ -289,6 +216,40 @@ void launch_few(const char *fn, int type, int y, const product_arguments &p) {
     else launch_few<F8, F16, EPILOGUE>(fn, p);
 }
 
+}  // namespace
+
+planned_forward plan_forward(int type, int y, int epilogue, product_arguments p, call_scratch &s) {
+    const int bytes = bytes_of(type);
+    planned_forward f = {place_operand({p.a, p.lda}, p.M, p.K, bytes, true, s), place_operand({p.b, p.ldb}, p.N, p.K, bytes, true, s),
+                         place_operand({p.b2, p.ldb2}, epilogue == GATED ? p.N : 0, p.K, bytes, true, s), {}};
+    p.lda = f.a.ld;
+    p.ldb = f.b.ld;
+    p.ldb2 = f.b2.ld;
+    f.q = plan_product(type, FORWARD, epilogue, y, p, 1, s);
+    return f;
+}
+void launch_forward(const char *fn, planned_forward &f, const call_scratch &s) {
+    f.q.p.a = settle(fn, f.a, s);
+    f.q.p.b = settle(fn, f.b, s);
+    f.q.p.b2 = settle(fn, f.b2, s);
+    launch_product(fn, f.q, s);
+}
+double tile_launch_cost(product_tile tile, long tiles, long slices, int bytes, bool gated) {
+    for (const tile_model &t : TILES_16_BITS)
+        if (bytes == 2 && t.tile == tile) return modelled(gated && tile == TILE_64 ? GATED_64_16_BITS : t, tiles, slices);
+    for (const tile_model &t : TILES_8_BITS)
+        if (bytes == 1 && t.tile == tile) return modelled(gated && tile == TILE_64 ? GATED_64_8_BITS : t, tiles, slices);
+    return 0.0;
+}
+void launch_gated_gradients(const char *fn, int type, const gated_backward_arguments &a) {
+    const unsigned blocks = (unsigned)((a.ldd / 16 * a.M + 255) / 256);
+    if (type == F16) hipLaunchKernelGGL(gated_backward_kernel<F16>, dim3(blocks), dim3(256), 0, stream(), a);
+    else hipLaunchKernelGGL(gated_backward_kernel<BF16>, dim3(blocks), dim3(256), 0, stream(), a);
+    check(hipGetLastError(), fn);
+}
+
+namespace {
+
 // A forward product: few tokens, or tiles
 int forward(const char *fn, int type, int y, int epilogue, product_arguments p) {
     if (p.M == 0 || p.N == 0) return 0;
@@ -302,17 +263,9 @@ int forward(const char *fn, int type, int y, int epilogue, product_arguments p) 
         }
     }
     call_scratch s;
-    const placed_operand a = place_operand({p.a, p.lda}, p.M, p.K, bytes, true, s), b = place_operand({p.b, p.ldb}, p.N, p.K, bytes, true, s),
-                         b2 = place_operand({p.b2, p.ldb2}, gated ? p.N : 0, p.K, bytes, true, s);
-    p.lda = a.ld;
-    p.ldb = b.ld;
-    p.ldb2 = b2.ld;
-    planned_product q = plan_product(type, FORWARD, epilogue, y, p, 1, s);
+    planned_forward f = plan_forward(type, y, epilogue, p, s);
     if (s.take(fn)) return 1;
-    q.p.a = settle(fn, a, s);
-    q.p.b = settle(fn, b, s);
-    q.p.b2 = settle(fn, b2, s);
-    launch_product(fn, q, s);
+    launch_forward(fn, f, s);
     return 0;
 }
 
@@ -411,34 +364,6 @@ column_sums launch_activation_backward(const char *fn, activation_backward_argum
     hipLaunchKernelGGL(activation_backward_kernel<E>, dim3((unsigned)plan.columns, (unsigned)plan.chunks), dim3(256), 0, stream(), a);
     check(hipGetLastError(), fn);
     return {a.partial, dbias, a.N, dbias ? plan.chunks : 0};
-}
-
-product_arguments product_of(long M, long N, long K) {
-    product_arguments p = {};
-    p.M = (int)M;
-    p.N = (int)N;
-    p.K = (int)K;
-    p.rows_above = p.split_row = p.M;
-    return p;
-}
-
-int refuse_result(const char *fn, uint64_t rows, uint64_t columns) {
-    if (((rows + 63) / 64) * ((columns + 63) / 64) <= MOST_TILES) return 0;
-    return refuse(fn, "result of %llu x %llu: more tiles than a launch holds", (unsigned long long)rows, (unsigned long long)columns);
-}
-// An operand whose rows overlap has no end behind its last row that the tiles could stop at where k runs down its columns.
-int refuse_overlap(const char *fn, const char *name, uint64_t rows, uint64_t columns, uint64_t ld) {
-    if (rows <= 1 || ld == 0 || ld >= columns) return 0;
-    return refuse(fn, "%s: rows of %llu are %llu apart", name, (unsigned long long)columns, (unsigned long long)ld);
-}
-// What both products refuse alike
-int refuse_product(const char *fn, uint64_t M, uint64_t N, uint64_t K, int activation, int type, int y) {
-    if (M > MOST || N > MOST || K > MOST) return refuse(fn, "product of %llu x %llu x %llu: dimensions of at most 2^30 - 1", (unsigned long long)M, (unsigned long long)N, (unsigned long long)K);
-    if ((int64_t)K * bytes_of(type) > MOST_ROW_BYTES) return refuse(fn, "K of %llu: rows of at most %lld bytes", (unsigned long long)K, (long long)MOST_ROW_BYTES);
-    if (activation < NONE || activation > SILU) return refuse(fn, "activation %d is not known", activation);
-    if (!known_type(type, false) && type != F8) return refuse(fn, "element type %d: float16, bfloat16 or float8_e4m3", type);
-    if (type == F8 ? !known_type(y, false) : y != type) return refuse(fn, "results of type %d from operands of type %d", y, type);
-    return refuse_result(fn, M, N);
 }
 
 }  // namespace
@@ -614,10 +539,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
     char *d = (char *)s.at(gradient);
     if (m > 0 && n > 0) {
         const gated_backward_arguments a = {dh, gate, up, d, d + 2 * half, m, n, ldh ? (long)ldh : n, ld_gate ? (long)ld_gate : n, ld_up ? (long)ld_up : n, ld, activation};
-        const unsigned blocks = (unsigned)((half / 8 * m + 255) / 256);
-        if (type == F16) hipLaunchKernelGGL(gated_backward_kernel<F16>, dim3(blocks), dim3(256), 0, stream(), a);
-        else hipLaunchKernelGGL(gated_backward_kernel<BF16>, dim3(blocks), dim3(256), 0, stream(), a);
-        check(hipGetLastError(), __FUNCTION__);
+        launch_gated_gradients(__FUNCTION__, type, a);
     }
     g.p.p.a = g.q.p.a = d;
     g.p.p.a_more = d + 2 * half;

@@ -366,9 +366,331 @@ PyObject *gated_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rows grouped by expert
+// 32-bit numbers, dense
+Tensor ints_of(PyObject *o, const char *name, const Tensor &x) {
+    const Tensor t = tensor_of(o, name);
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.is_cuda() && t.is_contiguous(), name, " holds dense ", name_of(at::kInt), " on the GPU, not ", name_of(t.scalar_type()), " of ", t.sizes(),
+                      " on ", t.device());
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " lives on another GPU");
+    return t;
+}
+const int32_t *ints(const Tensor &t) { return t.defined() ? (const int32_t *)t.data_ptr() : nullptr; }
+std::string shape_of(at::IntArrayRef leading, const std::string &last) {
+    std::string s = "[";
+    for (int64_t n : leading) s += std::to_string(n) + ", ";
+    return s + last + "]";
+}
+// [groups, outputs, columns], groups one below the other; outputs < 0: any number
+device_rows weights_of(PyObject *o, const char *name, int64_t groups, int64_t outputs, int64_t columns, const Tensor &x, ScalarType type, int64_t *found = nullptr) {
+    const Tensor t = tensor_of(o, name);
+    TORCH_CHECK_VALUE(t.dim() == 3 && t.size(0) == groups && (outputs < 0 || t.size(1) == outputs) && t.size(2) == columns, name, " holds matrices, [", groups, ", ",
+                      outputs < 0 ? std::string("outputs") : std::to_string(outputs), ", ", columns, "], not ", t.sizes());
+    if (found) *found = t.size(1);
+    return rows_of(t, name, {type}, &x);
+}
+const float *group_scales_of(PyObject *o, const char *name, int64_t groups, int64_t outputs, const Tensor &x) {
+    const Tensor t = tensor_of(o, name);
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == groups && t.size(1) == outputs && t.is_cuda() && t.is_contiguous(), name, " is dense, [", groups, ", ", outputs, "] of ",
+                      name_of(at::kFloat), " on the GPU, not ", name_of(t.scalar_type()), " of ", t.sizes());
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " lives on another GPU");
+    return (const float *)t.data_ptr();
+}
+// What places there are, of how many groups, and which rows of x they take
+struct grouping {
+    Tensor offsets, rows;
+    int64_t groups, places;
+};
+grouping grouping_of(PyObject *offsets, PyObject *rows, const Tensor &x, int64_t x_rows) {
+    grouping g = {ints_of(offsets, "offsets", x), Tensor(), 0, x_rows};
+    TORCH_CHECK_VALUE(g.offsets.dim() == 1 && g.offsets.size(0) >= 2, "offsets are those of the groups and the end, [groups + 1], not ", g.offsets.sizes());
+    g.groups = g.offsets.size(0) - 1;
+    if (given(rows)) {
+        g.rows = ints_of(rows, "rows", x);
+        TORCH_CHECK_VALUE(g.rows.dim() == 1, "rows are one number for each place, not ", g.rows.sizes());
+        g.places = g.rows.size(0);
+    }
+    return g;
+}
+device_rows places_of(PyObject *o, const char *name, int64_t places, int64_t columns, const Tensor &x) {
+    const Tensor t = tensor_of(o, name);
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.size(0) == places && (columns < 0 || t.size(1) == columns), name, " holds a row for each place, [", places, ", ",
+                      columns < 0 ? std::string("columns") : std::to_string(columns), "], not ", t.sizes());
+    return rows_of(t, name, {x.scalar_type()}, &x);
+}
+Tensor new_of(const Tensor &x, at::IntArrayRef shape, ScalarType type) { return at::empty(shape, x.options().dtype(type).requires_grad(false)); }
+
+// logits, k, normalise -> experts, weights, offsets, rows, places
+PyObject *route(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 3);
+    const Tensor logits = tensor_of(a[0], "logits");
+    const device_rows r = rows_of(logits, "logits", NORM_TYPES);
+    const int64_t k = PyLong_AsLongLong(a[1]);
+    if (k == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_VALUE(r.width >= 1 && r.width <= 1024, "logits of ", r.width, " experts: 1 to 1024");
+    TORCH_CHECK_VALUE(k >= 1 && k <= r.width && k <= 16, "k of ", k, ": 1 to 16, of ", r.width, " experts");
+    TORCH_CHECK_VALUE(r.rows <= 1 << 24, r.rows, " tokens: at most 2^24");
+    c10::SmallVector<int64_t, 6> shape(logits.sizes().begin(), logits.sizes().end());
+    shape.back() = k;
+    const Tensor experts = new_of(logits, shape, at::kInt), weights = new_of(logits, shape, at::kFloat), offsets = new_of(logits, {r.width + 1}, at::kInt), rows = new_of(logits, {r.rows * k}, at::kInt),
+                 places = new_of(logits, shape, at::kInt);
+    {
+        on_stream_of stream(logits);
+        stream.accepted(tiramisu_hip_route(r.p, (int32_t *)address(experts), (float *)address(weights), (int32_t *)address(offsets), (int32_t *)address(rows), (int32_t *)address(places), r.rows, r.width,
+                                           k, r.step, PyObject_IsTrue(a[2]) == 1, element_of(logits.scalar_type())));
+    }
+    return tuple_of({experts, weights, offsets, rows, places});
+    END_HANDLE_TH_ERRORS
+}
+
+// the choices of x's rows: [..., k] of ints or floats
+Tensor choices_of(PyObject *o, const char *name, const Tensor &x, int64_t k, ScalarType type) {
+    const Tensor t = tensor_of(o, name);
+    bool same = t.dim() == x.dim() && t.scalar_type() == type && t.is_cuda() && t.is_contiguous() && (k < 0 || t.size(t.dim() - 1) == k);
+    for (int64_t d = 0; same && d + 1 < x.dim(); d++) same = t.size(d) == x.size(d);
+    TORCH_CHECK_VALUE(same, name, " is dense, ", shape_of(x.sizes().slice(0, x.dim() - 1), k < 0 ? "k" : std::to_string(k)), " of ", name_of(type), " on the GPU, not ", name_of(t.scalar_type()), " of ",
+                      t.sizes());
+    TORCH_CHECK_VALUE(t.device() == x.device(), name, " lives on another GPU");
+    return t;
+}
+
+// dweights, logits, experts, normalise -> dlogits
+PyObject *route_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 4);
+    const Tensor logits = tensor_of(a[1], "logits");
+    const device_rows r = rows_of(logits, "logits", NORM_TYPES);
+    const Tensor experts = choices_of(a[2], "experts", logits, -1, at::kInt);
+    const int64_t k = experts.size(experts.dim() - 1);
+    const Tensor dweights = choices_of(a[0], "dweights", logits, k, at::kFloat), dlogits = new_like(logits, r.width, logits.scalar_type());
+    TORCH_CHECK_VALUE(r.width >= 1 && r.width <= 1024, "logits of ", r.width, " experts: 1 to 1024");
+    TORCH_CHECK_VALUE(k >= 1 && k <= r.width && k <= 16, "k of ", k, ": 1 to 16, of ", r.width, " experts");
+    {
+        on_stream_of stream(logits);
+        stream.accepted(tiramisu_hip_route_backward((const float *)address(dweights), r.p, ints(experts), address(dlogits), r.rows, r.width, k, r.step, PyObject_IsTrue(a[3]) == 1,
+                                                    element_of(logits.scalar_type())));
+    }
+    return tuple_of({dlogits});
+    END_HANDLE_TH_ERRORS
+}
+
+// x, weight, offsets, rows, x_scale, weight_scale, type -> y
+PyObject *grouped_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 7);
+    const Tensor x = tensor_of(a[0], "x");
+    const device_rows r = rows_of(x, "x", PRODUCT_TYPES);
+    const grouping g = grouping_of(a[2], a[3], x, r.rows);
+    int64_t outputs;
+    const device_rows weight = weights_of(a[1], "weight", g.groups, -1, r.width, x, x.scalar_type(), &outputs);
+    const ScalarType type = result_type(x, a[6]);
+    with_scales(x, {{a[4], "x_scale"}, {a[5], "weight_scale"}});
+    const float *const x_scale = given(a[4]) ? row_numbers(a[4], "x_scale", x, r.rows) : nullptr;
+    const float *const weight_scale = given(a[5]) ? group_scales_of(a[5], "weight_scale", g.groups, outputs, x) : nullptr;
+    const Tensor y = new_of(x, {g.places, outputs}, type);
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_grouped_linear(r.p, weight.p, ints(g.offsets), ints(g.rows), x_scale, weight_scale, address(y), g.places, r.rows, g.groups, outputs, r.width, r.step, weight.step,
+                                                    element_of(x.scalar_type()), element_of(type)));
+    }
+    return tuple_of({y});
+    END_HANDLE_TH_ERRORS
+}
+
+// dy, x, weight, offsets, rows -> dx, dweight
+PyObject *grouped_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 5);
+    const Tensor x = tensor_of(a[1], "x");
+    const device_rows r = rows_of(x, "x", HALVES);
+    const ScalarType type = x.scalar_type();
+    const grouping g = grouping_of(a[3], a[4], x, r.rows);
+    int64_t outputs;
+    const device_rows weight = weights_of(a[2], "weight", g.groups, -1, r.width, x, type, &outputs), dy = places_of(a[0], "dy", g.places, outputs, x);
+    const Tensor dx = new_of(x, {g.places, r.width}, type), dweight = new_of(x, {g.groups, outputs, r.width}, type);
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_grouped_linear_backward(dy.p, r.p, weight.p, ints(g.offsets), ints(g.rows), address(dx), address(dweight), g.places, r.rows, g.groups, outputs, r.width, dy.step,
+                                                             r.step, weight.step, element_of(type)));
+    }
+    return tuple_of({dx, dweight});
+    END_HANDLE_TH_ERRORS
+}
+
+// x, gate_weight, up_weight, offsets, rows, activation, x_scale, gate_scale, up_scale, type, keep_pre -> h, gate, up
+PyObject *grouped_gated_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 11);
+    const Tensor x = tensor_of(a[0], "x");
+    const device_rows r = rows_of(x, "x", PRODUCT_TYPES);
+    const grouping g = grouping_of(a[3], a[4], x, r.rows);
+    int64_t outputs;
+    const device_rows gate_weight = weights_of(a[1], "gate_weight", g.groups, -1, r.width, x, x.scalar_type(), &outputs),
+                      up_weight = weights_of(a[2], "up_weight", g.groups, outputs, r.width, x, x.scalar_type());
+    const ScalarType type = result_type(x, a[9]);
+    with_scales(x, {{a[6], "x_scale"}, {a[7], "gate_scale"}, {a[8], "up_scale"}});
+    const float *const x_scale = given(a[6]) ? row_numbers(a[6], "x_scale", x, r.rows) : nullptr;
+    const float *const gate_scale = given(a[7]) ? group_scales_of(a[7], "gate_scale", g.groups, outputs, x) : nullptr;
+    const float *const up_scale = given(a[8]) ? group_scales_of(a[8], "up_scale", g.groups, outputs, x) : nullptr;
+    const bool keep = PyObject_IsTrue(a[10]) == 1;
+    const Tensor h = new_of(x, {g.places, outputs}, type), gate = keep ? new_of(x, {g.places, outputs}, type) : Tensor(), up = keep ? new_of(x, {g.places, outputs}, type) : Tensor();
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_grouped_gated_linear(r.p, gate_weight.p, up_weight.p, ints(g.offsets), ints(g.rows), x_scale, gate_scale, up_scale, address(h), address(gate), address(up), g.places,
+                                                          r.rows, g.groups, outputs, r.width, r.step, gate_weight.step, up_weight.step, activation_of(a[5]), element_of(x.scalar_type()),
+                                                          element_of(type)));
+    }
+    return tuple_of({h, gate, up});
+    END_HANDLE_TH_ERRORS
+}
+
+// dh, x, gate_weight, up_weight, gate, up, offsets, rows, activation -> dx, dgate_weight, dup_weight
+PyObject *grouped_gated_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 9);
+    const Tensor x = tensor_of(a[1], "x");
+    const device_rows r = rows_of(x, "x", HALVES);
+    const ScalarType type = x.scalar_type();
+    const grouping g = grouping_of(a[6], a[7], x, r.rows);
+    int64_t outputs;
+    const device_rows gate_weight = weights_of(a[2], "gate_weight", g.groups, -1, r.width, x, type, &outputs), up_weight = weights_of(a[3], "up_weight", g.groups, outputs, r.width, x, type);
+    const device_rows dh = places_of(a[0], "dh", g.places, outputs, x), gate = places_of(a[4], "gate", g.places, outputs, x), up = places_of(a[5], "up", g.places, outputs, x);
+    const Tensor dx = new_of(x, {g.places, r.width}, type), dgate = new_of(x, {g.groups, outputs, r.width}, type), dup = new_of(x, {g.groups, outputs, r.width}, type);
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_grouped_gated_linear_backward(dh.p, r.p, gate_weight.p, up_weight.p, gate.p, up.p, ints(g.offsets), ints(g.rows), address(dx), address(dgate), address(dup), g.places,
+                                                                   r.rows, g.groups, outputs, r.width, dh.step, r.step, gate_weight.step, up_weight.step, gate.step, up.step, activation_of(a[8]),
+                                                                   element_of(type)));
+    }
+    return tuple_of({dx, dgate, dup});
+    END_HANDLE_TH_ERRORS
+}
+
+// x, places, weights, residual -> y
+PyObject *combine(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 4);
+    const Tensor x = tensor_of(a[0], "x");
+    const device_rows r = rows_of(x, "x", HALVES);
+    TORCH_CHECK_VALUE(x.dim() == 2, "x holds a row for each place, [places, columns], not ", x.sizes());
+    const Tensor places = ints_of(a[1], "places", x);
+    TORCH_CHECK_VALUE(places.dim() >= 1, "places are a token's, [..., k], not ", places.sizes());
+    const int64_t k = places.size(places.dim() - 1);
+    TORCH_CHECK_VALUE(k <= 1024, "places of ", k, " rows a token: at most 1024");
+    const Tensor weights = given(a[2]) ? choices_of(a[2], "weights", places, k, at::kFloat) : Tensor();
+    c10::SmallVector<int64_t, 6> shape(places.sizes().begin(), places.sizes().end());
+    shape.back() = r.width;
+    const Tensor y = new_of(x, shape, x.scalar_type());
+    device_rows residual = {0, 0, 0, nullptr};
+    if (given(a[3])) residual = rows_like(a[3], "residual", y, r.width, x.scalar_type());
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_combine_rows(r.p, ints(places), (const float *)address(weights), residual.p, address(y), tokens_of(places), k, r.rows, r.width, r.step, residual.step,
+                                                  element_of(x.scalar_type())));
+    }
+    return tuple_of({y});
+    END_HANDLE_TH_ERRORS
+}
+
+// dy, x, places, weights, rows -> dx, dweights
+PyObject *combine_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 5);
+    const Tensor x = tensor_of(a[1], "x");
+    const device_rows r = rows_of(x, "x", HALVES);
+    TORCH_CHECK_VALUE(x.dim() == 2, "x holds a row for each place, [places, columns], not ", x.sizes());
+    const Tensor places = ints_of(a[2], "places", x), owners = ints_of(a[4], "rows", x);
+    TORCH_CHECK_VALUE(places.dim() >= 1, "places are a token's, [..., k], not ", places.sizes());
+    TORCH_CHECK_VALUE(owners.dim() == 1 && owners.size(0) == r.rows, "rows are the token of each place, [", r.rows, "], not ", owners.sizes());
+    const int64_t k = places.size(places.dim() - 1);
+    TORCH_CHECK_VALUE(k <= 1024, "places of ", k, " rows a token: at most 1024");
+    const Tensor weights = given(a[3]) ? choices_of(a[3], "weights", places, k, at::kFloat) : Tensor();
+    const device_rows dy = rows_like(a[0], "dy", places, r.width, x.scalar_type());
+    const Tensor dx = new_of(x, {r.rows, r.width}, x.scalar_type()), dweights = weights.defined() ? at::empty_like(weights) : Tensor();
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_combine_rows_backward(dy.p, r.p, ints(places), ints(owners), (const float *)address(weights), address(dx), (float *)address(dweights), tokens_of(places), k, r.rows,
+                                                           r.width, dy.step, r.step, element_of(x.scalar_type())));
+    }
+    return tuple_of({dx, dweights});
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- 4-bit weights
+constexpr int64_t FOUR_BIT_GROUP = 32;
+// x -> q, scale
+PyObject *quantize_groups(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 1);
+    const Tensor x = tensor_of(a[0], "x");
+    const device_rows r = rows_of(x, "x", NORM_TYPES);
+    const Tensor q = new_like(x, (r.width + 1) / 2, at::kByte), scale = new_like(x, (r.width + FOUR_BIT_GROUP - 1) / FOUR_BIT_GROUP, at::kByte);
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_quantize_groups(r.p, address(q), (uint8_t *)address(scale), r.rows, r.width, r.step, element_of(x.scalar_type())));
+    }
+    return tuple_of({q, scale});
+    END_HANDLE_TH_ERRORS
+}
+// [outputs, columns] of bytes
+device_rows bytes_of(PyObject *o, const char *name, int64_t outputs, int64_t columns, const Tensor &x, int64_t *found = nullptr) {
+    const Tensor t = tensor_of(o, name);
+    TORCH_CHECK_VALUE(t.dim() == 2 && (outputs < 0 || t.size(0) == outputs) && t.size(1) == columns, name, " holds bytes, [", outputs < 0 ? std::string("outputs") : std::to_string(outputs), ", ", columns,
+                      "], not ", t.sizes());
+    if (found) *found = t.size(0);
+    return rows_of(t, name, {at::kByte}, &x);
+}
+
+// x, weight, weight_scale, bias, residual, activation -> y
+PyObject *four_bit_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 6);
+    const Tensor x = tensor_of(a[0], "x");
+    const device_rows r = rows_of(x, "x", HALVES);
+    const ScalarType type = x.scalar_type();
+    int64_t outputs;
+    const device_rows weight = bytes_of(a[1], "weight", -1, (r.width + 1) / 2, x, &outputs);
+    const device_rows scale = bytes_of(a[2], "weight_scale", outputs, (r.width + FOUR_BIT_GROUP - 1) / FOUR_BIT_GROUP, x);
+    const void *const bias = given(a[3]) ? vector_of(a[3], "bias", outputs, type, x) : nullptr;
+    device_rows residual = {0, 0, 0, nullptr};
+    if (given(a[4])) residual = rows_like(a[4], "residual", x, outputs, type);
+    const Tensor y = new_like(x, outputs, type);
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_four_bit_linear(r.p, weight.p, (const uint8_t *)scale.p, bias, residual.p, address(y), r.rows, outputs, r.width, r.step, weight.step, scale.step, residual.step,
+                                                     activation_of(a[5]), element_of(type)));
+    }
+    return tuple_of({y});
+    END_HANDLE_TH_ERRORS
+}
+
+// x, gate_weight, up_weight, gate_scale, up_scale, activation -> h
+PyObject *four_bit_gated_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    count(n, 6);
+    const Tensor x = tensor_of(a[0], "x");
+    const device_rows r = rows_of(x, "x", HALVES);
+    const ScalarType type = x.scalar_type();
+    const int64_t groups = (r.width + FOUR_BIT_GROUP - 1) / FOUR_BIT_GROUP;
+    int64_t outputs;
+    const device_rows gate = bytes_of(a[1], "gate_weight", -1, (r.width + 1) / 2, x, &outputs), up = bytes_of(a[2], "up_weight", outputs, (r.width + 1) / 2, x);
+    const device_rows gate_scale = bytes_of(a[3], "gate_scale", outputs, groups, x), up_scale = bytes_of(a[4], "up_scale", outputs, groups, x);
+    const Tensor h = new_like(x, outputs, type);
+    {
+        on_stream_of stream(x);
+        stream.accepted(tiramisu_hip_four_bit_gated_linear(r.p, gate.p, up.p, (const uint8_t *)gate_scale.p, (const uint8_t *)up_scale.p, address(h), r.rows, outputs, r.width, r.step, gate.step, up.step,
+                                                           gate_scale.step, up_scale.step, activation_of(a[5]), element_of(type)));
+    }
+    return tuple_of({h});
+    END_HANDLE_TH_ERRORS
+}
+
 #define OPERATOR(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {OPERATOR(rms_norm), OPERATOR(rms_norm_backward), OPERATOR(quantize_rows), OPERATOR(linear), OPERATOR(linear_backward),
-                         OPERATOR(gated_linear), OPERATOR(gated_linear_backward), {nullptr, nullptr, 0, nullptr}};
+                         OPERATOR(gated_linear), OPERATOR(gated_linear_backward), OPERATOR(route), OPERATOR(route_backward), OPERATOR(grouped_linear),
+                         OPERATOR(grouped_linear_backward), OPERATOR(grouped_gated_linear), OPERATOR(grouped_gated_linear_backward), OPERATOR(combine), OPERATOR(combine_backward),
+                         OPERATOR(quantize_groups), OPERATOR(four_bit_linear), OPERATOR(four_bit_gated_linear), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_operators", "The inner part of tiramisu_amd.operators.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

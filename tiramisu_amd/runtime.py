@@ -154,6 +154,17 @@ def wrappers():
         lib.tiramisu_hip_linear_backward.argtypes = [p] * 7 + [u] * 7 + [i] * 2
         lib.tiramisu_hip_gated_linear.argtypes = [p] * 9 + [u] * 6 + [i] * 3
         lib.tiramisu_hip_gated_linear_backward.argtypes = [p] * 9 + [u] * 9 + [i] * 2
+        lib.tiramisu_hip_route.argtypes = [p] * 6 + [u] * 4 + [i] * 2
+        lib.tiramisu_hip_route_backward.argtypes = [p] * 4 + [u] * 4 + [i] * 2
+        lib.tiramisu_hip_grouped_linear.argtypes = [p] * 7 + [u] * 7 + [i] * 2
+        lib.tiramisu_hip_grouped_linear_backward.argtypes = [p] * 7 + [u] * 8 + [i]
+        lib.tiramisu_hip_grouped_gated_linear.argtypes = [p] * 11 + [u] * 8 + [i] * 3
+        lib.tiramisu_hip_grouped_gated_linear_backward.argtypes = [p] * 11 + [u] * 11 + [i] * 2
+        lib.tiramisu_hip_combine_rows.argtypes = [p] * 5 + [u] * 6 + [i]
+        lib.tiramisu_hip_combine_rows_backward.argtypes = [p] * 7 + [u] * 6 + [i]
+        lib.tiramisu_hip_quantize_groups.argtypes = [p] * 3 + [u] * 3 + [i]
+        lib.tiramisu_hip_four_bit_linear.argtypes = [p] * 6 + [u] * 7 + [i] * 2
+        lib.tiramisu_hip_four_bit_gated_linear.argtypes = [p] * 6 + [u] * 8 + [i] * 2
         _wrappers = lib
     return _wrappers
 
