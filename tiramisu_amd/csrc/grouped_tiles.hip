@@ -4,6 +4,8 @@
 
 #include <atomic>
 
+#include "kernels/target_gfx950.h"
+
 namespace tgroups {
 namespace {
 
@@ -19,32 +21,47 @@ void allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &a
     asked.fetch_or(bit);
 }
 
-template <class C, int Y>
-void launch(const grouped_arguments &a, hipStream_t stream) {
+template <class C>
+long tiles_of(const grouped_arguments &a) {
     const long across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
-    const long tiles = C::A_ROWS ? most_row_tiles(a.rows, a.groups, C::BM) * across : (a.p.M + C::BM - 1L) / C::BM * across * a.groups;
+    return C::A_ROWS ? most_row_tiles(a.rows, a.groups, C::BM) * across : (a.p.M + C::BM - 1L) / C::BM * across * a.groups;
+}
+template <class C, class D, int Y>
+void launch(const grouped_arguments &a, hipStream_t stream) {
+    const long tiles = tiles_of<C>(a);
+    constexpr int LDS = C::LDS_BYTES > D::LDS_BYTES ? C::LDS_BYTES : D::LDS_BYTES;
     void (*kernel)(grouped_arguments);
-    if constexpr (C::A_ROWS) kernel = grouped_rows_kernel<C, Y>;
+    if constexpr (C::A_ROWS) kernel = grouped_rows_kernel<C, D, Y>;
     else kernel = grouped_weights_kernel<C, Y>;
     static std::atomic<unsigned long long> asked{0};
-    allow_lds((const void *)kernel, C::LDS_BYTES, asked);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), C::LDS_BYTES, stream, a);
+    allow_lds((const void *)kernel, LDS, asked);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), LDS, stream, a);
     check(hipGetLastError(), "tiramisu_hip_grouped_linear");
 }
 
 template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
-    typedef tile_config<E, 256, 256, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, E == F8 ? 32 : 16> tile_256;
+    static constexpr int F = E == F8 ? 32 : 16, SMALL_N = EPILOGUE == GATED ? 128 : 64;
+    typedef tile_config<E, 256, 256, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, F> tile_256;
+    typedef tile_config<E, 128, 256, 2, 4, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_256_end;
     typedef tile_config<E, 256, 128, 4, 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_256x128;
     typedef tile_config<E, 128, 128, 4, 2, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128;
-    typedef tile_config<E, 64, EPILOGUE == GATED ? 128 : 64, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
+    // (two stages: two workgroups to a compute unit, which cover each other's beginnings and ends where there is more than a round of tiles; us with four / with two, bf16:
+    // 8192 rows in 64 groups, gated 1024 x 2048 154 / 145, gradient of 16384 rows in 32 groups of 2048 x 2048 200 / 186, one round of 1500 x 700 19.7 / 23.7; 8 bits, 32768 rows 259 / 315)
+    typedef tile_config<E, 128, 128, 4, 2, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_pair;
+    typedef tile_config<E, 64, 128, 2, 4, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_end;
+    typedef tile_config<E, 64, 128, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_pair_end;
+    typedef tile_config<E, 64, SMALL_N, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
 };
 template <int E, int Y, bool A_ROWS, bool B_ROWS, int EPILOGUE>
 void launch_tile(product_tile tile, const grouped_arguments &a, hipStream_t stream) {
     typedef tiles_for<E, A_ROWS, B_ROWS, EPILOGUE> T;
-    if (tile == TILE_256) launch<typename T::tile_256, Y>(a, stream);
-    else if (tile == TILE_256x128) launch<typename T::tile_256x128, Y>(a, stream);
-    else if (tile == TILE_128) launch<typename T::tile_128, Y>(a, stream);
-    else launch<typename T::tile_64, Y>(a, stream);
+    if (tile == TILE_256) launch<typename T::tile_256, typename T::tile_256_end, Y>(a, stream);
+    else if (tile == TILE_256x128) launch<typename T::tile_256x128, typename T::tile_128, Y>(a, stream);
+    else if (tile == TILE_128) {
+        if constexpr (E != F8)
+            if (tiles_of<typename T::tile_128>(a) > ttarget::COMPUTE_UNITS) return launch<typename T::tile_128_pair, typename T::tile_128_pair_end, Y>(a, stream);
+        launch<typename T::tile_128, typename T::tile_128_end, Y>(a, stream);
+    } else launch<typename T::tile_64, typename T::tile_64, Y>(a, stream);
 }
 
 }  // namespace

@@ -24,10 +24,11 @@ __global__ __launch_bounds__(256) void combine_kernel(combine_arguments a) {
     const long across = (a.columns + 7) / 8, id = (long)blockIdx.x * 256 + threadIdx.x;
     if (id >= across * a.tokens) return;
     const long t = id / across, n = 8 * (id - t * across);
+    const long left = 2 * (a.columns - n);
     const int some = (int)min(8L, a.columns - n);
     typedef stored<E> T;
     u32x4 residual = {0, 0, 0, 0};
-    if (a.residual) residual = load_guarded<2>((const char *)((const T *)a.residual + t * a.ldr + n), 2 * some);
+    if (a.residual) residual = load_to_end<2>((const char *)((const T *)a.residual + t * a.ldr + n), left, 2 * a.columns);
     float sum[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) sum[i] = 0.f;
@@ -41,7 +42,7 @@ __global__ __launch_bounds__(256) void combine_kernel(combine_arguments a) {
             there[j] = place >= 0 && place < a.rows;
             w[j] = there[j] ? a.weights ? a.weights[t * a.k + j0 + j] : 1.f : 0.f;
             held[j] = u32x4{0, 0, 0, 0};
-            if (there[j]) held[j] = load_guarded<2>((const char *)((const T *)a.x + place * a.ldx + n), 2 * some);
+            if (there[j]) held[j] = load_to_end<2>((const char *)((const T *)a.x + place * a.ldx + n), left, 2 * a.columns);
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) {
@@ -80,12 +81,13 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(combine_backward_
     __shared__ float sums[TEAMS][WAVES][AHEAD];
     const int team = threadIdx.x / THREADS, x = threadIdx.x % THREADS, lane = threadIdx.x & 63;
     if ((long)blockIdx.x >= a.token_blocks) {
-        const long first = ((long)blockIdx.x - a.token_blocks) * 256;
-        for (long s = first + threadIdx.x / 64; s < min(first + 256, a.rows); s += 4) {
-            const int owner = a.owners[s];
-            if (owner >= 0 && owner < a.tokens) continue;
-            const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (long n = 8 * lane; n < a.columns; n += 512) store_some<E>((T *)a.dx + s * a.columns + n, (int)min(8L, a.columns - n), none);
+        // 64 rows to a wavefront, whose lanes read their owners at once
+        const long first = (((long)blockIdx.x - a.token_blocks) * 4 + threadIdx.x / 64) * 64, s = first + lane;
+        const int owner = s < a.rows ? a.owners[s] : 0;
+        for (unsigned long long none = __ballot(s < a.rows && (owner < 0 || owner >= a.tokens)); none; none &= none - 1) {
+            const long row = first + __builtin_ctzll(none);
+            const float zeros[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (long n = 8 * lane; n < a.columns; n += 512) store_some<E>((T *)a.dx + row * a.columns + n, (int)min(8L, a.columns - n), zeros);
         }
         return;
     }
@@ -103,15 +105,17 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(combine_backward_
             dot[j] = 0.f;
         }
         for (long n = 8 * x; mine && n < a.columns; n += 8 * THREADS) {
+            const long left = 2 * (a.columns - n);
             const int some = (int)min(8L, a.columns - n);
             float d[8];
+            const u32x4 held_d = load_to_end<2>((const char *)((const T *)a.dy + t * a.ldy + n), left, 2 * a.columns);
             u32x4 held[AHEAD];
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
                 held[j] = u32x4{0, 0, 0, 0};
-                if (a.dweights && place[j] >= 0) held[j] = load_guarded<2>((const char *)((const T *)a.x + place[j] * a.ldx + n), 2 * some);
+                if (a.dweights && place[j] >= 0) held[j] = load_to_end<2>((const char *)((const T *)a.x + place[j] * a.ldx + n), left, 2 * a.columns);
             }
-            load_some<E>((const T *)a.dy + t * a.ldy + n, some, d);
+            widen<E>(held_d, d);
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
                 if (place[j] < 0) continue;

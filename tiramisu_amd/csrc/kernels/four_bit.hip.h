@@ -147,13 +147,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void four_bit_few_kernel(four_bit_a
             uint32_t exponent[PARTS];
 #pragma unroll
             for (int q = 0; q < PARTS; q++) {
-                fw[q] = load_guarded<1>(w[q] + at, left);
+                fw[q] = load_to_end<1>(w[q] + at, left, bytes);
                 exponent[q] = left > 0 ? scale[q][at / 16] : 127;
             }
 #pragma unroll
             for (int step = 0; step < 4; step++)
 #pragma unroll
-                for (int i = 0; i < TILES; i++) fx[step][i] = load_guarded<2>(x[i] + 4 * at + 16 * step, left_x - 16 * step);
+                for (int i = 0; i < TILES; i++) fx[step][i] = load_to_end<2>(x[i] + 4 * at + 16 * step, left_x - 16 * step, 2L * p.K);
             multiply(fw, fx, exponent);
         }
     }

@@ -8,6 +8,7 @@
 #ifndef TIRAMISU_AMD_GROUPED_PRODUCTS_HIP_H
 #define TIRAMISU_AMD_GROUPED_PRODUCTS_HIP_H
 #include "linear_few_tokens.hip.h"
+#include "wave_reduce.hip.h"
 
 namespace tgroups {
 
@@ -27,14 +28,7 @@ __device__ __forceinline__ group_span span_of(const int *offsets, int g, int all
     const int first = min(max(offsets[g], 0), all), end = min(max(offsets[g + 1], first), all);
     return {first, end - first};
 }
-__device__ __forceinline__ int sum_up_to(int v, int lane) {                // over the lanes up to this one
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const int from = __shfl_up(v, o);
-        if (lane >= o) v += from;
-    }
-    return v;
-}
+__device__ __forceinline__ int sum_up_to(int v) { return twave::wave_group_sum<64>(v); }       // (its steps leave in every lane the sum over the lanes up to it)
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Consecutive workgroups go to the eight XCDs in turn: every XCD gets a run of consecutive tiles (as in tile_of).
@@ -61,8 +55,8 @@ __device__ __forceinline__ found_tile find_tile(const int *offsets, int groups, 
     };
     auto tiles_of = [&](const group_span &s) { return (s.rows + HEIGHT - 1) / HEIGHT * across; };
     group_span s = of_lane(0);
-    int tiles = tiles_of(s), upto = sum_up_to(tiles, lane), total = __builtin_amdgcn_readlane(upto, 63);
-    for (int c = 1; c < chunks; c++) total += __builtin_amdgcn_readlane(sum_up_to(tiles_of(of_lane(c)), lane), 63);
+    int tiles = tiles_of(s), upto = sum_up_to(tiles), total = __builtin_amdgcn_readlane(upto, 63);
+    for (int c = 1; c < chunks; c++) total += __builtin_amdgcn_readlane(sum_up_to(tiles_of(of_lane(c))), 63);
     const int everything = total + (all - last + HEIGHT - 1) / HEIGHT * across;
     if (id >= everything) return {-1, 0, 0, 0};
     int t = tile_in_runs(id, everything);
@@ -72,7 +66,7 @@ __device__ __forceinline__ found_tile find_tile(const int *offsets, int groups, 
         t -= here;
         s = of_lane(++c);
         tiles = tiles_of(s);
-        upto = sum_up_to(tiles, lane);
+        upto = sum_up_to(tiles);
     }
     const int owner = __builtin_ctzll(__ballot(upto > t) | 1ull << 63);
     return {c * 64 + owner, __builtin_amdgcn_readlane(s.first, owner), __builtin_amdgcn_readlane(s.rows, owner),
@@ -112,9 +106,12 @@ __device__ __forceinline__ product_arguments product_of_rows(const grouped_argum
     return p;
 }
 
-template <class C, int Y>
+// D: the tile for the last rows of a group that are no more than it is high, of C's width and half of its height or less (of 256 x 256 tiles a third would be half empty
+// where groups have some hundred rows).
+template <class C, class D, int Y>
 __global__ __launch_bounds__(C::NT) void grouped_rows_kernel(grouped_arguments a) {
 #ifdef __HIP_DEVICE_COMPILE__
+    static_assert(C::NT == D::NT && C::COLUMNS == D::COLUMNS && C::BM % D::BM == 0, "one workgroup's size and width");
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     const int across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
     const found_tile f = find_tile<C::BM>(a.offsets, a.groups, a.rows, across, blockIdx.x, threadIdx.x & 63);
@@ -124,7 +121,9 @@ __global__ __launch_bounds__(C::NT) void grouped_rows_kernel(grouped_arguments a
     const product_arguments p = product_of_rows<C::BYTES>(a, group, uniform(f.first), rows, picked);
     int row, column;
     tile_in_bands(uniform(f.tile), (rows + C::BM - 1) / C::BM, across, row, column);
-    compute_tile_at<C, Y, C::A_ROWS && C::B_ROWS>(p, row, column, 0, (lds_char *)shared_bytes, picked);
+    constexpr bool PICKED = C::A_ROWS && C::B_ROWS;
+    if (C::BM != D::BM && rows - row * C::BM <= D::BM) compute_tile_at<D, Y, PICKED>(p, row * (C::BM / D::BM), column, 0, (lds_char *)shared_bytes, picked);
+    else compute_tile_at<C, Y, PICKED>(p, row, column, 0, (lds_char *)shared_bytes, picked);
 #endif
 }
 

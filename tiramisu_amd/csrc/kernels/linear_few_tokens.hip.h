@@ -115,9 +115,9 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
             const long at = (long)u * 128 + 64 * half, left = bytes - at - 16 * group;
             u32x4 fw[PARTS], fx[TILES];
 #pragma unroll
-            for (int q = 0; q < PARTS; q++) fw[q] = load_guarded<BYTES>(w[q] + at, left);
+            for (int q = 0; q < PARTS; q++) fw[q] = load_to_end<BYTES>(w[q] + at, left, bytes);
 #pragma unroll
-            for (int i = 0; i < TILES; i++) fx[i] = load_guarded<BYTES>(x[i] + at, left);
+            for (int i = 0; i < TILES; i++) fx[i] = load_to_end<BYTES>(x[i] + at, left, bytes);
 #pragma unroll
             for (int q = 0; q < PARTS; q++)
 #pragma unroll

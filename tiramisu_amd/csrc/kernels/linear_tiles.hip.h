@@ -231,12 +231,12 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
     lb[0].start(b, ldb, n0, N, k0, K, wave, lane);
     if constexpr (HALVES == 2) lb[1].start(b2, ldb2, n0, N, k0, K, wave, lane);
 
-    auto issue_one = [&](int stage, int v) {
+    auto issue_one = [&](int stage, int v, bool ahead = false) {
         lds_char *const s = lds + stage * C::STAGE;
         if (v < C::LA) la.load(s, wave, v);
         else if (HALVES == 1 || v < C::LA + LB1) lb[0].load(s + C::A_STAGE, wave, v - C::LA);
         else lb[HALVES - 1].load(s + C::A_STAGE + C::B_STAGE / 2, wave, v - C::LA - LB1);
-        if (v == C::LA + C::LB - 1) {
+        if (v == (PICKED && ahead ? C::LA : C::LA + C::LB) - 1) {
             la.advance();
             lb[0].advance();
             if constexpr (HALVES == 2) lb[1].advance();
@@ -288,8 +288,9 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
 #pragma unroll
     for (int p = 0; p < ST; p++)
         if (p < KT) {
+            // (picked rows wait for their numbers: B's loads are ahead of theirs)
 #pragma unroll
-            for (int v = 0; v < PER; v++) issue_one(p, v);
+            for (int v = 0; v < PER; v++) issue_one(p, PICKED ? (v + C::LA) % PER : v, true);
         }
     if (KT >= ST) wait_loads<(ST - 1) * PER>(); else wait_loads<0>();
     __builtin_amdgcn_s_barrier();

@@ -124,6 +124,22 @@ __device__ __forceinline__ u32x4 load_guarded(const char *p, long left) {
     return w;
 }
 
+// The same for 16 bytes of a row of `whole` bytes of which `left` remain: in rows of 16 bytes and more by one load, of the row's last 16 bytes where fewer
+// remain (element by element, each behind a comparison of its own, a piece waits for memory eight times: gradients of a token's rows, 2000 x 3 x 1430 f16, 18.9 us, so 9.0).
+template <int BYTES>
+__device__ __forceinline__ u32x4 load_to_end(const char *p, long left, long whole) {
+    if (whole < 16) return load_guarded<BYTES>(p, left);
+    const u32x4 w = *reinterpret_cast<const u32x4_any *>(p + min(left - 16, 0L));
+    if (left >= 16) return w;
+    const int gone = 8 * (16 - (int)max(left, 0L));                       // bits that are not this piece's
+    unsigned long long low = ((unsigned long long)w[1] << 32) | w[0], high = ((unsigned long long)w[3] << 32) | w[2];
+    if (gone >= 64) { low = high; high = 0; }
+    const int by = gone & 63;
+    if (gone >= 128) low = 0;
+    else if (by) { low = (low >> by) | (high << (64 - by)); high >>= by; }
+    return u32x4{(uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32)};
+}
+
 // ... as fp32
 template <int E, int N>
 __device__ __forceinline__ void widen(u32x4 w, float (&v)[N]) {

@@ -1,7 +1,7 @@
 // A router's choice: the k best of a token's logits, their weights, and the tokens' places grouped by expert; and the gradient of the logits.
 //
 // LANES lanes of a wavefront hold the logits of a token, VALUES neighbouring ones each, as whole numbers that order them (zeros of either sign alike, NaN above
-// everything).  A choice is the largest number over the lanes and then the first lane, and its first value, that holds it: ties go to the lowest index.  Chosen
+// everything).  A choice is the largest number over the lanes and then the lowest index that holds it.  Chosen
 // ones become the least number; minus infinity is never chosen.  Sixteen lanes are one row of the cross-lane network, so that up to 128 experts take four tokens a wavefront
 // without a word through LDS.
 //
@@ -10,6 +10,8 @@
 // sums over its wavefronts.  One workgroup does both for few tokens.
 #ifndef TIRAMISU_AMD_ROUTE_HIP_H
 #define TIRAMISU_AMD_ROUTE_HIP_H
+#include <type_traits>
+
 #include "operator_elements.hip.h"
 
 namespace troute {
@@ -41,28 +43,40 @@ __device__ __forceinline__ float number_of(uint32_t o) {
 }
 constexpr uint32_t LEAST = 0x007fffffu;     // of minus infinity
 
-// The LANES consecutive lanes that a lane belongs to (16: a row of the cross-lane network)
+// f over the LANES consecutive lanes that a lane belongs to, in each of them: within a row of 16 by turns of the cross-lane network, across rows through LDS
 template <int LANES, class F, class T>
 __device__ __forceinline__ T over_lanes(T v, F f) {
-#pragma unroll
-    for (int o = 1; o < LANES; o *= 2) v = f(v, __shfl_xor(v, o));
+    static_assert(sizeof(T) == 4 && (LANES == 16 || LANES == 64), "rows of 16 lanes");
+    auto turned = [](T x, auto by) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + decltype(by)::value, 0xf, 0xf, false));        // row_ror
+    };
+    v = f(v, turned(v, std::integral_constant<int, 8>()));
+    v = f(v, turned(v, std::integral_constant<int, 4>()));
+    v = f(v, turned(v, std::integral_constant<int, 2>()));
+    v = f(v, turned(v, std::integral_constant<int, 1>()));
+    if constexpr (LANES == 64) {
+        v = f(v, __shfl_xor(v, 16));
+        v = f(v, __shfl_xor(v, 32));
+    }
     return v;
 }
 
+// A lane's VALUES logits of a token; minus infinity behind the last
 template <int E, int LANES, int VALUES>
 __device__ __forceinline__ void load_logits(const void *logits, long ld, long token, int experts, int at, float (&v)[VALUES]) {
-    const stored<E> *const row = (const stored<E> *)logits + token * ld;
-#pragma unroll
-    for (int i = 0; i < VALUES; i++) {
-        const int e = at * VALUES + i;
-        v[i] = e < experts ? load_one<E>(row + e) : -__builtin_inff();
+    const stored<E> *const row = (const stored<E> *)logits + token * ld + at * VALUES;
+    const int some = experts - at * VALUES;
+    if constexpr (VALUES * sizeof(stored<E>) % 16 == 0) {
+        if (some >= VALUES) return load_elements<E>(row, v);
     }
+#pragma unroll
+    for (int i = 0; i < VALUES; i++) v[i] = i < some ? load_one<E>(row + i) : -__builtin_inff();
 }
 
 // Chooses for `token`; lane j of the LANES writes the j-th.  All lanes of the wavefront call it; `there`: whether the token exists.
 template <int E, int LANES, int VALUES>
 __device__ __forceinline__ void choose(const route_arguments &a, long token, bool there, int lane) {
-    const int at = lane % LANES, base = lane - at;
+    const int at = lane % LANES;
     float v[VALUES];
     uint32_t order[VALUES];
     load_logits<E, LANES, VALUES>(a.logits, a.ld, there ? token : 0, a.experts, at, v);
@@ -76,13 +90,11 @@ __device__ __forceinline__ void choose(const route_arguments &a, long token, boo
     float z = 0.f, most = 0.f;
     for (int j = 0; j < a.k; j++) {
         const uint32_t top = over_lanes<LANES>(best, [](uint32_t x, uint32_t y) { return max(x, y); });
-        const unsigned long long holders = (__ballot(best == top) >> base) & (LANES == 64 ? ~0ull : (1ull << LANES) - 1);
-        const int owner = __builtin_ctzll(holders | 1ull << 63);
         int index = 0;
 #pragma unroll
         for (int i = VALUES - 1; i >= 0; i--) index = order[i] == top ? i : index;
-        index += at * VALUES;
-        const int expert = top > LEAST ? __shfl(index, base + owner) : -1;
+        index = over_lanes<LANES>(best == top ? at * VALUES + index : MOST_EXPERTS, [](int x, int y) { return min(x, y); });
+        const int expert = top > LEAST ? index : -1;
         const float value = number_of(top);
         if (j == 0) most = expert >= 0 ? value : 0.f;
         if (at == j) { mine = expert; z = value; }
@@ -244,7 +256,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_place_kernel(route_argume
     for (int w = t; w < sharers * a.experts; w += ROUTE_THREADS) {
         const int e = w % a.experts;
         int all = 0, early = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int b = w / a.experts; b < blocks; b += sharers) {
             const int c = a.counts[(long)b * a.experts + e];
             all += c;
