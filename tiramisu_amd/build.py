@@ -77,7 +77,8 @@ def build_compiler(force=True):
 WRAPPER_UNITS = [("hip_wrappers", "hip_wrappers.hip", []), ("operators", "operators.hip", []), ("expert_operators", "expert_operators.hip", [])] + \
     [("linear_tiles_" + e.lower(), "linear_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16")] + \
     [("linear_tiles_f8", "linear_tiles.hip", ["-DTIRAMISU_OPERAND=F8", "-DTIRAMISU_OPERAND_HAS_NO_GRADIENTS"])] + \
-    [("grouped_tiles_" + e.lower(), "grouped_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16", "F8")]
+    [("grouped_tiles_" + e.lower(), "grouped_tiles.hip", ["-DTIRAMISU_OPERAND=" + e]) for e in ("BF16", "F16")] + \
+    [("grouped_tiles_f8", "grouped_tiles.hip", ["-DTIRAMISU_OPERAND=F8", "-DTIRAMISU_OPERAND_HAS_NO_GRADIENTS"])]
 
 
 def build_wrappers(force=True):

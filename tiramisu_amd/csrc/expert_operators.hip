@@ -90,36 +90,41 @@ int refuse_grouped(const char *fn, uint64_t S, uint64_t T, uint64_t groups, uint
     return 0;
 }
 
-product_tile grouped_tile(const grouped_arguments &a, long slices, int bytes, bool gated) {
-    const double active = (double)std::min(a.groups, a.rows), each = a.rows / active;
+// ---- which tile, by the launch's model (operators.hip) for the tiles that the groups have if the rows are spread as routers spread them, a tenth more than evenly, a
+// group's last tile half empty where it has several; tiles of 256 x 128 and 64 x 64 take 1.1 and 1.25 times what it says where groups bring weights of their own, and the weights' bytes come
+// at 4.6 TB/s.  Of 20 launches (16 and 8 bits, 8 to 64 groups, 500 to 32768 rows) the choice is the fastest or within 6 % of it in 18.
+constexpr struct { product_tile tile; int rows, columns; double factor; } GROUPED_TILES[] = {{TILE_256, 256, 256, 1.0}, {TILE_256x128, 256, 128, 1.1}, {TILE_128, 128, 128, 1.0}, {TILE_64, 64, 64, 1.25}};
+double rows_tiles(const grouped_arguments &a, int rows, int columns, bool gated) {
+    const double active = (double)std::min(a.groups, a.rows);
+    return 1.1 * active * std::max(1.0, a.rows / active / rows + 0.5) * (double)(((gated ? 2L : 1L) * a.p.N + columns - 1) / columns);
+}
+product_tile grouped_tile(const grouped_arguments &a, int bytes, bool gated) {
+    const double weights = (gated ? 2.0 : 1.0) * std::min(a.groups, a.rows) * a.p.N * a.p.K * bytes / 4.6e6 + 3.0;
     product_tile best = TILE_64;
     double best_cost = 0;
-    const struct { product_tile tile; int rows, columns; } known[] = {{TILE_256, 256, 256}, {TILE_256x128, 256, 128}, {TILE_128, 128, 128}, {TILE_64, 64, gated ? 128 : 64}};
-    for (const auto &t : known) {
-        // (a group's last tile is half full where it has several)
-        const double down = active * std::max(1.0, each / t.rows + 0.5);
-        const long across = ((gated ? 2L : 1L) * a.p.N + t.columns - 1) / t.columns;
-        const double cost = tile_launch_cost(t.tile, std::max(1L, (long)(down * across)), std::max(1L, slices), bytes, gated);
+    for (const auto &t : GROUPED_TILES) {
+        const long tiles = std::max(1L, (long)rows_tiles(a, t.rows, gated && t.tile == TILE_64 ? 128 : t.columns, gated)), slices = std::max(1L, ((long)a.p.K * bytes + 127) / 128);
+        const double launch = t.factor * tile_launch_cost(t.tile, tiles, slices, bytes, gated), cost = std::max(launch, weights) + 0.2 * std::min(launch, weights);
         if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
     }
     return best;
 }
-product_tile weights_tile(const grouped_arguments &a, int bytes) {
+// Both gradients: as one launch of as many tiles as they have together, whose slices are theirs in the mean.
+product_tile gradients_tile(const grouped_arguments &a, const grouped_arguments &b, int pairs) {
     product_tile best = TILE_64;
     double best_cost = 0;
-    const struct { product_tile tile; int rows, columns; } known[] = {{TILE_256, 256, 256}, {TILE_256x128, 256, 128}, {TILE_128, 128, 128}, {TILE_64, 64, 64}};
-    for (const auto &t : known) {
-        const long tiles = (a.p.M + t.rows - 1L) / t.rows * ((a.p.N + t.columns - 1L) / t.columns) * a.groups;
-        const double cost = tile_launch_cost(t.tile, std::max(1L, tiles), std::max(1L, (long)a.rows / a.groups * bytes / 128), bytes, false);
+    for (const auto &t : GROUPED_TILES) {
+        const double down = a.p.y ? rows_tiles(a, t.rows, t.columns, false) : 0, across = b.p.y ? (double)((b.p.M + t.rows - 1L) / t.rows) * ((b.p.N + t.columns - 1L) / t.columns) * b.groups : 0;
+        const double slices = down * pairs * ((a.p.K + 63) / 64) + across * ((double)b.rows / b.groups / 64 + 0.5), tiles = std::max(1.0, down + across);
+        const double cost = t.factor * tile_launch_cost(t.tile, (long)tiles, std::max(1L, (long)(slices / tiles + 0.5)), 2, false);
         if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
     }
     return best;
 }
-
-void launch_tiles(int type, product_tile tile, product_layout layout, int epilogue, int y, const grouped_arguments &a) {
-    if (type == BF16) tgroups::launch_grouped_BF16(tile, layout, epilogue, y, a, stream());
-    else if (type == F16) tgroups::launch_grouped_F16(tile, layout, epilogue, y, a, stream());
-    else tgroups::launch_grouped_F8(tile, layout, epilogue, y, a, stream());
+void launch_gradients(int type, const grouped_arguments &a, const grouped_arguments &b, int pairs) {
+    if (!a.p.y && !b.p.y) return;
+    const product_tile tile = gradients_tile(a, b, pairs);
+    (type == BF16 ? tgroups::launch_grouped_gradients_BF16 : tgroups::launch_grouped_gradients_F16)(tile, a, b, stream());
 }
 
 template <int E, int Y, int EPILOGUE>
@@ -137,7 +142,9 @@ void launch_few(const char *fn, int type, int y, const grouped_arguments &a) {
     else launch_few<F8, F16, EPILOGUE>(fn, a);
 }
 
-// Rows of x as a product takes them: picked by it where it can, else moved, in the groups' order
+// (rows are picked at offsets of 31 bits)
+bool can_pick(const operand &x, long rows, long columns, int bytes) { return rows > 0 && loadable(x, bytes, true) && ((rows - 1) * x.ld + columns) * bytes < 0x7ffffff0L; }
+// Rows of x in the groups' order, where a product cannot pick them itself
 struct planned_rows {
     const void *x;
     const int *index;
@@ -165,6 +172,29 @@ const void *settle_rows(const char *fn, const planned_rows &q, const call_scratc
     return out;
 }
 
+// Rows of x as the gradient of the weights takes them, down whose columns k runs: picked there, or moved
+struct planned_weight_rows {
+    planned_rows moved;
+    placed_operand in_order;
+    const int *index;
+    long tokens;
+};
+planned_weight_rows plan_weight_rows(const void *x, const int *rows, long ldx, long S, long T, long K, call_scratch &s) {
+    planned_weight_rows q = {};
+    q.moved.place = q.in_order.place = call_scratch::NOWHERE;
+    q.tokens = T;
+    q.index = rows && can_pick({x, ldx}, T, K, 2) && ldx <= MOST_STEP ? rows : nullptr;
+    if (rows && !q.index) q.moved = plan_rows(x, rows, ldx, S, T, K, 2, s);
+    else q.in_order = place_operand({x, ldx}, rows ? 0 : S, K, 2, false, s);
+    return q;
+}
+void settle_weight_rows(const char *fn, const planned_weight_rows &q, grouped_arguments &b, const call_scratch &s) {
+    const bool moved = q.moved.place != call_scratch::NOWHERE;
+    b.p.b = moved ? settle_rows(fn, q.moved, s) : settle(fn, q.in_order, s);
+    b.p.ldb = moved ? q.moved.ld : q.in_order.ld;
+    if (q.index) b.picked = {q.index, q.tokens};
+}
+
 // Rows that a group has in the mean, up to which its weights' bytes bound it and wavefronts that load them straight into registers are faster than tiles.
 constexpr long FEW_ROWS_OF_A_GROUP = 8;
 
@@ -182,8 +212,7 @@ int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_argum
     }
     call_scratch s;
     const operand x = {a.p.a, a.p.lda};
-    // (rows are picked at offsets of 31 bits)
-    const bool pick = rows && loadable(x, bytes, true) && ((tokens - 1) * a.p.lda + K) * bytes < 0x7ffffff0L && tokens > 0;
+    const bool pick = rows && can_pick(x, tokens, K, bytes);
     planned_rows moved = {};
     placed_operand in_order = {};
     moved.place = in_order.place = call_scratch::NOWHERE;
@@ -211,7 +240,8 @@ int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_argum
     a.p.ldb2 = b2.ld;
     a.b_step = (long)a.p.N * b.ld;
     a.b2_step = (long)a.p.N * b2.ld;
-    launch_tiles(type, grouped_tile(a, (K * bytes + 127) / 128, bytes, gated), FORWARD, epilogue, y, a);
+    const product_tile tile = grouped_tile(a, bytes, gated);
+    (type == BF16 ? tgroups::launch_grouped_BF16 : type == F16 ? tgroups::launch_grouped_F16 : tgroups::launch_grouped_F8)(tile, epilogue, y, a, stream());
     return 0;
 }
 
@@ -357,31 +387,27 @@ int tiramisu_hip_grouped_linear_backward(const void *dy, const void *x, const vo
     const placed_operand d = place_operand({dy, ldy ? (long)ldy : (long)N}, (long)S, (long)N, 2, true, s);
     const placed_operand w = place_operand({weight, ldw ? (long)ldw : (long)K}, dx && S ? (long)(N * groups) : 0, (long)K, 2, false, s);
     const bool gradient = dweight && N > 0;
-    const planned_rows picked = plan_rows(x, rows, ldx ? (long)ldx : (long)K, gradient && rows ? (long)S : 0, (long)T, (long)K, 2, s);
-    const placed_operand xs = place_operand({x, ldx ? (long)ldx : (long)K}, gradient && !rows ? (long)S : 0, (long)K, 2, false, s);
+    const planned_weight_rows xs = plan_weight_rows(x, rows, ldx ? (long)ldx : (long)K, gradient ? (long)S : 0, (long)T, (long)K, s);
     if (s.take(__FUNCTION__)) return 1;
     const void *at = settle(__FUNCTION__, d, s);
+    grouped_arguments a = grouped_of(S, groups, K, N, offsets), b = grouped_of(N, groups, K, 0, offsets);
     if (dx && S > 0) {
-        grouped_arguments a = grouped_of(S, groups, K, N, offsets);
         a.p.a = at;
         a.p.lda = d.ld;
         a.p.b = settle(__FUNCTION__, w, s);
         a.p.ldb = w.ld;
         a.b_step = (long)N * w.ld;
         a.p.y = dx;
-        launch_tiles(type, grouped_tile(a, ((long)N + 63) / 64, 2, false), INPUT_GRADIENT, LINEAR, type, a);
     }
     if (gradient) {
-        grouped_arguments a = grouped_of(N, groups, K, 0, offsets);
-        a.rows = (int)S;
-        a.p.a = at;
-        a.p.lda = d.ld;
-        a.p.b = rows ? settle_rows(__FUNCTION__, picked, s) : settle(__FUNCTION__, xs, s);
-        a.p.ldb = rows ? picked.ld : xs.ld;
-        a.p.y = dweight;
-        a.y_step = (long)N * (long)K;
-        launch_tiles(type, weights_tile(a, 2), WEIGHT_GRADIENT, LINEAR, type, a);
+        b.rows = (int)S;
+        b.p.a = at;
+        b.p.lda = d.ld;
+        settle_weight_rows(__FUNCTION__, xs, b, s);
+        b.p.y = dweight;
+        b.y_step = (long)N * (long)K;
     }
+    launch_gradients(type, a, b, 1);
     return 0;
 }
 
@@ -405,13 +431,12 @@ int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, co
     const long of_weights = dx && m ? n * (long)groups : 0;
     const placed_operand wg = place_operand({gate_weight, ldg ? (long)ldg : k}, of_weights, k, 2, false, s), wu = place_operand({up_weight, ldu ? (long)ldu : k}, of_weights, k, 2, false, s);
     const bool weights = dgate_weight && n > 0;
-    const planned_rows picked = plan_rows(x, rows, ldx ? (long)ldx : k, weights && rows ? m : 0, (long)T, k, 2, s);
-    const placed_operand xs = place_operand({x, ldx ? (long)ldx : k}, weights && !rows ? m : 0, k, 2, false, s);
+    const planned_weight_rows xs = plan_weight_rows(x, rows, ldx ? (long)ldx : k, weights ? m : 0, (long)T, k, s);
     if (s.take(__FUNCTION__)) return 1;
     char *const d = (char *)s.at(gradient);
     if (m > 0 && n > 0) launch_gated_gradients(__FUNCTION__, type, {dh, gate, up, d, d + 2 * half, m, n, ldh ? (long)ldh : n, ld_gate ? (long)ld_gate : n, ld_up ? (long)ld_up : n, ld, activation});
+    grouped_arguments a = grouped_of(S, groups, K, N, offsets), b = grouped_of((uint64_t)(half + n), groups, K, 0, offsets);
     if (dx && m > 0) {
-        grouped_arguments a = grouped_of(S, groups, K, N, offsets);
         a.p.a = d;
         a.p.a_more = d + 2 * half;
         a.p.lda = ld;
@@ -422,23 +447,20 @@ int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, co
         a.b_step = n * wg.ld;
         a.b2_step = n * wu.ld;
         a.p.y = dx;
-        launch_tiles(type, grouped_tile(a, 2 * ((n + 63) / 64), 2, false), INPUT_GRADIENT, LINEAR, type, a);
     }
     if (weights) {
         // rows of the product: those of gate, up to `half` nothing, those of up
-        grouped_arguments a = grouped_of((uint64_t)(half + n), groups, K, 0, offsets);
-        a.rows = (int)m;
-        a.p.rows_above = (int)n;
-        a.p.split_row = (int)half;
-        a.p.a = d;
-        a.p.lda = ld;
-        a.p.b = rows ? settle_rows(__FUNCTION__, picked, s) : settle(__FUNCTION__, xs, s);
-        a.p.ldb = rows ? picked.ld : xs.ld;
-        a.p.y = dgate_weight;
-        a.p.y_below = dup_weight;
-        a.y_step = n * k;
-        launch_tiles(type, weights_tile(a, 2), WEIGHT_GRADIENT, LINEAR, type, a);
+        b.rows = (int)m;
+        b.p.rows_above = (int)n;
+        b.p.split_row = (int)half;
+        b.p.a = d;
+        b.p.lda = ld;
+        settle_weight_rows(__FUNCTION__, xs, b, s);
+        b.p.y = dgate_weight;
+        b.p.y_below = dup_weight;
+        b.y_step = n * k;
     }
+    launch_gradients(type, a, b, 2);
     return 0;
 }
 

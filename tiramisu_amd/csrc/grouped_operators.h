@@ -10,10 +10,13 @@ namespace tgroups {
 // Tiles of `height` rows that the rows of so many groups, and those behind them, can need at most
 inline long most_row_tiles(long rows, long groups, long height) { return rows / height + (groups + 1 < rows ? groups + 1 : rows); }
 
-// y: element type of the results
-void launch_grouped_F16(product_tile, product_layout, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
-void launch_grouped_BF16(product_tile, product_layout, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
-void launch_grouped_F8(product_tile, product_layout, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+// Forward; y: element type of the results
+void launch_grouped_F16(product_tile, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+void launch_grouped_BF16(product_tile, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+void launch_grouped_F8(product_tile, int epilogue, int y, const grouped_arguments &, hipStream_t stream);
+// The gradients of the rows and of the weights on the same tiles, in one launch; one without a place for its result (p.y) is not computed
+void launch_grouped_gradients_F16(product_tile, const grouped_arguments &rows, const grouped_arguments &weights, hipStream_t stream);
+void launch_grouped_gradients_BF16(product_tile, const grouped_arguments &rows, const grouped_arguments &weights, hipStream_t stream);
 
 }  // namespace tgroups
 #endif

@@ -24,18 +24,28 @@ void allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &a
 template <class C>
 long tiles_of(const grouped_arguments &a) {
     const long across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
-    return C::A_ROWS ? most_row_tiles(a.rows, a.groups, C::BM) * across : (a.p.M + C::BM - 1L) / C::BM * across * a.groups;
+    if (C::A_ROWS) return most_row_tiles(a.rows, a.groups, C::BM) * across;
+    return ((a.p.M + C::BM - 1L) / C::BM * across + XCDS - 1) / XCDS * XCDS * a.groups;
 }
 template <class C, class D, int Y>
 void launch(const grouped_arguments &a, hipStream_t stream) {
-    const long tiles = tiles_of<C>(a);
+    auto kernel = grouped_rows_kernel<C, D, Y>;
     constexpr int LDS = C::LDS_BYTES > D::LDS_BYTES ? C::LDS_BYTES : D::LDS_BYTES;
-    void (*kernel)(grouped_arguments);
-    if constexpr (C::A_ROWS) kernel = grouped_rows_kernel<C, D, Y>;
-    else kernel = grouped_weights_kernel<C, Y>;
     static std::atomic<unsigned long long> asked{0};
     allow_lds((const void *)kernel, LDS, asked);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), LDS, stream, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles_of<C>(a)), dim3(C::NT), LDS, stream, a);
+    check(hipGetLastError(), "tiramisu_hip_grouped_linear");
+}
+template <class C, class D, class G, int Y>
+void launch_gradients(const grouped_arguments &a, const grouped_arguments &b, hipStream_t stream) {
+    auto kernel = grouped_gradients_kernel<C, D, G, Y>;
+    constexpr int ROWS = C::LDS_BYTES > D::LDS_BYTES ? C::LDS_BYTES : D::LDS_BYTES, RING = G::STAGES * G::STAGE + 4 * PICKS, WEIGHTS = RING > G::LDS_BYTES ? RING : G::LDS_BYTES,
+                  LDS = ROWS > WEIGHTS ? ROWS : WEIGHTS;
+    static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+    static std::atomic<unsigned long long> asked{0};
+    allow_lds((const void *)kernel, LDS, asked);
+    const long start = a.p.y ? (tiles_of<C>(a) + XCDS - 1) / XCDS * XCDS : 0, tiles = start + (b.p.y ? tiles_of<G>(b) : 0);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(C::NT), b.picked.index ? LDS : ROWS > G::LDS_BYTES ? ROWS : G::LDS_BYTES, stream, a, b, (int)start);
     check(hipGetLastError(), "tiramisu_hip_grouped_linear");
 }
 
@@ -52,9 +62,9 @@ template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
     typedef tile_config<E, 64, 128, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_pair_end;
     typedef tile_config<E, 64, SMALL_N, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
 };
-template <int E, int Y, bool A_ROWS, bool B_ROWS, int EPILOGUE>
+template <int E, int Y, int EPILOGUE>
 void launch_tile(product_tile tile, const grouped_arguments &a, hipStream_t stream) {
-    typedef tiles_for<E, A_ROWS, B_ROWS, EPILOGUE> T;
+    typedef tiles_for<E, true, true, EPILOGUE> T;
     if (tile == TILE_256) launch<typename T::tile_256, typename T::tile_256_end, Y>(a, stream);
     else if (tile == TILE_256x128) launch<typename T::tile_256x128, typename T::tile_128, Y>(a, stream);
     else if (tile == TILE_128) {
@@ -68,15 +78,28 @@ void launch_tile(product_tile tile, const grouped_arguments &a, hipStream_t stre
 
 #define JOIN_NAMES(name, element) name##element
 #define NAME_OF(name, element) JOIN_NAMES(name, element)
-void NAME_OF(launch_grouped_, TIRAMISU_OPERAND)(product_tile tile, product_layout layout, int epilogue, int y, const grouped_arguments &a, hipStream_t stream) {
+void NAME_OF(launch_grouped_, TIRAMISU_OPERAND)(product_tile tile, int epilogue, int y, const grouped_arguments &a, hipStream_t stream) {
     constexpr int E = TIRAMISU_OPERAND;
-    if constexpr (E == F8) {                // with k along the rows, to either 16-bit type
-        if (epilogue == GATED) y == BF16 ? launch_tile<E, BF16, true, true, GATED>(tile, a, stream) : launch_tile<E, F16, true, true, GATED>(tile, a, stream);
-        else y == BF16 ? launch_tile<E, BF16, true, true, LINEAR>(tile, a, stream) : launch_tile<E, F16, true, true, LINEAR>(tile, a, stream);
-    } else if (epilogue == GATED) launch_tile<E, E, true, true, GATED>(tile, a, stream);
-    else if (layout == FORWARD) launch_tile<E, E, true, true, LINEAR>(tile, a, stream);
-    else if (layout == INPUT_GRADIENT) launch_tile<E, E, true, false, LINEAR>(tile, a, stream);
-    else launch_tile<E, E, false, false, LINEAR>(tile, a, stream);
+    if constexpr (E == F8) {                // to either 16-bit type
+        if (epilogue == GATED) y == BF16 ? launch_tile<E, BF16, GATED>(tile, a, stream) : launch_tile<E, F16, GATED>(tile, a, stream);
+        else y == BF16 ? launch_tile<E, BF16, LINEAR>(tile, a, stream) : launch_tile<E, F16, LINEAR>(tile, a, stream);
+    } else if (epilogue == GATED) launch_tile<E, E, GATED>(tile, a, stream);
+    else launch_tile<E, E, LINEAR>(tile, a, stream);
 }
+
+#ifndef TIRAMISU_OPERAND_HAS_NO_GRADIENTS
+void NAME_OF(launch_grouped_gradients_, TIRAMISU_OPERAND)(product_tile tile, const grouped_arguments &a, const grouped_arguments &b, hipStream_t stream) {
+    constexpr int E = TIRAMISU_OPERAND;
+    typedef tiles_for<E, true, false, LINEAR> R;
+    typedef tiles_for<E, false, false, LINEAR> W;
+    if (tile == TILE_256) launch_gradients<typename R::tile_256, typename R::tile_256_end, typename W::tile_256, E>(a, b, stream);
+    else if (tile == TILE_256x128) launch_gradients<typename R::tile_256x128, typename R::tile_128, typename W::tile_256x128, E>(a, b, stream);
+    else if (tile == TILE_128) {
+        if ((a.p.y ? tiles_of<typename R::tile_128>(a) : 0) + (b.p.y ? tiles_of<typename W::tile_128>(b) : 0) > ttarget::COMPUTE_UNITS)
+            launch_gradients<typename R::tile_128_pair, typename R::tile_128_pair_end, typename W::tile_128_pair, E>(a, b, stream);
+        else launch_gradients<typename R::tile_128, typename R::tile_128_end, typename W::tile_128, E>(a, b, stream);
+    } else launch_gradients<typename R::tile_64, typename R::tile_64, typename W::tile_64, E>(a, b, stream);
+}
+#endif
 
 }  // namespace tgroups

@@ -108,43 +108,63 @@ __device__ __forceinline__ product_arguments product_of_rows(const grouped_argum
 
 // D: the tile for the last rows of a group that are no more than it is high, of C's width and half of its height or less (of 256 x 256 tiles a third would be half empty
 // where groups have some hundred rows).
+#ifdef __HIP_DEVICE_COMPILE__               // (the host's compilation needs no body)
 template <class C, class D, int Y>
-__global__ __launch_bounds__(C::NT) void grouped_rows_kernel(grouped_arguments a) {
-#ifdef __HIP_DEVICE_COMPILE__
+__device__ __forceinline__ void rows_tile(const grouped_arguments &a, int id, lds_char *lds) {
     static_assert(C::NT == D::NT && C::COLUMNS == D::COLUMNS && C::BM % D::BM == 0, "one workgroup's size and width");
-    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     const int across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
-    const found_tile f = find_tile<C::BM>(a.offsets, a.groups, a.rows, across, blockIdx.x, threadIdx.x & 63);
+    const found_tile f = find_tile<C::BM>(a.offsets, a.groups, a.rows, across, id, threadIdx.x & 63);
     const int group = uniform(f.group), rows = uniform(f.rows);
     if (group < 0) return;
     picked_rows picked;
     const product_arguments p = product_of_rows<C::BYTES>(a, group, uniform(f.first), rows, picked);
     int row, column;
     tile_in_bands(uniform(f.tile), (rows + C::BM - 1) / C::BM, across, row, column);
-    constexpr bool PICKED = C::A_ROWS && C::B_ROWS;
-    if (C::BM != D::BM && rows - row * C::BM <= D::BM) compute_tile_at<D, Y, PICKED>(p, row * (C::BM / D::BM), column, 0, (lds_char *)shared_bytes, picked);
-    else compute_tile_at<C, Y, PICKED>(p, row, column, 0, (lds_char *)shared_bytes, picked);
-#endif
+    constexpr int PICK = C::A_ROWS && C::B_ROWS ? ROWS_OF_A : NOTHING;
+    if (C::BM != D::BM && rows - row * C::BM <= D::BM) compute_tile_at<D, Y, PICK>(p, row * (C::BM / D::BM), column, 0, lds, picked);
+    else compute_tile_at<C, Y, PICK>(p, row, column, 0, lds, picked);
 }
 
-// The gradient of the weights: a.p.M x a.p.N of every group, its rows the terms.  A group without rows has zeros.
+// Tiles of a group's gradient are dealt to all eight XCDs, so that each has its share of every group however many rows that has (a run of whole groups to each
+// left some with half as much again as others); where eight does not divide them, groups begin at different XCDs.
 template <class C, int Y>
-__global__ __launch_bounds__(C::NT) void grouped_weights_kernel(grouped_arguments a) {
-#ifdef __HIP_DEVICE_COMPILE__
-    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
-    const int down = (a.p.M + C::BM - 1) / C::BM, across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
-    const int t = tile_in_runs(blockIdx.x, down * across * a.groups), group = t / (down * across);
+__device__ __forceinline__ void weights_tile(const grouped_arguments &a, int id, lds_char *lds) {
+    const int down = (a.p.M + C::BM - 1) / C::BM, across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS, tiles = down * across, each = (tiles + XCDS - 1) / XCDS;
+    const int group = id / XCDS / each, tile = (id + group) % XCDS * each + id / XCDS % each;
+    if (tile >= tiles) return;
     const group_span s = span_of(a.offsets, group, a.rows);
     product_arguments p = a.p;
     const long first = uniform(s.first), g = group;
     p.K = uniform(s.rows);
     p.a = (const char *)p.a + first * p.lda * C::BYTES;
-    p.b = (const char *)p.b + first * p.ldb * C::BYTES;
     p.y = (char *)p.y + g * a.y_step * 2;
     if (p.y_below) p.y_below = (char *)p.y_below + g * a.y_step * 2;
     int row, column;
-    tile_in_bands(t - group * down * across, down, across, row, column);
-    compute_tile_at<C, Y>(p, row, column, 0, (lds_char *)shared_bytes);
+    tile_in_bands(tile, down, across, row, column);
+    if (a.picked.index) return compute_tile_at<C, Y, K_OF_B>(p, row, column, 0, lds, {a.picked.index + first, a.picked.all});
+    p.b = (const char *)p.b + first * p.ldb * C::BYTES;
+    compute_tile_at<C, Y>(p, row, column, 0, lds);
+}
+#endif
+
+template <class C, class D, int Y>
+__global__ __launch_bounds__(C::NT) void grouped_rows_kernel(grouped_arguments a) {
+#ifdef __HIP_DEVICE_COMPILE__
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    rows_tile<C, D, Y>(a, blockIdx.x, (lds_char *)shared_bytes);
+#endif
+}
+
+// Both gradients in one launch: of the rows (a: C, and D for the last ones of a group), a.p.M x a.p.N of every group's weights behind them (b: G, the rows its terms; a
+// group without rows has zeros).  `start`: b's first workgroup, a multiple of the XCDs.
+template <class C, class D, class G, int Y>
+__global__ __launch_bounds__(C::NT) void grouped_gradients_kernel(grouped_arguments a, grouped_arguments b, int start) {
+#ifdef __HIP_DEVICE_COMPILE__
+    static_assert(C::NT == G::NT, "one workgroup's size");
+    extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
+    const int id = blockIdx.x;
+    if (id < start) rows_tile<C, D, Y>(a, id, (lds_char *)shared_bytes);
+    else weights_tile<G, Y>(b, id - start, (lds_char *)shared_bytes);
 #endif
 }
 

@@ -130,6 +130,41 @@ struct operand_loader {
             offset[v] = from >= 0 && from < all ? (int)(from * ld * BYTES) + q * 16 : (int)0x80000000;      // (behind any descriptor's end)
         }
     }
+    // k down the columns, of which an index in LDS picks each from `all` rows (below 2^31 bytes): k is row list[k], k < count; others read as zero.  offset: of a
+    // lane's granules within a row; picks: the rows of the slice that is loaded next.
+    typedef const __attribute__((address_space(3))) int *lds_list;
+    __device__ __forceinline__ void start_picked_k(const void *p, long ld, long first, long rows, lds_list list_, int count_, long all, int wave, int lane) {
+        static_assert(!K_ALONG_ROWS, "k is picked where it runs down the columns");
+        base = (const char *)p + first * BYTES;
+        left = ((all - 1) * ld + (rows - first)) * BYTES;
+        step = 0;
+        along = 0;
+        list = list_;
+        count = count_;
+        row_bytes = (int)(ld * BYTES);
+        most = (int)all;
+#pragma unroll
+        for (int v = 0; v < LOADS; v++) {
+            const int g = (wave * LOADS + v) * 64 + lane, row = g / G;
+            offset[v] = ((g % G) ^ swizzle(row)) * 16;
+            at[v] = row;
+        }
+        pick();
+    }
+    lds_list list;
+    int count, row_bytes, most, at[K_ALONG_ROWS ? 1 : LOADS], picks[K_ALONG_ROWS ? 1 : LOADS];
+    __device__ __forceinline__ void pick() {
+#pragma unroll
+        for (int v = 0; v < LOADS; v++) {
+            const int k = along + at[v];
+            picks[v] = list[min(k, count - 1)];
+            picks[v] = k < count ? picks[v] : -1;
+        }
+    }
+    __device__ __forceinline__ void load_picked_k(lds_char *stage, int wave, int v) const {
+        const int from = picks[v] >= 0 && picks[v] < most ? picks[v] * row_bytes + offset[v] : (int)0x80000000;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(), (__attribute__((address_space(3))) void *)(stage + (wave * LOADS + v) * 1024), 16, from, 0, 0, 0);
+    }
     // (a dword that begins inside an operand and ends outside reads as zero: the end is moved to a whole one)
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor() const {
         const long n = (left + 3) & ~3L;
@@ -205,11 +240,14 @@ __device__ __forceinline__ S multiply(const fragment<E, AR> &rows, const fragmen
 // Adds the product of one pair of operands' rows from m0 and n0, K elements of k, to the accumulators.  b, b2: B's operand (GATED: gate and up).
 // (The operands are __restrict__ so that the compiler does not take a transposing read of LDS for one that may see a load still on its way there: it
 // waited for every load ahead of each of them, 205 us where 105 are enough.)
-// picked: rows of A that an index picks, see compute_tile_at.
-struct picked_rows { const int *index; long all; };       // index: of the product's row 0 (null: rows follow each other); all: rows of the operand
-template <class C, bool PICKED = false>
+// What an index picks of an operand: nothing, rows of A (k along them), or k of B (down its columns; the index lies in LDS, PICKS of it at a time).
+enum picking : int { NOTHING = 0, ROWS_OF_A = 1, K_OF_B = 2 };
+struct picked_rows { const int *index; long all; };       // index: of the product's row 0, or of its first k (null: rows follow each other); all: rows of the operand
+constexpr int PICKS = 4096;
+template <class C, int PICK = NOTHING>
 __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc)[C::TM][C::TN], const void *__restrict__ a, long lda, const void *__restrict__ b, long ldb, const void *__restrict__ b2, long ldb2, long M, long N,
-                                           long m0, long n0, long k0, long K, lds_char *lds, picked_rows picked = {nullptr, 0}) {
+                                           long m0, long n0, long k0, long K, lds_char *lds, picked_rows picked = {nullptr, 0},
+                                           const __attribute__((address_space(3))) int *list = nullptr) {
     constexpr int TM = C::TM, TN = C::TN, ST = C::STAGES, E = C::E;
     constexpr int F = C::F, Q = 128 / C::STEP;                             // matrix steps of a slice
     constexpr int HALVES = C::EPILOGUE == GATED ? 2 : 1;
@@ -221,6 +259,7 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
     operand_loader<C::BYTES, C::BM, C::A_ROWS, C::LA, F> la;
     // (GATED: rows of gate in the first half of B's stage, rows of up in the second)
     operand_loader<C::BYTES, C::BN / HALVES, C::B_ROWS, LB1, F> lb[HALVES];
+    constexpr bool PICKED = PICK == ROWS_OF_A;
     bool in_order = true;
     if constexpr (PICKED)
         if (picked.index) {
@@ -228,17 +267,22 @@ __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc
             in_order = false;
         }
     if (in_order) la.start(a, lda, m0, M, k0, K, wave, lane);
-    lb[0].start(b, ldb, n0, N, k0, K, wave, lane);
+    if constexpr (PICK == K_OF_B) lb[0].start_picked_k(b, ldb, n0, N, list, (int)K, picked.all, wave, lane);
+    else lb[0].start(b, ldb, n0, N, k0, K, wave, lane);
     if constexpr (HALVES == 2) lb[1].start(b2, ldb2, n0, N, k0, K, wave, lane);
 
     auto issue_one = [&](int stage, int v, bool ahead = false) {
         lds_char *const s = lds + stage * C::STAGE;
         if (v < C::LA) la.load(s, wave, v);
+        else if constexpr (PICK == K_OF_B) lb[0].load_picked_k(s + C::A_STAGE, wave, v - C::LA);
         else if (HALVES == 1 || v < C::LA + LB1) lb[0].load(s + C::A_STAGE, wave, v - C::LA);
         else lb[HALVES - 1].load(s + C::A_STAGE + C::B_STAGE / 2, wave, v - C::LA - LB1);
         if (v == (PICKED && ahead ? C::LA : C::LA + C::LB) - 1) {
             la.advance();
-            lb[0].advance();
+            if constexpr (PICK == K_OF_B) {
+                lb[0].along += 64;
+                lb[0].pick();
+            } else lb[0].advance();
             if constexpr (HALVES == 2) lb[1].advance();
         }
     };
@@ -460,10 +504,11 @@ __device__ __forceinline__ void tile_of(int id, int rows, int columns, int &row,
 }
 
 #ifdef __HIP_DEVICE_COMPILE__               // (the host's compilation needs no body, and rejects a second one of the same configuration)
-// The tile of the product in this row and column of tiles, of part `split` of k.  Y: type of bias, residual and outputs.  PICKED: rows of A may be
-// picked by an index, and their scales with them.
-template <class C, int Y, bool PICKED = false>
+// The tile of the product in this row and column of tiles, of part `split` of k.  Y: type of bias, residual and outputs.  ROWS_OF_A: rows of A may be
+// picked by an index, and their scales with them; K_OF_B: the rows of B are, of a whole product.
+template <class C, int Y, int PICK = NOTHING>
 __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int row, int column, int split, lds_char *lds, picked_rows picked = {nullptr, 0}) {
+    constexpr bool PICKED = PICK == ROWS_OF_A;
     const long m0 = (long)row * C::BM, n0 = (long)column * C::COLUMNS;
     constexpr int F = C::F, REGISTERS = F * F / 64;
     typename block_sums<F>::type acc[C::TM][C::TN];
@@ -501,7 +546,16 @@ __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int 
     if constexpr (EARLY) load_terms();
     const long k0 = p.partial ? (long)split * p.slices_per_split * C::BK : 0;
     const long K = p.partial ? min((long)p.slices_per_split * C::BK, p.K - k0) : p.K;
-    accumulate<C, PICKED>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds, picked);
+    if constexpr (PICK == K_OF_B) {
+        // the index of PICKS terms at a time, behind the ring
+        __attribute__((address_space(3))) int *const list = (__attribute__((address_space(3))) int *)(lds + C::STAGES * C::STAGE);
+        for (long from = 0; from < K; from += PICKS) {
+            const int some = (int)min((long)PICKS, K - from);
+            for (int i = threadIdx.x; i < some; i += C::NT) list[i] = picked.index[from + i];
+            __syncthreads();
+            accumulate<C, K_OF_B>(acc, (const char *)p.a + from * p.lda * C::BYTES, p.lda, p.b, p.ldb, nullptr, 0, p.M, p.N, m0, n0, 0, some, lds, picked, list);
+        }
+    } else accumulate<C, PICK>(acc, p.a, p.lda, p.b, p.ldb, p.b2, p.ldb2, p.M, p.N, m0, n0, k0, K, lds, picked);
     if constexpr (C::EPILOGUE == LINEAR && C::A_ROWS && !C::B_ROWS)        // (only the gradient of a gated layer's input has two)
         if (p.a_more) accumulate<C>(acc, p.a_more, p.lda, p.b_more, p.ldb_more, nullptr, 0, p.M, p.N, m0, n0, k0, K, lds);
 
