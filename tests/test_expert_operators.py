@@ -657,7 +657,7 @@ def test_what_the_c_abi_refuses(capfd):
         w.tiramisu_hip_grouped_gated_linear_backward(p, p, p, p, p, p, p, None, p, p, p, 8, 8, 2, 8, 8, 0, 0, 0, 7, 0, 0, 4, 2),
         w.tiramisu_hip_combine_rows(p, p, None, None, p, 4, 1025, 8, 8, 0, 0, 2), w.tiramisu_hip_combine_rows(p, p, None, None, p, 4, 2, 8, 8, 0, 0, 0),
         w.tiramisu_hip_combine_rows(p, None, None, None, p, 4, 2, 8, 8, 0, 0, 2), w.tiramisu_hip_combine_rows_backward(p, p, p, p, None, p, p, 4, 2, 8, 8, 0, 0, 2),
-        w.tiramisu_hip_combine_rows_backward(p, p, p, None, p, p, p, 4, 2, 8, 8, 0, 0, 2), w.tiramisu_hip_combine_rows_backward(p, p, p, p, p, p, p, 1 << 24, 2, 8, 8, 0, 0, 2),
+        w.tiramisu_hip_combine_rows_backward(p, p, p, None, p, p, p, 4, 2, 8, 8, 0, 0, 2), w.tiramisu_hip_combine_rows_backward(p, p, p, p, p, p, p, 1 << 25, 2, 8, 8, 0, 0, 2),
     ]
     assert calls == [1] * len(calls)
     messages = capfd.readouterr().err.strip().splitlines()

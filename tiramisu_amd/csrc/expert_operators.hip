@@ -3,6 +3,7 @@
 #include "operator_calls.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "../../include/tiramisu_hip_wrappers.h"
@@ -23,6 +24,7 @@ namespace {
 typedef unsigned long long ull;
 
 // ---- route
+using troute::ROUTE_FEW_THREADS;
 using troute::ROUTE_THREADS;
 using troute::route_arguments;
 using troute::route_backward_arguments;
@@ -41,15 +43,16 @@ void by_experts(int experts, F f) {
 constexpr long ROUTE_FEW = 256;             // tokens that one workgroup routes
 template <int E>
 int route(const char *fn, route_arguments a) {
-    const size_t lds = troute::route_lds_bytes(a.experts);
     if (a.tokens <= ROUTE_FEW) {
+        const size_t lds = troute::route_lds_bytes(a.experts, ROUTE_FEW_THREADS);
         by_experts(a.experts, [&](auto lanes, auto values) {
-            hipLaunchKernelGGL((troute::route_few_kernel<E, decltype(lanes)::value, decltype(values)::value>), dim3(1), dim3(ROUTE_THREADS), lds, stream(), a);
+            hipLaunchKernelGGL((troute::route_few_kernel<E, decltype(lanes)::value, decltype(values)::value>), dim3(1), dim3(ROUTE_FEW_THREADS), lds, stream(), a);
         });
         check(hipGetLastError(), fn);
         return 0;
     }
-    a.block = (int)std::max(32L, (a.tokens + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
+    const size_t lds = troute::route_lds_bytes(a.experts, ROUTE_THREADS);
+    a.block = (int)std::max(64L, (a.tokens + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
     const unsigned blocks = (unsigned)((a.tokens + a.block - 1) / a.block);
     call_scratch s;
     const uint64_t counts = s.want((uint64_t)blocks * a.experts * 4);
@@ -109,14 +112,17 @@ product_tile grouped_tile(const grouped_arguments &a, int bytes, bool gated) {
     }
     return best;
 }
-// Both gradients: as one launch of as many tiles as they have together, whose slices are theirs in the mean.
+// Both gradients: as one launch of as many tiles as they have together, whose slices are theirs in the mean; where there are few rounds, those of a group of twice the
+// mean's rows, whose tiles the launch waits for (6720 rows in 14 groups, 140 x 1053: 256 x 256 tiles 45 us, 128 x 128 34).
 product_tile gradients_tile(const grouped_arguments &a, const grouped_arguments &b, int pairs) {
     product_tile best = TILE_64;
     double best_cost = 0;
     for (const auto &t : GROUPED_TILES) {
         const double down = a.p.y ? rows_tiles(a, t.rows, t.columns, false) : 0, across = b.p.y ? (double)((b.p.M + t.rows - 1L) / t.rows) * ((b.p.N + t.columns - 1L) / t.columns) * b.groups : 0;
-        const double slices = down * pairs * ((a.p.K + 63) / 64) + across * ((double)b.rows / b.groups / 64 + 0.5), tiles = std::max(1.0, down + across);
-        const double cost = t.factor * tile_launch_cost(t.tile, (long)tiles, std::max(1L, (long)(slices / tiles + 0.5)), 2, false);
+        const double of_rows = pairs * ((a.p.K + 63) / 64), of_weights = (double)b.rows / b.groups / 64, tiles = std::max(1.0, down + across);
+        double slices = (down * of_rows + across * (of_weights + 0.5)) / tiles;
+        if (tiles <= 2 * ttarget::COMPUTE_UNITS) slices = std::max(slices, std::max(down ? of_rows : 0.0, across ? 2 * of_weights : 0.0));
+        const double cost = t.factor * tile_launch_cost(t.tile, (long)tiles, std::max(1L, (long)(slices + 0.5)), 2, false);
         if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
     }
     return best;
@@ -130,9 +136,19 @@ void launch_gradients(int type, const grouped_arguments &a, const grouped_argume
 template <int E, int Y, int EPILOGUE>
 void launch_few(const char *fn, const grouped_arguments &a) {
     const int active = std::min(a.groups, a.rows);
-    const dim3 grid((unsigned)((a.p.N + FEW_ROWS - 1L) / FEW_ROWS), (unsigned)active + 1);
-    hipLaunchKernelGGL((tgroups::grouped_few_kernel<E, Y, EPILOGUE, 1>), grid, dim3(64 * FEW_WAVES), few_lds_bytes(1, EPILOGUE == GATED), stream(), a);
-    check(hipGetLastError(), fn);
+    auto go = [&](auto kernel, int split) {
+        const long columns = FEW_ROWS * (FEW_WAVES / split);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p.N + columns - 1) / columns), (unsigned)active + 1), dim3(64 * FEW_WAVES), few_lds_bytes(1, EPILOGUE == GATED), stream(), a);
+        check(hipGetLastError(), fn);
+    };
+    // Wavefronts that share the k of 16 columns: half or a quarter of a workgroup's where rows are short (of up to 4 KB, 2 KB) and workgroups of as many more columns still are two to a
+    // compute unit: each then reads more for its look-up, launch and sums.  us with 8 / 4 / 2, bf16: 128 rows in 64 groups, 2048 x 1024 61 / 46 / 41, gated 1024 x 2048 87 / 79 / 86;
+    // 8 rows in 8 groups 10.9 / 8.9 / 9.2 and 14.4 / 14.8 / 19.6.
+    const long bytes = (long)a.p.K * bytes_of(E), workgroups = (a.p.N + FEW_ROWS - 1L) / FEW_ROWS * active;
+    if constexpr (EPILOGUE == LINEAR)
+        if (bytes <= 2048 && workgroups >= 8 * ttarget::COMPUTE_UNITS) return go(tgroups::grouped_few_kernel<E, Y, EPILOGUE, 1, 2>, 2);
+    if (bytes <= 4096 && workgroups >= 4 * ttarget::COMPUTE_UNITS) return go(tgroups::grouped_few_kernel<E, Y, EPILOGUE, 1, 4>, 4);
+    go(tgroups::grouped_few_kernel<E, Y, EPILOGUE, 1, 8>, 8);
 }
 template <int EPILOGUE>
 void launch_few(const char *fn, int type, int y, const grouped_arguments &a) {
@@ -195,8 +211,9 @@ void settle_weight_rows(const char *fn, const planned_weight_rows &q, grouped_ar
     if (q.index) b.picked = {q.index, q.tokens};
 }
 
-// Rows that a group has in the mean, up to which its weights' bytes bound it and wavefronts that load them straight into registers are faster than tiles.
-constexpr long FEW_ROWS_OF_A_GROUP = 8;
+// Rows that a group has in the mean, up to which wavefronts that load weights straight into registers are faster than tiles, which read each weight once for all rows of a group (us as
+// few / as tiles, 64 groups of 2, 4, 8, 16 rows: gated 1024 x 2048 bf16 83 / 94, 99 / 103, 121 / 111, 176 / 111, e4m3 42 / 43, 50 / 51, 62 / 59; 2048 x 1024 bf16 41 / 41, 50 / 48, 65 / 53).
+constexpr long FEW_ROWS_OF_A_GROUP = 3;
 
 int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_arguments a, const int *rows, long tokens) {
     if (a.rows == 0 || a.p.N == 0) return 0;
@@ -257,14 +274,49 @@ grouped_arguments grouped_of(uint64_t S, uint64_t groups, uint64_t N, uint64_t K
 // ---- 4-bit weights
 using tfour::four_bit_arguments;
 
-// Tokens up to which the weights' bytes bound the product, and which go in parts of 64; with more the weights are widened ahead of a product on tiles.
-constexpr long FOUR_BIT_FEW = 128;
+// more LDS than a launch gets unasked: asked for once on every device
+void allow_lds(const char *fn, const void *kernel, int bytes, std::atomic<unsigned long long> &asked) {
+    int device = 0;
+    check(hipGetDevice(&device), fn);
+    const unsigned long long bit = 1ull << (device & 63);
+    if (asked.load() & bit) return;
+    check(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), fn);
+    asked.fetch_or(bit);
+}
+// LDS of x: whole units of k, up to a chunk
+long four_bit_chunk_bytes(long K, int tiles) { return std::min(K / 128 * 128, (long)tfour::four_bit_chunk(tiles)) * 16 * tiles * 2; }
 
+// Wavefronts that share the k of 16 columns: as few as leave a workgroup to each compute unit, as x is read once by each (us with 8 / 4 / 2: one token, 16384 x 4096 19 / 14 / 20; 64 tokens 51 / 31 /
+// 21; 128 tokens, 4096 x 4096 26 / 16 / 20)
+int four_bit_split(long M, long N, bool gated) {
+    const long tiles = (N + FEW_ROWS - 1) / FEW_ROWS * ((M + 63) / 64);
+    return tiles <= ttarget::COMPUTE_UNITS ? 8 : gated || M <= 16 || tiles <= 2 * ttarget::COMPUTE_UNITS ? 4 : 2;
+}
+// What the kernel of few tokens takes, for every round of its workgroups the bytes of x and weights at what a compute unit takes in, and what widening the weights ahead of a product on tiles
+// does, in microseconds (few / widened: 4096 x 4096 with 128, 256 and 512 tokens 16 / 32, 21 / 37, 39 / 38; gated 8192 x 2048 with 128 and 256 23 / 45, 44 / 47).
+double four_bit_few_cost(long M, long N, long K, bool gated) {
+    const long teams = FEW_WAVES / four_bit_split(M, N, gated), workgroups = (N + FEW_ROWS * teams - 1) / (FEW_ROWS * teams) * ((M + 63) / 64);
+    const double rounds = (double)((workgroups + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
+    return 3.0 + rounds * (double)K * (2.0 * std::min(M, 64L) + 8.5 * (double)teams * (gated ? 2 : 1)) / 33e3;
+}
+double four_bit_widened_cost(const planned_forward &f, long N, long K, bool gated) { return 7.0 + (gated ? 2.0 : 1.0) * N * K * 2.53 / 5e6 + f.q.plan.cost; }
+template <int E, int EPILOGUE, int TILES, int SPLIT>
+void launch_four_few(const char *fn, const four_bit_arguments &a) {
+    constexpr int TEAMS = FEW_WAVES / SPLIT;
+    auto kernel = tfour::four_bit_few_kernel<E, EPILOGUE, TILES, SPLIT>;
+    static std::atomic<unsigned long long> asked{0};
+    allow_lds(fn, (const void *)kernel, 16 * TILES * 2 * tfour::four_bit_chunk(TILES), asked);
+    const long columns = FEW_ROWS * TEAMS, lds = std::max(four_bit_chunk_bytes(a.p.K, TILES), (long)few_lds_bytes(TILES, EPILOGUE == GATED));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a.p.N + columns - 1) / columns), (unsigned)((a.p.M + 16 * TILES - 1) / (16 * TILES))), dim3(64 * FEW_WAVES), (size_t)lds, stream(), a);
+    check(hipGetLastError(), fn);
+}
 template <int E, int EPILOGUE, int TILES>
 void launch_four_few(const char *fn, const four_bit_arguments &a) {
-    const dim3 grid((unsigned)((a.p.N + FEW_ROWS - 1L) / FEW_ROWS), (unsigned)((a.p.M + 16 * TILES - 1) / (16 * TILES)));
-    hipLaunchKernelGGL((tfour::four_bit_few_kernel<E, EPILOGUE, TILES>), grid, dim3(64 * FEW_WAVES), few_lds_bytes(TILES, EPILOGUE == GATED), stream(), a);
-    check(hipGetLastError(), fn);
+    const int split = four_bit_split(a.p.M, a.p.N, EPILOGUE == GATED);
+    if (split == 8) return launch_four_few<E, EPILOGUE, TILES, 8>(fn, a);
+    if constexpr (EPILOGUE == LINEAR && TILES > 1)
+        if (split == 2) return launch_four_few<E, EPILOGUE, TILES, 2>(fn, a);
+    launch_four_few<E, EPILOGUE, TILES, 4>(fn, a);
 }
 template <int E, int EPILOGUE>
 void launch_four_few(const char *fn, const four_bit_arguments &a) {
@@ -272,28 +324,34 @@ void launch_four_few(const char *fn, const four_bit_arguments &a) {
     else if (a.p.M <= 32) launch_four_few<E, EPILOGUE, 2>(fn, a);
     else launch_four_few<E, EPILOGUE, 4>(fn, a);
 }
+// Few tokens in parts of 64, or the weights widened ahead of a product on tiles
 template <int E>
 int four_bit(const char *fn, int epilogue, four_bit_arguments a) {
     if (a.p.M == 0 || a.p.N == 0) return 0;
     const bool gated = epilogue == GATED;
-    if (a.p.K > 0 && a.p.M <= FOUR_BIT_FEW && a.p.N <= MOST_FEW_COLUMNS) {
-        gated ? launch_four_few<E, GATED>(fn, a) : launch_four_few<E, LINEAR>(fn, a);
-        return 0;
-    }
+    const long N = a.p.N, K = a.p.K, to = (K + 7) / 8 * 8;
     call_scratch s;
-    const long N = a.p.N, K = a.p.K, to = (K + 7) / 8 * 8, groups = (K + tfour::GROUP - 1) / tfour::GROUP;
     const uint64_t wide[2] = {s.want((uint64_t)to * N * 2), gated ? s.want((uint64_t)to * N * 2) : call_scratch::NOWHERE};
     product_arguments p = a.p;
     p.b = p.b2 = nullptr;
     p.ldb = p.ldb2 = to;
     planned_forward f = plan_forward(E, E, epilogue, p, s);
+    if (K > 0 && N <= MOST_FEW_COLUMNS && (a.p.M <= 64 || four_bit_few_cost(a.p.M, N, K, gated) <= four_bit_widened_cost(f, N, K, gated))) {
+        call_scratch few;
+        const placed_operand x = place_operand({a.p.a, a.p.lda}, a.p.M, K, 2, true, few);
+        if (few.take(fn)) return 1;
+        a.p.a = settle(fn, x, few);
+        a.p.lda = x.ld;
+        gated ? launch_four_few<E, GATED>(fn, a) : launch_four_few<E, LINEAR>(fn, a);
+        return 0;
+    }
     if (s.take(fn)) return 1;
     f.b.from.p = s.at(wide[0]);
     f.b2.from.p = s.at(wide[1]);
     for (int i = 0; i < (gated ? 2 : 1) && K > 0; i++)
-        for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / groups); first < N; first += most) {
+        for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / (to / 8)); first < N; first += most) {
             const long n = std::min(most, N - first), ldq = i ? a.p.ldb2 : a.p.ldb, lds = i ? a.lds_2 : a.lds;
-            hipLaunchKernelGGL((tfour::widen_rows_kernel<E>), dim3((unsigned)((groups * n + 255) / 256)), dim3(256), 0, stream(), (const char *)(i ? a.p.b2 : a.p.b) + first * ldq,
+            hipLaunchKernelGGL((tfour::widen_rows_kernel<E>), dim3((unsigned)((to / 8 * n + 255) / 256)), dim3(256), 0, stream(), (const char *)(i ? a.p.b2 : a.p.b) + first * ldq,
                                (i ? a.scale_2 : a.scale) + first * lds, ldq, lds, n, K, (char *)s.at(wide[i]) + first * to * 2, to);
         }
     check(hipGetLastError(), fn);
@@ -486,19 +544,20 @@ int tiramisu_hip_combine_rows(const void *x, const int32_t *places, const float 
 
 int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int32_t *places, const int32_t *owners, const float *weights, void *dx, float *dweights, uint64_t tokens,
                                        uint64_t k, uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t ldx, int32_t type) {
-    if (tokens > (1 << 23) || rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu tokens of %llu columns: at most 2^23 of at most 2^26", (ull)tokens, (ull)columns);
+    if (rows > MOST || columns > MOST_COLUMNS) return refuse(__FUNCTION__, "%llu rows of %llu columns: at most 2^30 - 1 of at most 2^26", (ull)rows, (ull)columns);
     if (k > 1024) return refuse(__FUNCTION__, "%llu rows of a token: at most 1024", (ull)k);
+    if (tokens > MOST || tokens * k > 1 << 25) return refuse(__FUNCTION__, "%llu tokens of %llu rows: at most 2^25 rows of all", (ull)tokens, (ull)k);
     if (!known_type(type, false)) return refuse(__FUNCTION__, "element type %d: float16 or bfloat16", type);
     if ((tokens && columns && k && (!dy || !places)) || (rows && columns && dx && !owners) || (rows && columns && dweights && !x)) return refuse(__FUNCTION__, "dy, x, places and owners are needed");
     if (dweights && !weights) return refuse(__FUNCTION__, "a gradient of weights that are not given");
     timed record(__FUNCTION__);
     const long n = (long)columns;
-    const bool team = n >= 1024;
-    const long token_blocks = k == 0 ? 0 : team ? (long)tokens : ((long)tokens + 3) / 4, blocks = token_blocks + (dx && n ? ((long)rows + 255) / 256 : 0);
+    const bool wide = n > 256;
+    const long choices = wide ? 4 : 16, choice_blocks = ((long)tokens * (long)k + choices - 1) / choices, blocks = choice_blocks + (dx && n ? ((long)rows + 255) / 256 : 0);
     if (blocks == 0) return 0;
-    const tcombine::combine_backward_arguments a = {dy, x, places, owners, weights, n ? dx : nullptr, dweights, (long)tokens, (long)rows, n, ldy ? (long)ldy : n, ldx ? (long)ldx : n, (int)k, token_blocks};
-    auto kernel = type == F16 ? (team ? tcombine::combine_backward_kernel<F16, 256> : tcombine::combine_backward_kernel<F16, 64>)
-                              : (team ? tcombine::combine_backward_kernel<BF16, 256> : tcombine::combine_backward_kernel<BF16, 64>);
+    const tcombine::combine_backward_arguments a = {dy, x, places, owners, weights, n ? dx : nullptr, dweights, (long)tokens, (long)rows, n, ldy ? (long)ldy : n, ldx ? (long)ldx : n, (int)k, choice_blocks};
+    auto kernel = type == F16 ? (wide ? tcombine::combine_backward_kernel<F16, 64> : tcombine::combine_backward_kernel<F16, 16>)
+                              : (wide ? tcombine::combine_backward_kernel<BF16, 64> : tcombine::combine_backward_kernel<BF16, 16>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream(), a);
     check(hipGetLastError(), __FUNCTION__);
     return 0;

@@ -170,16 +170,16 @@ __global__ __launch_bounds__(C::NT) void grouped_gradients_kernel(grouped_argume
 
 // Few rows to a group: bound by the bytes of the weights of the groups that have rows.  grid: (columns in sixteens, groups that may have rows and one): workgroups
 // of the last row of the grid write the rows behind the groups.  A group's weights are read once for each TILES x 16 of its rows.
-template <int E, int Y, int EPILOGUE, int TILES>
+template <int E, int Y, int EPILOGUE, int TILES, int SPLIT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void grouped_few_kernel(grouped_arguments a) {
-    constexpr int BYTES = E == F8 ? 1 : 2;
+    constexpr int BYTES = E == F8 ? 1 : 2, COLUMNS = FEW_ROWS * (FEW_WAVES / SPLIT);
     const int lane = threadIdx.x & 63, wanted = blockIdx.y;
-    const long n0 = (long)blockIdx.x * FEW_ROWS;
+    const long n0 = (long)blockIdx.x * COLUMNS;
     if (wanted == (int)gridDim.y - 1) {
-        const int last = min(max(a.offsets[a.groups], 0), a.rows), some = (int)min((long)FEW_ROWS, a.p.N - n0);
-        for (long i = threadIdx.x; i < (long)(a.rows - last) * FEW_ROWS; i += 64 * FEW_WAVES) {
-            const long at = (last + i / FEW_ROWS) * a.p.N + n0 + i % FEW_ROWS;
-            if (i % FEW_ROWS >= some) continue;
+        const int last = min(max(a.offsets[a.groups], 0), a.rows), some = (int)min((long)COLUMNS, a.p.N - n0);
+        for (long i = threadIdx.x; i < (long)(a.rows - last) * COLUMNS; i += 64 * FEW_WAVES) {
+            const long at = (last + i / COLUMNS) * a.p.N + n0 + i % COLUMNS;
+            if (i % COLUMNS >= some) continue;
             ((uint16_t *)a.p.y)[at] = 0;
             if (a.p.pre) ((uint16_t *)a.p.pre)[at] = ((uint16_t *)a.p.pre2)[at] = 0;
         }
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void grouped_few_kernel(grouped_arg
         if (from > 0) __syncthreads();                     // (the sums of the rows before have been read)
         picked_rows picked;
         const product_arguments p = product_of_rows<BYTES>(a, group, first + from, min(rows - from, 16 * TILES), picked);
-        few_tokens<E, Y, EPILOGUE, TILES, true>(p, n0, picked);
+        few_tokens<E, Y, EPILOGUE, TILES, true, SPLIT>(p, n0, picked);
     }
 }
 

@@ -28,14 +28,15 @@ __device__ __forceinline__ f32x4 multiply_16(u32x4 rows, u32x4 columns, f32x4 c)
     }
 }
 
-// The 16 columns from n0 on.  PICKED: rows of x may be picked by an index; one that is none of x's gives a row of zeros.
-template <int E, int Y, int EPILOGUE, int TILES, bool PICKED = false>
+// The columns from n0 on: 16 to every SPLIT wavefronts, which share their k.  PICKED: rows of x may be picked by an index; one that is none of x's gives a row of zeros.
+template <int E, int Y, int EPILOGUE, int TILES, bool PICKED = false, int SPLIT = FEW_WAVES>
 __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, picked_rows picked = {nullptr, 0}) {
     constexpr int BYTES = E == F8 ? 1 : 2, PARTS = EPILOGUE == GATED ? 2 : 1, BATCH = TILES * PARTS >= 4 ? 2 : TILES * PARTS == 2 ? 4 : 8;
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     __attribute__((address_space(3))) f32x4 *const sums = (__attribute__((address_space(3))) f32x4 *)shared_bytes;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, team = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / SPLIT, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % SPLIT;
     const int l16 = lane & 15, group = lane >> 4;
+    n0 += team * FEW_ROWS;
     const long bytes = (long)p.K * BYTES;
 
     const char *w[PARTS], *x[TILES];
@@ -60,7 +61,7 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
         for (int i = 0; i < TILES; i++) acc[q][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // what the epilogue of 8 columns of row m reads, ahead of the product
-    const int id = threadIdx.x, m = id >> 1, c0 = 8 * (id & 1);
+    const int id = threadIdx.x % (64 * SPLIT), m = id >> 1, c0 = 8 * (id & 1);
     const long n = n0 + c0;
     const int some = (int)min(8L, p.N - n);
     const bool mine = m < p.M && m < 16 * TILES && some > 0;
@@ -83,13 +84,13 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
     // as many units at a time as are left, by halves
     auto take = [&](auto batch_c) {
         constexpr int B = decltype(batch_c)::value;
-        for (; u + (B - 1) * FEW_WAVES < whole; u += B * FEW_WAVES) {
+        for (; u + (B - 1) * SPLIT < whole; u += B * SPLIT) {
             u32x4 fw[B][2][PARTS], fx[B][2][TILES];
 #pragma unroll
             for (int b = 0; b < B; b++)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    const long at = (long)(u + b * FEW_WAVES) * 128 + 64 * half;
+                    const long at = (long)(u + b * SPLIT) * 128 + 64 * half;
 #pragma unroll
                     for (int q = 0; q < PARTS; q++) fw[b][half][q] = *reinterpret_cast<const u32x4_any *>(w[q] + at);
 #pragma unroll
@@ -109,7 +110,7 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
     if constexpr (BATCH >= 4) take(std::integral_constant<int, 4>());
     take(std::integral_constant<int, 2>());
     take(std::integral_constant<int, 1>());
-    for (; u < units; u += FEW_WAVES) {
+    for (; u < units; u += SPLIT) {
 #pragma unroll
         for (int half = 0; half < 2; half++) {
             const long at = (long)u * 128 + 64 * half, left = bytes - at - 16 * group;
@@ -129,7 +130,7 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
 #pragma unroll
     for (int q = 0; q < PARTS; q++)
 #pragma unroll
-        for (int i = 0; i < TILES; i++) sums[((wave * PARTS + q) * TILES + i) * 64 + lane] = acc[q][i];
+        for (int i = 0; i < TILES; i++) sums[(((team * SPLIT + wave) * PARTS + q) * TILES + i) * 64 + lane] = acc[q][i];
     __syncthreads();
     if (!mine) return;
     float z[PARTS][8];
@@ -138,10 +139,10 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
 #pragma unroll
         for (int i = 0; i < 8; i++) z[q][i] = 0.f;
 #pragma unroll
-        for (int v = 0; v < FEW_WAVES; v++)
+        for (int v = 0; v < SPLIT; v++)
 #pragma unroll
             for (int four = 0; four < 2; four++) {
-                const f32x4 s = sums[((v * PARTS + q) * TILES + (m >> 4)) * 64 + (c0 / 4 + four) * 16 + (m & 15)];
+                const f32x4 s = sums[(((team * SPLIT + v) * PARTS + q) * TILES + (m >> 4)) * 64 + (c0 / 4 + four) * 16 + (m & 15)];
 #pragma unroll
                 for (int i = 0; i < 4; i++) z[q][4 * four + i] += s[i];
             }

@@ -189,13 +189,13 @@ __device__ __forceinline__ int sum_before(int experts, INTS count, INTS sums) {
     return all;
 }
 
-constexpr int ROUTE_THREADS = 512;
+constexpr int ROUTE_THREADS = 1024, ROUTE_FEW_THREADS = 512;
 typedef __attribute__((address_space(3))) int lds_int;
-inline int route_lds_bytes(int experts) { return ((ROUTE_THREADS / 64 + 2) * experts + 64) * 4; }
+inline int route_lds_bytes(int experts, int threads) { return ((threads / 64 + 2) * experts + 64) * 4; }
 
-template <int E, int LANES, int VALUES>
+template <int E, int LANES, int VALUES, int THREADS>
 __device__ __forceinline__ void choose_block(const route_arguments &a, long first, long end) {
-    constexpr int TOKENS = ROUTE_THREADS / LANES;
+    constexpr int TOKENS = THREADS / LANES;
     for (long from = first; from < end; from += TOKENS) {
         const long token = from + threadIdx.x / LANES;
         choose<E, LANES, VALUES>(a, token, token < end, threadIdx.x & 63);
@@ -204,25 +204,25 @@ __device__ __forceinline__ void choose_block(const route_arguments &a, long firs
 
 // Everything, for few tokens: one workgroup
 template <int E, int LANES, int VALUES>
-__global__ __launch_bounds__(ROUTE_THREADS) void route_few_kernel(route_arguments a) {
+__global__ __launch_bounds__(ROUTE_FEW_THREADS) void route_few_kernel(route_arguments a) {
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
-    lds_int *const next = (lds_int *)shared_bytes, *const hist = next + a.experts, *const sums = hist + ROUTE_THREADS / 64 * a.experts;
+    lds_int *const next = (lds_int *)shared_bytes, *const hist = next + a.experts, *const sums = hist + ROUTE_FEW_THREADS / 64 * a.experts;
     const int t = threadIdx.x;
-    for (int e = t; e < a.experts; e += ROUTE_THREADS) next[e] = 0;
-    choose_block<E, LANES, VALUES>(a, 0, a.tokens);
+    for (int e = t; e < a.experts; e += ROUTE_FEW_THREADS) next[e] = 0;
+    choose_block<E, LANES, VALUES, ROUTE_FEW_THREADS>(a, 0, a.tokens);
     __syncthreads();
     const long all = a.tokens * a.k;
-    for (long i = t; i < all; i += ROUTE_THREADS) {
+    for (long i = t; i < all; i += ROUTE_FEW_THREADS) {
         const int e = a.chosen[i];
         if (e >= 0) __hip_atomic_fetch_add(next + e, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     }
     __syncthreads();
-    const int total = sum_before<ROUTE_THREADS>(a.experts, next, sums);
-    for (int e = t; e < a.experts; e += ROUTE_THREADS) a.offsets[e] = next[e];
+    const int total = sum_before<ROUTE_FEW_THREADS>(a.experts, next, sums);
+    for (int e = t; e < a.experts; e += ROUTE_FEW_THREADS) a.offsets[e] = next[e];
     if (t == 0) a.offsets[a.experts] = total;
     __syncthreads();
-    place<ROUTE_THREADS>(a, 0, all, next, hist);
-    for (long i = total + t; i < all; i += ROUTE_THREADS) a.rows[i] = -1;
+    place<ROUTE_FEW_THREADS>(a, 0, all, next, hist);
+    for (long i = total + t; i < all; i += ROUTE_FEW_THREADS) a.rows[i] = -1;
 }
 
 // A block of tokens: their choices, and how many of each expert
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(ROUTE_THREADS) void route_choose_kernel(route_argum
     const int t = threadIdx.x;
     const long first = (long)blockIdx.x * a.block, end = min(first + a.block, a.tokens);
     for (int e = t; e < a.experts; e += ROUTE_THREADS) count[e] = 0;
-    choose_block<E, LANES, VALUES>(a, first, end);
+    choose_block<E, LANES, VALUES, ROUTE_THREADS>(a, first, end);
     __syncthreads();
     for (long i = first * a.k + t; i < end * a.k; i += ROUTE_THREADS) {
         const int e = a.chosen[i];
