@@ -210,7 +210,7 @@ expr cublas_gemm(const buffer &A, const buffer &B, buffer &C, expr M, expr N, ex
                  expr transposeA = expr(), expr transposeB = expr());
 
 /** Operators of a transformer's feed-forward sublayer as library calls on GPU buffers (this back-end's own; tiramisu_hip_wrappers.h
-  * says what they compute), used like cublas_gemm.  All buffers of a call hold one type: p_bfloat16 (rms_norm also p_float32), rows dense.
+  * says what they compute), used like cublas_gemm.  All buffers of a call hold one type but where it says otherwise: p_bfloat16 (rms_norm also p_float32), rows dense.
   * A call that the runtime refuses ends the process. */
 enum class hip_activation { none = 0, relu = 1, gelu = 2, gelu_tanh = 3, silu = 4 };
 /** y = s / sqrt(mean(s^2) + eps) * weight of each row, s = x + residual where a residual is given, stored in \p sum then. */
@@ -222,6 +222,21 @@ expr hip_linear(const buffer &x, const buffer &weight, buffer &y, expr M, expr N
 /** h = activation(x gate_weight^T) * (x up_weight^T); both weights N x K. */
 expr hip_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, buffer &h, expr M, expr N, expr K,
                       hip_activation activation = hip_activation::silu);
+/** A feed-forward sublayer with experts.  The k experts of each token with the largest of its `experts` logits (p_bfloat16 or p_float32): \p chosen and \p places
+  * [tokens][k], \p offsets [experts + 1] and \p rows [tokens k] hold p_int32, \p weights [tokens][k] p_float32. */
+expr hip_route(const buffer &logits, buffer &chosen, buffer &weights, buffer &offsets, buffer &rows, buffer &places, expr tokens, expr experts, expr k, bool normalise = true);
+/** y[s] = x[rows[s]] weight[g]^T for the places s of group g, offsets[g] to offsets[g + 1]; weight is groups x N x K, x T x K, y S x N.  Without \p rows x has the S rows themselves. */
+expr hip_grouped_linear(const buffer &x, const buffer &weight, const buffer &offsets, buffer &y, expr S, expr T, expr groups, expr N, expr K, const buffer *rows = nullptr);
+/** h[s] = activation(x[rows[s]] gate_weight[g]^T) * (x[rows[s]] up_weight[g]^T). */
+expr hip_grouped_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, const buffer &offsets, buffer &h, expr S, expr T, expr groups, expr N, expr K,
+                              const buffer *rows = nullptr, hip_activation activation = hip_activation::silu);
+/** y[t] = residual[t] + sum over j < k of weights[t][j] x[places[t][j]]; x is S x columns, weights (without: ones) hold p_float32. */
+expr hip_combine_rows(const buffer &x, const buffer &places, buffer &y, expr tokens, expr k, expr S, expr columns, const buffer *weights = nullptr, const buffer *residual = nullptr);
+/** hip_linear and hip_gated_linear with weights in 4 bits: values N x (K + 1) / 2 and scales N x (K + 31) / 32, both p_uint8. */
+expr hip_four_bit_linear(const buffer &x, const buffer &weight, const buffer &scale, buffer &y, expr M, expr N, expr K, hip_activation activation = hip_activation::none,
+                         const buffer *bias = nullptr, const buffer *residual = nullptr);
+expr hip_four_bit_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, const buffer &gate_scale, const buffer &up_scale, buffer &h, expr M, expr N, expr K,
+                               hip_activation activation = hip_activation::silu);
 
 std::string str_from_tiramisu_type_expr(expr_t t);
 std::string str_tiramisu_type_op(op_t o);

@@ -267,6 +267,7 @@ int tiramisu_hip_exchange_scratch_source(struct tiramisu_hip_scratch_source *sou
 /* For generated code: no buffer in the place of one that may be left out, and what becomes of a refused call there -- the reference's failure
  * model, the process ends with status 1 behind the operator's message. */
 float *tiramisu_hip_no_buffer(void);
+int32_t *tiramisu_hip_no_numbers(void);
 int tiramisu_hip_require(int32_t status);
 
 /* ---- per-launch timing.  Between profile_start and profile_stop every tiramisu_hip_launch

@@ -440,4 +440,64 @@ expr hip_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &
                                                        u64_of(M), u64_of(N), u64_of(K), dense, dense, dense, expr((int32_t)activation), type, type});
 }
 
+namespace {
+
+expr numbers_argument(const buffer *b) { return b ? buffer_argument(b) : expr(o_call, "tiramisu_hip_no_numbers", {}, p_uint64); }
+void holds(const char *op, primitive_t type, std::initializer_list<const buffer *> buffers) {
+    for (const buffer *b : buffers)
+        if (b && b->get_elements_type() != type)
+            ERROR(std::string(op) + ": buffer " + b->get_name() + " holds " + str_from_tiramisu_type_primitive(b->get_elements_type()) + ", not " + str_from_tiramisu_type_primitive(type), true);
+}
+
+}  // namespace
+
+expr hip_route(const buffer &logits, buffer &chosen, buffer &weights, buffer &offsets, buffer &rows, buffer &places, expr tokens, expr experts, expr k, bool normalise) {
+    const expr type = element_of("hip_route", logits, {}, true), dense = expr((uint64_t)0);
+    holds("hip_route", p_int32, {&chosen, &offsets, &rows, &places});
+    holds("hip_route", p_float32, {&weights});
+    return operator_call("tiramisu_hip_route", {buffer_argument(&logits), buffer_argument(&chosen), buffer_argument(&weights), buffer_argument(&offsets), buffer_argument(&rows),
+                                                buffer_argument(&places), u64_of(tokens), u64_of(experts), u64_of(k), dense, expr((int32_t)normalise), type});
+}
+
+expr hip_grouped_linear(const buffer &x, const buffer &weight, const buffer &offsets, buffer &y, expr S, expr T, expr groups, expr N, expr K, const buffer *rows) {
+    const expr type = element_of("hip_grouped_linear", x, {&weight, &y}, false), dense = expr((uint64_t)0);
+    holds("hip_grouped_linear", p_int32, {&offsets, rows});
+    return operator_call("tiramisu_hip_grouped_linear", {buffer_argument(&x), buffer_argument(&weight), buffer_argument(&offsets), numbers_argument(rows), buffer_argument(nullptr),
+                                                         buffer_argument(nullptr), buffer_argument(&y), u64_of(S), u64_of(T), u64_of(groups), u64_of(N), u64_of(K), dense, dense, type, type});
+}
+
+expr hip_grouped_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, const buffer &offsets, buffer &h, expr S, expr T, expr groups, expr N, expr K,
+                              const buffer *rows, hip_activation activation) {
+    const expr type = element_of("hip_grouped_gated_linear", x, {&gate_weight, &up_weight, &h}, false), dense = expr((uint64_t)0);
+    holds("hip_grouped_gated_linear", p_int32, {&offsets, rows});
+    return operator_call("tiramisu_hip_grouped_gated_linear", {buffer_argument(&x), buffer_argument(&gate_weight), buffer_argument(&up_weight), buffer_argument(&offsets), numbers_argument(rows),
+                                                               buffer_argument(nullptr), buffer_argument(nullptr), buffer_argument(nullptr), buffer_argument(&h), buffer_argument(nullptr),
+                                                               buffer_argument(nullptr), u64_of(S), u64_of(T), u64_of(groups), u64_of(N), u64_of(K), dense, dense, dense,
+                                                               expr((int32_t)activation), type, type});
+}
+
+expr hip_combine_rows(const buffer &x, const buffer &places, buffer &y, expr tokens, expr k, expr S, expr columns, const buffer *weights, const buffer *residual) {
+    const expr type = element_of("hip_combine_rows", x, {&y, residual}, false), dense = expr((uint64_t)0);
+    holds("hip_combine_rows", p_int32, {&places});
+    holds("hip_combine_rows", p_float32, {weights});
+    return operator_call("tiramisu_hip_combine_rows", {buffer_argument(&x), buffer_argument(&places), buffer_argument(weights), buffer_argument(residual), buffer_argument(&y), u64_of(tokens),
+                                                       u64_of(k), u64_of(S), u64_of(columns), dense, dense, type});
+}
+
+expr hip_four_bit_linear(const buffer &x, const buffer &weight, const buffer &scale, buffer &y, expr M, expr N, expr K, hip_activation activation, const buffer *bias, const buffer *residual) {
+    const expr type = element_of("hip_four_bit_linear", x, {&y, bias, residual}, false), dense = expr((uint64_t)0);
+    holds("hip_four_bit_linear", p_uint8, {&weight, &scale});
+    return operator_call("tiramisu_hip_four_bit_linear", {buffer_argument(&x), buffer_argument(&weight), buffer_argument(&scale), buffer_argument(bias), buffer_argument(residual),
+                                                          buffer_argument(&y), u64_of(M), u64_of(N), u64_of(K), dense, dense, dense, dense, expr((int32_t)activation), type});
+}
+
+expr hip_four_bit_gated_linear(const buffer &x, const buffer &gate_weight, const buffer &up_weight, const buffer &gate_scale, const buffer &up_scale, buffer &h, expr M, expr N, expr K,
+                               hip_activation activation) {
+    const expr type = element_of("hip_four_bit_gated_linear", x, {&h}, false), dense = expr((uint64_t)0);
+    holds("hip_four_bit_gated_linear", p_uint8, {&gate_weight, &up_weight, &gate_scale, &up_scale});
+    return operator_call("tiramisu_hip_four_bit_gated_linear", {buffer_argument(&x), buffer_argument(&gate_weight), buffer_argument(&up_weight), buffer_argument(&gate_scale),
+                                                                buffer_argument(&up_scale), buffer_argument(&h), u64_of(M), u64_of(N), u64_of(K), dense, dense, dense, dense, dense,
+                                                                expr((int32_t)activation), type});
+}
+
 }  // namespace tiramisu

@@ -455,11 +455,14 @@ template <int Y>
 __device__ __forceinline__ void load_residual(const product_arguments &p, float (&r)[8], long m, long n, int some) {
     load_some<Y>((const stored<Y> *)p.residual + m * p.ldr + n, some, r);
 }
-template <int Y>
+// PAST: past the caches
+template <int Y, bool PAST = false>
 __device__ __forceinline__ void store_linear(const product_arguments &p, const float (&z)[8], long m, long n, int some) {
     typedef stored<Y> T;
-    if (m < p.rows_above) store_some<Y>((T *)p.y + m * p.N + n, some, z);
-    else if (m >= p.split_row) store_some<Y>((T *)p.y_below + (m - p.split_row) * p.N + n, some, z);
+    if (m >= p.rows_above && m < p.split_row) return;
+    T *const to = m < p.rows_above ? (T *)p.y + m * p.N + n : (T *)p.y_below + (m - p.split_row) * p.N + n;
+    if constexpr (PAST) store_some_past<Y>(to, some, z);
+    else store_some<Y>(to, some, z);
 }
 template <int Y>
 __device__ __forceinline__ void finish_linear(const product_arguments &p, const column_terms &c, float (&z)[8], const float (&r)[8], float row_scale, long m, long n,
@@ -641,7 +644,7 @@ __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int 
                             for (int e = 0; e < 8; e++) z[e] += r[pass][e];
                         }
                     }
-                    store_linear<Y>(p, z, first + pass * DOWN, n, some);
+                    store_linear<Y, !C::A_ROWS>(p, z, first + pass * DOWN, n, some);
                 }
             } else {
                 // (many instructions: not unrolled)

@@ -109,6 +109,18 @@ __device__ __forceinline__ void store_some(stored<E> *p, int n, const float (&v)
         if (i < n) store_one<E>(p + i, v[i]);
 }
 
+// Results that are read much later, if at all by this device's next kernels: past the caches, where operands stay (gradients of the weights of 32 groups, 268 MB: 369 -> 356 us with
+// those of the rows; gated 4096 x 4096 x 2048 239 -> 233).  16-bit types.
+template <int E>
+__device__ __forceinline__ void store_some_past(stored<E> *p, int n, const float (&v)[8]) {
+    if (n < 8) return store_some<E>(p, n, v);
+    typedef stored<E> pair __attribute__((ext_vector_type(2)));
+    u32x4 w;
+#pragma unroll
+    for (int c = 0; c < 4; c++) w[c] = __builtin_bit_cast(uint32_t, pair{(stored<E>)v[2 * c], (stored<E>)v[2 * c + 1]});
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any *>(p));
+}
+
 // 16 bytes at `p` of which `left` exist; the others are zero and not read
 template <int BYTES>
 __device__ __forceinline__ u32x4 load_guarded(const char *p, long left) {

@@ -550,6 +550,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
 }
 
 float *tiramisu_hip_no_buffer(void) { return nullptr; }       // (a pointer that is also one to scales)
+int32_t *tiramisu_hip_no_numbers(void) { return nullptr; }
 
 int tiramisu_hip_require(int32_t status) {
     if (status != 0) exit(1);

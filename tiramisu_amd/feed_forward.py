@@ -1,9 +1,9 @@
-"""A transformer's feed-forward sublayer on the operators of ``tiramisu_amd.operators``: trained in 16 bits, served in 16 or in 8.
+"""A transformer's feed-forward sublayer on the operators of ``tiramisu_amd.operators``: trained in 16 bits, served in 16, in 8 or with weights in 4.
 
     sum = x + residual,  n = rms_norm(sum),  h = silu(n gate^T) * (n up^T),  y = sum + h down^T
 
 ``python -m tiramisu_amd.feed_forward`` trains one on random data for some steps, then serves tokens with what it learnt and says how far 8 bits
-are from 16.  (The same forward pass as a Tiramisu program: tiramisu_amd/programs/feed_forward.cpp.)
+and 4-bit weights are from 16.  (The same forward pass as a Tiramisu program: tiramisu_amd/programs/feed_forward.cpp.)
 """
 from typing import NamedTuple
 
@@ -57,6 +57,10 @@ class FeedForward:
         """The sublayer with its matrices as 8-bit rows with scales, laid out once."""
         return EightBitFeedForward(self)
 
+    def in_4_bits(self):
+        """The sublayer with its matrices in 4 bits with a scale for each 32 of a row, laid out once."""
+        return FourBitFeedForward(self)
+
 
 class EightBitFeedForward:
     """Serves a ``FeedForward`` with 8-bit matrices: the norm's results leave it in 8 bits, the gated layer's are brought to 8 bits ahead of the down
@@ -72,6 +76,19 @@ class EightBitFeedForward:
                                    up_scale=self.up.scale, dtype=self.dtype).h
         h = operators.quantize_rows(h)
         return operators.linear(h.q, self.down.q, residual=n.sum, x_scale=h.scale, weight_scale=self.down.scale, dtype=self.dtype).y
+
+
+class FourBitFeedForward:
+    """Serves a ``FeedForward`` with 4-bit matrices, a quarter of the bytes that bound a single token; activations stay in 16 bits."""
+
+    def __init__(self, layer):
+        self.norm, self.activation, self.eps = layer.norm, layer.activation, layer.eps
+        self.gate, self.up, self.down = [operators.quantize_groups(w) for w in (layer.gate, layer.up, layer.down)]
+
+    def serve(self, x, residual):
+        n = operators.rms_norm(x, self.norm, residual=residual, eps=self.eps)
+        h = operators.four_bit_gated_linear(n.y, self.gate.q, self.up.q, self.gate.scale, self.up.scale, activation=self.activation).h
+        return operators.four_bit_linear(h, self.down.q, self.down.scale, residual=n.sum).y
 
 
 def disturbed(layer, by, generator=None):
@@ -107,12 +124,12 @@ def main():
     layer = disturbed(teacher, 0.5, generator)
     errors = train(layer, teacher, 60, 2048, generator=generator)
     print("mean squared error: %.4f at first, %.4f after %d steps" % (errors[0], errors[-1], len(errors)))
-    small = layer.in_8_bits()
+    small, smallest = layer.in_8_bits(), layer.in_4_bits()
     for tokens in (1, 16, 2048):
         x, residual = [torch.randn((tokens, 1024), device="cuda", generator=generator).to(torch.bfloat16) for _ in range(2)]
-        y, y8 = layer.serve(x, residual).float(), small.serve(x, residual).float()
-        branch = y - (x + residual).float()
-        print("%4d tokens: 8 bits are %.3f of the sublayer's own part away from 16" % (tokens, float((y8 - y).norm() / branch.norm())))
+        y, y8, y4 = [served.serve(x, residual).float() for served in (layer, small, smallest)]
+        branch = (y - (x + residual).float()).norm()
+        print("%4d tokens: 8 bits are %.3f of the sublayer's own part away from 16, 4-bit weights %.3f" % (tokens, float((y8 - y).norm() / branch), float((y4 - y).norm() / branch)))
 
 
 if __name__ == "__main__":
