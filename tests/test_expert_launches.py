@@ -19,14 +19,16 @@ GATED_16 = {"few 8": (30, 19, 93, 330), "few 4": (16, 8, 2100, 330), "64x128/3":
 LINEAR_8 = {"few 8": (30, 19, 93, 332), "few 4": (16, 8, 2100, 3000), "few 2": (20, 9, 4100, 332), "64x64/3": (83, 3, 93, 140), "128x128/4": (250, 8, 2029, 392), "256x128/3": (36058, 51, 71, 44),
             "256x256/2": (30200, 22, 235, 36)}
 GATED_8 = {"few 8": (30, 19, 93, 332), "few 4": (16, 8, 2100, 332), "64x128/3": (83, 3, 93, 140), "128x128/4": (14642, 11, 13, 36), "256x128/3": (28360, 65, 9, 820), "256x256/2": (11240, 4, 617, 36)}
-LINEAR_BACKWARD = {"64x64/3": (130, 9, 12, 34), "128x128/2": (103, 112, 14, 74), "128x128/4": (101, 21, 12, 446), "256x128/3": (4599, 96, 202, 78), "256x256/2": (3277, 30, 134, 986)}
-GATED_BACKWARD = {"64x64/3": (130, 9, 11, 34), "128x128/2": (103, 112, 13, 74), "128x128/4": (101, 21, 11, 446), "256x128/3": (3520, 105, 113, 82), "256x256/2": (4001, 13, 1130, 1026)}
+LINEAR_BACKWARD = {"64x64/3": (130, 9, 12, 34), "128x128/2": (103, 112, 14, 74), "128x128/4": (101, 21, 12, 446), "256x128/3": (4599, 96, 202, 78), "256x256/2": (3277, 30, 134, 986),
+                   "64x64/3 split": (1125, 1, 12, 34), "128x128/2 split": (12152, 4, 10, 38), "128x128/4 split": (6115, 3, 12, 74), "256x128/3 split": (11936, 1, 1416, 66), "256x256/2 split": (20158, 1, 132, 2098)}
+GATED_BACKWARD = {"64x64/3": (130, 9, 11, 34), "128x128/2": (103, 112, 13, 74), "128x128/4": (101, 21, 11, 446), "256x128/3": (3520, 105, 113, 82), "256x256/2": (4001, 13, 1130, 1026),
+                  "64x64/3 split": (1125, 1, 11, 34), "128x128/2 split": (12152, 4, 9, 38), "128x128/4 split": (6115, 3, 11, 74), "256x128/3 split": (13090, 1, 787, 74), "256x256/2 split": (23260, 1, 99, 1134)}
 # (M, N, K): k in several chunks of LDS and behind their last whole unit
 FOUR_BIT = {"few 1 8": (5, 100, 4330), "few 1 4": (9, 4203, 330), "few 2 8": (20, 100, 2330), "few 2 4": (31, 4203, 331), "few 2 2": (17, 8301, 200), "few 4 8": (50, 100, 2330), "few 4 4": (64, 4203, 130),
             "few 4 2": (33, 8301, 1290), "few 4 8, in parts": (130, 100, 500), "widened": (3001, 700, 1333)}
 FOUR_BIT_GATED = {"few 1 8": (5, 100, 4330), "few 1 4": (9, 4203, 330), "few 2 8": (20, 100, 2330), "few 2 4": (31, 4203, 331), "few 4 8": (50, 100, 2330), "few 4 4": (64, 8301, 130), "widened": (3001, 700, 1333)}
 # tokens, experts, k
-ROUTES = [(tokens, count, k) for tokens in (9, 300) for count, k in ((9, 2), (25, 3), (50, 16), (120, 4), (250, 4), (900, 3))]
+ROUTES = [(tokens, count, k) for tokens in (9, 300) for count, k in ((9, 2), (25, 3), (50, 16), (120, 4), (250, 4), (500, 5), (900, 3))]
 
 
 def sizes(table):
@@ -49,6 +51,7 @@ def described():
         elif bits: parts.append("few %%s %%s" %% bits.groups())
         elif "widen" in k and "widened" not in parts: parts.append("widened")
         elif c and "tgroups" in k: parts.append("%%sx%%s/%%s" %% c[0])
+        elif "weights_finish" in k: parts[-1] += " split"
     return ", ".join(parts)
 tables = json.loads(%r)
 def say(kind, table, call):

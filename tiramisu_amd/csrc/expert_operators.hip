@@ -36,14 +36,18 @@ void by_experts(int experts, F f) {
     else if (experts <= 32) f(std::integral_constant<int, 16>(), std::integral_constant<int, 2>());
     else if (experts <= 64) f(std::integral_constant<int, 16>(), std::integral_constant<int, 4>());
     else if (experts <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
-    else if (experts <= 256) f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    else if (experts <= 256) f(std::integral_constant<int, 16>(), std::integral_constant<int, 16>());
+    else if (experts <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
     else f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
 }
 
-constexpr long ROUTE_FEW = 256;             // tokens that one workgroup routes
+// Tokens that one workgroup routes; with more, blocks of tokens do, in two launches (us as one / as blocks, 8 of 64 experts: 32 tokens 5.7 / 9.5, 64 7.7 / 10.0, 128 12.9 / 10.1; of 600, a wavefront to a
+// token: 16 tokens 14 / 16, 32 24 / 16.5).
+long experts_lanes(int experts) { return experts <= 256 ? 16 : 64; }
+long route_few(int experts) { return experts_lanes(experts) == 16 ? 80 : 24; }
 template <int E>
 int route(const char *fn, route_arguments a) {
-    if (a.tokens <= ROUTE_FEW) {
+    if (a.tokens <= route_few(a.experts)) {
         const size_t lds = troute::route_lds_bytes(a.experts, ROUTE_FEW_THREADS);
         by_experts(a.experts, [&](auto lanes, auto values) {
             hipLaunchKernelGGL((troute::route_few_kernel<E, decltype(lanes)::value, decltype(values)::value>), dim3(1), dim3(ROUTE_FEW_THREADS), lds, stream(), a);
@@ -52,7 +56,7 @@ int route(const char *fn, route_arguments a) {
         return 0;
     }
     const size_t lds = troute::route_lds_bytes(a.experts, ROUTE_THREADS);
-    a.block = (int)std::max(64L, (a.tokens + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
+    a.block = (int)std::max(experts_lanes(a.experts) == 16 ? 64L : 16L, (a.tokens + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
     const unsigned blocks = (unsigned)((a.tokens + a.block - 1) / a.block);
     call_scratch s;
     const uint64_t counts = s.want((uint64_t)blocks * a.experts * 4);
@@ -113,24 +117,45 @@ product_tile grouped_tile(const grouped_arguments &a, int bytes, bool gated) {
     return best;
 }
 // Both gradients: as one launch of as many tiles as they have together, whose slices are theirs in the mean; where there are few rounds, those of a group of twice the
-// mean's rows, whose tiles the launch waits for (6720 rows in 14 groups, 140 x 1053: 256 x 256 tiles 45 us, 128 x 128 34).
-product_tile gradients_tile(const grouped_arguments &a, const grouped_arguments &b, int pairs) {
-    product_tile best = TILE_64;
+// mean's rows, whose tiles the launch waits for (6720 rows in 14 groups, 140 x 1053: 256 x 256 tiles 45 us, 128 x 128 34).  The terms of the weights' tiles may be shared by several workgroups, whose
+// sums, written and read again at 5 TB/s, a launch more adds (14252 rows in 3 groups, 192 x 103: 50 us, so 28).
+struct gradients_plan { product_tile tile; int splits; };
+gradients_plan plan_gradients(const grouped_arguments &a, const grouped_arguments &b, int pairs) {
+    gradients_plan best = {TILE_64, 1};
     double best_cost = 0;
-    for (const auto &t : GROUPED_TILES) {
-        const double down = a.p.y ? rows_tiles(a, t.rows, t.columns, false) : 0, across = b.p.y ? (double)((b.p.M + t.rows - 1L) / t.rows) * ((b.p.N + t.columns - 1L) / t.columns) * b.groups : 0;
-        const double of_rows = pairs * ((a.p.K + 63) / 64), of_weights = (double)b.rows / b.groups / 64, tiles = std::max(1.0, down + across);
-        double slices = (down * of_rows + across * (of_weights + 0.5)) / tiles;
-        if (tiles <= 2 * ttarget::COMPUTE_UNITS) slices = std::max(slices, std::max(down ? of_rows : 0.0, across ? 2 * of_weights : 0.0));
-        const double cost = t.factor * tile_launch_cost(t.tile, (long)tiles, std::max(1L, (long)(slices + 0.5)), 2, false);
-        if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
-    }
+    for (const auto &t : GROUPED_TILES)
+        for (int splits = 1; splits <= 16; splits *= 2) {
+            const double of_rows = pairs * ((a.p.K + 63) / 64), of_weights = (double)b.rows / b.groups / 64 / splits;
+            const double down = a.p.y ? rows_tiles(a, t.rows, t.columns, false) : 0;
+            const double across = b.p.y ? (double)((b.p.M + t.rows - 1L) / t.rows) * ((b.p.N + t.columns - 1L) / t.columns) * b.groups * splits : 0, tiles = std::max(1.0, down + across);
+            if (splits > 1 && (!b.p.y || of_weights < 2.0 || tiles > 4 * ttarget::COMPUTE_UNITS)) break;
+            double slices = (down * of_rows + across * (of_weights + 0.5)) / tiles;
+            if (tiles <= 2 * ttarget::COMPUTE_UNITS) slices = std::max(slices, std::max(down ? of_rows : 0.0, across ? 2 * of_weights : 0.0));
+            double cost = t.factor * tile_launch_cost(t.tile, (long)tiles, std::max(1L, (long)(slices + 0.5)), 2, false);
+            if (splits > 1) cost += 4.0 + 2.0 * splits * b.groups * b.p.M * b.p.N * 4 / 5e6;
+            if (best_cost == 0 || cost < best_cost) { best = {t.tile, splits}; best_cost = cost; }
+        }
     return best;
 }
-void launch_gradients(int type, const grouped_arguments &a, const grouped_arguments &b, int pairs) {
+struct planned_gradients {
+    gradients_plan plan;
+    uint64_t partial;
+};
+planned_gradients plan_gradients(grouped_arguments &a, grouped_arguments &b, int pairs, call_scratch &s) {
+    planned_gradients g = {plan_gradients(a, b, pairs), call_scratch::NOWHERE};
+    b.splits = g.plan.splits;
+    if (b.splits > 1) g.partial = s.want((uint64_t)b.splits * b.groups * b.p.M * b.p.N * 4);
+    return g;
+}
+void launch_gradients(const char *fn, int type, const planned_gradients &g, const grouped_arguments &a, grouped_arguments &b, const call_scratch &s) {
     if (!a.p.y && !b.p.y) return;
-    const product_tile tile = gradients_tile(a, b, pairs);
-    (type == BF16 ? tgroups::launch_grouped_gradients_BF16 : tgroups::launch_grouped_gradients_F16)(tile, a, b, stream());
+    b.p.partial = (float *)s.at(g.partial);
+    (type == BF16 ? tgroups::launch_grouped_gradients_BF16 : tgroups::launch_grouped_gradients_F16)(g.plan.tile, a, b, stream());
+    if (b.splits == 1) return;
+    const unsigned blocks = (unsigned)(((b.p.N + 7L) / 8 * b.p.M * b.groups + 255) / 256);
+    if (type == BF16) hipLaunchKernelGGL(tgroups::grouped_weights_finish_kernel<BF16>, dim3(blocks), dim3(256), 0, stream(), b);
+    else hipLaunchKernelGGL(tgroups::grouped_weights_finish_kernel<F16>, dim3(blocks), dim3(256), 0, stream(), b);
+    check(hipGetLastError(), fn);
 }
 
 template <int E, int Y, int EPILOGUE>
@@ -160,55 +185,68 @@ void launch_few(const char *fn, int type, int y, const grouped_arguments &a) {
 
 // (rows are picked at offsets of 31 bits)
 bool can_pick(const operand &x, long rows, long columns, int bytes) { return rows > 0 && loadable(x, bytes, true) && ((rows - 1) * x.ld + columns) * bytes < 0x7ffffff0L; }
-// Rows of x in the groups' order, where a product cannot pick them itself
-struct planned_rows {
-    const void *x;
-    const int *index;
-    long ldx, rows, tokens, columns;
-    int bytes;
-    uint64_t place;
-    long ld;
-};
-planned_rows plan_rows(const void *x, const int *index, long ldx, long rows, long tokens, long columns, int bytes, call_scratch &s) {
-    planned_rows q = {x, index, ldx, rows, tokens, columns, bytes, call_scratch::NOWHERE, (columns * bytes + 15) / 16 * 16 / bytes};
-    if (rows > 0 && columns > 0) q.place = s.want((uint64_t)q.ld * bytes * rows);
-    return q;
-}
-const void *settle_rows(const char *fn, const planned_rows &q, const call_scratch &s) {
-    if (q.place == call_scratch::NOWHERE) return q.x;
-    char *out = (char *)s.at(q.place);
-    const long to = q.ld * q.bytes;
-    for (long first = 0, most = std::max(1L, MOST_PIECES_A_LAUNCH / (to / 16)); first < q.rows; first += most) {
-        const long n = std::min(most, q.rows - first);
-        auto kernel = q.bytes == 1 ? tgroups::pick_rows_kernel<1> : tgroups::pick_rows_kernel<2>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((to / 16 * n + 255) / 256)), dim3(256), 0, stream(), (const char *)q.x, out + first * to, q.index + first, n, q.tokens, q.columns * q.bytes,
-                           q.ldx * q.bytes, to);
-    }
-    check(hipGetLastError(), fn);
-    return out;
-}
 
+// Operands that have to be moved ahead of a call's product: up to three, all in one launch (gated gradients at odd sizes had five launches, so three: 552 rows in 29 groups, 443 x 131, 28 -> 23 us).
+class operand_moves {
+public:
+    explicit operand_moves(int bytes_) : bytes(bytes_) {}
+    // An operand in its order: its address, and where it has to be moved what will be there
+    const void *settle(const placed_operand &q, const call_scratch &s) {
+        if (q.place == call_scratch::NOWHERE) return q.from.p;
+        return add({(const char *)q.from.p, (char *)s.at(q.place), nullptr, q.rows, q.rows, q.columns * bytes, q.from.ld * bytes, q.ld * bytes});
+    }
+    // Rows of x in the groups' order
+    const void *settle(const void *x, const int *index, long ldx, long tokens, long rows, long columns, long ld, uint64_t place, const call_scratch &s) {
+        return add({(const char *)x, (char *)s.at(place), index, rows, tokens, columns * bytes, ldx * bytes, ld * bytes});
+    }
+    void launch(const char *fn) const {
+        if (count == 0) return;
+        long blocks = 1;
+        for (int i = 0; i < count; i++) blocks = std::max(blocks, (moves.of[i].to / 16 * moves.of[i].rows + 255) / 256);
+        auto kernel = bytes == 1 ? tgroups::move_operands_kernel<1> : tgroups::move_operands_kernel<2>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(blocks, 1L << 20), (unsigned)count), dim3(256), 0, stream(), moves);
+        check(hipGetLastError(), fn);
+    }
+
+private:
+    const void *add(const tgroups::row_move &m) {
+        moves.of[count++] = m;
+        return m.out;
+    }
+    int bytes, count = 0;
+    tgroups::row_moves moves = {};
+};
+// Rows of x where a product cannot pick them itself: a place for them, rows at multiples of 16 bytes
+struct planned_rows { uint64_t place; long ld; };
+planned_rows plan_rows(long rows, long columns, int bytes, call_scratch &s) {
+    const long ld = (columns * bytes + 15) / 16 * 16 / bytes;
+    return {rows > 0 && columns > 0 ? s.want((uint64_t)ld * bytes * rows) : call_scratch::NOWHERE, ld};
+}
 // Rows of x as the gradient of the weights takes them, down whose columns k runs: picked there, or moved
 struct planned_weight_rows {
+    const void *x;
+    const int *rows;
+    long ldx, places, tokens, columns;
+    bool pick;
     planned_rows moved;
     placed_operand in_order;
-    const int *index;
-    long tokens;
 };
 planned_weight_rows plan_weight_rows(const void *x, const int *rows, long ldx, long S, long T, long K, call_scratch &s) {
-    planned_weight_rows q = {};
-    q.moved.place = q.in_order.place = call_scratch::NOWHERE;
-    q.tokens = T;
-    q.index = rows && can_pick({x, ldx}, T, K, 2) && ldx <= MOST_STEP ? rows : nullptr;
-    if (rows && !q.index) q.moved = plan_rows(x, rows, ldx, S, T, K, 2, s);
+    planned_weight_rows q = {x, rows, ldx, S, T, K, rows && can_pick({x, ldx}, T, K, 2) && ldx <= MOST_STEP, {call_scratch::NOWHERE, 0}, {}};
+    q.in_order.place = call_scratch::NOWHERE;
+    if (rows && !q.pick) q.moved = plan_rows(S, K, 2, s);
     else q.in_order = place_operand({x, ldx}, rows ? 0 : S, K, 2, false, s);
     return q;
 }
-void settle_weight_rows(const char *fn, const planned_weight_rows &q, grouped_arguments &b, const call_scratch &s) {
-    const bool moved = q.moved.place != call_scratch::NOWHERE;
-    b.p.b = moved ? settle_rows(fn, q.moved, s) : settle(fn, q.in_order, s);
-    b.p.ldb = moved ? q.moved.ld : q.in_order.ld;
-    if (q.index) b.picked = {q.index, q.tokens};
+void settle_weight_rows(const planned_weight_rows &q, grouped_arguments &b, operand_moves &moves, const call_scratch &s) {
+    if (q.moved.place != call_scratch::NOWHERE) {
+        b.p.b = moves.settle(q.x, q.rows, q.ldx, q.tokens, q.places, q.columns, q.moved.ld, q.moved.place, s);
+        b.p.ldb = q.moved.ld;
+        return;
+    }
+    b.p.b = moves.settle(q.in_order, s);
+    b.p.ldb = q.in_order.ld;
+    if (q.pick) b.picked = {q.rows, q.tokens};
 }
 
 // Rows that a group has in the mean, up to which wavefronts that load weights straight into registers are faster than tiles, which read each weight once for all rows of a group (us as
@@ -230,16 +268,17 @@ int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_argum
     call_scratch s;
     const operand x = {a.p.a, a.p.lda};
     const bool pick = rows && can_pick(x, tokens, K, bytes);
-    planned_rows moved = {};
+    planned_rows moved = {call_scratch::NOWHERE, 0};
     placed_operand in_order = {};
-    moved.place = in_order.place = call_scratch::NOWHERE;
-    if (rows && !pick) moved = plan_rows(a.p.a, rows, a.p.lda, a.rows, tokens, K, bytes, s);
+    in_order.place = call_scratch::NOWHERE;
+    if (rows && !pick) moved = plan_rows(a.rows, K, bytes, s);
     else if (!rows) in_order = place_operand(x, a.rows, K, bytes, true, s);
     const uint64_t scales = rows && !pick && a.p.a_scale ? s.want((uint64_t)a.rows * 4) : call_scratch::NOWHERE;
     const placed_operand b = place_operand({a.p.b, a.p.ldb}, all, K, bytes, true, s), b2 = place_operand({a.p.b2, a.p.ldb2}, gated ? all : 0, K, bytes, true, s);
     if (s.take(fn)) return 1;
+    operand_moves moves(bytes);
     if (rows && !pick) {
-        a.p.a = settle_rows(fn, moved, s);
+        if (moved.place != call_scratch::NOWHERE) a.p.a = moves.settle(a.p.a, rows, a.p.lda, tokens, a.rows, K, moved.ld, moved.place, s);
         a.p.lda = moved.ld;
         a.picked = {nullptr, a.rows};
         if (a.p.a_scale) {
@@ -248,11 +287,12 @@ int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_argum
             a.p.a_scale = (const float *)s.at(scales);
         }
     } else if (!rows) {
-        a.p.a = settle(fn, in_order, s);
+        a.p.a = moves.settle(in_order, s);
         a.p.lda = in_order.ld;
     }
-    a.p.b = settle(fn, b, s);
-    a.p.b2 = settle(fn, b2, s);
+    a.p.b = moves.settle(b, s);
+    a.p.b2 = moves.settle(b2, s);
+    moves.launch(fn);
     a.p.ldb = b.ld;
     a.p.ldb2 = b2.ld;
     a.b_step = (long)a.p.N * b.ld;
@@ -268,6 +308,7 @@ grouped_arguments grouped_of(uint64_t S, uint64_t groups, uint64_t N, uint64_t K
     a.offsets = offsets;
     a.groups = (int)groups;
     a.rows = (int)S;
+    a.splits = 1;
     return a;
 }
 
@@ -292,12 +333,12 @@ int four_bit_split(long M, long N, bool gated) {
     const long tiles = (N + FEW_ROWS - 1) / FEW_ROWS * ((M + 63) / 64);
     return tiles <= ttarget::COMPUTE_UNITS ? 8 : gated || M <= 16 || tiles <= 2 * ttarget::COMPUTE_UNITS ? 4 : 2;
 }
-// What the kernel of few tokens takes, for every round of its workgroups the bytes of x and weights at what a compute unit takes in, and what widening the weights ahead of a product on tiles
+// What the kernel of few tokens takes, for every round of its workgroups a beginning and an end and the bytes of x and weights at what a compute unit takes in, and what widening the weights ahead of a product on tiles
 // does, in microseconds (few / widened: 4096 x 4096 with 128, 256 and 512 tokens 16 / 32, 21 / 37, 39 / 38; gated 8192 x 2048 with 128 and 256 23 / 45, 44 / 47).
 double four_bit_few_cost(long M, long N, long K, bool gated) {
     const long teams = FEW_WAVES / four_bit_split(M, N, gated), workgroups = (N + FEW_ROWS * teams - 1) / (FEW_ROWS * teams) * ((M + 63) / 64);
     const double rounds = (double)((workgroups + ttarget::COMPUTE_UNITS - 1) / ttarget::COMPUTE_UNITS);
-    return 3.0 + rounds * (double)K * (2.0 * std::min(M, 64L) + 8.5 * (double)teams * (gated ? 2 : 1)) / 33e3;
+    return 3.0 + (rounds - 1) * 4.0 + rounds * (double)K * (2.0 * std::min(M, 64L) + 8.5 * (double)teams * (gated ? 2 : 1)) / 33e3;
 }
 double four_bit_widened_cost(const planned_forward &f, long N, long K, bool gated) { return 7.0 + (gated ? 2.0 : 1.0) * N * K * 2.53 / 5e6 + f.q.plan.cost; }
 template <int E, int EPILOGUE, int TILES, int SPLIT>
@@ -446,26 +487,22 @@ int tiramisu_hip_grouped_linear_backward(const void *dy, const void *x, const vo
     const placed_operand w = place_operand({weight, ldw ? (long)ldw : (long)K}, dx && S ? (long)(N * groups) : 0, (long)K, 2, false, s);
     const bool gradient = dweight && N > 0;
     const planned_weight_rows xs = plan_weight_rows(x, rows, ldx ? (long)ldx : (long)K, gradient ? (long)S : 0, (long)T, (long)K, s);
-    if (s.take(__FUNCTION__)) return 1;
-    const void *at = settle(__FUNCTION__, d, s);
     grouped_arguments a = grouped_of(S, groups, K, N, offsets), b = grouped_of(N, groups, K, 0, offsets);
-    if (dx && S > 0) {
-        a.p.a = at;
-        a.p.lda = d.ld;
-        a.p.b = settle(__FUNCTION__, w, s);
-        a.p.ldb = w.ld;
-        a.b_step = (long)N * w.ld;
-        a.p.y = dx;
-    }
-    if (gradient) {
-        b.rows = (int)S;
-        b.p.a = at;
-        b.p.lda = d.ld;
-        settle_weight_rows(__FUNCTION__, xs, b, s);
-        b.p.y = dweight;
-        b.y_step = (long)N * (long)K;
-    }
-    launch_gradients(type, a, b, 1);
+    a.p.y = S > 0 ? dx : nullptr;
+    b.p.y = gradient ? dweight : nullptr;
+    b.rows = (int)S;
+    const planned_gradients g = plan_gradients(a, b, 1, s);
+    if (s.take(__FUNCTION__)) return 1;
+    operand_moves moves(2);
+    a.p.a = b.p.a = moves.settle(d, s);
+    a.p.lda = b.p.lda = d.ld;
+    a.p.b = moves.settle(w, s);
+    a.p.ldb = w.ld;
+    a.b_step = (long)N * w.ld;
+    settle_weight_rows(xs, b, moves, s);
+    b.y_step = (long)N * (long)K;
+    moves.launch(__FUNCTION__);
+    launch_gradients(__FUNCTION__, type, g, a, b, s);
     return 0;
 }
 
@@ -490,35 +527,32 @@ int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, co
     const placed_operand wg = place_operand({gate_weight, ldg ? (long)ldg : k}, of_weights, k, 2, false, s), wu = place_operand({up_weight, ldu ? (long)ldu : k}, of_weights, k, 2, false, s);
     const bool weights = dgate_weight && n > 0;
     const planned_weight_rows xs = plan_weight_rows(x, rows, ldx ? (long)ldx : k, weights ? m : 0, (long)T, k, s);
+    // rows of the weights' product: those of gate, up to `half` nothing, those of up
+    grouped_arguments a = grouped_of(S, groups, K, N, offsets), b = grouped_of((uint64_t)(half + n), groups, K, 0, offsets);
+    a.p.y = m > 0 ? dx : nullptr;
+    b.p.y = weights ? dgate_weight : nullptr;
+    b.p.y_below = weights ? dup_weight : nullptr;
+    b.p.rows_above = (int)n;
+    b.p.split_row = (int)half;
+    b.rows = (int)m;
+    const planned_gradients g = plan_gradients(a, b, 2, s);
     if (s.take(__FUNCTION__)) return 1;
     char *const d = (char *)s.at(gradient);
     if (m > 0 && n > 0) launch_gated_gradients(__FUNCTION__, type, {dh, gate, up, d, d + 2 * half, m, n, ldh ? (long)ldh : n, ld_gate ? (long)ld_gate : n, ld_up ? (long)ld_up : n, ld, activation});
-    grouped_arguments a = grouped_of(S, groups, K, N, offsets), b = grouped_of((uint64_t)(half + n), groups, K, 0, offsets);
-    if (dx && m > 0) {
-        a.p.a = d;
-        a.p.a_more = d + 2 * half;
-        a.p.lda = ld;
-        a.p.b = settle(__FUNCTION__, wg, s);
-        a.p.b_more = settle(__FUNCTION__, wu, s);
-        a.p.ldb = wg.ld;
-        a.p.ldb_more = wu.ld;
-        a.b_step = n * wg.ld;
-        a.b2_step = n * wu.ld;
-        a.p.y = dx;
-    }
-    if (weights) {
-        // rows of the product: those of gate, up to `half` nothing, those of up
-        b.rows = (int)m;
-        b.p.rows_above = (int)n;
-        b.p.split_row = (int)half;
-        b.p.a = d;
-        b.p.lda = ld;
-        settle_weight_rows(__FUNCTION__, xs, b, s);
-        b.p.y = dgate_weight;
-        b.p.y_below = dup_weight;
-        b.y_step = n * k;
-    }
-    launch_gradients(type, a, b, 2);
+    operand_moves moves(2);
+    a.p.a = b.p.a = d;
+    a.p.a_more = d + 2 * half;
+    a.p.lda = b.p.lda = ld;
+    a.p.b = moves.settle(wg, s);
+    a.p.b_more = moves.settle(wu, s);
+    a.p.ldb = wg.ld;
+    a.p.ldb_more = wu.ld;
+    a.b_step = n * wg.ld;
+    a.b2_step = n * wu.ld;
+    settle_weight_rows(xs, b, moves, s);
+    b.y_step = n * k;
+    moves.launch(__FUNCTION__);
+    launch_gradients(__FUNCTION__, type, g, a, b, s);
     return 0;
 }
 
@@ -553,7 +587,7 @@ int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int3
     timed record(__FUNCTION__);
     const long n = (long)columns;
     const bool wide = n > 256;
-    const long choices = wide ? 4 : 16, choice_blocks = ((long)tokens * (long)k + choices - 1) / choices, blocks = choice_blocks + (dx && n ? ((long)rows + 255) / 256 : 0);
+    const long choices = wide ? 4 : 16, choice_blocks = ((long)tokens * (long)k + choices - 1) / choices, blocks = choice_blocks + (dx && n ? ((long)rows + 63) / 64 : 0);
     if (blocks == 0) return 0;
     const tcombine::combine_backward_arguments a = {dy, x, places, owners, weights, n ? dx : nullptr, dweights, (long)tokens, (long)rows, n, ldy ? (long)ldy : n, ldx ? (long)ldx : n, (int)k, choice_blocks};
     auto kernel = type == F16 ? (wide ? tcombine::combine_backward_kernel<F16, 64> : tcombine::combine_backward_kernel<F16, 16>)

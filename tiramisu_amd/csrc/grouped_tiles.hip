@@ -25,7 +25,7 @@ template <class C>
 long tiles_of(const grouped_arguments &a) {
     const long across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
     if (C::A_ROWS) return most_row_tiles(a.rows, a.groups, C::BM) * across;
-    return ((a.p.M + C::BM - 1L) / C::BM * across + XCDS - 1) / XCDS * XCDS * a.groups;
+    return ((a.p.M + C::BM - 1L) / C::BM * across + XCDS - 1) / XCDS * XCDS * a.groups * a.splits;
 }
 template <class C, class D, int Y>
 void launch(const grouped_arguments &a, hipStream_t stream) {

@@ -82,13 +82,14 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(combine_backward_
     typedef stored<E> T;
     const int lane = threadIdx.x & 63, at = threadIdx.x % LANES;
     if ((long)blockIdx.x >= a.choice_blocks) {
-        // 64 rows to a wavefront, whose lanes read their owners at once
-        const long first = (((long)blockIdx.x - a.choice_blocks) * 4 + threadIdx.x / 64) * 64, s = first + lane;
+        // 16 rows to a wavefront, whose lanes read their owners at once; LANES to a row
+        const long first = (((long)blockIdx.x - a.choice_blocks) * 4 + threadIdx.x / 64) * 16, s = first + lane % 16;
         const int owner = s < a.rows ? a.owners[s] : 0;
-        for (unsigned long long none = __ballot(s < a.rows && (owner < 0 || owner >= a.tokens)); none; none &= none - 1) {
-            const long row = first + __builtin_ctzll(none);
+        const bool none = s < a.rows && (owner < 0 || owner >= a.tokens);
+        for (int i = lane / LANES; i < 16; i += 64 / LANES) {
             const float zeros[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (long n = 8 * lane; n < a.columns; n += 512) store_some<E>((T *)a.dx + row * a.columns + n, (int)min(8L, a.columns - n), zeros);
+            if (!__shfl((int)none, i)) continue;
+            for (long n = 8 * at; n < a.columns; n += 8 * LANES) store_some<E>((T *)a.dx + (first + i) * a.columns + n, (int)min(8L, a.columns - n), zeros);
         }
         return;
     }

@@ -21,6 +21,7 @@ struct grouped_arguments {
     picked_rows picked;                     // forward: x's rows (index null: x holds the grouped rows themselves)
     long b_step, b2_step;                   // elements from group to group of the weights (input's gradient, gated: b2 is the second pair's)
     long y_step;                            // gradient of the weights: elements from group to group of the result
+    int splits;                             // ... workgroups that share the terms of a tile: sums to p.partial, [group][split][M][N]
 };
 
 struct group_span { int first, rows; };
@@ -130,20 +131,25 @@ __device__ __forceinline__ void rows_tile(const grouped_arguments &a, int id, ld
 template <class C, int Y>
 __device__ __forceinline__ void weights_tile(const grouped_arguments &a, int id, lds_char *lds) {
     const int down = (a.p.M + C::BM - 1) / C::BM, across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS, tiles = down * across, each = (tiles + XCDS - 1) / XCDS;
-    const int group = id / XCDS / each, tile = (id + group) % XCDS * each + id / XCDS % each;
+    const int split = id / (XCDS * each * a.groups), in = id - split * XCDS * each * a.groups;
+    const int group = in / XCDS / each, tile = (in + group) % XCDS * each + in / XCDS % each;
     if (tile >= tiles) return;
     const group_span s = span_of(a.offsets, group, a.rows);
     product_arguments p = a.p;
     const long first = uniform(s.first), g = group;
     p.K = uniform(s.rows);
+    if (a.splits > 1) {
+        p.partial += g * a.splits * p.M * p.N;
+        p.slices_per_split = ((p.K + 63) / 64 + a.splits - 1) / a.splits;
+    }
     p.a = (const char *)p.a + first * p.lda * C::BYTES;
     p.y = (char *)p.y + g * a.y_step * 2;
     if (p.y_below) p.y_below = (char *)p.y_below + g * a.y_step * 2;
     int row, column;
     tile_in_bands(tile, down, across, row, column);
-    if (a.picked.index) return compute_tile_at<C, Y, K_OF_B>(p, row, column, 0, lds, {a.picked.index + first, a.picked.all});
+    if (a.picked.index) return compute_tile_at<C, Y, K_OF_B>(p, row, column, split, lds, {a.picked.index + first, a.picked.all});
     p.b = (const char *)p.b + first * p.ldb * C::BYTES;
-    compute_tile_at<C, Y>(p, row, column, 0, lds);
+    compute_tile_at<C, Y>(p, row, column, split, lds);
 }
 #endif
 
@@ -209,16 +215,44 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void grouped_few_kernel(grouped_arg
     }
 }
 
-// Rows that an index picks, `across` pieces of 16 bytes each, to rows `to` bytes apart: where the tiles cannot pick them themselves.  One that is none of x's is zero.
-template <int BYTES>
-__global__ __launch_bounds__(256) void pick_rows_kernel(const char *in, char *out, const int *index, long rows, long all, long bytes, long from, long to) {
-    const long across = to / 16, id = (long)blockIdx.x * 256 + threadIdx.x;
-    if (id >= across * rows) return;
-    const long m = id / across, c = 16 * (id - m * across), row = index[m];
-    u32x4 w = {0, 0, 0, 0};
-    if (row >= 0 && row < all) w = load_guarded<BYTES>(in + row * from + c, bytes - c);
-    *reinterpret_cast<u32x4 *>(out + m * to + c) = w;
+// The sums of the gradient of the weights, added in order: 8 columns of a row of a group to a thread
+template <int Y>
+__global__ __launch_bounds__(256) void grouped_weights_finish_kernel(grouped_arguments a) {
+    const long across = (a.p.N + 7) / 8, id = (long)blockIdx.x * 256 + threadIdx.x, all = across * a.p.M;
+    if (id >= all * a.groups) return;
+    const long g = id / all, m = (id - g * all) / across, n = 8 * (id - g * all - m * across);
+    const int some = (int)min(8L, a.p.N - n);
+    product_arguments p = a.p;
+    p.y = (char *)p.y + g * a.y_step * 2;
+    if (p.y_below) p.y_below = (char *)p.y_below + g * a.y_step * 2;
+    float z[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) z[i] = 0.f;
+    for (int s = 0; s < a.splits; s++) {
+        float v[8];
+        load_some<F32>(p.partial + ((g * a.splits + s) * p.M + m) * p.N + n, some, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] += v[i];
+    }
+    store_linear<Y, true>(p, z, m, n, some);
 }
+
+// Rows to where the tiles can load them, 16 bytes at a time, `to` bytes apart (a multiple of 16; the rest of a row is zero): in their order, or those that an index picks, zeros where it picks
+// none of x's.  Up to three operands in one launch, blockIdx.y.
+struct row_move { const char *in; char *out; const int *index; long rows, all, bytes, from, to; };
+struct row_moves { row_move of[3]; };
+template <int BYTES>
+__global__ __launch_bounds__(256) void move_operands_kernel(row_moves moves) {
+    const row_move m = moves.of[blockIdx.y];
+    const long across = m.to / 16, all = across * m.rows;
+    for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < all; id += (long)gridDim.x * 256) {
+        const long r = id / across, c = 16 * (id - r * across), row = m.index ? m.index[r] : r;
+        u32x4 w = {0, 0, 0, 0};
+        if (row >= 0 && row < m.all) w = load_to_end<BYTES>(m.in + row * m.from + c, m.bytes - c, m.bytes);
+        *reinterpret_cast<u32x4 *>(m.out + r * m.to + c) = w;
+    }
+}
+
 // ... and their scales
 static __global__ __launch_bounds__(256) void pick_scales_kernel(const float *in, float *out, const int *index, long rows, long all) {
     const long m = (long)blockIdx.x * 256 + threadIdx.x;

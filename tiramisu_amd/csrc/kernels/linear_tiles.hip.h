@@ -508,7 +508,7 @@ __device__ __forceinline__ void tile_of(int id, int rows, int columns, int &row,
 
 #ifdef __HIP_DEVICE_COMPILE__               // (the host's compilation needs no body, and rejects a second one of the same configuration)
 // The tile of the product in this row and column of tiles, of part `split` of k.  Y: type of bias, residual and outputs.  ROWS_OF_A: rows of A may be
-// picked by an index, and their scales with them; K_OF_B: the rows of B are, of a whole product.
+// picked by an index, and their scales with them; K_OF_B: the rows of B are.
 template <class C, int Y, int PICK = NOTHING>
 __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int row, int column, int split, lds_char *lds, picked_rows picked = {nullptr, 0}) {
     constexpr bool PICKED = PICK == ROWS_OF_A;
@@ -552,8 +552,8 @@ __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int 
     if constexpr (PICK == K_OF_B) {
         // the index of PICKS terms at a time, behind the ring
         __attribute__((address_space(3))) int *const list = (__attribute__((address_space(3))) int *)(lds + C::STAGES * C::STAGE);
-        for (long from = 0; from < K; from += PICKS) {
-            const int some = (int)min((long)PICKS, K - from);
+        for (long from = k0; from < k0 + K; from += PICKS) {
+            const int some = (int)min((long)PICKS, k0 + K - from);
             for (int i = threadIdx.x; i < some; i += C::NT) list[i] = picked.index[from + i];
             __syncthreads();
             accumulate<C, K_OF_B>(acc, (const char *)p.a + from * p.lda * C::BYTES, p.lda, p.b, p.ldb, nullptr, 0, p.M, p.N, m0, n0, 0, some, lds, picked, list);

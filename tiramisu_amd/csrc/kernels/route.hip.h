@@ -2,8 +2,8 @@
 //
 // LANES lanes of a wavefront hold the logits of a token, VALUES neighbouring ones each, as whole numbers that order them (zeros of either sign alike, NaN above
 // everything).  A choice is the largest number over the lanes and then the lowest index that holds it.  Chosen
-// ones become the least number; minus infinity is never chosen.  Sixteen lanes are one row of the cross-lane network, so that up to 128 experts take four tokens a wavefront
-// without a word through LDS.
+// ones become the least number; minus infinity is never chosen.  Sixteen lanes are one row of the cross-lane network, so that up to 256 experts take four tokens a wavefront
+// without a word through LDS (200 experts, 16384 tokens: 29.8 us with a wavefront to a token, so 20).
 //
 // Places are counted, without atomics whose order could be seen: assignments, in order of token and rank, are the experts' in the order that they come.  Blocks of
 // tokens count theirs while they choose; the second kernel adds the blocks before its own and ranks its own by ballots (a wavefront's lanes of one expert) and by
@@ -43,7 +43,7 @@ __device__ __forceinline__ float number_of(uint32_t o) {
 }
 constexpr uint32_t LEAST = 0x007fffffu;     // of minus infinity
 
-// f over the LANES consecutive lanes that a lane belongs to, in each of them: within a row of 16 by turns of the cross-lane network, across rows through LDS
+// f over the LANES consecutive lanes that a lane belongs to, in each of them: within a row of 16 by turns of the cross-lane network, across rows by scalars
 template <int LANES, class F, class T>
 __device__ __forceinline__ T over_lanes(T v, F f) {
     static_assert(sizeof(T) == 4 && (LANES == 16 || LANES == 64), "rows of 16 lanes");
@@ -55,8 +55,8 @@ __device__ __forceinline__ T over_lanes(T v, F f) {
     v = f(v, turned(v, std::integral_constant<int, 2>()));
     v = f(v, turned(v, std::integral_constant<int, 1>()));
     if constexpr (LANES == 64) {
-        v = f(v, __shfl_xor(v, 16));
-        v = f(v, __shfl_xor(v, 32));
+        auto of_row = [&](int lane) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); };
+        return f(f(of_row(0), of_row(16)), f(of_row(32), of_row(48)));
     }
     return v;
 }
