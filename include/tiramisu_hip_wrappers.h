@@ -246,7 +246,8 @@ int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, co
  * the rest float16 or bfloat16. */
 int tiramisu_hip_combine_rows(const void *x, const int32_t *places, const float *weights, const void *residual, void *y, uint64_t tokens, uint64_t k, uint64_t rows, uint64_t columns,
                               uint64_t ldx, uint64_t ldr, int32_t type);
-/* dx[places[t][j]] = weights[t][j] dy[t] (each row is in `places` once at most), zeros where owners (the token of each row: tiramisu_hip_route's rows) name no token;
+/* dx[places[t][j]] = weights[t][j] dy[t] (each row is in `places` once at most), zeros where owners (the token of each row: tiramisu_hip_route's rows) name no token or one whose
+ * places have left the row out;
  * dweights[t][j] = dy[t] . x[places[t][j]].  Either may be null. */
 int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int32_t *places, const int32_t *owners, const float *weights, void *dx, float *dweights, uint64_t tokens,
                                        uint64_t k, uint64_t rows, uint64_t columns, uint64_t ldy, uint64_t ldx, int32_t type);

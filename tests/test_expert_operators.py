@@ -386,6 +386,97 @@ def test_picked_rows_beyond_2_gib():
         assert torch.equal(operators.grouped_linear_backward(dy, far, w, offsets, rows=rows).dweight, operators.grouped_linear_backward(dy, x, w, offsets, rows=rows).dweight)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("each", [1, 9])
+def test_as_many_groups_as_there_may_be(each):
+    check_grouped([each * (i % 3) for i in range(1024)], 5, 40, 72, torch.bfloat16)
+    check_grouped_backward([each * (i % 3) for i in range(1024)], 5, 40, 72, torch.bfloat16)
+
+
+def linear_bound(z, x, w):
+    return rounded(z, sum_error(x.shape[1], x.abs() @ w.abs().t()), torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_weights_beyond_4_gib():
+    """The last of 40 groups' weights begin behind 2^32 bytes, and so does its gradient."""
+    E, N = 40, 8192
+    g = generator(73)
+    w = torch.empty((E, N, N), dtype=torch.bfloat16, device="cuda")
+    w[-1] = normal((N, N), torch.bfloat16, g, N ** -0.5)
+    wd = w[-1].double()
+    for S, n in ((30, 20), (400, 130)):                   # few rows, and tiles
+        x, dy = normal((S, N), torch.bfloat16, g), normal((S, N), torch.bfloat16, g)
+        offsets = torch.full((E + 1,), S - n, dtype=torch.int32, device="cuda")
+        offsets[-1] = S
+        offsets[0] = 0
+        w[0] = 0
+        xd, dd = x[-n:].double(), dy[-n:].double()
+        z = xd @ wd.t()
+        y = operators.grouped_linear(x, w, offsets)
+        close(y[-n:], z, linear_bound(z, xd, wd), "y")
+        assert not bool(y[:-n].any())
+        got = operators.grouped_linear_backward(dy, x, w, offsets)
+        z = dd @ wd
+        close(got.dx[-n:], z, linear_bound(z, dd, wd.t()), "dx")
+        z = dd.t() @ xd
+        close(got.dweight[-1], z, linear_bound(z, dd.t(), xd.t()), "dweight")
+        assert not bool(got.dweight[1:-1].any())
+
+
+@pytest.mark.gpu
+def test_results_beyond_4_gib():
+    """Places whose rows begin behind 2^32 bytes of what is stored, kept, read again and combined."""
+    S, N, K, last = 600000, 4096, 24, 300
+    g = generator(79)
+    x, w, v = normal((S, K), torch.bfloat16, g), normal((2, N, K), torch.bfloat16, g), normal((2, N, K), torch.bfloat16, g)
+    offsets = torch.tensor([0, S - last, S], dtype=torch.int32, device="cuda")
+    xd, wd, vd = x[-last:].double(), w[1].double(), v[1].double()
+    z, u = xd @ wd.t(), xd @ vd.t()
+    y = operators.grouped_linear(x, w, offsets)
+    close(y[-last:], z, linear_bound(z, xd, wd), "y")
+    got = operators.grouped_gated_linear(x, w, v, offsets, keep_pre=True)
+    close(got.gate[-last:], z, linear_bound(z, xd, wd), "gate")
+    close(got.up[-last:], u, linear_bound(u, xd, vd), "up")
+    back = operators.grouped_linear_backward(y, x, w, offsets)
+    yd = y[-last:].double()
+    z = yd @ wd
+    close(back.dx[-last:], z, linear_bound(z, yd, wd.t()), "dx")
+    z = yd.t() @ xd
+    close(back.dweight[1], z, linear_bound(z, yd.t(), xd.t()), "dweight")
+    places = torch.arange(S - 8, S, dtype=torch.int32, device="cuda").view(4, 2)
+    weights = torch.randn((4, 2), device="cuda", generator=g)
+    sums = (y[-8:].double().view(4, 2, N) * weights.double()[..., None]).sum(1)
+    close(operators.combine(y, places, weights), sums, rounded(sums, 4 * 2.0 ** -24 * (y[-8:].double().view(4, 2, N) * weights.double()[..., None]).abs().sum(1), torch.bfloat16), "combined")
+    owners = torch.full((S,), -1, dtype=torch.int32, device="cuda")
+    owners[-8:] = torch.arange(4, device="cuda", dtype=torch.int32).repeat_interleave(2)
+    dy = normal((4, N), torch.bfloat16, g)
+    c = operators.combine_backward(dy, y, places, weights, owners)
+    z = (dy.double()[:, None] * weights.double()[..., None]).view(8, N)
+    close(c.dx[-8:], z, rounded(z, 2.0 ** -24 * z.abs(), torch.bfloat16), "combine's dx")
+    assert not bool(c.dx[:-8].any())
+
+
+@pytest.mark.gpu
+def test_terms_of_a_group_shared_by_workgroups_and_picked():
+    """The weights' gradient alone, whose workgroups each have more terms than an index in LDS holds at a time."""
+    S, T, N, K = 300000, 5000, 72, 80
+    g = generator(83)
+    dy, x = normal((S, N), torch.bfloat16, g), normal((T, K), torch.bfloat16, g)
+    rows = torch.randint(-1, T + 1, (S,), device="cuda", generator=g, dtype=torch.int32)
+    offsets = torch.tensor([0, S - 70, S - 9], dtype=torch.int32, device="cuda")
+    dweight = torch.full((2, N, K), math.nan, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    assert runtime.wrappers().tiramisu_hip_grouped_linear_backward(dy.data_ptr(), x.data_ptr(), None, offsets.data_ptr(), rows.data_ptr(), None, dweight.data_ptr(), S, T, 2, N, K, 0, 0, 0, 2) == 0
+    torch.cuda.synchronize()
+    there = (rows >= 0) & (rows < T)
+    xd, dd = torch.where(there[:, None], x.double()[rows.clamp(0, T - 1).long()], 0.0), dy.double()
+    for e, (first, end) in enumerate(((0, S - 70), (S - 70, S - 9))):
+        a, b = dd[first:end].t(), xd[first:end].t()
+        z = a @ b.t()
+        close(dweight[e], z, linear_bound(z, a, b), "dweight")
+
+
 # ---------------------------------------------------------------- combine
 
 COMBINES = [(1, 1, 1, 1), (3, 2, 7, 5), (5, 8, 64, 100), (40, 3, 1430, 130), (130, 9, 1001, 2000), (17, 20, 264, 340), (9, 4, 4100, 36), (2, 0, 40, 3)]
@@ -441,6 +532,23 @@ def test_combine_backward(tokens, k, N, places, dtype):
         if weights is not None:
             terms = torch.where(there[..., None], x.double()[at.clamp(0, places - 1).long()], 0.0) * dy.double()[:, None]
             close(got.dweights, terms.sum(2), (N + 4) * 2.0 ** -24 * terms.abs().sum(2) + 2.0 ** -140, "dweights")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [40, 1001])
+def test_choices_left_out_after_the_route(N):
+    """A choice that is dropped by -1 in `places`, with `rows` as they were: its row has a gradient of zeros."""
+    g = generator(89)
+    r = operators.route(torch.randn((150, 7), device="cuda", generator=g), 3)
+    places = r.places.masked_fill(torch.rand((150, 3), device="cuda", generator=g) < 0.3, -1)
+    x, dy = normal((450, N), torch.bfloat16, g), normal((150, N), torch.bfloat16, g)
+    dropped = torch.full((450,), True, device="cuda")
+    dropped[places[places >= 0].long()] = False
+    for _ in range(3):
+        torch.full((450, N), math.nan, device="cuda", dtype=torch.bfloat16)          # (what the allocator hands out next)
+        got = operators.combine_backward(dy, x, places, r.weights, r.rows)
+        assert not bool(got.dx[dropped].any()) and bool(torch.isfinite(got.dx.float()).all())
+        assert bool((got.dweights[places < 0] == 0).all())
 
 
 @pytest.mark.gpu
@@ -583,6 +691,66 @@ def test_calls_follow_the_work_on_a_side_stream():
 
 
 @pytest.mark.gpu
+def test_calls_on_two_streams_at_once():
+    """Eager calls with scratch (moved operands, shared terms), one stream beside the other: the results of calls on their own."""
+    cases = []
+    for seed, (S, E, N, K) in enumerate(((9000, 3, 102, 103), (4001, 2, 77, 131))):
+        g = generator(91 + seed)
+        x, w, dy = normal((S, K), torch.float16, g), normal((E, N, K), torch.float16, g, 0.1), normal((S, N), torch.float16, g)
+        offsets = torch.linspace(0, S, E + 1, device="cuda").int()
+        cases.append((dy, x, w, offsets))
+    expected = [[t.clone() for t in operators.grouped_linear_backward(*c)] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(operators.grouped_linear_backward(*cases[i]))
+    torch.cuda.synchronize()
+    for results, was in zip(got, expected):
+        for r in results:
+            assert all(torch.equal(u, v) for u, v in zip(r, was))
+
+
+@pytest.mark.gpu
+def test_shared_terms_in_a_graph():
+    g = generator(97)
+    x, w, dy = normal((14000, 103), torch.float16, g), normal((3, 192, 103), torch.float16, g, 0.1), normal((14000, 192), torch.float16, g)
+    offsets = torch.tensor([0, 5000, 9000, 14000], dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        out = operators.grouped_linear_backward(dy, x, w, offsets)
+    for ends in ([0, 14000, 14000, 14000], [0, 10, 20, 30], [0, 4000, 9001, 13000]):
+        offsets.copy_(torch.tensor(ends, dtype=torch.int32))
+        dy.copy_(normal(dy.shape, torch.float16, generator(ends[1])))
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(got, operators.grouped_linear_backward(dy, x, w, offsets)))
+
+
+@pytest.mark.gpu
+def test_calls_in_inference_mode():
+    args, dy = sublayer_inputs(40, 6, 136, 72, torch.bfloat16, 13)
+    expected = sublayer(*args, 2, dy)
+    with torch.inference_mode():
+        got = sublayer(*args, 2, dy)
+        r = operators.route(operators.linear(args[0], args[1]).y, 2)
+        assert r.weights.sum(-1).shape == (40,) and int(r.offsets[-1]) == 80
+    assert all(torch.equal(u, v) for u, v in zip(got, expected))
+    # the results of a route are tensors like others: changed in place, kept by autograd
+    r = operators.route(operators.linear(args[0], args[1]).y, 2)
+    kept = r.weights.clone()
+    scale = torch.ones(2, device="cuda", requires_grad=True)
+    (r.weights * scale).sum().backward()
+    assert torch.allclose(scale.grad, kept.sum(0), rtol=1e-5)
+    r.weights.mul_(2)
+    assert torch.equal(r.weights, kept * 2)
+
+
+@pytest.mark.gpu
 def test_launches_are_recorded_by_the_profile():
     args, dy = sublayer_inputs(4, 3, 64, 64, torch.bfloat16, 5)
     records = runtime.profile(lambda: sublayer(*args, 2, dy))
@@ -662,3 +830,12 @@ def test_what_the_c_abi_refuses(capfd):
     assert calls == [1] * len(calls)
     messages = capfd.readouterr().err.strip().splitlines()
     assert len(messages) == len(calls) and all(m.startswith("Error at tiramisu_hip_") for m in messages)
+
+
+def test_the_c_abi_refuses_sizes_that_pass_64_bits(capfd):
+    w, p = runtime.wrappers(), 4096
+    calls = [w.tiramisu_hip_grouped_gated_linear(p, p, p, p, None, None, None, None, p, None, None, 8, 8, 2, n, 8, 0, 0, 0, 4, 2, 2) for n in (1 << 63, (1 << 63) + 4, (1 << 64) - 1)]
+    calls += [w.tiramisu_hip_grouped_gated_linear_backward(p, p, p, p, p, p, p, None, p, p, p, 8, 8, 2, 1 << 63, 8, 0, 0, 0, 0, 0, 0, 4, 2), w.tiramisu_hip_grouped_linear(p, p, p, None, None, None, p, 1 << 63, 1 << 63, 2, 8, 8, 0, 0, 2, 2),
+              w.tiramisu_hip_combine_rows(p, p, None, None, p, 1 << 63, 2, 8, 8, 0, 0, 2), w.tiramisu_hip_combine_rows_backward(p, p, p, p, p, p, p, 1 << 63, 2, 8, 8, 0, 0, 2)]
+    assert calls == [1] * len(calls)
+    assert len(capfd.readouterr().err.strip().splitlines()) == len(calls)

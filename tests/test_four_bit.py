@@ -144,6 +144,21 @@ def test_operands_within_larger_tensors(M, N, K, first, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("K", [33, 97, 129, 255])
+@pytest.mark.parametrize("M", [1, 40, 200])
+def test_the_half_of_a_byte_behind_an_odd_row(M, K):
+    """It is no weight, whatever it holds: with the row's last scale it would be infinity in float16."""
+    x, (w,), _, _ = four_bit_inputs(M, 40, K, torch.float16, 59)
+    last = w.q[:, K // 32 * 16:]
+    last.zero_()
+    w.scale[:, -1] = 127 + 30
+    clean = operators.four_bit_linear(x, w.q, w.scale).y, operators.four_bit_gated_linear(x, w.q, w.q, w.scale, w.scale).h
+    last[:, -1] = 0x70
+    assert bool(torch.isfinite(clean[0]).all()) and torch.equal(operators.four_bit_linear(x, w.q, w.scale).y, clean[0])
+    assert torch.equal(operators.four_bit_gated_linear(x, w.q, w.q, w.scale, w.scale).h, clean[1])
+
+
+@pytest.mark.gpu
 def test_infinities_reach_their_own_rows_only():
     for M in (3, 50, 200):
         x, (w,), _, _ = four_bit_inputs(M, 40, 100, torch.bfloat16, 53)

@@ -446,7 +446,7 @@ int tiramisu_hip_grouped_linear(const void *x, const void *weight, const int32_t
 int tiramisu_hip_grouped_gated_linear(const void *x, const void *gate_weight, const void *up_weight, const int32_t *offsets, const int32_t *rows, const float *x_scale,
                                       const float *gate_scale, const float *up_scale, void *h, void *gate, void *up, uint64_t S, uint64_t T, uint64_t groups, uint64_t N, uint64_t K,
                                       uint64_t ldx, uint64_t ldg, uint64_t ldu, int32_t activation, int32_t type, int32_t h_type) {
-    if (const int rc = refuse_grouped(__FUNCTION__, S, T, groups, 2 * N, K, activation, type, h_type)) return rc;
+    if (const int rc = refuse_grouped(__FUNCTION__, S, T, groups, 2 * std::min(N, MOST), K, activation, type, h_type)) return rc;
     if (S == 0 || N == 0) return 0;
     if (!offsets || !h || (K && ((T && !x) || !gate_weight || !up_weight))) return refuse(__FUNCTION__, "x, both weights, offsets and h are needed");
     if (!rows && T != S) return refuse(__FUNCTION__, "%llu rows of x for %llu places", (ull)T, (ull)S);

@@ -84,8 +84,13 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(combine_backward_
     if ((long)blockIdx.x >= a.choice_blocks) {
         // 16 rows to a wavefront, whose lanes read their owners at once; LANES to a row
         const long first = (((long)blockIdx.x - a.choice_blocks) * 4 + threadIdx.x / 64) * 16, s = first + lane % 16;
-        const int owner = s < a.rows ? a.owners[s] : 0;
-        const bool none = s < a.rows && (owner < 0 || owner >= a.tokens);
+        const int owner = s < a.rows ? a.owners[s] : -1;
+        bool written = false;                              // (the four lanes of a row share its token's choices)
+        if (owner >= 0 && owner < a.tokens)
+            for (int j = lane / 16; j < a.k; j += 4) written = written || a.places[(long)owner * a.k + j] == s;
+        written = __shfl_xor((int)written, 16) || written;
+        written = __shfl_xor((int)written, 32) || written;
+        const bool none = s < a.rows && !written;
         for (int i = lane / LANES; i < 16; i += 64 / LANES) {
             const float zeros[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             if (!__shfl((int)none, i)) continue;

@@ -153,11 +153,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void four_bit_few_kernel(four_bit_a
     // behind the whole units, from memory
     if (whole * 128 < p.K && wave == whole % SPLIT) {
         const long at = whole * 64L, left = bytes - at - 16 * piece, left_x = 2L * p.K - 4 * at - 64 * piece;
+        const int weights = (int)(p.K - 2 * at) - 32 * piece;
         u32x4 fw[PARTS], fx[4][TILES];
         uint32_t exponent[PARTS];
 #pragma unroll
         for (int q = 0; q < PARTS; q++) {
             fw[q] = load_to_end<1>(w[q] + at, left, bytes);
+            // (of an odd number of weights the last byte's high half is none, whatever it holds: in float16 a large scale would make it infinity, and its product with x's zero NaN)
+#pragma unroll
+            for (int i = 0; i < 4; i++) fw[q][i] &= weights >= 8 * i + 8 ? 0xffffffffu : weights <= 8 * i ? 0u : (1u << (4 * (weights - 8 * i))) - 1;
             exponent[q] = left > 0 ? scale[q][whole * 4L + piece] : 127;
         }
 #pragma unroll

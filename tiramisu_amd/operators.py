@@ -209,7 +209,7 @@ def combine(x, places, weights=None, residual=None):
 
 def combine_backward(dy, x, places, weights, rows):
     """Gradients of ``combine``: of x, and of the weights where there are some (None: ones).  Each place is in ``places`` once at most; ``rows``, the token of each place, is that of
-    the route: a place that is no token's has a gradient of zeros."""
+    the route: a place that is no token's, or that its token's ``places`` have left out since, has a gradient of zeros."""
     return CombineGradients(*_operators.combine_backward(dy, x, places, weights, rows))
 
 
