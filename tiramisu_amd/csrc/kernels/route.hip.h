@@ -148,6 +148,7 @@ __device__ __forceinline__ void place(const route_arguments &a, long first, long
             a.places[i] = at;
             a.rows[at] = (int)(i / a.k);
         } else if (i < end) a.places[i] = -1;
+        if (from + THREADS >= end) break;
         __syncthreads();
         for (int x = t; x < a.experts; x += THREADS)
             for (int w = 0; w < WAVES; w++) next[x] += hist[w * a.experts + x];
