@@ -839,3 +839,10 @@ def test_the_c_abi_refuses_sizes_that_pass_64_bits(capfd):
               w.tiramisu_hip_combine_rows(p, p, None, None, p, 1 << 63, 2, 8, 8, 0, 0, 2), w.tiramisu_hip_combine_rows_backward(p, p, p, p, p, p, p, 1 << 63, 2, 8, 8, 0, 0, 2)]
     assert calls == [1] * len(calls)
     assert len(capfd.readouterr().err.strip().splitlines()) == len(calls)
+
+
+def test_the_c_abi_refuses_more_workgroups_than_a_launch_holds(capfd):
+    w, p = runtime.wrappers(), 4096
+    calls = [w.tiramisu_hip_combine_rows_backward(p, p, p, p, p, p, p, 4, 2, (1 << 30) - 1, 8, 0, 0, 2)]
+    assert calls == [1] * len(calls)
+    assert len(capfd.readouterr().err.strip().splitlines()) == len(calls)

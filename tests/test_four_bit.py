@@ -170,6 +170,17 @@ def test_infinities_reach_their_own_rows_only():
 
 
 @pytest.mark.gpu
+def test_more_tokens_than_parts_that_a_launch_has():
+    """Four million tokens of a narrow product: the last are those of a call of their own."""
+    M, N, K = 64 * 65535 + 65, 16, 64
+    x, (w,), _, _ = four_bit_inputs(M, N, K, torch.bfloat16, 61)
+    y = operators.four_bit_linear(x, w.q, w.scale).y
+    xd, wd = x[-70:].double(), widened(w.q, w.scale, K)
+    z = xd @ wd.t()
+    close(y[-70:], z, rounded(z, sum_error(K, xd.abs() @ wd.abs().t()), torch.bfloat16), "y")
+
+
+@pytest.mark.gpu
 def test_no_tokens_and_no_terms():
     x, (w,), _, _ = four_bit_inputs(4, 40, 64, torch.bfloat16, 3)
     assert operators.four_bit_linear(x[:0], w.q, w.scale).y.shape == (0, 40) and operators.four_bit_gated_linear(x[:0], w.q, w.q, w.scale, w.scale).h.shape == (0, 40)

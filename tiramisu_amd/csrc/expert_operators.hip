@@ -99,7 +99,8 @@ int refuse_grouped(const char *fn, uint64_t S, uint64_t T, uint64_t groups, uint
 
 // ---- which tile, by the launch's model (operators.hip) for the tiles that the groups have if the rows are spread as routers spread them, a tenth more than evenly, a
 // group's last tile half empty where it has several; tiles of 256 x 128 and 64 x 64 take 1.1 and 1.25 times what it says where groups bring weights of their own, and the weights' bytes come
-// at 4.6 TB/s.  Of 20 launches (16 and 8 bits, 8 to 64 groups, 500 to 32768 rows) the choice is the fastest or within 6 % of it in 18.
+// at 4.6 TB/s.  Of 240 launches (16 and 8 bits, 2 to 128 groups, 64 to 32768 rows, groups uneven) the choice is 4 % behind the fastest of the four in the geometric mean, 46 % at worst (groups of
+// about 64 rows, 5120 x 2560: 31 us, 21 on 256 x 128).
 constexpr struct { product_tile tile; int rows, columns; double factor; } GROUPED_TILES[] = {{TILE_256, 256, 256, 1.0}, {TILE_256x128, 256, 128, 1.1}, {TILE_128, 128, 128, 1.0}, {TILE_64, 64, 64, 1.25}};
 double rows_tiles(const grouped_arguments &a, int rows, int columns, bool gated) {
     const double active = (double)std::min(a.groups, a.rows);
@@ -365,6 +366,7 @@ void launch_four_few(const char *fn, const four_bit_arguments &a) {
     else if (a.p.M <= 32) launch_four_few<E, EPILOGUE, 2>(fn, a);
     else launch_four_few<E, EPILOGUE, 4>(fn, a);
 }
+constexpr long MOST_PARTS = 65535;          // workgroups of a launch in a direction other than the first
 // Few tokens in parts of 64, or the weights widened ahead of a product on tiles
 template <int E>
 int four_bit(const char *fn, int epilogue, four_bit_arguments a) {
@@ -377,7 +379,7 @@ int four_bit(const char *fn, int epilogue, four_bit_arguments a) {
     p.b = p.b2 = nullptr;
     p.ldb = p.ldb2 = to;
     planned_forward f = plan_forward(E, E, epilogue, p, s);
-    if (K > 0 && N <= MOST_FEW_COLUMNS && (a.p.M <= 64 || four_bit_few_cost(a.p.M, N, K, gated) <= four_bit_widened_cost(f, N, K, gated))) {
+    if (K > 0 && N <= MOST_FEW_COLUMNS && a.p.M <= 64 * MOST_PARTS && (a.p.M <= 64 || four_bit_few_cost(a.p.M, N, K, gated) <= four_bit_widened_cost(f, N, K, gated))) {
         call_scratch few;
         const placed_operand x = place_operand({a.p.a, a.p.lda}, a.p.M, K, 2, true, few);
         if (few.take(fn)) return 1;
@@ -584,11 +586,12 @@ int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int3
     if (!known_type(type, false)) return refuse(__FUNCTION__, "element type %d: float16 or bfloat16", type);
     if ((tokens && columns && k && (!dy || !places)) || (rows && columns && dx && !owners) || (rows && columns && dweights && !x)) return refuse(__FUNCTION__, "dy, x, places and owners are needed");
     if (dweights && !weights) return refuse(__FUNCTION__, "a gradient of weights that are not given");
-    timed record(__FUNCTION__);
     const long n = (long)columns;
     const bool wide = n > 256;
     const long choices = wide ? 4 : 16, choice_blocks = ((long)tokens * (long)k + choices - 1) / choices, blocks = choice_blocks + (dx && n ? ((long)rows + 63) / 64 : 0);
     if (blocks == 0) return 0;
+    if (blocks >= 1L << 24) return refuse(__FUNCTION__, "%llu rows and %llu choices: more workgroups than a launch holds", (ull)rows, (ull)(tokens * k));
+    timed record(__FUNCTION__);
     const tcombine::combine_backward_arguments a = {dy, x, places, owners, weights, n ? dx : nullptr, dweights, (long)tokens, (long)rows, n, ldy ? (long)ldy : n, ldx ? (long)ldx : n, (int)k, choice_blocks};
     auto kernel = type == F16 ? (wide ? tcombine::combine_backward_kernel<F16, 64> : tcombine::combine_backward_kernel<F16, 16>)
                               : (wide ? tcombine::combine_backward_kernel<BF16, 64> : tcombine::combine_backward_kernel<BF16, 16>);
