@@ -13,9 +13,9 @@ from test_operators import F8, HALVES
 
 # launches: (rows, groups, N, K)
 LINEAR_16 = {"few 8": (30, 19, 93, 330), "few 4": (16, 8, 2100, 1030), "few 2": (20, 9, 4100, 330), "64x64/3": (83, 3, 93, 142), "128x128/4": (418, 117, 67, 42), "128x128/2": (164, 52, 815, 38),
-             "256x128/3": (29169, 23, 67, 134), "256x256/2": (5294, 25, 1601, 162)}
+             "256x128/3": (29169, 23, 67, 134), "256x256/2": (5294, 25, 1601, 162), "192x128/2": (5929, 11, 1026, 142)}
 GATED_16 = {"few 8": (30, 19, 93, 330), "few 4": (16, 8, 2100, 330), "64x128/3": (83, 3, 93, 142), "128x128/4": (40, 3, 93, 42), "128x128/2": (24628, 82, 9, 38), "256x128/3": (32239, 2, 9, 158),
-            "256x256/2": (18525, 77, 205, 154)}
+            "256x256/2": (18525, 77, 205, 154), "192x128/2": (2853, 9, 1104, 132)}
 LINEAR_8 = {"few 8": (30, 19, 93, 332), "few 4": (16, 8, 2100, 3000), "few 2": (20, 9, 4100, 332), "64x64/3": (83, 3, 93, 140), "128x128/4": (250, 8, 2029, 392), "256x128/3": (36058, 51, 71, 44),
             "256x256/2": (30200, 22, 235, 36)}
 GATED_8 = {"few 8": (30, 19, 93, 332), "few 4": (16, 8, 2100, 332), "64x128/3": (83, 3, 93, 140), "128x128/4": (14642, 11, 13, 36), "256x128/3": (28360, 65, 9, 820), "256x256/2": (11240, 4, 617, 36)}

@@ -98,10 +98,11 @@ int refuse_grouped(const char *fn, uint64_t S, uint64_t T, uint64_t groups, uint
 }
 
 // ---- which tile, by the launch's model (operators.hip) for the tiles that the groups have if the rows are spread as routers spread them, a tenth more than evenly, a
-// group's last tile half empty where it has several; tiles of 256 x 128 and 64 x 64 take 1.1 and 1.25 times what it says where groups bring weights of their own, and the weights' bytes come
-// at 4.6 TB/s.  Of 240 launches (16 and 8 bits, 2 to 128 groups, 64 to 32768 rows, groups uneven) the choice is 4 % behind the fastest of the four in the geometric mean, 46 % at worst (groups of
-// about 64 rows, 5120 x 2560: 31 us, 21 on 256 x 128).
-constexpr struct { product_tile tile; int rows, columns; double factor; } GROUPED_TILES[] = {{TILE_256, 256, 256, 1.0}, {TILE_256x128, 256, 128, 1.1}, {TILE_128, 128, 128, 1.0}, {TILE_64, 64, 64, 1.25}};
+// group's last tile half empty where it has several; what the model says is multiplied by `factor`, as groups bring weights of their own, whose bytes come at 4.6 TB/s.  192 x 128 are 16 bits' and forward.  Of 585
+// launches of 16 bits and 135 of 8 (2 to 128 groups, 64 to 32768 rows, groups uneven) the choice is 5 % and 3 % behind the fastest tile in the geometric mean (16 bits without 192 x 128: 6 %), a third to a half at worst:
+// few tiles of few rows, or a round that begins with a few tiles, as the groups' sizes are not known here.
+constexpr struct { product_tile tile; int rows, columns; double factor; } GROUPED_TILES[] = {{TILE_256, 256, 256, 1.0}, {TILE_256x128, 256, 128, 1.1}, {TILE_192x128, 192, 128, 1.05}, {TILE_128, 128, 128, 1.0},
+                                                                                             {TILE_64, 64, 64, 1.25}};
 double rows_tiles(const grouped_arguments &a, int rows, int columns, bool gated) {
     const double active = (double)std::min(a.groups, a.rows);
     return 1.1 * active * std::max(1.0, a.rows / active / rows + 0.5) * (double)(((gated ? 2L : 1L) * a.p.N + columns - 1) / columns);
@@ -111,6 +112,7 @@ product_tile grouped_tile(const grouped_arguments &a, int bytes, bool gated) {
     product_tile best = TILE_64;
     double best_cost = 0;
     for (const auto &t : GROUPED_TILES) {
+        if (t.tile == TILE_192x128 && bytes == 1) continue;
         const long tiles = std::max(1L, (long)rows_tiles(a, t.rows, gated && t.tile == TILE_64 ? 128 : t.columns, gated)), slices = std::max(1L, ((long)a.p.K * bytes + 127) / 128);
         const double launch = t.factor * tile_launch_cost(t.tile, tiles, slices, bytes, gated), cost = std::max(launch, weights) + 0.2 * std::min(launch, weights);
         if (best_cost == 0 || cost < best_cost) { best = t.tile; best_cost = cost; }
@@ -125,7 +127,7 @@ gradients_plan plan_gradients(const grouped_arguments &a, const grouped_argument
     gradients_plan best = {TILE_64, 1};
     double best_cost = 0;
     for (const auto &t : GROUPED_TILES)
-        for (int splits = 1; splits <= 16; splits *= 2) {
+        for (int splits = 1; splits <= 16 && t.tile != TILE_192x128; splits *= 2) {
             const double of_rows = pairs * ((a.p.K + 63) / 64), of_weights = (double)b.rows / b.groups / 64 / splits;
             const double down = a.p.y ? rows_tiles(a, t.rows, t.columns, false) : 0;
             const double across = b.p.y ? (double)((b.p.M + t.rows - 1L) / t.rows) * ((b.p.N + t.columns - 1L) / t.columns) * b.groups * splits : 0, tiles = std::max(1.0, down + across);

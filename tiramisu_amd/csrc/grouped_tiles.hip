@@ -60,6 +60,10 @@ template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
     typedef tile_config<E, 128, 128, 4, 2, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_pair;
     typedef tile_config<E, 64, 128, 2, 4, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_end;
     typedef tile_config<E, 64, 128, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_pair_end;
+    // Two to a compute unit, whose LDS they fill, four wavefronts of 96 x 64 each: they read LDS as little as those of 256 x 128 and cover each other's beginnings and ends
+    // (8192 rows in 8 groups bf16, 2048 x 2048, as 256 x 256 / 256 x 128 / 128 x 128 / so: 89 / 81 / 80 / 65 us, gated 158 / 151 / 157 / 131).
+    typedef tile_config<E, 192, 128, 2, 2, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_192x128;
+    typedef tile_config<E, 96, 128, 1, 4, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_192x128_end;
     typedef tile_config<E, 64, SMALL_N, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
 };
 template <int E, int Y, int EPILOGUE>
@@ -71,6 +75,8 @@ void launch_tile(product_tile tile, const grouped_arguments &a, hipStream_t stre
         if constexpr (E != F8)
             if (tiles_of<typename T::tile_128>(a) > ttarget::COMPUTE_UNITS) return launch<typename T::tile_128_pair, typename T::tile_128_pair_end, Y>(a, stream);
         launch<typename T::tile_128, typename T::tile_128_end, Y>(a, stream);
+    } else if (tile == TILE_192x128) {
+        if constexpr (E != F8) launch<typename T::tile_192x128, typename T::tile_192x128_end, Y>(a, stream);
     } else launch<typename T::tile_64, typename T::tile_64, Y>(a, stream);
 }
 

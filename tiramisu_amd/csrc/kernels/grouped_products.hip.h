@@ -153,8 +153,9 @@ __device__ __forceinline__ void weights_tile(const grouped_arguments &a, int id,
 }
 #endif
 
+// (192 rows: registers for two workgroups to a compute unit, which the LDS has room for)
 template <class C, class D, int Y>
-__global__ __launch_bounds__(C::NT) void grouped_rows_kernel(grouped_arguments a) {
+__global__ __launch_bounds__(C::NT, C::BM == 192 ? 2 : 1) void grouped_rows_kernel(grouped_arguments a) {
 #ifdef __HIP_DEVICE_COMPILE__
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     rows_tile<C, D, Y>(a, blockIdx.x, (lds_char *)shared_bytes);

@@ -235,6 +235,11 @@ void launch_forward(const char *fn, planned_forward &f, const call_scratch &s) {
     launch_product(fn, f.q, s);
 }
 double tile_launch_cost(product_tile tile, long tiles, long slices, int bytes, bool gated) {
+    if (tile == TILE_192x128) {             // two to a compute unit, the last round maybe alone (fitted to 585 launches of 2 to 128 groups)
+        const long pairs = (tiles - 1) / (2 * ttarget::COMPUTE_UNITS), rest = tiles - pairs * 2 * ttarget::COMPUTE_UNITS;
+        const double pair = 4.0 + 1.2 * (double)slices, alone = 3.0 + 0.88 * (double)slices;
+        return 3.0 + (double)pairs * pair + (rest > ttarget::COMPUTE_UNITS ? pair : alone);
+    }
     for (const tile_model &t : TILES_16_BITS)
         if (bytes == 2 && t.tile == tile) return modelled(gated && tile == TILE_64 ? GATED_64_16_BITS : t, tiles, slices);
     for (const tile_model &t : TILES_8_BITS)
