@@ -846,3 +846,22 @@ def test_the_c_abi_refuses_more_workgroups_than_a_launch_holds(capfd):
     calls = [w.tiramisu_hip_combine_rows_backward(p, p, p, p, p, p, p, 4, 2, (1 << 30) - 1, 8, 0, 0, 2)]
     assert calls == [1] * len(calls)
     assert len(capfd.readouterr().err.strip().splitlines()) == len(calls)
+
+
+def test_gradients_of_combine_without_columns_or_without_a_result():
+    """Places are read wherever something is launched, also of rows without columns: without them such a call is refused.  Where no result is wanted, nothing is launched."""
+    out = host_runtime.printed(r"""
+p = 1 << 20
+def says(*a):
+    rc = w.tiramisu_hip_combine_rows_backward(*a, 0, 0, 2)
+    return rc, len(launches())
+# dy, x, places, owners, weights, dx, dweights, tokens, k, rows, columns
+assert says(p, p, None, p, p, p, p, 4, 2, 8, 0) == (1, 0)
+assert says(None, None, None, None, p, None, p, 4, 2, 0, 0) == (1, 0)
+assert says(p, p, None, p, p, p, p, 4, 2, 8, 8) == (1, 0)
+assert says(p, p, p, p, p, p, p, 4, 2, 8, 0) == (0, 1)
+assert says(p, p, p, p, p, None, None, 4, 2, 8, 8) == (0, 0)
+assert says(p, p, p, p, p, p, None, 4, 2, 8, 0) == (0, 0)
+assert says(None, None, None, None, p, None, p, 4, 0, 0, 8) == (0, 0)
+""")
+    assert out == ""

@@ -586,9 +586,11 @@ int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int3
     if (k > 1024) return refuse(__FUNCTION__, "%llu rows of a token: at most 1024", (ull)k);
     if (tokens > MOST || tokens * k > 1 << 25) return refuse(__FUNCTION__, "%llu tokens of %llu rows: at most 2^25 rows of all", (ull)tokens, (ull)k);
     if (!known_type(type, false)) return refuse(__FUNCTION__, "element type %d: float16 or bfloat16", type);
-    if ((tokens && columns && k && (!dy || !places)) || (rows && columns && dx && !owners) || (rows && columns && dweights && !x)) return refuse(__FUNCTION__, "dy, x, places and owners are needed");
+    // (the kernel reads places whether or not the rows have columns)
+    if ((tokens && k && (!places || (columns && !dy))) || (rows && columns && dx && !owners) || (rows && columns && dweights && !x)) return refuse(__FUNCTION__, "dy, x, places and owners are needed");
     if (dweights && !weights) return refuse(__FUNCTION__, "a gradient of weights that are not given");
     const long n = (long)columns;
+    if (!dweights && !(dx && n)) return 0;
     const bool wide = n > 256;
     const long choices = wide ? 4 : 16, choice_blocks = ((long)tokens * (long)k + choices - 1) / choices, blocks = choice_blocks + (dx && n ? ((long)rows + 63) / 64 : 0);
     if (blocks == 0) return 0;
