@@ -215,7 +215,8 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
                                        uint64_t ldx, uint64_t ldg, uint64_t ldu, uint64_t ld_gate, uint64_t ld_up, int32_t activation, int32_t type);
 /* ---- operators of a feed-forward sublayer with experts, and of 4-bit weights: the rules above, the numbers of types and activations below them.
  *      Rows grouped by expert: `offsets` (groups + 1 of them, rising, in GPU memory; the host never reads them) say where each group's S places begin and end;
- *      places behind the last group's are rows of zeros in results, and give nothing to gradients.  `rows` (may be null: x holds the S places' rows, T = S) picks
+ *      places ahead of the first group's (a call for some of the experts: offsets and weights of these alone) and behind the last one's are rows of zeros in results, and give nothing
+ *      to gradients.  `rows` (may be null: x holds the S places' rows, T = S) picks
  *      the row of x, of T, for each place; numbers that are none of x's give rows of zeros.  Group g's weight is N x K, all of them one below the other. ---- */
 
 /* The k largest of each token's `count` logits (ties to the lowest index, NaN above everything, minus infinity never), and their weights: softmax

@@ -865,3 +865,63 @@ assert says(p, p, p, p, p, p, None, 4, 2, 8, 0) == (0, 0)
 assert says(None, None, None, None, p, None, p, 4, 0, 0, 8) == (0, 0)
 """)
     assert out == ""
+
+
+# sizes of all groups, the share of them, places behind the last, N, K: few rows and tiles, shares that begin with empty groups, that are empty, that are all
+SHARES = [([3, 0, 2, 1, 4, 0, 2, 1], 2, 5, 1, 70, 64), ([2] * 9, 8, 9, 0, 33, 40), ([1] * 20, 0, 20, 2, 20, 24), ([130, 7, 0, 300, 70, 1], 1, 3, 5, 130, 72), ([130, 7, 0, 300, 70, 1], 3, 6, 0, 264, 200),
+          ([600, 520, 0, 700], 2, 3, 9, 300, 136), ([70, 300], 1, 2, 0, 1, 33), ([5000, 3, 2000, 900], 1, 4, 40, 300, 264)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES + [F8])
+@pytest.mark.parametrize("sizes,low,high,behind,N,K", SHARES)
+def test_some_of_the_groups(sizes, low, high, behind, N, K, dtype):
+    """A share of the experts: its own offsets and weights with the places of all.  The others' places are rows of zeros, whatever the operands hold there."""
+    out = torch.float16 if dtype == torch.float16 else torch.bfloat16
+    share, S = slice(low, high), sum(sizes) + behind
+    mine = torch.zeros((S, 1), dtype=torch.bool, device="cuda")
+    mine[sum(sizes[:low]):sum(sizes[:high])] = True
+
+    def zeros_elsewhere(got, name):
+        assert not bool(got.masked_fill(mine, 0).any()), name
+
+    for picked in (False, True):
+        offsets, rows, x, xs, ws, scales, xd, wds = grouped_inputs(sizes, behind, N, K, dtype, 101 + N, weights=2, picked=picked)
+        if not picked and dtype != F8:
+            x = torch.where(mine, x, math.nan)
+        own = offsets[low:high + 1]
+        z = [torch.where(mine, by_group(sizes, behind, xd, wd, product), 0.0) for wd in wds]
+        error = [sum_error(K, by_group(sizes, behind, xd, wd, sizes_of)) + by_group(sizes, behind, xd, wd, cut(dtype)) for wd in wds]
+        for _ in range(2):
+            torch.full((S, N), math.nan, device="cuda", dtype=out)          # (what the allocator hands out next)
+            y = operators.grouped_linear(x, ws[0][share], own, rows=rows, x_scale=xs, weight_scale=None if xs is None else scales[0][share], dtype=out)
+            zeros_elsewhere(y, "y")
+            close(y, z[0], rounded(z[0], error[0], out), "y")
+        unwritten = [torch.full((S, N), math.nan, device="cuda", dtype=out) for _ in range(3)]
+        del unwritten
+        got = operators.grouped_gated_linear(x, ws[0][share], ws[1][share], own, rows=rows, x_scale=xs, gate_scale=None if xs is None else scales[0][share],
+                                             up_scale=None if xs is None else scales[1][share], dtype=out, keep_pre=True)
+        for t, exact, bound, name in ((got.gate, z[0], error[0], "gate"), (got.up, z[1], error[1], "up")):
+            zeros_elsewhere(t, name)
+            close(t, exact, rounded(exact, bound, out), name)
+        zeros_elsewhere(got.h, "h")
+        assert bool(torch.isfinite(got.h.float()).all())
+        if dtype == F8:
+            continue
+        g = generator(103)
+        dy, gate, up = [torch.where(mine, normal((S, N), dtype, g), math.nan) for _ in range(3)]
+        d = torch.where(mine, dy, 0).double()
+        at = [sum(sizes[:e]) for e in range(low, high)]
+        spans = [slice(a, a + n) for a, n in zip(at, sizes[low:high])]
+        most = max(sizes[low:high])
+        for _ in range(2):
+            torch.full((S, K), math.nan, device="cuda", dtype=dtype)
+            back = operators.grouped_linear_backward(dy, x, ws[0][share], own, rows=rows)
+            zeros_elsewhere(back.dx, "dx")
+            exact = by_group(sizes, behind, d, wds[0], lambda a, w: a @ w)
+            close(back.dx, exact, backward_bound(dtype, exact, N, by_group(sizes, behind, d.abs(), wds[0].abs(), lambda a, w: a @ w)) + torch.zeros_like(exact), "dx")
+            exact = torch.stack([d[s].t() @ xd[s] for s in spans])
+            close(back.dweight, exact, backward_bound(dtype, exact, most, torch.stack([d[s].abs().t() @ xd[s].abs() for s in spans])), "dweight")
+        both = operators.grouped_gated_linear_backward(dy, x, ws[0][share], ws[1][share], gate, up, own, rows=rows)
+        zeros_elsewhere(both.dx, "gated dx")
+        assert all(bool(torch.isfinite(t.float()).all()) for t in both)

@@ -7,8 +7,8 @@
 
 namespace tgroups {
 
-// Tiles of `height` rows that the rows of so many groups, and those behind them, can need at most
-inline long most_row_tiles(long rows, long groups, long height) { return rows / height + (groups + 1 < rows ? groups + 1 : rows); }
+// Tiles of `height` rows that the rows of so many groups, and those ahead of them and behind them, can need at most
+inline long most_row_tiles(long rows, long groups, long height, long others = 2) { return rows / height + (groups + others < rows ? groups + others : rows); }
 
 // Forward; y: element type of the results
 void launch_grouped_F16(product_tile, int epilogue, int y, const grouped_arguments &, hipStream_t stream);

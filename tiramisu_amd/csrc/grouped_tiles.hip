@@ -22,11 +22,13 @@ void allow_lds(const void *kernel, int bytes, std::atomic<unsigned long long> &a
 }
 
 template <class C>
-long tiles_of(const grouped_arguments &a) {
+long tiles_of(const grouped_arguments &a, long others = 2) {
     const long across = (a.p.N + C::COLUMNS - 1) / C::COLUMNS;
-    if (C::A_ROWS) return most_row_tiles(a.rows, a.groups, C::BM) * across;
+    if (C::A_ROWS) return most_row_tiles(a.rows, a.groups, C::BM, others) * across;
     return ((a.p.M + C::BM - 1L) / C::BM * across + XCDS - 1) / XCDS * XCDS * a.groups * a.splits;
 }
+// Whether tiles are two to a compute unit: by those of a launch for all groups, whose rows none are ahead of
+bool more_than_a_round(long tiles) { return tiles > ttarget::COMPUTE_UNITS; }
 template <class C, class D, int Y>
 void launch(const grouped_arguments &a, hipStream_t stream) {
     auto kernel = grouped_rows_kernel<C, D, Y>;
@@ -73,7 +75,7 @@ void launch_tile(product_tile tile, const grouped_arguments &a, hipStream_t stre
     else if (tile == TILE_256x128) launch<typename T::tile_256x128, typename T::tile_128, Y>(a, stream);
     else if (tile == TILE_128) {
         if constexpr (E != F8)
-            if (tiles_of<typename T::tile_128>(a) > ttarget::COMPUTE_UNITS) return launch<typename T::tile_128_pair, typename T::tile_128_pair_end, Y>(a, stream);
+            if (more_than_a_round(tiles_of<typename T::tile_128>(a, 1))) return launch<typename T::tile_128_pair, typename T::tile_128_pair_end, Y>(a, stream);
         launch<typename T::tile_128, typename T::tile_128_end, Y>(a, stream);
     } else if (tile == TILE_192x128) {
         if constexpr (E != F8) launch<typename T::tile_192x128, typename T::tile_192x128_end, Y>(a, stream);
@@ -101,7 +103,7 @@ void NAME_OF(launch_grouped_gradients_, TIRAMISU_OPERAND)(product_tile tile, con
     if (tile == TILE_256) launch_gradients<typename R::tile_256, typename R::tile_256_end, typename W::tile_256, E>(a, b, stream);
     else if (tile == TILE_256x128) launch_gradients<typename R::tile_256x128, typename R::tile_128, typename W::tile_256x128, E>(a, b, stream);
     else if (tile == TILE_128) {
-        if ((a.p.y ? tiles_of<typename R::tile_128>(a) : 0) + (b.p.y ? tiles_of<typename W::tile_128>(b) : 0) > ttarget::COMPUTE_UNITS)
+        if (more_than_a_round((a.p.y ? tiles_of<typename R::tile_128>(a, 1) : 0) + (b.p.y ? tiles_of<typename W::tile_128>(b) : 0)))
             launch_gradients<typename R::tile_128_pair, typename R::tile_128_pair_end, typename W::tile_128_pair, E>(a, b, stream);
         else launch_gradients<typename R::tile_128, typename R::tile_128_end, typename W::tile_128, E>(a, b, stream);
     } else launch_gradients<typename R::tile_64, typename R::tile_64, typename W::tile_64, E>(a, b, stream);

@@ -3,7 +3,8 @@
 // has as many workgroups as the groups could need at most, every workgroup looks up which tile of which group is its own, and those left over end at once.
 //
 // Looking up is a sum over the groups' tiles, 64 groups at a time across the lanes of a wavefront, and each wavefront does it for itself: no barrier, no
-// launch ahead that would plan, and no table.  Rows behind the last group's are rows of zeros: one more group, whose product has no terms.
+// launch ahead that would plan, and no table.  Rows ahead of the first group's (of a launch for some of the experts) and behind the last one's are rows of zeros: two more
+// groups, whose products have no terms.
 // Offsets are bounded by the number of rows before they are used, so that no offsets whatever lead outside of the operands.
 #ifndef TIRAMISU_AMD_GROUPED_PRODUCTS_HIP_H
 #define TIRAMISU_AMD_GROUPED_PRODUCTS_HIP_H
@@ -45,11 +46,11 @@ __device__ __forceinline__ void tile_in_bands(int t, int rows, int columns, int 
     row = band * BAND + in - column * height;
 }
 
-// Whose tile workgroup `id` computes, of tiles that are HEIGHT rows high and `across` to a row: group < 0: nobody's; group == groups: the rows' behind the groups.
+// Whose tile workgroup `id` computes, of tiles that are HEIGHT rows high and `across` to a row: group < 0: nobody's; group == groups: the rows' ahead of the groups or behind them.
 struct found_tile { int group, first, rows, tile; };
 template <int HEIGHT>
 __device__ __forceinline__ found_tile find_tile(const int *offsets, int groups, int all, int across, int id, int lane) {
-    const int chunks = (groups + 63) / 64, last = uniform(min(max(offsets[groups], 0), all));
+    const int chunks = (groups + 63) / 64, head = uniform(min(max(offsets[0], 0), all)), last = uniform(min(max(offsets[groups], 0), all));
     auto of_lane = [&](int chunk) {
         const int g = chunk * 64 + lane;
         return g < groups ? span_of(offsets, g, all) : group_span{0, 0};
@@ -58,10 +59,11 @@ __device__ __forceinline__ found_tile find_tile(const int *offsets, int groups, 
     group_span s = of_lane(0);
     int tiles = tiles_of(s), upto = sum_up_to(tiles), total = __builtin_amdgcn_readlane(upto, 63);
     for (int c = 1; c < chunks; c++) total += __builtin_amdgcn_readlane(sum_up_to(tiles_of(of_lane(c))), 63);
-    const int everything = total + (all - last + HEIGHT - 1) / HEIGHT * across;
+    const int ahead = (head + HEIGHT - 1) / HEIGHT * across, everything = total + ahead + (all - last + HEIGHT - 1) / HEIGHT * across;
     if (id >= everything) return {-1, 0, 0, 0};
     int t = tile_in_runs(id, everything);
-    if (t >= total) return {groups, last, all - last, t - total};
+    if (t >= total + ahead) return {groups, last, all - last, t - total - ahead};
+    if (t >= total) return {groups, 0, head, t - total};
     int c = 0;
     for (int here; t >= (here = __builtin_amdgcn_readlane(upto, 63)) && c + 1 < chunks;) {
         t -= here;
@@ -176,16 +178,16 @@ __global__ __launch_bounds__(C::NT) void grouped_gradients_kernel(grouped_argume
 }
 
 // Few rows to a group: bound by the bytes of the weights of the groups that have rows.  grid: (columns in sixteens, groups that may have rows and one): workgroups
-// of the last row of the grid write the rows behind the groups.  A group's weights are read once for each TILES x 16 of its rows.
+// of the last row of the grid write the rows ahead of the groups and behind them.  A group's weights are read once for each TILES x 16 of its rows.
 template <int E, int Y, int EPILOGUE, int TILES, int SPLIT>
 __global__ __launch_bounds__(64 * FEW_WAVES) void grouped_few_kernel(grouped_arguments a) {
     constexpr int BYTES = E == F8 ? 1 : 2, COLUMNS = FEW_ROWS * (FEW_WAVES / SPLIT);
     const int lane = threadIdx.x & 63, wanted = blockIdx.y;
     const long n0 = (long)blockIdx.x * COLUMNS;
     if (wanted == (int)gridDim.y - 1) {
-        const int last = min(max(a.offsets[a.groups], 0), a.rows), some = (int)min((long)COLUMNS, a.p.N - n0);
-        for (long i = threadIdx.x; i < (long)(a.rows - last) * COLUMNS; i += 64 * FEW_WAVES) {
-            const long at = (last + i / COLUMNS) * a.p.N + n0 + i % COLUMNS;
+        const int head = min(max(a.offsets[0], 0), a.rows), last = min(max(a.offsets[a.groups], 0), a.rows), some = (int)min((long)COLUMNS, a.p.N - n0);
+        for (long i = threadIdx.x; i < (long)(head + a.rows - last) * COLUMNS; i += 64 * FEW_WAVES) {
+            const long row = i / COLUMNS, at = (row < head ? row : last + row - head) * a.p.N + n0 + i % COLUMNS;
             if (i % COLUMNS >= some) continue;
             ((uint16_t *)a.p.y)[at] = 0;
             if (a.p.pre) ((uint16_t *)a.p.pre)[at] = ((uint16_t *)a.p.pre2)[at] = 0;

@@ -180,8 +180,8 @@ def route_backward(dweights, logits, experts, normalise=True):
 
 def grouped_linear(x, weight, offsets, rows=None, x_scale=None, weight_scale=None, dtype=None):
     """y[s] = x[s] weight[g]^T for the places s from offsets[g] to offsets[g + 1] (int32, on the GPU), with weight [groups, N, K] and the types of ``linear``
-    (``weight_scale`` [groups, N]).  With ``rows`` place s takes the row x[rows[s]] instead, and the result has a row for each of ``rows``.  Places behind the last
-    group's, and those whose number is none of x's, are rows of zeros."""
+    (``weight_scale`` [groups, N]).  With ``rows`` place s takes the row x[rows[s]] instead, and the result has a row for each of ``rows``.  Places ahead of the first
+    group's and behind the last one's, and those whose number is none of x's, are rows of zeros; so ``weight[a:b]`` with ``offsets[a:b + 1]`` are the results of these groups alone."""
     return _operators.grouped_linear(x, weight, offsets, rows, x_scale, weight_scale, _result_type(dtype))[0]
 
 
