@@ -217,7 +217,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
  *      Rows grouped by expert: `offsets` (groups + 1 of them, rising, in GPU memory; the host never reads them) say where each group's S places begin and end;
  *      places ahead of the first group's (a call for some of the experts: offsets and weights of these alone) and behind the last one's are rows of zeros in results, and give nothing
  *      to gradients.  `rows` (may be null: x holds the S places' rows, T = S) picks
- *      the row of x, of T, for each place; numbers that are none of x's give rows of zeros.  Group g's weight is N x K, all of them one below the other. ---- */
+ *      the row of x, of T, for each place; numbers that are none of x's give rows of zeros, whatever weights and scales hold (in dweight: dy times zeros).  Group g's weight is N x K, all of them one below the other. ---- */
 
 /* The k largest of each token's `count` logits (ties to the lowest index, NaN above everything, minus infinity never), and their weights: softmax
  * over the chosen ones (normalise) or over all.  A place that no expert is left for has expert -1 and weight 0.  Places by expert, in order of token and rank: offsets

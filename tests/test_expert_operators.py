@@ -925,3 +925,31 @@ def test_some_of_the_groups(sizes, low, high, behind, N, K, dtype):
         both = operators.grouped_gated_linear_backward(dy, x, ws[0][share], ws[1][share], gate, up, own, rows=rows)
         zeros_elsewhere(both.dx, "gated dx")
         assert all(bool(torch.isfinite(t.float()).all()) for t in both)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", HALVES + [F8])
+@pytest.mark.parametrize("sizes,behind,N,K", [([2, 0, 1, 3], 2, 70, 64), ([1] * 20, 3, 2100, 330), ([30, 0, 9], 20, 33, 70), ([40, 30], 9, 66, 71), ([130, 0, 60, 4], 30, 140, 200), ([700, 520, 3], 5, 264, 136),
+                                              ([2600, 100, 1400], 100, 1104, 132), ([5000, 10, 3000], 50, 640, 264)])
+def test_rows_that_are_none_of_x_are_zeros_whatever_the_weights_hold(sizes, behind, N, K, dtype):
+    """Infinities and NaN in weights and in their scales do not reach places that take no row of x, nor those behind the groups: few rows, all tiles, rows moved ahead of them."""
+    offsets, rows, x, xs, ws, scales, _, _ = grouped_inputs(sizes, behind, N, K, dtype, 107, weights=2, picked=True)
+    T, S = x.shape[0], sum(sizes) + behind
+    nobody = ~((rows >= 0) & (rows < T))
+    nobody[sum(sizes):] = True
+    assert int(nobody.sum()) > behind
+    for w in ws:
+        w[:, 0, 0] = math.nan
+        w[:, N // 2, K - 1] = math.nan if dtype == F8 else math.inf
+        w[0] = math.nan
+    for s in scales:
+        if s is not None:
+            s[:, 1], s[0] = math.inf, math.nan
+    odd = torch.zeros((T, K + 3), device="cuda").to(dtype)                  # rows at odd elements: moved ahead of tiles
+    odd[:, 1:K + 1] = x
+    for view in (x, odd[:, 1:K + 1]):
+        y = operators.grouped_linear(view, ws[0], offsets, rows=rows, x_scale=xs, weight_scale=scales[0])
+        assert y.shape == (S, N) and not bool(y[nobody].any()) and bool(torch.isnan(y[~nobody][:, 0]).all())
+        for activation in ("silu", "gelu"):
+            got = operators.grouped_gated_linear(view, ws[0], ws[1], offsets, rows=rows, activation=activation, x_scale=xs, gate_scale=scales[0], up_scale=scales[1], keep_pre=True)
+            assert not any(bool(t[nobody].any()) for t in got) and all(bool(torch.isnan(t[~nobody][:, 0]).all()) for t in got)

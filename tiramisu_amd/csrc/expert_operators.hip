@@ -261,7 +261,7 @@ int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_argum
     const int bytes = bytes_of(type);
     const bool gated = epilogue == GATED;
     const long K = a.p.K, all = (long)a.groups * a.p.N;
-    a.picked = {rows, rows ? tokens : a.rows};
+    a.picked = {rows, rows ? tokens : a.rows, rows, tokens};
     a.b_step = (long)a.p.N * a.p.ldb;
     a.b2_step = (long)a.p.N * a.p.ldb2;
     if (K > 0 && a.p.N <= MOST_FEW_COLUMNS && a.rows <= FEW_ROWS_OF_A_GROUP * std::min(a.groups, a.rows)) {
@@ -283,7 +283,7 @@ int grouped_forward(const char *fn, int type, int y, int epilogue, grouped_argum
     if (rows && !pick) {
         if (moved.place != call_scratch::NOWHERE) a.p.a = moves.settle(a.p.a, rows, a.p.lda, tokens, a.rows, K, moved.ld, moved.place, s);
         a.p.lda = moved.ld;
-        a.picked = {nullptr, a.rows};
+        a.picked = {nullptr, a.rows, rows, tokens};
         if (a.p.a_scale) {
             hipLaunchKernelGGL(tgroups::pick_scales_kernel, dim3((unsigned)((a.rows + 255L) / 256)), dim3(256), 0, stream(), a.p.a_scale, (float *)s.at(scales), rows, (long)a.rows, tokens);
             check(hipGetLastError(), fn);

@@ -19,7 +19,7 @@ struct grouped_arguments {
     product_arguments p;                    // addresses of the first group's; M: rows in all (gradient of the weights: rows of a group's result)
     const int *offsets;                     // groups + 1
     int groups, rows;                       // rows in all
-    picked_rows picked;                     // forward: x's rows (index null: x holds the grouped rows themselves)
+    picked_rows picked;                     // forward: x's rows (index null: x holds the grouped rows themselves, from the caller or moved)
     long b_step, b2_step;                   // elements from group to group of the weights (input's gradient, gated: b2 is the second pair's)
     long y_step;                            // gradient of the weights: elements from group to group of the result
     int splits;                             // ... workgroups that share the terms of a tile: sums to p.partial, [group][split][M][N]
@@ -82,6 +82,7 @@ __device__ __forceinline__ product_arguments product_of_rows(const grouped_argum
     product_arguments p = a.p;
     picked = a.picked;
     const long f = first;
+    if (picked.given) picked.given += f;
     if (picked.index) picked.index += f;
     else {
         p.a = (const char *)p.a + f * p.lda * BYTES;

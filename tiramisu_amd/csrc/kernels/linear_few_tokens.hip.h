@@ -30,7 +30,7 @@ __device__ __forceinline__ f32x4 multiply_16(u32x4 rows, u32x4 columns, f32x4 c)
 
 // The columns from n0 on: 16 to every SPLIT wavefronts, which share their k.  PICKED: rows of x may be picked by an index; one that is none of x's gives a row of zeros.
 template <int E, int Y, int EPILOGUE, int TILES, bool PICKED = false, int SPLIT = FEW_WAVES>
-__device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, picked_rows picked = {nullptr, 0}) {
+__device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, picked_rows picked = {}) {
     constexpr int BYTES = E == F8 ? 1 : 2, PARTS = EPILOGUE == GATED ? 2 : 1, BATCH = TILES * PARTS >= 4 ? 2 : TILES * PARTS == 2 ? 4 : 8;
     extern __shared__ __attribute__((aligned(16))) char shared_bytes[];
     __attribute__((address_space(3))) f32x4 *const sums = (__attribute__((address_space(3))) f32x4 *)shared_bytes;
@@ -147,15 +147,16 @@ __device__ __forceinline__ void few_tokens(const product_arguments &p, long n0, 
                 for (int i = 0; i < 4; i++) z[q][4 * four + i] += s[i];
             }
     }
-    if constexpr (PICKED)
-        if (!there) {
-#pragma unroll
-            for (int q = 0; q < PARTS; q++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) z[q][i] = 0.f;
-        }
     column_terms columns;
     widen_column_pieces<Y>(p, pieces, columns);
+    if constexpr (PICKED)
+        if (!there) {                                      // (and no scale, which may be NaN, makes it something else)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                z[0][i] = z[PARTS - 1][i] = 0.f;
+                if (E == F8) columns.scale[i] = columns.scale_2[i] = 0.f;
+            }
+        }
     if constexpr (EPILOGUE == GATED) finish_gated<Y>(p, columns, z[0], z[1], scale, m, n, some);
     else {
         float r[8];

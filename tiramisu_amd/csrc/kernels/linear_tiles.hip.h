@@ -242,11 +242,13 @@ __device__ __forceinline__ S multiply(const fragment<E, AR> &rows, const fragmen
 // waited for every load ahead of each of them, 205 us where 105 are enough.)
 // What an index picks of an operand: nothing, rows of A (k along them), or k of B (down its columns; the index lies in LDS, PICKS of it at a time).
 enum picking : int { NOTHING = 0, ROWS_OF_A = 1, K_OF_B = 2 };
-struct picked_rows { const int *index; long all; };       // index: of the product's row 0, or of its first k (null: rows follow each other); all: rows of the operand
+// index: of the product's row 0, or of its first k (null: rows follow each other); all: rows of the operand.  given, of: the index and number of rows that a caller gave, also
+// where the operand has been moved into the groups' order since (null: none).
+struct picked_rows { const int *index; long all; const int *given; long of; };
 constexpr int PICKS = 4096;
 template <class C, int PICK = NOTHING>
 __device__ __forceinline__ void accumulate(typename block_sums<C::F>::type (&acc)[C::TM][C::TN], const void *__restrict__ a, long lda, const void *__restrict__ b, long ldb, const void *__restrict__ b2, long ldb2, long M, long N,
-                                           long m0, long n0, long k0, long K, lds_char *lds, picked_rows picked = {nullptr, 0},
+                                           long m0, long n0, long k0, long K, lds_char *lds, picked_rows picked = {},
                                            const __attribute__((address_space(3))) int *list = nullptr) {
     constexpr int TM = C::TM, TN = C::TN, ST = C::STAGES, E = C::E;
     constexpr int F = C::F, Q = 128 / C::STEP;                             // matrix steps of a slice
@@ -508,9 +510,9 @@ __device__ __forceinline__ void tile_of(int id, int rows, int columns, int &row,
 
 #ifdef __HIP_DEVICE_COMPILE__               // (the host's compilation needs no body, and rejects a second one of the same configuration)
 // The tile of the product in this row and column of tiles, of part `split` of k.  Y: type of bias, residual and outputs.  ROWS_OF_A: rows of A may be
-// picked by an index, and their scales with them; K_OF_B: the rows of B are.
+// picked by an index, and their scales with them, and a row that takes none of A's is a row of zeros whatever B holds; K_OF_B: the rows of B are.
 template <class C, int Y, int PICK = NOTHING>
-__device__ __forceinline__ void compute_tile_at(const product_arguments &p, int row, int column, int split, lds_char *lds, picked_rows picked = {nullptr, 0}) {
+__device__ __forceinline__ void compute_tile_at(const product_arguments &p, int row, int column, int split, lds_char *lds, picked_rows picked = {}) {
     constexpr bool PICKED = PICK == ROWS_OF_A;
     const long m0 = (long)row * C::BM, n0 = (long)column * C::COLUMNS;
     constexpr int F = C::F, REGISTERS = F * F / 64;
@@ -565,6 +567,15 @@ __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int 
     if constexpr (!EARLY) load_terms();
     column_terms columns;
     if (TERMS && some > 0 && !p.partial) widen_column_pieces<Y>(p, pieces, columns);
+
+    // What row lane % 32 of each strip takes of A, on its way during the epilogue
+    int taken[STRIPS];
+    if constexpr (PICKED)
+#pragma unroll
+        for (int i = 0; i < STRIPS; i++) {
+            const long m = m0 + wm * C::WM + i * 32 + lane % 32;
+            taken[i] = picked.given && m < p.M ? picked.given[m] : 0;
+        }
 
     // A wavefront's strips of 32 rows, through LDS of its own: stored by columns of the accumulators, read by rows.
     const int at = lane % F, group = lane / F;
@@ -660,6 +671,26 @@ __device__ __forceinline__ void compute_tile_at(const product_arguments &p, int 
             }
         }
         order_lanes();
+    }
+    // Rows that take none of A's have been computed like the others, zeros times weights and scales, which an infinity makes NaN: the lanes that stored them store zeros
+    // behind that (clearing sums on their way instead costs every row: 4096 x 2 of 8 gated, 2048 x 2048, 158 -> 162 us, so 160; 1000 x 2 of 12 in 8 bits 21.0 -> 21.9, so 21.4).
+    if constexpr (PICKED) {
+#pragma unroll
+        for (int i = 0; i < STRIPS; i++) {
+            const long first = m0 + wm * C::WM + i * 32;
+            const uint32_t none = (uint32_t)__ballot(picked.given && first + lane % 32 < p.M && (taken[i] < 0 || taken[i] >= picked.of));
+            if (none == 0) continue;
+#pragma unroll 1
+            for (int row = r0; row < 32; row += DOWN) {
+                if (!((none >> row) & 1) || some <= 0) continue;
+                const float zeros[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                typedef stored<Y> T;
+                const long to = (first + row) * p.N + n;
+                store_some<Y>((T *)p.y + to, some, zeros);
+                if (p.pre) store_some<Y>((T *)p.pre + to, some, zeros);
+                if (C::EPILOGUE == GATED && p.pre) store_some<Y>((T *)p.pre2 + to, some, zeros);
+            }
+        }
     }
 }
 // Tile `id` of the product

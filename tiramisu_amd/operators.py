@@ -181,13 +181,13 @@ def route_backward(dweights, logits, experts, normalise=True):
 def grouped_linear(x, weight, offsets, rows=None, x_scale=None, weight_scale=None, dtype=None):
     """y[s] = x[s] weight[g]^T for the places s from offsets[g] to offsets[g + 1] (int32, on the GPU), with weight [groups, N, K] and the types of ``linear``
     (``weight_scale`` [groups, N]).  With ``rows`` place s takes the row x[rows[s]] instead, and the result has a row for each of ``rows``.  Places ahead of the first
-    group's and behind the last one's, and those whose number is none of x's, are rows of zeros; so ``weight[a:b]`` with ``offsets[a:b + 1]`` are the results of these groups alone."""
+    group's and behind the last one's, and those whose number is none of x's, are rows of zeros, whatever weights and scales hold; so ``weight[a:b]`` with ``offsets[a:b + 1]`` are the results of these groups alone."""
     return _operators.grouped_linear(x, weight, offsets, rows, x_scale, weight_scale, _result_type(dtype))[0]
 
 
 def grouped_linear_backward(dy, x, weight, offsets, rows=None):
     """Gradients of ``grouped_linear`` (16-bit operands): dx of each place (with ``rows`` the gradient of x is ``combine(dx, places)``) and of the weights, zeros for
-    a group without places."""
+    a group without places.  A place whose number is none of x's counts as dy times zeros there."""
     return GroupedLinearGradients(*_operators.grouped_linear_backward(dy, x, weight, offsets, rows))
 
 
