@@ -256,7 +256,8 @@ int tiramisu_hip_combine_rows_backward(const void *dy, const void *x, const int3
  * power of two, as its exponent and 127 (e8m0), that is the smallest by which the largest of them is at most 6; 1 for zeros, 255 (NaN) where one is not finite.  Dense results. */
 int tiramisu_hip_quantize_groups(const void *x, void *q, uint8_t *scale, uint64_t rows, uint64_t columns, uint64_t ldx, int32_t type);
 /* tiramisu_hip_linear and tiramisu_hip_gated_linear with weights in 4 bits; ldq, ldg, ldu, lds, ldgs, ldus: bytes from row to row of values and scales.  x, bias, residual and results
- * are float16 or bfloat16; weights are multiplied as numbers of that type, which bfloat16 holds exactly and float16 within its range. */
+ * are float16 or bfloat16; weights are multiplied as numbers of that type: exact in bfloat16 (6 x 2^126, 2 x 2^127 and what else is 2^128 or more, of
+ * scales 253 and 254, is infinite) and within float16's range, beyond which they are infinite and below which rounded to multiples of 2^-24. */
 int tiramisu_hip_four_bit_linear(const void *x, const void *q, const uint8_t *scale, const void *bias, const void *residual, void *y, uint64_t M, uint64_t N, uint64_t K, uint64_t ldx,
                                  uint64_t ldq, uint64_t lds, uint64_t ldr, int32_t activation, int32_t type);
 int tiramisu_hip_four_bit_gated_linear(const void *x, const void *gate_q, const void *up_q, const uint8_t *gate_scale, const uint8_t *up_scale, void *h, uint64_t M, uint64_t N,

@@ -242,3 +242,29 @@ def test_what_the_c_abi_refuses(capfd):
     assert calls == [1] * len(calls)
     messages = capfd.readouterr().err.strip().splitlines()
     assert len(messages) == len(calls) and all(m.startswith("Error at tiramisu_hip_") for m in messages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,times,K", [(1, 1, 32), (40, 1, 32), (200, 1, 32), (3001, 44, 1344)])
+def test_the_least_and_the_largest_scales(M, times, K):
+    """Exponents 0, 253 and 254 in bfloat16, through registers and through the widened copy: exact down to 2^-128, and infinite where the value is 2^128 or more."""
+    for byte in (0, 253, 254):
+        q = torch.zeros((16 * times, K // 2), device="cuda", dtype=torch.uint8)
+        q[:, 0] = torch.arange(16, device="cuda", dtype=torch.uint8).repeat(times)
+        scale = torch.full((16 * times, K // 32), byte, device="cuda", dtype=torch.uint8)
+        exact = widened(q, scale, K)[:, 0]
+        expected = torch.where(exact.abs() >= 2.0 ** 128, exact.sign() * math.inf, exact)
+        got = operators.four_bit_linear(torch.ones((M, K), device="cuda", dtype=torch.bfloat16), q, scale).y
+        print(byte, got[0, :16].tolist(), flush=True)
+        assert torch.equal(got.double(), expected.nan_to_num(0, math.inf, -math.inf).expand(M, -1))
+
+
+@pytest.mark.gpu
+def test_groups_of_the_largest_numbers():
+    """float32 numbers that the nearest values of their group bring to 2^128 keep their scale and value; in a product such a weight is infinite, as bfloat16 has no number there."""
+    x = torch.zeros((2, 32), device="cuda")
+    x[0, 0], x[1, 0] = 3.4e38, 2.0 ** 127
+    r = operators.quantize_groups(x)
+    assert [int(v) for v in r.scale[:, 0]] == [253, 252] and widened(r.q, r.scale, 32)[:, 0].tolist() == [2.0 ** 128, 2.0 ** 127]
+    y = operators.four_bit_linear(torch.ones((1, 32), device="cuda", dtype=torch.bfloat16), r.q, r.scale).y
+    assert y[0].tolist() == [math.inf, 2.0 ** 127]

@@ -1,6 +1,7 @@
 // Products with weights in 4 bits: e2m1 values (a sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6), two to a byte with the first in the low half,
 // and for each 32 along a row a power of two, as its exponent and 127 (e8m0).  gfx950 converts a pair of values, scaled, to a pair of 16-bit numbers in one
-// instruction; a value has two significant bits, so bfloat16 holds every scaled one exactly, and float16 those within its range.
+// instruction; a value has two significant bits, so bfloat16 holds every scaled one below 2^128 exactly, down to 2^-128 (which the matrix instruction takes as it is), and
+// float16 those within its range; larger ones are infinite.
 #ifndef TIRAMISU_AMD_FOUR_BIT_HIP_H
 #define TIRAMISU_AMD_FOUR_BIT_HIP_H
 #include "linear_few_tokens.hip.h"

@@ -222,8 +222,8 @@ def quantize_groups(x):
 
 
 def four_bit_linear(x, weight, weight_scale, bias=None, residual=None, activation="none"):
-    """``linear`` with a weight in 4 bits (``quantize_groups``' values and scales); x, bias and residual float16 or bfloat16.  Weights are multiplied as numbers of x's type, which bfloat16
-    holds exactly and float16 within its range."""
+    """``linear`` with a weight in 4 bits (``quantize_groups``' values and scales); x, bias and residual float16 or bfloat16.  Weights are multiplied as numbers of x's type, which are exact in
+    bfloat16 below 2^128 and in float16 within its range, and infinite beyond."""
     return Linear(*_operators.four_bit_linear(x, weight, weight_scale, bias, residual, _activation(activation)))
 
 
