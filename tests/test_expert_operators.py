@@ -953,3 +953,17 @@ def test_rows_that_are_none_of_x_are_zeros_whatever_the_weights_hold(sizes, behi
         for activation in ("silu", "gelu"):
             got = operators.grouped_gated_linear(view, ws[0], ws[1], offsets, rows=rows, activation=activation, x_scale=xs, gate_scale=scales[0], up_scale=scales[1], keep_pre=True)
             assert not any(bool(t[nobody].any()) for t in got) and all(bool(torch.isnan(t[~nobody][:, 0]).all()) for t in got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(1025, 8195), (1024, 8191)])
+def test_gradients_of_weights_around_the_size_that_goes_past_the_caches(N, K):
+    """2^27 bytes of eight groups' gradients and some less or more, rows at odd elements; terms of a tile shared among workgroups or not."""
+    dtype, sizes = torch.bfloat16, [70, 0, 3, 130, 1, 0, 40, 9]
+    offsets, _, x, _, (w,), _, xd, _ = grouped_inputs(sizes, 5, N, K, dtype, 127)
+    dy = normal((x.shape[0], N), dtype, generator(131))
+    got, d, at = operators.grouped_linear_backward(dy, x, w, offsets).dweight, dy.double(), 0
+    for e, n in enumerate(sizes):
+        a, b = d[at:at + n].t(), xd[at:at + n]
+        at += n
+        close(got[e], a @ b, backward_bound(dtype, a @ b, n, a.abs() @ b.abs()), "group %d" % e)

@@ -702,3 +702,20 @@ def test_what_the_c_abi_refuses(capfd):
     assert w.tiramisu_hip_rms_norm(p, None, p, p, None, None, None, 4, 1 << 27, 0, 0, 1e-6, 2, 2) == 1
     messages = capfd.readouterr().err.strip().splitlines()
     assert len(messages) == 20 and all(m.startswith("Error at tiramisu_hip_") for m in messages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(8200, 8195), (8192, 8191), (8192, 8192)])
+def test_gradients_of_weights_around_the_size_that_goes_past_the_caches(N, K):
+    """2^27 bytes of weights' gradients and some less or more, dense rows at odd elements among them."""
+    M, dtype, g = 70, torch.bfloat16, generator(113)
+    x, w, dy = normal((M, K), dtype, g), normal((N, K), dtype, g, K ** -0.5), normal((M, N), dtype, g)
+    xd, dd = x.double(), dy.double()
+    exact = dd.t() @ xd
+    close(operators.linear_backward(dy, x, w).dweight, exact, backward_bound(dtype, exact, M, dd.t().abs() @ xd.abs()), "dweight")
+    n = N // 2
+    gate, up = normal((M, n), dtype, g), normal((M, n), dtype, g)
+    got = operators.gated_linear_backward(dy[:, :n].contiguous(), x, w[:n], w[n:], gate, up, activation="none")
+    for ours, dz, name in ((got.dgate_weight, dd[:, :n] * up.double(), "dgate_weight"), (got.dup_weight, dd[:, :n] * gate.double(), "dup_weight")):
+        exact = dz.t() @ xd
+        close(ours, exact, backward_bound(dtype, exact, M, dz.t().abs() @ xd.abs()), name)

@@ -494,6 +494,7 @@ int tiramisu_hip_grouped_linear_backward(const void *dy, const void *x, const vo
     grouped_arguments a = grouped_of(S, groups, K, N, offsets), b = grouped_of(N, groups, K, 0, offsets);
     a.p.y = S > 0 ? dx : nullptr;
     b.p.y = gradient ? dweight : nullptr;
+    b.p.past = groups * N * K * 2 >= PAST_THE_CACHES;
     b.rows = (int)S;
     const planned_gradients g = plan_gradients(a, b, 1, s);
     if (s.take(__FUNCTION__)) return 1;
@@ -536,6 +537,7 @@ int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, co
     a.p.y = m > 0 ? dx : nullptr;
     b.p.y = weights ? dgate_weight : nullptr;
     b.p.y_below = weights ? dup_weight : nullptr;
+    b.p.past = 2 * groups * N * K * 2 >= PAST_THE_CACHES;
     b.p.rows_above = (int)n;
     b.p.split_row = (int)half;
     b.rows = (int)m;

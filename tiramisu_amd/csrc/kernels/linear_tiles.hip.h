@@ -52,6 +52,7 @@ struct product_arguments {
     void *y_below;                          // rows from `split_row` on go here (row split_row first); rows from `rows_above` to it nowhere
     int split_row, rows_above;
     int activation;
+    int past;                               // gradient of weights: stored past the caches
     float *partial;                         // sums only, [split][M][N] (GATED: [split][2][M][N]); null: the whole product in one workgroup
     int slices_per_split;
 };
@@ -457,13 +458,13 @@ template <int Y>
 __device__ __forceinline__ void load_residual(const product_arguments &p, float (&r)[8], long m, long n, int some) {
     load_some<Y>((const stored<Y> *)p.residual + m * p.ldr + n, some, r);
 }
-// PAST: past the caches
-template <int Y, bool PAST = false>
+// WEIGHTS: a gradient of weights, which may go past the caches
+template <int Y, bool WEIGHTS = false>
 __device__ __forceinline__ void store_linear(const product_arguments &p, const float (&z)[8], long m, long n, int some) {
     typedef stored<Y> T;
     if (m >= p.rows_above && m < p.split_row) return;
     T *const to = m < p.rows_above ? (T *)p.y + m * p.N + n : (T *)p.y_below + (m - p.split_row) * p.N + n;
-    if constexpr (PAST) store_some_past<Y>(to, some, z);
+    if (WEIGHTS && p.past) store_some_past<Y>(to, some, z);
     else store_some<Y>(to, some, z);
 }
 template <int Y>

@@ -31,6 +31,11 @@ constexpr long MOST_FEW_COLUMNS = 1 << 26;               // of a product of few 
 constexpr int64_t MOST_ROW_BYTES = 1 << 22;              // of an operand with k along its rows: a tile's offsets stay below 2^31
 constexpr int64_t MOST_STEP = 1 << 23;                   // elements from k to k of one with k down its columns: the same
 
+// Gradients of weights of so many bytes in all go past the caches: smaller ones are still there for the optimiser that reads them next (backward pass and its reader, which adds them
+// to 32-bit weights, us past the caches / through them, bf16: 4 MB 32.2 / 30.3, 17 MB 85.7 / 84.8, 34 MB 93.1 / 91.3, copied instead 78.1 / 75.8, 67 MB copied 227.9 / 223.8), larger ones only
+// put operands out of them (134 MB 511.9 / 521.5, 268 MB 657.0 / 679.5, those of 32 groups without a reader 356 / 369).
+constexpr uint64_t PAST_THE_CACHES = 1 << 27;
+
 inline bool known_type(int type, bool with_f32) { return type == F16 || type == BF16 || (with_f32 && type == F32); }
 inline int bytes_of(int type) { return type == F32 ? 4 : type == F8 ? 1 : 2; }
 

@@ -495,6 +495,7 @@ int tiramisu_hip_linear_backward(const void *dy, const void *x, const void *weig
     q.ldb = xs.ld;
     p.y = dx;
     q.y = dweight;
+    q.past = N * K * 2 >= PAST_THE_CACHES;
     planned_gradients g = plan_gradients(type, p, 1, q, s);
     if (s.take(__FUNCTION__)) return 1;
     column_sums sums = {};
@@ -538,6 +539,7 @@ int tiramisu_hip_gated_linear_backward(const void *dh, const void *x, const void
         q.y_below = dup_weight;
         q.rows_above = (int)n;
         q.split_row = (int)half;
+        q.past = 2 * N * K * 2 >= PAST_THE_CACHES;
     }
     planned_gradients g = plan_gradients(type, p, 2, q, s);
     if (s.take(__FUNCTION__)) return 1;
