@@ -100,7 +100,7 @@ int refuse_grouped(const char *fn, uint64_t S, uint64_t T, uint64_t groups, uint
 // ---- which tile, by the launch's model (operators.hip) for the tiles that the groups have if the rows are spread as routers spread them, a tenth more than evenly, a
 // group's last tile half empty where it has several; what the model says is multiplied by `factor`, as groups bring weights of their own, whose bytes come at 4.6 TB/s.  192 x 128 are 16 bits' and forward.  Of 585
 // launches of 16 bits and 135 of 8 (2 to 128 groups, 64 to 32768 rows, groups uneven) the choice is 5 % and 3 % behind the fastest tile in the geometric mean (16 bits without 192 x 128: 6 %), a third to a half at worst:
-// few tiles of few rows, or a round that begins with a few tiles, as the groups' sizes are not known here.
+// few tiles of few rows, or a round that begins with a few tiles, as the groups' sizes are not known here (4096 rows in 16 groups, 2048 x 6144: 175 us on the 256 x 256 that this takes, 146 on 192 x 128).
 constexpr struct { product_tile tile; int rows, columns; double factor; } GROUPED_TILES[] = {{TILE_256, 256, 256, 1.0}, {TILE_256x128, 256, 128, 1.1}, {TILE_192x128, 192, 128, 1.05}, {TILE_128, 128, 128, 1.0},
                                                                                              {TILE_64, 64, 64, 1.25}};
 double rows_tiles(const grouped_arguments &a, int rows, int columns, bool gated) {
@@ -526,6 +526,8 @@ int tiramisu_hip_grouped_gated_linear_backward(const void *dh, const void *x, co
     if (K == 0) return 0;
     timed record(__FUNCTION__);
     const long m = (long)S, n = (long)N, k = (long)K, half = (n + 7) / 8 * 8, ld = 2 * half;        // [dgate | dup] in rows of 2 x `half` elements
+    // (dgate and dup are operands of two products, of 16 bits as the matrix instructions take them: kept in 32 they would be two operands each, at twice the products' work.  Gradients are off by
+    // 0.0024 of their size, 0.0017 with 32 bits.)
     call_scratch s;
     const uint64_t gradient = s.want((uint64_t)std::max(1L, m) * std::max(1L, ld) * 2);
     const long of_weights = dx && m ? n * (long)groups : 0;

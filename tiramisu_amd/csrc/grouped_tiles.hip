@@ -63,7 +63,7 @@ template <int E, bool A_ROWS, bool B_ROWS, int EPILOGUE> struct tiles_for {
     typedef tile_config<E, 64, 128, 2, 4, 4, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_end;
     typedef tile_config<E, 64, 128, 2, 4, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_128_pair_end;
     // Two to a compute unit, whose LDS they fill, four wavefronts of 96 x 64 each: they read LDS as little as those of 256 x 128 and cover each other's beginnings and ends
-    // (8192 rows in 8 groups bf16, 2048 x 2048, as 256 x 256 / 256 x 128 / 128 x 128 / so: 89 / 81 / 80 / 65 us, gated 158 / 151 / 157 / 131).
+    // (8192 rows in 8 groups bf16, 2048 x 2048, as 256 x 256 / 256 x 128 / 128 x 128 / so: 89 / 81 / 80 / 65 us, gated, which the rule leaves on the first, 158 / 151 / 157 / 131).
     typedef tile_config<E, 192, 128, 2, 2, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_192x128;
     typedef tile_config<E, 96, 128, 1, 4, 2, A_ROWS, B_ROWS, EPILOGUE, 16> tile_192x128_end;
     typedef tile_config<E, 64, SMALL_N, 2, EPILOGUE == GATED ? 4 : 2, 3, A_ROWS, B_ROWS, EPILOGUE, 16> tile_64;
